@@ -7,6 +7,8 @@ operations or, where ``own`` is set, through ``nvcr_b200.tokens``.
 
 The 4-bit form is the same everywhere: a group of consecutive values is held as codes c in 0..15 with an FP16
 scale s and an FP16 minimum m, and stands for c * s + m. Two codes share a byte, the even index in the low half.
+Appending takes m = fp16(min), s = fp16((max - min) / 15), or 2^-24 where that is 0 and the range is not, and
+c = clamp(rint((x - m) / s), 0, 15), from FP32.
 """
 import math
 
@@ -113,6 +115,7 @@ def _codes(x, group):
     low, high = g.amin(-1), g.amax(-1)
     minimums = low.half()
     scales = ((high - low) * torch.tensor(1.0 / 15.0, dtype=torch.float32, device=x.device)).half()
+    scales = torch.where((scales == 0) & (high > low), torch.full_like(scales, 2.0 ** -24), scales)
     s = scales.float().unsqueeze(-1)
     codes = torch.where(s > 0, torch.round((g - minimums.float().unsqueeze(-1)) / s), torch.zeros_like(g))
     return codes.clamp(0, 15).to(torch.uint8).flatten(-2), scales, minimums
@@ -403,6 +406,7 @@ def _exact_append(s):
         parts = x.double().reshape(*x.shape[:-1], -1, case["group"])
         low, high = parts.min(-1, keepdim=True).values, parts.max(-1, keepdim=True).values
         m, step = low.half().double(), ((high - low) / 15).half().double()
+        step = step.clamp(min=2.0 ** -24) * (high > low)  # the smallest FP16 for a range too small for it
         level = torch.where(step > 0, (parts - m) / step.clamp(min=1e-30), torch.zeros_like(parts)).round()
         return (level.clamp(0, 15) * step + m).reshape(x.shape)
 
