@@ -11,7 +11,8 @@
  * Every output is bit-identical to the reference's CPU executor run_cpu
  * (src/deterministic/program.cpp:702-820); NaN payloads are unspecified.
  * The nvcr_sm100_fx_* functions at the end load and run programs of the other
- * profile, nvcr.fx.v1 (reference src/deterministic/fx_program.hpp:70-79).
+ * profile, nvcr.fx.v1 (reference src/deterministic/fx_program.hpp:70-79), and the
+ * nvcr_sm100_token_* functions are the operators of a token model's step.
  *
  * Plain C types only. Every function returns NVCR_SM100_OK (0) or
  * 1 + the reference's nvcr::ErrorCode value (include/nvcr/common/error.hpp:11-34),
@@ -365,6 +366,116 @@ int nvcr_sm100_dcvc_yuv420p8_to_ycbcr_padded(const uint8_t* input, int32_t width
 int nvcr_sm100_dcvc_ycbcr_padded_to_yuv420p8(const uint16_t* input, int32_t batch, int32_t channels, int32_t height,
                                              int32_t width, int32_t visible_width, int32_t visible_height,
                                              uint8_t* output, void* stream);
+
+/* Token operators: one step of a token model in low-bit form (an autoregressive
+ * context model over a codec's symbols, or a language model beside the codec).
+ * No counterpart in the reference. All tensors are in device memory, strides
+ * are in elements, last dimensions are contiguous, and every call enqueues on
+ * `stream` (a cudaStream_t; NULL for the default stream) and returns; a refused
+ * call (NVCR_SM100_INVALID_ARGUMENT) enqueues nothing.
+ *
+ * The 4-bit group form: `group` consecutive values (32, 64 or 128) are held as
+ * codes c in 0..15, two a byte with the even index in the low half, an FP16
+ * scale s and an FP16 minimum m, and stand for c * s + m. */
+#define NVCR_SM100_TOKEN_F16 0
+#define NVCR_SM100_TOKEN_BF16 1
+#define NVCR_SM100_TOKEN_F32 2
+
+/* Norms after and before a block with its gate and residual, in one pass:
+ *   p = post ? N(block; post_weight, post_bias) : block
+ *   hidden = residual_scale * residual + gate * p
+ *   normed = N(hidden; pre_weight, pre_bias)
+ * N(v) = v / sqrt(mean(v^2) + epsilon) * (weight + weight_offset) + bias, of
+ * v - mean(v) when `layer` is not 0. `rows` rows of `width` values of `type`;
+ * residual and gate may be NULL (no term; one), a gate_stride of 0 gives every
+ * row the same gate; NULL weights are one and NULL biases zero; hidden and
+ * normed are contiguous and either may be NULL. FP32 inside; normed is taken
+ * from the unrounded sum. hidden may be residual's buffer and normed block's
+ * (same rows and strides); no other overlap. */
+int nvcr_sm100_token_norm(int type, int layer, int post, const void* block, int64_t block_stride, const void* residual,
+                          int64_t residual_stride, const void* gate, int64_t gate_stride, const void* post_weight,
+                          const void* post_bias, const void* pre_weight, const void* pre_bias, void* hidden,
+                          void* normed, int64_t rows, int32_t width, float residual_scale, float weight_offset,
+                          float epsilon, void* stream);
+
+/* A paged cache of keys and values in 4 bits; slot p * page_size + i is place i
+ * of page p. The buffers are the caller's. head_dim is 64, 128 or 256, group
+ * 32, 64 or 128 with 1, 2 or 4 groups a head, page_size a multiple of 16.
+ * Kernels OR into *status (may be NULL) what they find wrong in device data,
+ * and leave the token or page concerned out: 1 a slot past the end, 2 a
+ * position outside the rotation table, 4 a page number outside the cache, 8 a
+ * length or an offset outside what the call said. */
+typedef struct nvcr_sm100_token_cache {
+    uint8_t* key_codes;    /* [pages][kv_heads][page_size][head_dim / 2] */
+    uint16_t* key_scales;  /* [pages][kv_heads][page_size][head_dim / group][2]: FP16 scale, minimum */
+    uint8_t* value_codes;
+    uint16_t* value_scales;
+    uint32_t* status;
+    int32_t pages;
+    int32_t kv_heads;
+    int32_t page_size;
+    int32_t head_dim;
+    int32_t group;
+} nvcr_sm100_token_cache;
+
+/* Stores `tokens` tokens' keys and values (F16 or BF16) at their slots; a
+ * negative slot is a padding token and is not stored, and slots are distinct.
+ * With positions, keys are rotated before they are stored and queries (may be
+ * NULL) into `rotated` [tokens][query_heads][head_dim]: the first `rotary`
+ * (even) channels of a head, as pairs (i, i + rotary / 2), or (2 i, 2 i + 1)
+ * when `interleaved` is not 0, by row positions[token] of the FP32 tables
+ * cosines and sines [table_rows][rotary / 2]. Without positions (NULL) queries
+ * are copied. A token whose position is outside the table is not stored and
+ * its rotated queries are NaN. Each group is stored with m = fp16(min), s =
+ * fp16((max - min) * (1 / 15)), or 2^-24 where that is 0 and the range is not,
+ * and c = clamp(rint((x - m) / s), 0, 15), from FP32; a group whose range is
+ * past FP16's, or that holds a NaN or an infinity, stands for non-finite values. */
+int nvcr_sm100_token_append(const nvcr_sm100_token_cache* cache, int type, const void* keys, int64_t key_stride,
+                            int64_t key_head_stride, const void* values, int64_t value_stride,
+                            int64_t value_head_stride, const int64_t* slots, int64_t tokens, const void* queries,
+                            int64_t query_stride, int64_t query_head_stride, int32_t query_heads, void* rotated,
+                            const int32_t* positions, const float* cosines, const float* sines, int64_t table_rows,
+                            int32_t rotary, int interleaved, void* stream);
+
+/* The values that `count` slots' codes stand for, as keys and values
+ * [count][kv_heads][head_dim] of `type`; zeros for a slot outside the cache. */
+int nvcr_sm100_token_read(const nvcr_sm100_token_cache* cache, int type, const int64_t* slots, int64_t count,
+                          void* keys, void* values, void* stream);
+
+/* Working memory of nvcr_sm100_token_attend on the current device. A context
+ * serves one call at a time: calls that share it belong on one stream. */
+typedef struct nvcr_sm100_token_context nvcr_sm100_token_context;
+int nvcr_sm100_token_context_create(nvcr_sm100_token_context** context);
+void nvcr_sm100_token_context_destroy(nvcr_sm100_token_context* context);
+
+/* Attention of `tokens` new tokens of `batch` sequences over their cached keys
+ * and values (the new tokens' own already appended). Sequence b's new tokens
+ * are query_offsets[b] .. query_offsets[b + 1] - 1 (NULL: token b), at most
+ * max_queries of them; its length, new tokens included, is lengths[b], at most
+ * max_length; place t is on page page_table[b * table_stride + t / page_size],
+ * and page_table has table_pages columns. A token sees the places up to its
+ * own. Query head h reads cache head h / (heads / kv_heads). Scores are scaled
+ * by `scale`; output [tokens][heads][head_dim] of `type` (F16 or BF16), zeros
+ * for a token that sees nothing. FP32 softmax and sums. */
+int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_token_cache* cache, int type,
+                            const void* queries, int64_t query_stride, int64_t query_head_stride, int64_t tokens,
+                            int32_t heads, const int32_t* page_table, int64_t table_stride, int32_t table_pages,
+                            const int32_t* lengths, int32_t batch, const int32_t* query_offsets, int32_t max_queries,
+                            int32_t max_length, float scale, void* output, void* stream);
+
+/* Weights in the 4-bit group form, laid out once for nvcr_sm100_token_multiply:
+ * codes [outputs][inputs / 2], scales and minimums [outputs][inputs / group],
+ * inputs a multiple of group. The packed buffers' sizes in bytes come first. */
+int nvcr_sm100_token_packed_bytes(int32_t outputs, int32_t inputs, int32_t group, size_t* code_bytes,
+                                  size_t* scale_bytes);
+int nvcr_sm100_token_pack(const uint8_t* codes, const uint16_t* scales, const uint16_t* minimums, int32_t outputs,
+                          int32_t inputs, int32_t group, void* packed_codes, void* packed_scales, void* stream);
+/* y[r][n] = sum_k x[r][k] w[n][k] + bias[n] for `rows` rows of x (F16 or BF16);
+ * bias may be NULL; y is contiguous. Made for a few rows: each 16 rows read
+ * the weights once. FP32 sums. */
+int nvcr_sm100_token_multiply(int type, const void* x, int64_t x_stride, int64_t rows, const void* packed_codes,
+                              const void* packed_scales, int32_t outputs, int32_t inputs, int32_t group,
+                              const void* bias, void* y, void* stream);
 
 #ifdef __cplusplus
 }

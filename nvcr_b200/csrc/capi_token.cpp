@@ -1,0 +1,256 @@
+// The token operators of include/nvcr_sm100.h: argument checks and launches.
+
+#include "../../include/nvcr_sm100.h"
+
+#include "capi_internal.hpp"
+#include "token_kernels.hpp"
+
+#include <cmath>
+#include <cstdint>
+#include <exception>
+#include <limits>
+#include <new>
+#include <string>
+
+struct nvcr_sm100_token_context {
+    int device;
+};
+
+namespace {
+
+using nvcr_sm100::Code;
+using nvcr_sm100::Error;
+using nvcr_sm100::report_error;
+using nvcr_sm100::report_ok;
+namespace token = nvcr_sm100::token;
+
+int refuse(const char* reason) { return report_error(Error{Code::invalid_argument, reason}); }
+
+int launched(cudaError_t status) {
+    if (status == cudaSuccess) return report_ok();
+    return report_error(Error{Code::backend_error, cudaGetErrorString(status)});
+}
+
+template <typename F>
+int guarded(F&& body) {
+    try {
+        return body();
+    } catch (const std::bad_alloc&) {
+        return report_error(Error{Code::resource_exhausted, "host allocation failed"});
+    } catch (const std::exception& exception) {
+        return report_error(Error{Code::internal_error, exception.what()});
+    } catch (...) {
+        return report_error(Error{Code::internal_error, "unknown exception"});
+    }
+}
+
+bool half_type(int type) { return type == NVCR_SM100_TOKEN_F16 || type == NVCR_SM100_TOKEN_BF16; }
+bool any_type(int type) { return half_type(type) || type == NVCR_SM100_TOKEN_F32; }
+
+constexpr std::int64_t most_rows = std::numeric_limits<std::int32_t>::max();
+
+// Null when the cache's shape and buffers can be used, else why not.
+const char* cache_refusal(const nvcr_sm100_token_cache* cache) {
+    if (cache == nullptr || cache->key_codes == nullptr || cache->key_scales == nullptr ||
+        cache->value_codes == nullptr || cache->value_scales == nullptr) {
+        return "null cache buffer";
+    }
+    if (cache->pages <= 0 || cache->kv_heads <= 0 || cache->kv_heads > 65535) return "cache pages or heads out of range";
+    if (cache->page_size <= 0 || cache->page_size % 16 != 0) return "cache page_size must be a positive multiple of 16";
+    if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256) {
+        return "cache head_dim must be 64, 128 or 256";
+    }
+    if ((cache->group != 32 && cache->group != 64 && cache->group != 128) || cache->group > cache->head_dim ||
+        cache->head_dim > 4 * cache->group) {
+        return "cache group must be 32, 64 or 128, with 1, 2 or 4 groups a head";
+    }
+    for (const void* buffer : {static_cast<const void*>(cache->key_codes), static_cast<const void*>(cache->key_scales),
+                               static_cast<const void*>(cache->value_codes),
+                               static_cast<const void*>(cache->value_scales)}) {
+        if (reinterpret_cast<std::uintptr_t>(buffer) % 16 != 0) return "cache buffers must be 16-byte aligned";
+    }
+    return nullptr;
+}
+
+token::Cache cache_of(const nvcr_sm100_token_cache& cache) {
+    return {cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.status,
+            cache.pages,     cache.kv_heads,   cache.page_size,   cache.head_dim,     cache.group};
+}
+
+bool matrix_shape(std::int32_t outputs, std::int32_t inputs, std::int32_t group) {
+    return outputs > 0 && inputs > 0 && (group == 32 || group == 64 || group == 128) && inputs % group == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int nvcr_sm100_token_norm(int type, int layer, int post, const void* block, int64_t block_stride, const void* residual,
+                          int64_t residual_stride, const void* gate, int64_t gate_stride, const void* post_weight,
+                          const void* post_bias, const void* pre_weight, const void* pre_bias, void* hidden,
+                          void* normed, int64_t rows, int32_t width, float residual_scale, float weight_offset,
+                          float epsilon, void* stream) {
+    return guarded([&] {
+        if (!any_type(type)) return refuse("unknown type");
+        if (rows < 0 || rows > most_rows || width <= 0) return refuse("rows or width out of range");
+        if (rows > 0 && hidden == nullptr && normed == nullptr) return refuse("neither hidden nor normed is wanted");
+        if (rows > 0 && block == nullptr) return refuse("null block");
+        if (!(epsilon >= 0.0f)) return refuse("epsilon must not be negative");
+        return launched(token::block_norm({static_cast<token::Type>(type), layer != 0, post != 0, block, block_stride,
+                                           residual, residual_stride, gate, gate_stride, post_weight, post_bias,
+                                           pre_weight, pre_bias, hidden, normed, rows, width, residual_scale,
+                                           weight_offset, epsilon},
+                                          static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_append(const nvcr_sm100_token_cache* cache, int type, const void* keys, int64_t key_stride,
+                            int64_t key_head_stride, const void* values, int64_t value_stride,
+                            int64_t value_head_stride, const int64_t* slots, int64_t tokens, const void* queries,
+                            int64_t query_stride, int64_t query_head_stride, int32_t query_heads, void* rotated,
+                            const int32_t* positions, const float* cosines, const float* sines, int64_t table_rows,
+                            int32_t rotary, int interleaved, void* stream) {
+    return guarded([&] {
+        if (const char* reason = cache_refusal(cache)) return refuse(reason);
+        if (!half_type(type)) return refuse("type must be F16 or BF16");
+        if (tokens < 0 || tokens > most_rows) return refuse("tokens out of range");
+        if (tokens > 0 && (keys == nullptr || values == nullptr || slots == nullptr)) {
+            return refuse("null keys, values or slots");
+        }
+        if (queries != nullptr && (rotated == nullptr || query_heads <= 0 || query_heads > 65535)) {
+            return refuse("queries need an output and 1 to 65535 heads");
+        }
+        if (positions != nullptr) {
+            if (cosines == nullptr || sines == nullptr || table_rows <= 0) return refuse("null or empty rotation table");
+            if (rotary <= 0 || rotary % 2 != 0 || rotary > cache->head_dim) {
+                return refuse("rotary must be even, positive and at most head_dim");
+            }
+        }
+        return launched(token::append(cache_of(*cache),
+                                      {static_cast<token::Type>(type), keys, key_stride, key_head_stride, values,
+                                       value_stride, value_head_stride, slots, tokens, queries, query_stride,
+                                       query_head_stride, query_heads, rotated, positions, cosines, sines, table_rows,
+                                       rotary, interleaved != 0},
+                                      static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_read(const nvcr_sm100_token_cache* cache, int type, const int64_t* slots, int64_t count,
+                          void* keys, void* values, void* stream) {
+    return guarded([&] {
+        if (const char* reason = cache_refusal(cache)) return refuse(reason);
+        if (!any_type(type)) return refuse("unknown type");
+        if (count < 0 || count > most_rows) return refuse("count out of range");
+        if (count > 0 && (slots == nullptr || keys == nullptr || values == nullptr)) {
+            return refuse("null slots, keys or values");
+        }
+        return launched(token::read(cache_of(*cache), static_cast<token::Type>(type), slots, count, keys, values,
+                                    static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_context_create(nvcr_sm100_token_context** context) {
+    return guarded([&] {
+        if (context == nullptr) return refuse("null argument");
+        *context = nullptr;
+        int device = 0;
+        const cudaError_t status = cudaGetDevice(&device);
+        if (status != cudaSuccess) return launched(status);
+        *context = new nvcr_sm100_token_context{device};
+        return report_ok();
+    });
+}
+
+void nvcr_sm100_token_context_destroy(nvcr_sm100_token_context* context) { delete context; }
+
+int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_token_cache* cache, int type,
+                            const void* queries, int64_t query_stride, int64_t query_head_stride, int64_t tokens,
+                            int32_t heads, const int32_t* page_table, int64_t table_stride, int32_t table_pages,
+                            const int32_t* lengths, int32_t batch, const int32_t* query_offsets, int32_t max_queries,
+                            int32_t max_length, float scale, void* output, void* stream) {
+    return guarded([&] {
+        if (context == nullptr) return refuse("null context");
+        if (const char* reason = cache_refusal(cache)) return refuse(reason);
+        if (!half_type(type)) return refuse("type must be F16 or BF16");
+        if (tokens < 0 || tokens > most_rows || batch < 0 || batch > 65535) return refuse("tokens or batch out of range");
+        if (heads <= 0 || heads > 65535 || heads % cache->kv_heads != 0) {
+            return refuse("heads must be a positive multiple of the cache's heads");
+        }
+        if (max_queries <= 0 || max_queries > 65535) return refuse("max_queries out of range");
+        if (query_offsets == nullptr && tokens != batch) return refuse("without query_offsets there is one token a sequence");
+        if (max_length < 0 || table_pages < 0 ||
+            max_length > static_cast<std::int64_t>(table_pages) * cache->page_size) {
+            return refuse("max_length needs more pages than page_table has");
+        }
+        if (!std::isfinite(scale)) return refuse("scale must be finite");
+        if (tokens > 0 && batch > 0 &&
+            (queries == nullptr || page_table == nullptr || lengths == nullptr || output == nullptr)) {
+            return refuse("null queries, page_table, lengths or output");
+        }
+        int device = 0;
+        const cudaError_t status = cudaGetDevice(&device);
+        if (status != cudaSuccess) return launched(status);
+        if (device != context->device) {
+            return report_error(Error{Code::invalid_state, "the context belongs to device " +
+                                                               std::to_string(context->device)});
+        }
+        return launched(token::attend(cache_of(*cache),
+                                      {static_cast<token::Type>(type), queries, query_stride, query_head_stride, tokens,
+                                       heads, page_table, table_stride, lengths, batch, query_offsets, max_queries,
+                                       max_length, scale, output},
+                                      static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_packed_bytes(int32_t outputs, int32_t inputs, int32_t group, size_t* code_bytes,
+                                  size_t* scale_bytes) {
+    return guarded([&] {
+        if (code_bytes == nullptr || scale_bytes == nullptr) return refuse("null argument");
+        if (!matrix_shape(outputs, inputs, group)) return refuse("inputs must be a multiple of a group of 32, 64 or 128");
+        *code_bytes = token::packed_code_bytes(outputs, inputs);
+        *scale_bytes = token::packed_scale_bytes(outputs, inputs, group);
+        return report_ok();
+    });
+}
+
+int nvcr_sm100_token_pack(const uint8_t* codes, const uint16_t* scales, const uint16_t* minimums, int32_t outputs,
+                          int32_t inputs, int32_t group, void* packed_codes, void* packed_scales, void* stream) {
+    return guarded([&] {
+        if (!matrix_shape(outputs, inputs, group)) return refuse("inputs must be a multiple of a group of 32, 64 or 128");
+        if (codes == nullptr || scales == nullptr || minimums == nullptr || packed_codes == nullptr ||
+            packed_scales == nullptr) {
+            return refuse("null argument");
+        }
+        if (reinterpret_cast<std::uintptr_t>(packed_codes) % 16 != 0 ||
+            reinterpret_cast<std::uintptr_t>(packed_scales) % 16 != 0) {
+            return refuse("packed buffers must be 16-byte aligned");
+        }
+        return launched(token::pack(codes, scales, minimums, outputs, inputs, group,
+                                    static_cast<std::uint8_t*>(packed_codes), static_cast<std::uint16_t*>(packed_scales),
+                                    static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_multiply(int type, const void* x, int64_t x_stride, int64_t rows, const void* packed_codes,
+                              const void* packed_scales, int32_t outputs, int32_t inputs, int32_t group,
+                              const void* bias, void* y, void* stream) {
+    return guarded([&] {
+        if (!half_type(type)) return refuse("type must be F16 or BF16");
+        if (!matrix_shape(outputs, inputs, group)) return refuse("inputs must be a multiple of a group of 32, 64 or 128");
+        if (rows < 0 || rows > 65535) return refuse("rows out of range");
+        if (packed_codes == nullptr || packed_scales == nullptr || (rows > 0 && (x == nullptr || y == nullptr))) {
+            return refuse("null argument");
+        }
+        if (reinterpret_cast<std::uintptr_t>(packed_codes) % 16 != 0 ||
+            reinterpret_cast<std::uintptr_t>(packed_scales) % 16 != 0) {
+            return refuse("packed buffers must be 16-byte aligned");
+        }
+        return launched(token::multiply({static_cast<token::Type>(type), x, x_stride, rows,
+                                         static_cast<const std::uint8_t*>(packed_codes),
+                                         static_cast<const std::uint16_t*>(packed_scales), outputs, inputs, group, bias,
+                                         y},
+                                        static_cast<cudaStream_t>(stream)));
+    });
+}
+
+}  // extern "C"

@@ -84,7 +84,9 @@ EXPORTS = [
     "nvcr_sm100_dcvc_clamp_reciprocal_with_quant", "nvcr_sm100_dcvc_add_in_place", "nvcr_sm100_dcvc_multiply_broadcast",
     "nvcr_sm100_dcvc_add_and_multiply", "nvcr_sm100_dcvc_replicate_pad", "nvcr_sm100_dcvc_crop_spatial",
     "nvcr_sm100_dcvc_rgb24_to_ycbcr_padded", "nvcr_sm100_dcvc_yuv420p8_to_ycbcr_padded",
-    "nvcr_sm100_dcvc_ycbcr_padded_to_yuv420p8",
+    "nvcr_sm100_dcvc_ycbcr_padded_to_yuv420p8", "nvcr_sm100_token_norm", "nvcr_sm100_token_append",
+    "nvcr_sm100_token_read", "nvcr_sm100_token_context_create", "nvcr_sm100_token_context_destroy",
+    "nvcr_sm100_token_attend", "nvcr_sm100_token_packed_bytes", "nvcr_sm100_token_pack", "nvcr_sm100_token_multiply",
 ]
 
 _lib: ctypes.CDLL | None = None
@@ -99,6 +101,7 @@ def library() -> ctypes.CDLL:
         raise FileNotFoundError(f"{LIBRARY} is not built; run nvcr_b200.build.build()")
     lib = ctypes.CDLL(str(LIBRARY))
     vp, sz, i32p = ctypes.c_void_p, ctypes.c_size_t, ctypes.POINTER(ctypes.c_int32)
+    i64 = ctypes.c_int64
     tp = ctypes.POINTER(Tensor)
     handle_out = ctypes.POINTER(ctypes.c_void_p)
     signatures = {
@@ -175,6 +178,21 @@ def library() -> ctypes.CDLL:
         "nvcr_sm100_dcvc_yuv420p8_to_ycbcr_padded": (ctypes.c_int, [vp, ctypes.c_int32, ctypes.c_int32, vp,
                                                                     ctypes.c_int32, ctypes.c_int32, vp]),
         "nvcr_sm100_dcvc_ycbcr_padded_to_yuv420p8": (ctypes.c_int, [vp] + [ctypes.c_int32] * 6 + [vp, vp]),
+        "nvcr_sm100_token_norm": (ctypes.c_int, [ctypes.c_int] * 3 + [vp, i64] * 3 + [vp] * 6 + [i64, ctypes.c_int32] +
+                                  [ctypes.c_float] * 3 + [vp]),
+        "nvcr_sm100_token_append": (ctypes.c_int, [vp, ctypes.c_int, vp, i64, i64, vp, i64, i64, vp, i64, vp, i64, i64,
+                                                   ctypes.c_int32, vp, vp, vp, vp, i64, ctypes.c_int32, ctypes.c_int,
+                                                   vp]),
+        "nvcr_sm100_token_read": (ctypes.c_int, [vp, ctypes.c_int, vp, i64, vp, vp, vp]),
+        "nvcr_sm100_token_context_create": (ctypes.c_int, [handle_out]),
+        "nvcr_sm100_token_context_destroy": (None, [vp]),
+        "nvcr_sm100_token_attend": (ctypes.c_int, [vp, vp, ctypes.c_int, vp, i64, i64, i64, ctypes.c_int32, vp, i64,
+                                                   ctypes.c_int32, vp, ctypes.c_int32, vp, ctypes.c_int32,
+                                                   ctypes.c_int32, ctypes.c_float, vp, vp]),
+        "nvcr_sm100_token_packed_bytes": (ctypes.c_int, [ctypes.c_int32] * 3 + [ctypes.POINTER(sz)] * 2),
+        "nvcr_sm100_token_pack": (ctypes.c_int, [vp] * 3 + [ctypes.c_int32] * 3 + [vp] * 3),
+        "nvcr_sm100_token_multiply": (ctypes.c_int, [ctypes.c_int, vp, i64, i64, vp, vp] + [ctypes.c_int32] * 3 +
+                                      [vp] * 3),
     }
     for name, (restype, argtypes) in signatures.items():
         function = getattr(lib, name)

@@ -1,0 +1,322 @@
+"""The token operators through the C ABI: one step of a token model in low-bit form.
+
+``block_norm`` is the norms after and before a block with its gate and residual;
+``PagedCache`` holds keys and values in 4 bits, rotated on the way in;
+``TokenContext.attend`` is attention over such a cache; ``PackedMatrix`` is a
+4-bit weight matrix with group scales. Tensors are torch tensors on the current
+CUDA device; work is enqueued on torch's current stream unless ``stream`` names
+another (then the caller orders the two, and keeps the tensors alive). What the
+operators refuse raises ``ExecutorError``; there is no CPU fallback.
+
+The 4-bit group form, of caches and weights alike: a group of consecutive values
+is held as codes c in 0..15, two a byte with the even index in the low half, an
+FP16 scale s and an FP16 minimum m, and stands for ``c * s + m``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .executor import ErrorCode, ExecutorError, _check, _stream_handle, library
+
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_KINDS = {"rms": 0, "layer": 1}
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("key_codes", ctypes.c_void_p), ("key_scales", ctypes.c_void_p), ("value_codes", ctypes.c_void_p),
+                ("value_scales", ctypes.c_void_p), ("status", ctypes.c_void_p), ("pages", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("group", ctypes.c_int32)]
+
+
+def _refuse(message: str) -> None:
+    raise ExecutorError(ErrorCode.invalid_argument, message)
+
+
+def _require(condition: bool, message: str) -> None:
+    if not condition:
+        _refuse(message)
+
+
+def _stream(stream, tensor: torch.Tensor) -> int | None:
+    if stream is not None:
+        return _stream_handle(stream)
+    _require(tensor.is_cuda, "tensors must be on a CUDA device")
+    return torch._C._cuda_getCurrentRawStream(tensor.device.index)
+
+
+def _like(tensor: torch.Tensor | None, name: str, shape: tuple, first: torch.Tensor) -> int | None:
+    """The address of an optional contiguous tensor of a shape, of `first`'s type and device."""
+    if tensor is None:
+        return None
+    if tensor.dtype is not first.dtype or tensor.device != first.device or tensor.shape != shape \
+            or not tensor.is_contiguous():
+        _refuse(f"{name} must be a contiguous {first.dtype} tensor of shape {tuple(shape)} on {first.device}")
+    return tensor.data_ptr()
+
+
+def _whole(tensor: torch.Tensor, name: str, kind: torch.dtype, shape: tuple, device: torch.device) -> int:
+    if tensor.dtype is not kind or tensor.device != device or tensor.shape != shape or not tensor.is_contiguous():
+        _refuse(f"{name} must be a contiguous {kind} tensor of shape {tuple(shape)} on {device}")
+    return tensor.data_ptr()
+
+
+def _heads(tensor: torch.Tensor, name: str, tokens: int, heads: int, dim: int, first: torch.Tensor) -> int:
+    """The address of a [tokens, heads, dim] tensor whose channels are contiguous (its other strides are free)."""
+    if tensor.dtype is not first.dtype or tensor.device != first.device or tensor.shape != (tokens, heads, dim) \
+            or (tensor.stride(2) != 1 and tensor.numel() > 0):
+        _refuse(f"{name} must be a {first.dtype} tensor of shape {(tokens, heads, dim)} on {first.device} "
+                "with contiguous channels")
+    return tensor.data_ptr()
+
+
+def block_norm(block: torch.Tensor, *, residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+               post: bool = False, post_weight: torch.Tensor | None = None, post_bias: torch.Tensor | None = None,
+               pre_weight: torch.Tensor | None = None, pre_bias: torch.Tensor | None = None, kind: str = "rms",
+               residual_scale: float = 1.0, weight_offset: float = 0.0, epsilon: float = 1e-6,
+               hidden: bool = True, normed: bool = True, stream=None):
+    """``(hidden, normed)`` of a block's output [rows, width] (float16, bfloat16 or float32):
+
+    p = N(block; post_weight, post_bias) if `post` else block;  hidden = residual_scale * residual + gate * p;
+    normed = N(hidden; pre_weight, pre_bias). N is the root-mean-square norm ("rms") or the layer norm ("layer"),
+    with weights taken as weight + weight_offset. `gate` is [width] or [rows, width]. block, residual and a gate of
+    rows may have any row stride. ``hidden=False`` or ``normed=False`` leaves that output out (None)."""
+    _require(block.dim() == 2 and block.dtype in _TYPES, "block must be a [rows, width] tensor of a float type")
+    _require(kind in _KINDS, f"kind must be one of {sorted(_KINDS)}")
+    _require(hidden or normed, "neither hidden nor normed is wanted")
+    rows, width = block.shape
+    strides = [0, 0, 0]
+    for i, (name, tensor) in enumerate((("block", block), ("residual", residual), ("gate", gate))):
+        if tensor is None or (i == 2 and tensor.dim() == 1):
+            continue
+        if tensor.shape != block.shape or tensor.dtype is not block.dtype or tensor.device != block.device \
+                or (tensor.stride(1) != 1 and width > 1):
+            _refuse(f"{name} must be a {block.dtype} tensor of shape {(rows, width)} on {block.device} "
+                    "with contiguous rows")
+        strides[i] = tensor.stride(0)
+    channel = (width,)
+    gate_address = None
+    if gate is not None:
+        gate_address = gate.data_ptr() if gate.dim() == 2 else _like(gate, "gate", channel, block)
+    handle = _stream(stream, block)
+    sums = torch.empty((rows, width), dtype=block.dtype, device=block.device) if hidden else None
+    out = torch.empty((rows, width), dtype=block.dtype, device=block.device) if normed else None
+    status = library().nvcr_sm100_token_norm(
+        _TYPES[block.dtype], _KINDS[kind], int(post), block.data_ptr(), strides[0],
+        None if residual is None else residual.data_ptr(), strides[1], gate_address, strides[2],
+        _like(post_weight, "post_weight", channel, block), _like(post_bias, "post_bias", channel, block),
+        _like(pre_weight, "pre_weight", channel, block), _like(pre_bias, "pre_bias", channel, block),
+        None if sums is None else sums.data_ptr(), None if out is None else out.data_ptr(), rows, width,
+        residual_scale, weight_offset, epsilon, handle)
+    if status:
+        _check(status)
+    return sums, out
+
+
+class PagedCache:
+    """A paged cache of keys and values in 4 bits, over the caller's tensors:
+    codes uint8 [pages, kv_heads, page_size, head_dim / 2] and scales float16
+    [pages, kv_heads, page_size, head_dim / group, 2] (scale, minimum), for
+    keys and for values. Slot p * page_size + i is place i of page p."""
+
+    def __init__(self, key_codes: torch.Tensor, key_scales: torch.Tensor, value_codes: torch.Tensor,
+                 value_scales: torch.Tensor) -> None:
+        _require(key_codes.dim() == 4 and key_scales.dim() == 5, "codes have 4 dimensions and scales 5")
+        _require(key_codes.is_cuda, "a cache is on a CUDA device")
+        pages, kv_heads, page_size, half = key_codes.shape
+        groups = key_scales.shape[3]
+        _require(groups > 0 and (2 * half) % groups == 0, "scales hold a whole number of groups")
+        device = key_codes.device
+        code_shape, scale_shape = (pages, kv_heads, page_size, half), (pages, kv_heads, page_size, groups, 2)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.tensors = (key_codes, key_scales, value_codes, value_scales)
+        self._struct = _Cache(_whole(key_codes, "key_codes", torch.uint8, code_shape, device),
+                              _whole(key_scales, "key_scales", torch.float16, scale_shape, device),
+                              _whole(value_codes, "value_codes", torch.uint8, code_shape, device),
+                              _whole(value_scales, "value_scales", torch.float16, scale_shape, device),
+                              self.status.data_ptr(), pages, kv_heads, page_size, 2 * half, 2 * half // groups)
+        self._address = ctypes.addressof(self._struct)
+        self.device, self.pages, self.kv_heads, self.page_size = device, pages, kv_heads, page_size
+        self.head_dim, self.group = 2 * half, 2 * half // groups
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, group: int = 64,
+              device: str | torch.device = "cuda") -> "PagedCache":
+        """A cache of zeros."""
+        _require(head_dim > 0 and group > 0 and head_dim % group == 0 and head_dim % 2 == 0,
+                 "head_dim must be even and a multiple of group")
+        place = (pages, kv_heads, page_size)
+        codes = [torch.zeros(place + (head_dim // 2,), dtype=torch.uint8, device=device) for _ in range(2)]
+        scales = [torch.zeros(place + (head_dim // group, 2), dtype=torch.float16, device=device) for _ in range(2)]
+        return cls(codes[0], scales[0], codes[1], scales[1])
+
+    def append(self, keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor, *,
+               queries: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+               cosines: torch.Tensor | None = None, sines: torch.Tensor | None = None, interleaved: bool = False,
+               stream=None) -> torch.Tensor | None:
+        """Stores keys and values [tokens, kv_heads, head_dim] (float16 or bfloat16) at int64 `slots` (negative: not
+        stored; else distinct). With int32 `positions`, keys are rotated before they are stored, and `queries`
+        [tokens, heads, head_dim] into the tensor that is returned, by rows of the float32 tables `cosines` and
+        `sines` [rows, rotary / 2]: pairs (i, i + rotary / 2), or (2 i, 2 i + 1) if `interleaved`."""
+        _require(keys.dim() == 3 and keys.dtype in (torch.float16, torch.bfloat16) and keys.device == self.device,
+                 "keys must be a float16 or bfloat16 tensor of three dimensions on the cache's device")
+        tokens = keys.shape[0]
+        key_address = _heads(keys, "keys", tokens, self.kv_heads, self.head_dim, keys)
+        value_address = _heads(values, "values", tokens, self.kv_heads, self.head_dim, keys)
+        slot_address = _whole(slots, "slots", torch.int64, (tokens,), self.device)
+        rotated = query_address = position_address = cosine_address = sine_address = None
+        query_heads = query_stride = query_head_stride = table_rows = rotary = 0
+        if queries is not None:
+            _require(queries.dim() == 3, "queries have three dimensions")
+            query_heads = queries.shape[1]
+            query_address = _heads(queries, "queries", tokens, query_heads, self.head_dim, keys)
+            query_stride, query_head_stride = queries.stride(0), queries.stride(1)
+            rotated = torch.empty((tokens, query_heads, self.head_dim), dtype=keys.dtype, device=self.device)
+        if positions is not None:
+            _require(cosines is not None and sines is not None and cosines.dim() == 2, "positions need rotation tables")
+            position_address = _whole(positions, "positions", torch.int32, (tokens,), self.device)
+            table_rows, rotary = cosines.shape[0], 2 * cosines.shape[1]
+            cosine_address = _whole(cosines, "cosines", torch.float32, (table_rows, rotary // 2), self.device)
+            sine_address = _whole(sines, "sines", torch.float32, (table_rows, rotary // 2), self.device)
+        status = library().nvcr_sm100_token_append(
+            self._address, _TYPES[keys.dtype], key_address, keys.stride(0), keys.stride(1), value_address,
+            values.stride(0), values.stride(1), slot_address, tokens, query_address, query_stride, query_head_stride,
+            query_heads, None if rotated is None else rotated.data_ptr(), position_address, cosine_address,
+            sine_address, table_rows, rotary, int(interleaved), _stream(stream, keys))
+        if status:
+            _check(status)
+        return rotated
+
+    def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16,
+             stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values [n, kv_heads, head_dim] that the codes at int64 `slots` stand for (zeros outside)."""
+        _require(slots.dim() == 1 and dtype in _TYPES, "slots have one dimension and dtype is a float type")
+        count = slots.shape[0]
+        slot_address = _whole(slots, "slots", torch.int64, (count,), self.device)
+        keys = torch.empty((count, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        values = torch.empty((count, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        status = library().nvcr_sm100_token_read(self._address, _TYPES[dtype], slot_address, count, keys.data_ptr(),
+                                                 values.data_ptr(), _stream(stream, slots))
+        if status:
+            _check(status)
+        return keys, values
+
+    def check(self) -> None:
+        """Waits for the device and raises if a kernel met a slot, position, page number or length out of range since
+        the last check (the token or page was left out)."""
+        found = int(self.status.item())
+        if found:
+            self.status.zero_()
+            names = [name for bit, name in ((1, "slot"), (2, "position"), (4, "page number"), (8, "length or offset"))
+                     if found & bit]
+            _refuse(f"out of range on the device: {', '.join(names)}")
+
+
+class TokenContext:
+    """Working memory of attention on the current device; calls that share one belong on one stream."""
+
+    def __init__(self) -> None:
+        handle = ctypes.c_void_p()
+        _check(library().nvcr_sm100_token_context_create(ctypes.byref(handle)))
+        self._handle = handle
+
+    def close(self) -> None:
+        if self._handle:
+            library().nvcr_sm100_token_context_destroy(self._handle)
+            self._handle = ctypes.c_void_p()
+
+    def __enter__(self) -> "TokenContext":
+        return self
+
+    def __exit__(self, *exc) -> None:
+        self.close()
+
+    def __del__(self) -> None:
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def attend(self, queries: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor, *,
+               max_length: int, query_offsets: torch.Tensor | None = None, max_queries: int = 1,
+               scale: float | None = None, stream=None) -> torch.Tensor:
+        """Attention of queries [tokens, heads, head_dim] over the cache, the new tokens' own keys and values already
+        appended. int32 `lengths` [batch] (at most `max_length`) count the new tokens; sequence b's pages are row b
+        of the int32 `page_table`; its new tokens are query_offsets[b] .. query_offsets[b + 1] - 1 (int32 [batch + 1],
+        at most `max_queries` each; None: token b). A token sees the places up to its own; one that sees none gives
+        zeros. `scale` defaults to 1 / sqrt(head_dim)."""
+        _require(queries.dim() == 3 and queries.dtype in (torch.float16, torch.bfloat16)
+                 and queries.device == cache.device,
+                 "queries must be a float16 or bfloat16 tensor of three dimensions on the cache's device")
+        tokens, heads, dim = queries.shape
+        query_address = _heads(queries, "queries", tokens, heads, cache.head_dim, queries)
+        _require(lengths.dim() == 1 and page_table.dim() == 2, "lengths have one dimension and page_table two")
+        batch, columns = lengths.shape[0], page_table.shape[1]
+        if page_table.dtype is not torch.int32 or page_table.device != cache.device or page_table.shape[0] != batch \
+                or (page_table.stride(1) != 1 and columns > 1):
+            _refuse(f"page_table must be an int32 tensor of {batch} rows on {cache.device} with contiguous rows")
+        length_address = _whole(lengths, "lengths", torch.int32, (batch,), cache.device)
+        offset_address = None if query_offsets is None else _whole(query_offsets, "query_offsets", torch.int32,
+                                                                   (batch + 1,), cache.device)
+        out = torch.empty((tokens, heads, dim), dtype=queries.dtype, device=queries.device)
+        status = library().nvcr_sm100_token_attend(
+            self._handle, cache._address, _TYPES[queries.dtype], query_address, queries.stride(0), queries.stride(1),
+            tokens, heads, page_table.data_ptr(), page_table.stride(0), columns, length_address, batch, offset_address,
+            max_queries, max_length, dim ** -0.5 if scale is None else scale, out.data_ptr(), _stream(stream, queries))
+        if status:
+            _check(status)
+        return out
+
+
+class PackedMatrix:
+    """A 4-bit weight matrix [outputs, inputs] with group scales, laid out once:
+    codes uint8 [outputs, inputs / 2], scales and minimums float16 [outputs, inputs / group]."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, minimums: torch.Tensor, stream=None) -> None:
+        _require(codes.dim() == 2 and scales.dim() == 2, "codes and scales have two dimensions")
+        _require(codes.is_cuda, "weights are on a CUDA device")
+        outputs, inputs, groups = codes.shape[0], 2 * codes.shape[1], scales.shape[1]
+        _require(groups > 0 and inputs % groups == 0, "scales hold a whole number of groups")
+        device, group = codes.device, inputs // groups
+        addresses = (_whole(codes, "codes", torch.uint8, (outputs, inputs // 2), device),
+                     _whole(scales, "scales", torch.float16, (outputs, groups), device),
+                     _whole(minimums, "minimums", torch.float16, (outputs, groups), device))
+        code_bytes, scale_bytes = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        _check(library().nvcr_sm100_token_packed_bytes(outputs, inputs, group, ctypes.byref(code_bytes),
+                                                       ctypes.byref(scale_bytes)))
+        self.outputs, self.inputs, self.group, self.device = outputs, inputs, group, device
+        self.codes = torch.empty(code_bytes.value, dtype=torch.uint8, device=device)
+        self.scales = torch.empty(scale_bytes.value, dtype=torch.uint8, device=device)
+        self._addresses = (self.codes.data_ptr(), self.scales.data_ptr())
+        _check(library().nvcr_sm100_token_pack(*addresses, outputs, inputs, group, *self._addresses,
+                                               _stream(stream, codes)))
+
+    @classmethod
+    def quantise(cls, weights: torch.Tensor, group: int = 64, stream=None) -> "PackedMatrix":
+        """From a float matrix [outputs, inputs], each group by its own range."""
+        _require(weights.dim() == 2 and group > 0 and weights.shape[1] % group == 0,
+                 "weights have two dimensions and inputs are a multiple of group")
+        parts = weights.float().unflatten(1, (-1, group))
+        low, high = parts.amin(-1), parts.amax(-1)
+        minimums, scales = low.half(), ((high - low) / 15).half()
+        steps = scales.float().unsqueeze(-1)
+        codes = torch.where(steps > 0, torch.round((parts - minimums.float().unsqueeze(-1)) / steps), 0.0)
+        codes = codes.clamp(0, 15).to(torch.uint8).flatten(1)
+        return cls(codes[:, 0::2] | codes[:, 1::2] << 4, scales, minimums, stream)
+
+    def multiply(self, x: torch.Tensor, bias: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """x [rows, inputs] (float16 or bfloat16, any row stride) times the matrix's transpose, plus bias [outputs]."""
+        if x.dim() != 2 or x.shape[1] != self.inputs or x.dtype not in (torch.float16, torch.bfloat16) \
+                or x.device != self.device or x.stride(1) != 1:
+            _refuse(f"x must be a float16 or bfloat16 tensor of shape (rows, {self.inputs}) on {self.device} "
+                    "with contiguous rows")
+        rows = x.shape[0]
+        y = torch.empty((rows, self.outputs), dtype=x.dtype, device=x.device)
+        status = library().nvcr_sm100_token_multiply(
+            _TYPES[x.dtype], x.data_ptr(), x.stride(0), rows, *self._addresses, self.outputs, self.inputs, self.group,
+            _like(bias, "bias", (self.outputs,), x), y.data_ptr(), _stream(stream, x))
+        if status:
+            _check(status)
+        return y
