@@ -5,16 +5,34 @@
 #include "capi_internal.hpp"
 #include "token_kernels.hpp"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <exception>
 #include <limits>
+#include <memory>
+#include <mutex>
 #include <new>
 #include <string>
+#include <vector>
 
 struct nvcr_sm100_token_context {
-    int device;
+    int device = 0;
+    nvcr_sm100::token::AttendWorkspace workspace{};
 };
+
+int nvcr_sm100::token::sm_count() {
+    static const int count = [] {
+        int device = 0, found = 0;
+        if (cudaGetDevice(&device) != cudaSuccess ||
+            cudaDeviceGetAttribute(&found, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || found <= 0) {
+            cudaGetLastError();
+            return 148;
+        }
+        return found;
+    }();
+    return count;
+}
 
 namespace {
 
@@ -24,10 +42,18 @@ using nvcr_sm100::report_error;
 using nvcr_sm100::report_ok;
 namespace token = nvcr_sm100::token;
 
+// Workspaces of destroyed contexts, ready for the next ones: their tickets are
+// zero between calls. `contexts` counts those made, so `spares` never grows
+// past its reservation.
+std::mutex spare_lock;
+std::vector<std::unique_ptr<nvcr_sm100_token_context>> spares;
+std::size_t contexts = 0;
+
 int refuse(const char* reason) { return report_error(Error{Code::invalid_argument, reason}); }
 
 int launched(cudaError_t status) {
     if (status == cudaSuccess) return report_ok();
+    if (status == cudaErrorInvalidValue) return refuse("a size is past what a launch can hold");
     return report_error(Error{Code::backend_error, cudaGetErrorString(status)});
 }
 
@@ -154,14 +180,49 @@ int nvcr_sm100_token_context_create(nvcr_sm100_token_context** context) {
         if (context == nullptr) return refuse("null argument");
         *context = nullptr;
         int device = 0;
-        const cudaError_t status = cudaGetDevice(&device);
+        cudaError_t status = cudaGetDevice(&device);
         if (status != cudaSuccess) return launched(status);
-        *context = new nvcr_sm100_token_context{device};
+        std::lock_guard<std::mutex> guard(spare_lock);
+        auto spare = std::find_if(spares.begin(), spares.end(), [&](const auto& c) { return c->device == device; });
+        if (spare != spares.end()) {
+            *context = spare->release();
+            spares.erase(spare);
+            return report_ok();
+        }
+        spares.reserve(++contexts);  // so that destroying one needs no memory
+        auto made = std::make_unique<nvcr_sm100_token_context>();
+        made->device = device;
+        const std::size_t ticket_bytes = (token::attend_ticket_bytes() + 255) / 256 * 256;
+        unsigned char* memory = nullptr;
+        status = cudaMalloc(&memory, ticket_bytes + token::attend_partial_bytes());
+        if (status == cudaErrorMemoryAllocation) {
+            cudaGetLastError();
+            return report_error(Error{Code::resource_exhausted, "no device memory for the context's workspace"});
+        }
+        if (status == cudaSuccess) status = cudaMemset(memory, 0, ticket_bytes);
+        // the memset is on the default stream, which other streams need not wait for
+        if (status == cudaSuccess) status = cudaStreamSynchronize(nullptr);
+        if (status != cudaSuccess) {
+            cudaFree(memory);
+            return launched(status);
+        }
+        made->workspace = {reinterpret_cast<float*>(memory + ticket_bytes), reinterpret_cast<unsigned*>(memory)};
+        *context = made.release();
         return report_ok();
     });
 }
 
-void nvcr_sm100_token_context_destroy(nvcr_sm100_token_context* context) { delete context; }
+void nvcr_sm100_token_context_destroy(nvcr_sm100_token_context* context) {
+    if (context == nullptr) return;
+    // Waits for the calls that use the workspace, as freeing it would, then keeps it for the next context.
+    int current = 0;
+    const bool switched = cudaGetDevice(&current) == cudaSuccess && current != context->device &&
+        cudaSetDevice(context->device) == cudaSuccess;
+    cudaDeviceSynchronize();
+    if (switched) cudaSetDevice(current);
+    std::lock_guard<std::mutex> guard(spare_lock);
+    spares.emplace_back(context);
+}
 
 int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_token_cache* cache, int type,
                             const void* queries, int64_t query_stride, int64_t query_head_stride, int64_t tokens,
@@ -198,7 +259,7 @@ int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_
                                       {static_cast<token::Type>(type), queries, query_stride, query_head_stride, tokens,
                                        heads, page_table, table_stride, lengths, batch, query_offsets, max_queries,
                                        max_length, scale, output},
-                                      static_cast<cudaStream_t>(stream)));
+                                      context->workspace, static_cast<cudaStream_t>(stream)));
     });
 }
 

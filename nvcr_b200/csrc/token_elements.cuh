@@ -4,6 +4,8 @@
 
 #include "token_kernels.hpp"
 
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -48,5 +50,24 @@ __device__ __forceinline__ float warp_sum(float v) {
     for (int offset = 16; offset > 0; offset /= 2) v += __shfl_xor_sync(0xffffffffu, v, offset);
     return v;
 }
+
+// A kernel's dynamic shared memory above 48 KB, allowed once on each device.
+class SharedAllowance {
+public:
+    template <typename Kernel>
+    cudaError_t allow(Kernel* kernel, int bytes) {
+        int device = 0;
+        cudaError_t status = cudaGetDevice(&device);
+        if (status != cudaSuccess) return status;
+        const unsigned long long bit = 1ull << (device & 63);
+        if (device < 64 && (devices_.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+        status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (status == cudaSuccess) devices_.fetch_or(bit, std::memory_order_relaxed);
+        return status;
+    }
+
+private:
+    std::atomic<unsigned long long> devices_{0};
+};
 
 }  // namespace nvcr_sm100::token

@@ -16,6 +16,10 @@
 
 namespace nvcr_sm100::token {
 
+// Streaming multiprocessors of the current device (looked up once; a process
+// drives GPUs of one kind).
+int sm_count();
+
 enum class Type : int { f16 = 0, bf16 = 1, f32 = 2 };
 
 // Bits of a cache's status word: what a kernel found wrong in device data.
@@ -103,7 +107,14 @@ struct AttendArgs {
     float scale;
     void* output;  // [tokens][heads][head_dim]
 };
-cudaError_t attend(const Cache& cache, const AttendArgs& args, cudaStream_t stream);
+// Where ranges of one sequence's length are joined; tickets are zero between calls.
+struct AttendWorkspace {
+    float* partials;
+    unsigned* tickets;
+};
+std::size_t attend_partial_bytes();
+std::size_t attend_ticket_bytes();
+cudaError_t attend(const Cache& cache, const AttendArgs& args, const AttendWorkspace& workspace, cudaStream_t stream);
 
 struct MultiplyArgs {
     Type type;
