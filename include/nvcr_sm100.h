@@ -455,8 +455,8 @@ void nvcr_sm100_token_context_destroy(nvcr_sm100_token_context* context);
  * max_length; place t is on page page_table[b * table_stride + t / page_size],
  * and page_table has table_pages columns. A token sees the places up to its
  * own. Query head h reads cache head h / (heads / kv_heads). Scores are scaled
- * by `scale`; output [tokens][heads][head_dim] of `type` (F16 or BF16), zeros
- * for a token that sees nothing. FP32 softmax and sums. */
+ * by `scale`; output [tokens][heads][head_dim] of `type` (F16 or BF16), 16-byte
+ * aligned, zeros for a token that sees nothing. FP32 softmax and sums. */
 int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_token_cache* cache, int type,
                             const void* queries, int64_t query_stride, int64_t query_head_stride, int64_t tokens,
                             int32_t heads, const int32_t* page_table, int64_t table_stride, int32_t table_pages,

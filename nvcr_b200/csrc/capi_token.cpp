@@ -90,6 +90,9 @@ const char* cache_refusal(const nvcr_sm100_token_cache* cache) {
         cache->head_dim > 4 * cache->group) {
         return "cache group must be 32, 64 or 128, with 1, 2 or 4 groups a head";
     }
+    if (static_cast<std::int64_t>(cache->pages) * cache->kv_heads > most_rows / (cache->page_size / 16)) {
+        return "cache has 2^31 runs of 16 places or more";
+    }
     for (const void* buffer : {static_cast<const void*>(cache->key_codes), static_cast<const void*>(cache->key_scales),
                                static_cast<const void*>(cache->value_codes),
                                static_cast<const void*>(cache->value_scales)}) {
@@ -248,6 +251,7 @@ int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_
             (queries == nullptr || page_table == nullptr || lengths == nullptr || output == nullptr)) {
             return refuse("null queries, page_table, lengths or output");
         }
+        if (reinterpret_cast<std::uintptr_t>(output) % 16 != 0) return refuse("output must be 16-byte aligned");
         int device = 0;
         const cudaError_t status = cudaGetDevice(&device);
         if (status != cudaSuccess) return launched(status);
