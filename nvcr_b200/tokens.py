@@ -21,6 +21,7 @@ import torch
 from .executor import ErrorCode, ExecutorError, _check, _stream_handle, library
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_HALVES = (torch.float16, torch.bfloat16)
 _KINDS = {"rms": 0, "layer": 1}
 
 
@@ -40,34 +41,45 @@ def _require(condition: bool, message: str) -> None:
         _refuse(message)
 
 
-def _stream(stream, tensor: torch.Tensor) -> int | None:
+def _stream(stream, index: int) -> int | None:
     if stream is not None:
         return _stream_handle(stream)
-    _require(tensor.is_cuda, "tensors must be on a CUDA device")
-    return torch._C._cuda_getCurrentRawStream(tensor.device.index)
+    if index < 0:
+        _refuse("tensors must be on a CUDA device")
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _like(tensor: torch.Tensor | None, name: str, shape: tuple, first: torch.Tensor) -> int | None:
-    """The address of an optional contiguous tensor of a shape, of `first`'s type and device."""
+def _channels(tensor: torch.Tensor | None, name: str, width: int, first: torch.Tensor) -> int | None:
+    """The address of an optional contiguous vector of `width`, of `first`'s type and device."""
     if tensor is None:
         return None
-    if tensor.dtype is not first.dtype or tensor.device != first.device or tensor.shape != shape \
+    if tensor.dtype is not first.dtype or tensor.shape != (width,) or tensor.get_device() != first.get_device() \
             or not tensor.is_contiguous():
-        _refuse(f"{name} must be a contiguous {first.dtype} tensor of shape {tuple(shape)} on {first.device}")
+        _refuse(f"{name} must be a contiguous {first.dtype} tensor of shape {(width,)} on {first.device}")
     return tensor.data_ptr()
 
 
-def _whole(tensor: torch.Tensor, name: str, kind: torch.dtype, shape: tuple, device: torch.device) -> int:
-    if tensor.dtype is not kind or tensor.device != device or tensor.shape != shape or not tensor.is_contiguous():
-        _refuse(f"{name} must be a contiguous {kind} tensor of shape {tuple(shape)} on {device}")
+def _rows(tensor: torch.Tensor, name: str, first: torch.Tensor) -> int:
+    """The address of a [rows, width] tensor like `first` (its row stride is free)."""
+    if tensor.dtype is not first.dtype or tensor.shape != first.shape or tensor.get_device() != first.get_device() \
+            or (tensor.stride(1) != 1 and tensor.shape[1] > 1):
+        _refuse(f"{name} must be a {first.dtype} tensor of shape {tuple(first.shape)} on {first.device} "
+                "with contiguous rows")
     return tensor.data_ptr()
 
 
-def _heads(tensor: torch.Tensor, name: str, tokens: int, heads: int, dim: int, first: torch.Tensor) -> int:
+def _whole(tensor: torch.Tensor, name: str, kind: torch.dtype, shape: tuple, index: int) -> int:
+    """The address of a contiguous tensor of a type and shape on CUDA device `index`."""
+    if tensor.dtype is not kind or tensor.shape != shape or tensor.get_device() != index or not tensor.is_contiguous():
+        _refuse(f"{name} must be a contiguous {kind} tensor of shape {tuple(shape)} on cuda:{index}")
+    return tensor.data_ptr()
+
+
+def _heads(tensor: torch.Tensor, name: str, shape: tuple, first: torch.Tensor) -> int:
     """The address of a [tokens, heads, dim] tensor whose channels are contiguous (its other strides are free)."""
-    if tensor.dtype is not first.dtype or tensor.device != first.device or tensor.shape != (tokens, heads, dim) \
+    if tensor.dtype is not first.dtype or tensor.shape != shape or tensor.get_device() != first.get_device() \
             or (tensor.stride(2) != 1 and tensor.numel() > 0):
-        _refuse(f"{name} must be a {first.dtype} tensor of shape {(tokens, heads, dim)} on {first.device} "
+        _refuse(f"{name} must be a {first.dtype} tensor of shape {tuple(shape)} on {first.device} "
                 "with contiguous channels")
     return tensor.data_ptr()
 
@@ -83,32 +95,31 @@ def block_norm(block: torch.Tensor, *, residual: torch.Tensor | None = None, gat
     normed = N(hidden; pre_weight, pre_bias). N is the root-mean-square norm ("rms") or the layer norm ("layer"),
     with weights taken as weight + weight_offset. `gate` is [width] or [rows, width]. block, residual and a gate of
     rows may have any row stride. ``hidden=False`` or ``normed=False`` leaves that output out (None)."""
-    _require(block.dim() == 2 and block.dtype in _TYPES, "block must be a [rows, width] tensor of a float type")
-    _require(kind in _KINDS, f"kind must be one of {sorted(_KINDS)}")
-    _require(hidden or normed, "neither hidden nor normed is wanted")
+    code, layer = _TYPES.get(block.dtype), _KINDS.get(kind)
+    if code is None or block.dim() != 2:
+        _refuse("block must be a [rows, width] tensor of a float type")
+    if layer is None:
+        _refuse(f"kind must be one of {sorted(_KINDS)}")
+    if not (hidden or normed):
+        _refuse("neither hidden nor normed is wanted")
     rows, width = block.shape
-    strides = [0, 0, 0]
-    for i, (name, tensor) in enumerate((("block", block), ("residual", residual), ("gate", gate))):
-        if tensor is None or (i == 2 and tensor.dim() == 1):
-            continue
-        if tensor.shape != block.shape or tensor.dtype is not block.dtype or tensor.device != block.device \
-                or (tensor.stride(1) != 1 and width > 1):
-            _refuse(f"{name} must be a {block.dtype} tensor of shape {(rows, width)} on {block.device} "
-                    "with contiguous rows")
-        strides[i] = tensor.stride(0)
-    channel = (width,)
-    gate_address = None
+    block_address, residual_address, gate_address = _rows(block, "block", block), None, None
+    residual_stride = gate_stride = 0
+    if residual is not None:
+        residual_address, residual_stride = _rows(residual, "residual", block), residual.stride(0)
     if gate is not None:
-        gate_address = gate.data_ptr() if gate.dim() == 2 else _like(gate, "gate", channel, block)
-    handle = _stream(stream, block)
-    sums = torch.empty((rows, width), dtype=block.dtype, device=block.device) if hidden else None
-    out = torch.empty((rows, width), dtype=block.dtype, device=block.device) if normed else None
+        if gate.dim() == 1:
+            gate_address = _channels(gate, "gate", width, block)
+        else:
+            gate_address, gate_stride = _rows(gate, "gate", block), gate.stride(0)
+    weights = (_channels(post_weight, "post_weight", width, block), _channels(post_bias, "post_bias", width, block),
+               _channels(pre_weight, "pre_weight", width, block), _channels(pre_bias, "pre_bias", width, block))
+    handle = _stream(stream, block.get_device())
+    sums = torch.empty_like(block, memory_format=torch.contiguous_format) if hidden else None
+    out = torch.empty_like(block, memory_format=torch.contiguous_format) if normed else None
     status = library().nvcr_sm100_token_norm(
-        _TYPES[block.dtype], _KINDS[kind], int(post), block.data_ptr(), strides[0],
-        None if residual is None else residual.data_ptr(), strides[1], gate_address, strides[2],
-        _like(post_weight, "post_weight", channel, block), _like(post_bias, "post_bias", channel, block),
-        _like(pre_weight, "pre_weight", channel, block), _like(pre_bias, "pre_bias", channel, block),
-        None if sums is None else sums.data_ptr(), None if out is None else out.data_ptr(), rows, width,
+        code, layer, post, block_address, block.stride(0), residual_address, residual_stride, gate_address, gate_stride,
+        *weights, None if sums is None else sums.data_ptr(), None if out is None else out.data_ptr(), rows, width,
         residual_scale, weight_offset, epsilon, handle)
     if status:
         _check(status)
@@ -128,18 +139,18 @@ class PagedCache:
         pages, kv_heads, page_size, half = key_codes.shape
         groups = key_scales.shape[3]
         _require(groups > 0 and (2 * half) % groups == 0, "scales hold a whole number of groups")
-        device = key_codes.device
+        device, index = key_codes.device, key_codes.get_device()
         code_shape, scale_shape = (pages, kv_heads, page_size, half), (pages, kv_heads, page_size, groups, 2)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self.tensors = (key_codes, key_scales, value_codes, value_scales)
-        self._struct = _Cache(_whole(key_codes, "key_codes", torch.uint8, code_shape, device),
-                              _whole(key_scales, "key_scales", torch.float16, scale_shape, device),
-                              _whole(value_codes, "value_codes", torch.uint8, code_shape, device),
-                              _whole(value_scales, "value_scales", torch.float16, scale_shape, device),
+        self._struct = _Cache(_whole(key_codes, "key_codes", torch.uint8, code_shape, index),
+                              _whole(key_scales, "key_scales", torch.float16, scale_shape, index),
+                              _whole(value_codes, "value_codes", torch.uint8, code_shape, index),
+                              _whole(value_scales, "value_scales", torch.float16, scale_shape, index),
                               self.status.data_ptr(), pages, kv_heads, page_size, 2 * half, 2 * half // groups)
         self._address = ctypes.addressof(self._struct)
         self.device, self.pages, self.kv_heads, self.page_size = device, pages, kv_heads, page_size
-        self.head_dim, self.group = 2 * half, 2 * half // groups
+        self.head_dim, self.group, self._index = 2 * half, 2 * half // groups, index
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, group: int = 64,
@@ -160,31 +171,36 @@ class PagedCache:
         stored; else distinct). With int32 `positions`, keys are rotated before they are stored, and `queries`
         [tokens, heads, head_dim] into the tensor that is returned, by rows of the float32 tables `cosines` and
         `sines` [rows, rotary / 2]: pairs (i, i + rotary / 2), or (2 i, 2 i + 1) if `interleaved`."""
-        _require(keys.dim() == 3 and keys.dtype in (torch.float16, torch.bfloat16) and keys.device == self.device,
-                 "keys must be a float16 or bfloat16 tensor of three dimensions on the cache's device")
+        index = self._index
+        if keys.dim() != 3 or keys.dtype not in _HALVES or keys.get_device() != index:
+            _refuse("keys must be a float16 or bfloat16 tensor of three dimensions on the cache's device")
         tokens = keys.shape[0]
-        key_address = _heads(keys, "keys", tokens, self.kv_heads, self.head_dim, keys)
-        value_address = _heads(values, "values", tokens, self.kv_heads, self.head_dim, keys)
-        slot_address = _whole(slots, "slots", torch.int64, (tokens,), self.device)
-        rotated = query_address = position_address = cosine_address = sine_address = None
+        shape = (tokens, self.kv_heads, self.head_dim)
+        key_address, value_address = _heads(keys, "keys", shape, keys), _heads(values, "values", shape, keys)
+        slot_address = _whole(slots, "slots", torch.int64, (tokens,), index)
+        rotated = query_address = rotated_address = position_address = cosine_address = sine_address = None
         query_heads = query_stride = query_head_stride = table_rows = rotary = 0
         if queries is not None:
-            _require(queries.dim() == 3, "queries have three dimensions")
+            if queries.dim() != 3:
+                _refuse("queries have three dimensions")
             query_heads = queries.shape[1]
-            query_address = _heads(queries, "queries", tokens, query_heads, self.head_dim, keys)
+            query_address = _heads(queries, "queries", (tokens, query_heads, self.head_dim), keys)
             query_stride, query_head_stride = queries.stride(0), queries.stride(1)
-            rotated = torch.empty((tokens, query_heads, self.head_dim), dtype=keys.dtype, device=self.device)
+            rotated = torch.empty_like(queries, memory_format=torch.contiguous_format)
+            rotated_address = rotated.data_ptr()
         if positions is not None:
-            _require(cosines is not None and sines is not None and cosines.dim() == 2, "positions need rotation tables")
-            position_address = _whole(positions, "positions", torch.int32, (tokens,), self.device)
-            table_rows, rotary = cosines.shape[0], 2 * cosines.shape[1]
-            cosine_address = _whole(cosines, "cosines", torch.float32, (table_rows, rotary // 2), self.device)
-            sine_address = _whole(sines, "sines", torch.float32, (table_rows, rotary // 2), self.device)
+            if cosines is None or sines is None or cosines.dim() != 2:
+                _refuse("positions need rotation tables")
+            position_address = _whole(positions, "positions", torch.int32, (tokens,), index)
+            table_rows, half = table = cosines.shape
+            rotary = 2 * half
+            cosine_address = _whole(cosines, "cosines", torch.float32, table, index)
+            sine_address = _whole(sines, "sines", torch.float32, table, index)
         status = library().nvcr_sm100_token_append(
             self._address, _TYPES[keys.dtype], key_address, keys.stride(0), keys.stride(1), value_address,
             values.stride(0), values.stride(1), slot_address, tokens, query_address, query_stride, query_head_stride,
-            query_heads, None if rotated is None else rotated.data_ptr(), position_address, cosine_address,
-            sine_address, table_rows, rotary, int(interleaved), _stream(stream, keys))
+            query_heads, rotated_address, position_address, cosine_address, sine_address, table_rows, rotary,
+            interleaved, _stream(stream, index))
         if status:
             _check(status)
         return rotated
@@ -192,13 +208,15 @@ class PagedCache:
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16,
              stream=None) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values [n, kv_heads, head_dim] that the codes at int64 `slots` stand for (zeros outside)."""
-        _require(slots.dim() == 1 and dtype in _TYPES, "slots have one dimension and dtype is a float type")
+        code = _TYPES.get(dtype)
+        if slots.dim() != 1 or code is None:
+            _refuse("slots have one dimension and dtype is a float type")
         count = slots.shape[0]
-        slot_address = _whole(slots, "slots", torch.int64, (count,), self.device)
+        slot_address = _whole(slots, "slots", torch.int64, (count,), self._index)
         keys = torch.empty((count, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
-        values = torch.empty((count, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
-        status = library().nvcr_sm100_token_read(self._address, _TYPES[dtype], slot_address, count, keys.data_ptr(),
-                                                 values.data_ptr(), _stream(stream, slots))
+        values = torch.empty_like(keys)
+        status = library().nvcr_sm100_token_read(self._address, code, slot_address, count, keys.data_ptr(),
+                                                 values.data_ptr(), _stream(stream, self._index))
         if status:
             _check(status)
         return keys, values
@@ -247,24 +265,26 @@ class TokenContext:
         of the int32 `page_table`; its new tokens are query_offsets[b] .. query_offsets[b + 1] - 1 (int32 [batch + 1],
         at most `max_queries` each; None: token b). A token sees the places up to its own; one that sees none gives
         zeros. `scale` defaults to 1 / sqrt(head_dim)."""
-        _require(queries.dim() == 3 and queries.dtype in (torch.float16, torch.bfloat16)
-                 and queries.device == cache.device,
-                 "queries must be a float16 or bfloat16 tensor of three dimensions on the cache's device")
+        index = cache._index
+        if queries.dim() != 3 or queries.dtype not in _HALVES or queries.get_device() != index:
+            _refuse("queries must be a float16 or bfloat16 tensor of three dimensions on the cache's device")
         tokens, heads, dim = queries.shape
-        query_address = _heads(queries, "queries", tokens, heads, cache.head_dim, queries)
-        _require(lengths.dim() == 1 and page_table.dim() == 2, "lengths have one dimension and page_table two")
-        batch, columns = lengths.shape[0], page_table.shape[1]
-        if page_table.dtype is not torch.int32 or page_table.device != cache.device or page_table.shape[0] != batch \
+        query_address = _heads(queries, "queries", (tokens, heads, cache.head_dim), queries)
+        if lengths.dim() != 1 or page_table.dim() != 2:
+            _refuse("lengths have one dimension and page_table two")
+        batch, columns = page_table.shape
+        if page_table.dtype is not torch.int32 or page_table.get_device() != index or lengths.shape[0] != batch \
                 or (page_table.stride(1) != 1 and columns > 1):
-            _refuse(f"page_table must be an int32 tensor of {batch} rows on {cache.device} with contiguous rows")
-        length_address = _whole(lengths, "lengths", torch.int32, (batch,), cache.device)
+            _refuse(f"page_table must be an int32 tensor of {lengths.shape[0]} rows on {cache.device} "
+                    "with contiguous rows")
+        length_address = _whole(lengths, "lengths", torch.int32, (batch,), index)
         offset_address = None if query_offsets is None else _whole(query_offsets, "query_offsets", torch.int32,
-                                                                   (batch + 1,), cache.device)
-        out = torch.empty((tokens, heads, dim), dtype=queries.dtype, device=queries.device)
+                                                                   (batch + 1,), index)
+        out = torch.empty_like(queries, memory_format=torch.contiguous_format)
         status = library().nvcr_sm100_token_attend(
             self._handle, cache._address, _TYPES[queries.dtype], query_address, queries.stride(0), queries.stride(1),
             tokens, heads, page_table.data_ptr(), page_table.stride(0), columns, length_address, batch, offset_address,
-            max_queries, max_length, dim ** -0.5 if scale is None else scale, out.data_ptr(), _stream(stream, queries))
+            max_queries, max_length, dim ** -0.5 if scale is None else scale, out.data_ptr(), _stream(stream, index))
         if status:
             _check(status)
         return out
@@ -279,19 +299,19 @@ class PackedMatrix:
         _require(codes.is_cuda, "weights are on a CUDA device")
         outputs, inputs, groups = codes.shape[0], 2 * codes.shape[1], scales.shape[1]
         _require(groups > 0 and inputs % groups == 0, "scales hold a whole number of groups")
-        device, group = codes.device, inputs // groups
-        addresses = (_whole(codes, "codes", torch.uint8, (outputs, inputs // 2), device),
-                     _whole(scales, "scales", torch.float16, (outputs, groups), device),
-                     _whole(minimums, "minimums", torch.float16, (outputs, groups), device))
+        device, index, group = codes.device, codes.get_device(), inputs // groups
+        addresses = (_whole(codes, "codes", torch.uint8, (outputs, inputs // 2), index),
+                     _whole(scales, "scales", torch.float16, (outputs, groups), index),
+                     _whole(minimums, "minimums", torch.float16, (outputs, groups), index))
         code_bytes, scale_bytes = ctypes.c_size_t(0), ctypes.c_size_t(0)
         _check(library().nvcr_sm100_token_packed_bytes(outputs, inputs, group, ctypes.byref(code_bytes),
                                                        ctypes.byref(scale_bytes)))
-        self.outputs, self.inputs, self.group, self.device = outputs, inputs, group, device
+        self.outputs, self.inputs, self.group, self.device, self._index = outputs, inputs, group, device, index
         self.codes = torch.empty(code_bytes.value, dtype=torch.uint8, device=device)
         self.scales = torch.empty(scale_bytes.value, dtype=torch.uint8, device=device)
         self._addresses = (self.codes.data_ptr(), self.scales.data_ptr())
         _check(library().nvcr_sm100_token_pack(*addresses, outputs, inputs, group, *self._addresses,
-                                               _stream(stream, codes)))
+                                               _stream(stream, index)))
 
     @classmethod
     def quantise(cls, weights: torch.Tensor, group: int = 64, stream=None) -> "PackedMatrix":
@@ -308,15 +328,15 @@ class PackedMatrix:
 
     def multiply(self, x: torch.Tensor, bias: torch.Tensor | None = None, stream=None) -> torch.Tensor:
         """x [rows, inputs] (float16 or bfloat16, any row stride) times the matrix's transpose, plus bias [outputs]."""
-        if x.dim() != 2 or x.shape[1] != self.inputs or x.dtype not in (torch.float16, torch.bfloat16) \
-                or x.device != self.device or x.stride(1) != 1:
+        if x.dim() != 2 or x.shape[1] != self.inputs or x.dtype not in _HALVES or x.get_device() != self._index \
+                or x.stride(1) != 1:
             _refuse(f"x must be a float16 or bfloat16 tensor of shape (rows, {self.inputs}) on {self.device} "
                     "with contiguous rows")
         rows = x.shape[0]
-        y = torch.empty((rows, self.outputs), dtype=x.dtype, device=x.device)
+        y = x.new_empty((rows, self.outputs))
         status = library().nvcr_sm100_token_multiply(
             _TYPES[x.dtype], x.data_ptr(), x.stride(0), rows, *self._addresses, self.outputs, self.inputs, self.group,
-            _like(bias, "bias", (self.outputs,), x), y.data_ptr(), _stream(stream, x))
+            _channels(bias, "bias", self.outputs, x), y.data_ptr(), _stream(stream, self._index))
         if status:
             _check(status)
         return y

@@ -239,6 +239,21 @@ APPENDS = [  # dim, group, kv_heads, heads, page, tokens, rotary, interleaved, t
 
 @pytest.mark.parametrize("dim,group,kv_heads,heads,page,tokens,rotary,interleaved,name", APPENDS)
 def test_append_and_read(cuda, dim, group, kv_heads, heads, page, tokens, rotary, interleaved, name):
+    check_append(dim, group, kv_heads, heads, page, tokens, rotary, interleaved, name, 1)
+
+
+@pytest.mark.parametrize("dim,group,kv_heads,heads,page,tokens,rotary,interleaved,name", APPENDS + [
+    (128, 64, 8, 32, 16, 2000, 128, False, "bfloat16"),
+    (128, 32, 4, 20, 64, 700, 32, False, "float16"),
+    (256, 64, 2, 2, 16, 65, 16, False, "bfloat16"),
+    (64, 32, 2, 8, 32, 500, 8, True, "float16"),
+    (256, 128, 1, 3, 16, 9, 128, True, "bfloat16"),
+])
+def test_append_and_read_aligned(cuda, dim, group, kv_heads, heads, page, tokens, rotary, interleaved, name):
+    check_append(dim, group, kv_heads, heads, page, tokens, rotary, interleaved, name, 0)
+
+
+def check_append(dim, group, kv_heads, heads, page, tokens, rotary, interleaved, name, pad):
     import torch
 
     from nvcr_b200.tokens import PagedCache
@@ -249,7 +264,7 @@ def test_append_and_read(cuda, dim, group, kv_heads, heads, page, tokens, rotary
     for i, t in enumerate(cache.tensors):
         t.view(torch.uint8).fill_(17 + i)
     before = [t.clone() for t in cache.tensors]
-    rows = normal((tokens, heads + 2 * kv_heads, dim + 1), 3, 1.5, 0.3).to(kind)[:, :, 1:]  # odd strides and start
+    rows = normal((tokens, heads + 2 * kv_heads, dim + pad), 3, 1.5, 0.3).to(kind)[:, :, pad:]  # 1: odd strides and start
     queries, keys, values = rows.split([heads, kv_heads, kv_heads], 1)
     make = torch.Generator(device="cuda").manual_seed(4)
     slots = torch.randperm(pages * page, generator=make, device="cuda")[:tokens]
