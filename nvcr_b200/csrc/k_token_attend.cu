@@ -102,14 +102,6 @@ __device__ __forceinline__ float2 pair_at(const std::uint8_t* scales, int byte) 
     return __half22float2(*reinterpret_cast<const __half2*>(scales + byte));
 }
 
-// n / d for n < 2^31 as (umulhi(n, multiplier) + n) >> shift (Granlund and
-// Montgomery's division by an invariant).
-struct Divisor {
-    unsigned multiplier, shift;
-};
-
-__device__ __forceinline__ unsigned divide(unsigned n, Divisor d) { return (__umulhi(n, d.multiplier) + n) >> d.shift; }
-
 struct Work {
     Cache cache;
     AttendArgs a;
@@ -834,13 +826,6 @@ cudaError_t launch_shape(Work& work, cudaStream_t stream) {
                        : launch_rows<T, 128, 128>(work, stream);
     }
     return g == 64 ? launch_rows<T, 256, 64>(work, stream) : launch_rows<T, 256, 128>(work, stream);
-}
-
-Divisor divisor(unsigned d) {
-    Divisor made{0, 0};
-    while ((1u << made.shift) < d) ++made.shift;
-    made.multiplier = static_cast<unsigned>((((1ull << made.shift) - d) << 32) / d + 1);
-    return made;
 }
 
 }  // namespace

@@ -24,20 +24,46 @@ __device__ __forceinline__ void note(const Cache& cache, unsigned bit) {
 // A group's scale and minimum, and the codes of its values.
 struct GroupForm {
     __half scale, minimum;
-    float s, m;
+    float s, m, inverse;
     __device__ __forceinline__ GroupForm(float low, float high) {
         minimum = __float2half_rn(low);
         scale = __float2half_rn((high - low) * (1.0f / 15.0f));
         if (high > low && __half2float(scale) == 0.0f) scale = __ushort_as_half(1);
         m = __half2float(minimum), s = __half2float(scale);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(s));
+        if (s == 0.0f) inverse = 0.0f;
     }
-    __device__ __forceinline__ unsigned code(float x) const {
-        const float level = s > 0.0f ? rintf(__fdiv_rn(x - m, s)) : 0.0f;
-        return static_cast<unsigned>(fminf(fmaxf(level, 0.0f), 15.0f));  // fmaxf takes a NaN to 0
+    // The codes of N values, packed, on the FP32 and integer pipes alone (conversions run at a quarter of their rate):
+    // adding 1.5 * 2^23 rounds to the nearest integer, ties to even, in the low bits. A product with the reciprocal is
+    // within 2^-18 of the quotient (which is below 16, or clamped), so only where one is that close to a tie are the
+    // values divided.
+    template <int N>
+    __device__ __forceinline__ unsigned codes(const float (&x)[N]) const {
+        unsigned packed = 0, offset = 0;
+        bool tie = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float level = clamped((x[i] - m) * inverse), sum = level + 12582912.0f;
+            tie |= fabsf(level - (sum - 12582912.0f)) > 0.49999f;
+            packed += __float_as_uint(sum) << (4 * i);
+            offset += 0x4b400000u << (4 * i);
+        }
+        if (tie) {
+            packed = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float level = s > 0.0f ? clamped(__fdiv_rn(x[i] - m, s)) : 0.0f;
+                packed += __float_as_uint(level + 12582912.0f) << (4 * i);
+            }
+        }
+        return packed - offset;
     }
     __device__ __forceinline__ unsigned bits() const {
         return __half_as_ushort(scale) | static_cast<unsigned>(__half_as_ushort(minimum)) << 16;
     }
+
+private:
+    static __device__ __forceinline__ float clamped(float v) { return fminf(fmaxf(v, 0.0f), 15.0f); }  // a NaN is 0
 };
 
 // Any strides, alignment and rotation: one warp a (token, head) of keys, values
@@ -102,21 +128,21 @@ __global__ void append_kernel(Cache cache, AppendArgs a) {
         high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, offset));
     }
     const GroupForm form(low, high);
+    const unsigned packed = form.codes(x);
     const std::int64_t page = slot / cache.page_size;
     const std::int64_t place = (page * cache.kv_heads + head) * cache.page_size + slot % cache.page_size;
     std::uint8_t* codes = (is_key ? cache.key_codes : cache.value_codes) + place * (D / 2) + lane * (per_lane / 2);
 #pragma unroll
-    for (int i = 0; i < per_lane / 2; ++i) codes[i] = static_cast<std::uint8_t>(form.code(x[2 * i]) | form.code(x[2 * i + 1]) << 4);
+    for (int i = 0; i < per_lane / 2; ++i) codes[i] = static_cast<std::uint8_t>(packed >> (8 * i));
     if (lane % lanes == 0) {
         reinterpret_cast<unsigned*>(is_key ? cache.key_scales : cache.value_scales)[place * (D / cache.group) + lane / lanes] =
             form.bits();
     }
 }
 
-// Eight elements of a 16-bit type in one access.
+// Eight elements of a 16-bit type from one 16-byte access, and eight of any type to memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T* from, float (&x)[8]) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(from);
+__device__ __forceinline__ void unpack8(const uint4& raw, float (&x)[8]) {
     const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -150,98 +176,121 @@ __device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
     }
 }
 
-// Eight channels a thread, D / 8 threads a (token, run of `heads_each` heads): a
-// thread reads its angles' cosines and sines once and its heads in 16-byte
-// accesses; a key's or query's rotation partner, eight channels elsewhere in the
-// head, is a second load of a line that is in L1. Takes aligned tensors and
-// rotations of whole octets (pairs (i, i + rotary / 2): rotary a multiple of 16;
-// (2 i, 2 i + 1): of 8).
-template <typename T, int D>
-__global__ void __launch_bounds__(256) append_octets_kernel(Cache cache, AppendArgs a, int heads_each) {
+// Eight channels a thread, D / 8 threads a (token, run of H heads of queries,
+// keys or values): a thread reads its angles' cosines and sines once, loads all
+// its heads in 16-byte accesses before it uses any (HBM-bound: that keeps enough
+// bytes in flight), and a key's or query's rotation partner, eight channels
+// elsewhere in the head, as a second load of a line that is in L1. Takes aligned
+// tensors and rotations of whole octets (pairs (i, i + rotary / 2): rotary a
+// multiple of 16; (2 i, 2 i + 1): of 8).
+template <typename T, int D, int H>
+__global__ void __launch_bounds__(256, 4) append_octets_kernel(Cache cache, AppendArgs a, Divisor runs_per_page) {
     constexpr int lanes = D / 8;
     const int lane = threadIdx.x % lanes, channel = 8 * lane;
-    const std::int64_t token = static_cast<std::int64_t>(blockIdx.x) * (blockDim.x / lanes) + threadIdx.x / lanes;
+    const std::int64_t token = static_cast<std::int64_t>(blockIdx.x) * (256 / lanes) + threadIdx.x / lanes;
     const bool valid = token < a.tokens;  // threads past the end stay for the shuffles
-    const int query_heads = a.queries != nullptr ? a.query_heads : 0;
-    const int all = query_heads + 2 * cache.kv_heads;
-    const int first = blockIdx.y * heads_each, last = min(all, first + heads_each);
-    const std::int64_t slot = valid ? a.slots[token] : -1;
-    bool placed = true;
-    float cosine[8], sine[8];
+    const int query_runs = a.queries != nullptr ? (a.query_heads + H - 1) / H : 0;
+    const int kv_runs = (cache.kv_heads + H - 1) / H;
+    int run = blockIdx.y;
+    const bool is_query = run < query_runs, is_key = !is_query && run < query_runs + kv_runs;
+    run -= is_query ? 0 : is_key ? query_runs : query_runs + kv_runs;
+    const int first = run * H, last = min(is_query ? a.query_heads : cache.kv_heads, first + H);
+    const std::int64_t head_stride = is_query ? a.query_head_stride : is_key ? a.key_head_stride : a.value_head_stride;
+    const T* const source =
+        (is_query  ? static_cast<const T*>(a.queries) + token * a.query_stride
+             : is_key ? static_cast<const T*>(a.keys) + token * a.key_stride
+                      : static_cast<const T*>(a.values) + token * a.value_stride) +
+        first * head_stride + channel;
     const int half = a.rotary / 2;
-    bool turned = false;
-    if (a.positions != nullptr && valid) {
-        const std::int64_t position = a.positions[token];
-        placed = position >= 0 && position < a.table_rows;
-        if (!placed && lane == 0) note(cache, status_position);
-        turned = placed && channel < a.rotary;
-        if (turned) {
-            const float* cosines = a.cosines + position * half;
-            const float* sines = a.sines + position * half;
-            if (a.interleaved) {
+    const bool second = !a.interleaved && channel >= half;
+    const bool turns = a.positions != nullptr && (is_query || is_key) && channel < a.rotary;
+    const bool partners = turns && !a.interleaved;
+    uint4 raw[H], partner[H];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) cosine[i] = cosines[channel / 2 + i / 2], sine[i] = sines[channel / 2 + i / 2];
-            } else {
-                const int angle = channel < half ? channel : channel - half;
+    for (int h = 0; h < H; ++h) {
+        raw[h] = partner[h] = {0u, 0u, 0u, 0u};
+        if (valid && first + h < last) {
+            raw[h] = *reinterpret_cast<const uint4*>(source + h * head_stride);
+            if (partners) partner[h] = *reinterpret_cast<const uint4*>(source + h * head_stride + (second ? -half : half));
+        }
+    }
+    std::int64_t slot = -1, position = 0;
+    if (valid && !is_query) slot = a.slots[token];
+    if (valid && a.positions != nullptr) position = a.positions[token];
+    const bool placed = a.positions == nullptr || (position >= 0 && position < a.table_rows);
+    if (!placed && lane == 0) note(cache, status_position);
+    // x cos - partner sin for a pair's first element, x cos + partner sin for its second: the sign goes to the sine
+    float cosine[8], sine[8];
+    if (turns && placed && valid) {
+        const float4* cosines = reinterpret_cast<const float4*>(a.cosines + position * half);
+        const float4* sines = reinterpret_cast<const float4*>(a.sines + position * half);
+        if (a.interleaved) {
+            const float4 c = cosines[lane], s = sines[lane];
+            cosine[0] = cosine[1] = c.x, cosine[2] = cosine[3] = c.y, cosine[4] = cosine[5] = c.z, cosine[6] = cosine[7] = c.w;
+            sine[1] = s.x, sine[3] = s.y, sine[5] = s.z, sine[7] = s.w;
+            sine[0] = -s.x, sine[2] = -s.y, sine[4] = -s.z, sine[6] = -s.w;
+        } else {
+            const int at = (second ? channel - half : channel) / 4;
+            const float sign = second ? 1.0f : -1.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) cosine[i] = cosines[angle + i], sine[i] = sines[angle + i];
+            for (int i = 0; i < 2; ++i) {
+                const float4 c = cosines[at + i], s = sines[at + i];
+                cosine[4 * i] = c.x, cosine[4 * i + 1] = c.y, cosine[4 * i + 2] = c.z, cosine[4 * i + 3] = c.w;
+                sine[4 * i] = sign * s.x, sine[4 * i + 1] = sign * s.y;
+                sine[4 * i + 2] = sign * s.z, sine[4 * i + 3] = sign * s.w;
             }
         }
     }
-    const bool second = !a.interleaved && channel >= half;
-    const int partner = second ? -half : half;
+    T* const rotated = static_cast<T*>(a.rotated) + (token * a.query_heads + first) * D + channel;
     const std::int64_t limit = static_cast<std::int64_t>(cache.pages) * cache.page_size;
-    const bool stored = valid && placed && slot >= 0 && slot < limit;
-    if (valid && slot >= limit && lane == 0) note(cache, status_slot);
-    const std::int64_t page = stored ? slot / cache.page_size : 0;
-    const std::int64_t place = page * cache.kv_heads * cache.page_size + (stored ? slot - page * cache.page_size : 0);
-#pragma unroll 2
-    for (int h = first; h < last; ++h) {
-        const bool is_query = h < query_heads, is_key = !is_query && h < query_heads + cache.kv_heads;
-        const int head = is_query ? h : is_key ? h - query_heads : h - query_heads - cache.kv_heads;
-        if (is_query && !valid) continue;
-        float x[8] = {}, other[8] = {};
-        if (valid) {
-            const T* source = is_query ? static_cast<const T*>(a.queries) + token * a.query_stride + head * a.query_head_stride
-                : is_key ? static_cast<const T*>(a.keys) + token * a.key_stride + head * a.key_head_stride
-                         : static_cast<const T*>(a.values) + token * a.value_stride + head * a.value_head_stride;
-            load8(source + channel, x);
-            if (turned && (is_query || is_key)) {
-                if (a.interleaved) {
+    const bool stored = placed && slot >= 0 && slot < limit;
+    if (slot >= limit && lane == 0) note(cache, status_slot);
+    std::int64_t place = 0;
+    if (stored) {  // slots are below 2^35, their runs of 16 below 2^31
+        const std::int64_t page = divide(static_cast<unsigned>(slot >> 4), runs_per_page);
+        place = (page * cache.kv_heads + first) * cache.page_size + (slot - page * cache.page_size);
+    }
+    const int group_lanes = cache.group / 8;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) other[i] = x[i ^ 1];
-                } else {
-                    load8(source + channel + partner, other);
-                }
+    for (int h = 0; h < H; ++h) {
+        if (first + h >= last) break;
+        float x[8];
+        unpack8<T>(raw[h], x);
+        if (turns && placed) {
+            float turned[8];
+            if (a.interleaved) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float one = __fmul_rn(x[i], cosine[i]), two = __fmul_rn(other[i], sine[i]);
-                    x[i] = (a.interleaved ? i % 2 == 1 : second) ? __fadd_rn(one, two) : __fsub_rn(one, two);
-                }
+                for (int i = 0; i < 8; ++i) turned[i] = __fadd_rn(__fmul_rn(x[i], cosine[i]), __fmul_rn(x[i ^ 1], sine[i]));
+            } else {
+                float other[8];
+                unpack8<T>(partner[h], other);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) turned[i] = __fadd_rn(__fmul_rn(x[i], cosine[i]), __fmul_rn(other[i], sine[i]));
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = turned[i];
         }
         if (is_query) {
             if (!placed) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = NAN;
             }
-            store8(static_cast<T*>(a.rotated) + (token * a.query_heads + head) * D + channel, x);
+            if (valid) store8(rotated + h * D, x);
             continue;
         }
         float low = x[0], high = x[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) low = min_nan(low, x[i]), high = max_nan(high, x[i]);
-        const int group_lanes = cache.group / 8;
-        for (int offset = 1; offset < group_lanes; offset *= 2) {
+#pragma unroll
+        for (int offset = 1; offset < 16; offset *= 2) {
+            if (offset >= group_lanes) break;
             low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, offset));
             high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, offset));
         }
         if (!stored) continue;
         const GroupForm form(low, high);
-        unsigned codes = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) codes |= form.code(x[i]) << (4 * i);
-        const std::int64_t at = place + static_cast<std::int64_t>(head) * cache.page_size;
+        const unsigned codes = form.codes(x);
+        const std::int64_t at = place + h * cache.page_size;
         reinterpret_cast<unsigned*>(is_key ? cache.key_codes : cache.value_codes)[at * lanes + lane] = codes;
         if (lane % group_lanes == 0) {
             reinterpret_cast<unsigned*>(is_key ? cache.key_scales : cache.value_scales)[at * (lanes / group_lanes) +
@@ -250,39 +299,46 @@ __global__ void __launch_bounds__(256) append_octets_kernel(Cache cache, AppendA
     }
 }
 
-// Eight channels a thread of one stored token's keys, then of its values.
+// Eight channels a thread of one stored token's keys and values.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) read_kernel(Cache cache, const std::int64_t* slots, std::int64_t count, T* keys,
-                                                   T* values) {
+                                                   T* values, Divisor by_heads, Divisor runs_per_page) {
     constexpr int lanes = D / 8;
-    const std::int64_t per_kind = count * cache.kv_heads * lanes;
     const std::int64_t i = static_cast<std::int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const bool is_value = blockIdx.y == 1;
-    if (i >= per_kind) return;
+    if (i >= count * cache.kv_heads * lanes) return;
     const int lane = static_cast<int>(i % lanes);
-    const unsigned head_token = static_cast<unsigned>(i / lanes);  // count times heads is below 2^32
-    const unsigned token = head_token / cache.kv_heads, head = head_token - token * cache.kv_heads;
-    T* out = (is_value ? values : keys) + i * 8;
+    const unsigned head_token = static_cast<unsigned>(i / lanes);  // count times heads is below 2^31
+    const unsigned token = divide(head_token, by_heads), head = head_token - token * cache.kv_heads;
     const std::int64_t slot = slots[token];
-    float x[8] = {};
+    unsigned codes[2] = {}, pairs[2] = {};
     if (slot >= 0 && slot < static_cast<std::int64_t>(cache.pages) * cache.page_size) {
-        const std::int64_t page = slot / cache.page_size;
+        const std::int64_t page = divide(static_cast<unsigned>(slot >> 4), runs_per_page);
         const std::int64_t at = (page * cache.kv_heads + head) * cache.page_size + slot - page * cache.page_size;
-        const unsigned codes = reinterpret_cast<const unsigned*>(is_value ? cache.value_codes : cache.key_codes)[at * lanes + lane];
         const int group_lanes = cache.group / 8;
-        const unsigned pair = reinterpret_cast<const unsigned*>(is_value ? cache.value_scales : cache.key_scales)
-            [at * (lanes / group_lanes) + lane / group_lanes];
-        const float s = half_bits(static_cast<std::uint16_t>(pair)), m = half_bits(static_cast<std::uint16_t>(pair >> 16));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf(static_cast<float>(codes >> (4 * e) & 15u), s, m);
+        const std::int64_t code_at = at * lanes + lane, pair_at = at * (lanes / group_lanes) + lane / group_lanes;
+        codes[0] = reinterpret_cast<const unsigned*>(cache.key_codes)[code_at];
+        codes[1] = reinterpret_cast<const unsigned*>(cache.value_codes)[code_at];
+        pairs[0] = reinterpret_cast<const unsigned*>(cache.key_scales)[pair_at];
+        pairs[1] = reinterpret_cast<const unsigned*>(cache.value_scales)[pair_at];
     } else if (slot >= 0) {
         note(cache, status_slot);
     }
-    if (reinterpret_cast<std::uintptr_t>(out) % 16 == 0) {
-        store8(out, x);
-    } else {
+    const bool aligned = (reinterpret_cast<std::uintptr_t>(keys) | reinterpret_cast<std::uintptr_t>(values)) % 16 == 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) out[e] = narrow<T>(x[e]);
+    for (int kind = 0; kind < 2; ++kind) {
+        const float2 pair = __half22float2(reinterpret_cast<const __half2&>(pairs[kind]));
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {  // 2^23 + code, less 2^23: no conversion
+            x[e] = fmaf(__uint_as_float((codes[kind] >> (4 * e) & 15u) | 0x4b000000u) - 8388608.0f, pair.x, pair.y);
+        }
+        T* const out = (kind == 0 ? keys : values) + i * 8;
+        if (aligned) {
+            store8(out, x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = narrow<T>(x[e]);
+        }
     }
 }
 
@@ -295,16 +351,23 @@ cudaError_t append_shape(const Cache& cache, const AppendArgs& a, cudaStream_t s
     const bool octets = aligned(a.keys, a.key_stride, a.key_head_stride) &&
         aligned(a.values, a.value_stride, a.value_head_stride) &&
         aligned(a.queries, a.query_stride, a.query_head_stride) && aligned(a.rotated, 0, 0) &&
-        (a.positions == nullptr || a.rotary % (a.interleaved ? 8 : 16) == 0);
+        (a.positions == nullptr || (a.rotary % (a.interleaved ? 8 : 16) == 0 && aligned(a.cosines, 0, 0) &&
+                                    aligned(a.sines, 0, 0)));
     if (octets) {
         constexpr int tokens_each = 256 / (D / 8);
         const std::int64_t token_blocks = (a.tokens + tokens_each - 1) / tokens_each;
-        // More heads a thread share the angles; fewer keep a few tokens' threads many.
-        const std::int64_t room = token_blocks * heads / (16 * static_cast<std::int64_t>(sm_count()));
-        const int heads_each = static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>(8, room)));
-        const dim3 grid(static_cast<unsigned>(token_blocks), static_cast<unsigned>((heads + heads_each - 1) / heads_each));
-        if (grid.y > 65535) return cudaErrorInvalidValue;
-        append_octets_kernel<T, D><<<grid, 256, 0, stream>>>(cache, a, heads_each);
+        // Four heads a thread share the angles and are in flight together; one keeps a few tokens' threads many.
+        const int each = token_blocks * heads >= 16 * static_cast<std::int64_t>(sm_count()) ? 4 : 1;
+        const int query_heads = a.queries != nullptr ? a.query_heads : 0;
+        const std::int64_t runs = (query_heads + each - 1) / each + 2 * ((cache.kv_heads + each - 1) / each);
+        if (runs > 65535) return cudaErrorInvalidValue;
+        const dim3 grid(static_cast<unsigned>(token_blocks), static_cast<unsigned>(runs));
+        const Divisor runs_per_page = divisor(static_cast<unsigned>(cache.page_size / 16));
+        if (each == 4) {
+            append_octets_kernel<T, D, 4><<<grid, 256, 0, stream>>>(cache, a, runs_per_page);
+        } else {
+            append_octets_kernel<T, D, 1><<<grid, 256, 0, stream>>>(cache, a, runs_per_page);
+        }
     } else {
         const std::int64_t blocks = (a.tokens * heads + 7) / 8;
         if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
@@ -326,14 +389,16 @@ template <typename T>
 cudaError_t read_typed(const Cache& cache, const std::int64_t* slots, std::int64_t count, void* keys, void* values,
                        cudaStream_t stream) {
     const std::int64_t heads = count * cache.kv_heads, blocks = (heads * (cache.head_dim / 8) + 255) / 256;
-    if (heads > 0xffffffffll || blocks > 0x7fffffff) return cudaErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(blocks), 2);
+    if (heads > 0x7fffffff || blocks > 0x7fffffff) return cudaErrorInvalidValue;
+    const unsigned grid = static_cast<unsigned>(blocks);
     T* const k = static_cast<T*>(keys);
     T* const v = static_cast<T*>(values);
+    const Divisor by_heads = divisor(static_cast<unsigned>(cache.kv_heads));
+    const Divisor runs = divisor(static_cast<unsigned>(cache.page_size / 16));
     switch (cache.head_dim) {
-    case 64: read_kernel<T, 64><<<grid, 256, 0, stream>>>(cache, slots, count, k, v); break;
-    case 128: read_kernel<T, 128><<<grid, 256, 0, stream>>>(cache, slots, count, k, v); break;
-    default: read_kernel<T, 256><<<grid, 256, 0, stream>>>(cache, slots, count, k, v); break;
+    case 64: read_kernel<T, 64><<<grid, 256, 0, stream>>>(cache, slots, count, k, v, by_heads, runs); break;
+    case 128: read_kernel<T, 128><<<grid, 256, 0, stream>>>(cache, slots, count, k, v, by_heads, runs); break;
+    default: read_kernel<T, 256><<<grid, 256, 0, stream>>>(cache, slots, count, k, v, by_heads, runs); break;
     }
     return cudaGetLastError();
 }

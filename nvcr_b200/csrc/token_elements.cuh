@@ -51,6 +51,21 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// n / d for n < 2^31 as (umulhi(n, multiplier) + n) >> shift (Granlund and
+// Montgomery's division by an invariant).
+struct Divisor {
+    unsigned multiplier, shift;
+};
+
+__device__ __forceinline__ unsigned divide(unsigned n, Divisor d) { return (__umulhi(n, d.multiplier) + n) >> d.shift; }
+
+inline Divisor divisor(unsigned d) {
+    Divisor made{0, 0};
+    while ((1u << made.shift) < d) ++made.shift;
+    made.multiplier = static_cast<unsigned>((((1ull << made.shift) - d) << 32) / d + 1);
+    return made;
+}
+
 // A kernel's dynamic shared memory above 48 KB, allowed once on each device.
 class SharedAllowance {
 public:
