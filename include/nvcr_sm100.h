@@ -465,7 +465,7 @@ int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_
 
 /* Weights in the 4-bit group form, laid out once for nvcr_sm100_token_multiply:
  * codes [outputs][inputs / 2], scales and minimums [outputs][inputs / group],
- * inputs a multiple of group. The packed buffers' sizes in bytes come first. */
+ * inputs a multiple of group and at most 98304. The packed buffers' sizes in bytes come first. */
 int nvcr_sm100_token_packed_bytes(int32_t outputs, int32_t inputs, int32_t group, size_t* code_bytes,
                                   size_t* scale_bytes);
 int nvcr_sm100_token_pack(const uint8_t* codes, const uint16_t* scales, const uint16_t* minimums, int32_t outputs,

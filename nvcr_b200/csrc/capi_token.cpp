@@ -106,8 +106,9 @@ token::Cache cache_of(const nvcr_sm100_token_cache& cache) {
             cache.pages,     cache.kv_heads,   cache.page_size,   cache.head_dim,     cache.group};
 }
 
+// 8 rows of 98304 inputs fit the shared memory of a cluster of eight blocks.
 bool matrix_shape(std::int32_t outputs, std::int32_t inputs, std::int32_t group) {
-    return outputs > 0 && inputs > 0 && (group == 32 || group == 64 || group == 128) && inputs % group == 0;
+    return outputs > 0 && inputs > 0 && inputs <= 98304 && (group == 32 || group == 64 || group == 128) && inputs % group == 0;
 }
 
 }  // namespace
@@ -271,7 +272,7 @@ int nvcr_sm100_token_packed_bytes(int32_t outputs, int32_t inputs, int32_t group
                                   size_t* scale_bytes) {
     return guarded([&] {
         if (code_bytes == nullptr || scale_bytes == nullptr) return refuse("null argument");
-        if (!matrix_shape(outputs, inputs, group)) return refuse("inputs must be a multiple of a group of 32, 64 or 128");
+        if (!matrix_shape(outputs, inputs, group)) return refuse("inputs must be a multiple of a group of 32, 64 or 128, and at most 98304");
         *code_bytes = token::packed_code_bytes(outputs, inputs);
         *scale_bytes = token::packed_scale_bytes(outputs, inputs, group);
         return report_ok();
@@ -281,7 +282,7 @@ int nvcr_sm100_token_packed_bytes(int32_t outputs, int32_t inputs, int32_t group
 int nvcr_sm100_token_pack(const uint8_t* codes, const uint16_t* scales, const uint16_t* minimums, int32_t outputs,
                           int32_t inputs, int32_t group, void* packed_codes, void* packed_scales, void* stream) {
     return guarded([&] {
-        if (!matrix_shape(outputs, inputs, group)) return refuse("inputs must be a multiple of a group of 32, 64 or 128");
+        if (!matrix_shape(outputs, inputs, group)) return refuse("inputs must be a multiple of a group of 32, 64 or 128, and at most 98304");
         if (codes == nullptr || scales == nullptr || minimums == nullptr || packed_codes == nullptr ||
             packed_scales == nullptr) {
             return refuse("null argument");
@@ -301,7 +302,7 @@ int nvcr_sm100_token_multiply(int type, const void* x, int64_t x_stride, int64_t
                               const void* bias, void* y, void* stream) {
     return guarded([&] {
         if (!half_type(type)) return refuse("type must be F16 or BF16");
-        if (!matrix_shape(outputs, inputs, group)) return refuse("inputs must be a multiple of a group of 32, 64 or 128");
+        if (!matrix_shape(outputs, inputs, group)) return refuse("inputs must be a multiple of a group of 32, 64 or 128, and at most 98304");
         if (rows < 0 || rows > 65535) return refuse("rows out of range");
         if (packed_codes == nullptr || packed_scales == nullptr || (rows > 0 && (x == nullptr || y == nullptr))) {
             return refuse("null argument");

@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
     __shared__ bool joint_last;
     __shared__ __align__(16) __half joint_query[NT][D * 8];  // [word][lane][fragment registers]
     __shared__ float joint_query_sum[rows][groups], joint_factor[rows];
+    join_chain();
     const Cache& cache = work.cache;
     const AttendArgs& a = work.a;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = lane / 4, j = lane % 4;
@@ -802,8 +803,8 @@ cudaError_t launch(Work& work, cudaStream_t stream) {
         std::max(1, (work.a.max_length + unit - 1) / unit);
     if (units > 0x7fffffff) return cudaErrorInvalidValue;
     const std::int64_t grid = std::min<std::int64_t>(std::min(resident<D, NT> * sm_count(), most_blocks), units);
-    attend_kernel<T, D, G, NT><<<static_cast<unsigned>(grid), 32 * warps, bytes, stream>>>(work);
-    return cudaGetLastError();
+    return kernels::launch_overlapped(attend_kernel<T, D, G, NT>, dim3(static_cast<unsigned>(grid)), dim3(32 * warps), bytes,
+                                      stream, static_cast<const Work&>(work));
 }
 
 template <typename T, int D, int G>

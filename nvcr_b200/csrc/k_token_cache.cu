@@ -72,6 +72,7 @@ private:
 template <typename T, int D>
 __global__ void append_kernel(Cache cache, AppendArgs a) {
     constexpr int per_lane = D / 32;
+    join_chain();
     const int lane = threadIdx.x % 32;
     const int heads = 2 * cache.kv_heads + (a.queries != nullptr ? a.query_heads : 0);
     const std::int64_t item = (static_cast<std::int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
@@ -186,6 +187,7 @@ __device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
 template <typename T, int D, int H>
 __global__ void __launch_bounds__(256, 4) append_octets_kernel(Cache cache, AppendArgs a, Divisor runs_per_page) {
     constexpr int lanes = D / 8;
+    join_chain();
     const int lane = threadIdx.x % lanes, channel = 8 * lane;
     const std::int64_t token = static_cast<std::int64_t>(blockIdx.x) * (256 / lanes) + threadIdx.x / lanes;
     const bool valid = token < a.tokens;  // threads past the end stay for the shuffles
@@ -304,6 +306,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) read_kernel(Cache cache, const std::int64_t* slots, std::int64_t count, T* keys,
                                                    T* values, Divisor by_heads, Divisor runs_per_page) {
     constexpr int lanes = D / 8;
+    join_chain();
     const std::int64_t i = static_cast<std::int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= count * cache.kv_heads * lanes) return;
     const int lane = static_cast<int>(i % lanes);
@@ -363,17 +366,13 @@ cudaError_t append_shape(const Cache& cache, const AppendArgs& a, cudaStream_t s
         if (runs > 65535) return cudaErrorInvalidValue;
         const dim3 grid(static_cast<unsigned>(token_blocks), static_cast<unsigned>(runs));
         const Divisor runs_per_page = divisor(static_cast<unsigned>(cache.page_size / 16));
-        if (each == 4) {
-            append_octets_kernel<T, D, 4><<<grid, 256, 0, stream>>>(cache, a, runs_per_page);
-        } else {
-            append_octets_kernel<T, D, 1><<<grid, 256, 0, stream>>>(cache, a, runs_per_page);
-        }
-    } else {
-        const std::int64_t blocks = (a.tokens * heads + 7) / 8;
-        if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
-        append_kernel<T, D><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(cache, a);
+        return kernels::launch_overlapped(each == 4 ? append_octets_kernel<T, D, 4> : append_octets_kernel<T, D, 1>, grid,
+                                          dim3(256), 0, stream, cache, a, runs_per_page);
     }
-    return cudaGetLastError();
+    const std::int64_t blocks = (a.tokens * heads + 7) / 8;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+    return kernels::launch_overlapped(append_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, cache,
+                                      a);
 }
 
 template <typename T>
@@ -395,12 +394,9 @@ cudaError_t read_typed(const Cache& cache, const std::int64_t* slots, std::int64
     T* const v = static_cast<T*>(values);
     const Divisor by_heads = divisor(static_cast<unsigned>(cache.kv_heads));
     const Divisor runs = divisor(static_cast<unsigned>(cache.page_size / 16));
-    switch (cache.head_dim) {
-    case 64: read_kernel<T, 64><<<grid, 256, 0, stream>>>(cache, slots, count, k, v, by_heads, runs); break;
-    case 128: read_kernel<T, 128><<<grid, 256, 0, stream>>>(cache, slots, count, k, v, by_heads, runs); break;
-    default: read_kernel<T, 256><<<grid, 256, 0, stream>>>(cache, slots, count, k, v, by_heads, runs); break;
-    }
-    return cudaGetLastError();
+    const auto kernel = cache.head_dim == 64 ? read_kernel<T, 64> : cache.head_dim == 128 ? read_kernel<T, 128>
+                                                                                        : read_kernel<T, 256>;
+    return kernels::launch_overlapped(kernel, dim3(grid), dim3(256), 0, stream, cache, slots, count, k, v, by_heads, runs);
 }
 
 }  // namespace

@@ -13,10 +13,14 @@
 // latency-bound where they are small. So they are laid out once in the order in
 // which lanes want them: 16 outputs x 64 inputs are 512 consecutive bytes, 16 a
 // lane; a lane loads whole fragments with one 16-byte load, straight to
-// registers, several steps of 128 inputs ahead. A block's eight warps share the
-// inputs of 16, 32 or 64 outputs and are summed in shared memory; where that
-// leaves SMs idle, up to eight blocks of a cluster share the inputs and are
-// summed over distributed shared memory, in order: no workspace, one launch.
+// registers, a few steps of 128 inputs ahead. x goes to shared memory once, as
+// fragments, with its groups' sums. A block of 16 warps, one an SM, takes up to 16
+// consecutive tiles of 16 outputs; their steps in a row are divided evenly among
+// the warps, so a warp streams without a barrier to its end, whatever the sizes,
+// and leaves a sum in shared memory wherever its part of a tile ends. Where tiles
+// are fewer than SMs, or x is larger than shared memory, up to eight blocks of a
+// cluster divide the inputs and are summed over distributed shared memory. All
+// sums are in a fixed order: no atomics, no workspace, one launch.
 #include "token_elements.cuh"
 
 #include <algorithm>
@@ -29,8 +33,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int warps = 8;
+constexpr int warps = 16;
 constexpr int step_inputs = 128;
+constexpr int most_tiles = 16;  // of a block
 
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
@@ -55,233 +60,289 @@ __host__ __device__ constexpr int tiles_of(int outputs) { return (outputs + 15) 
 __host__ __device__ constexpr int steps_of(int inputs) { return (inputs + step_inputs - 1) / step_inputs; }
 
 struct Shape {
-    int steps;
-    int tiles;
-    bool aligned;  // x can be read 16 bytes at a time
+    int steps;       // of 128 inputs
+    int tiles;       // of 16 outputs
+    int part_steps;  // of each block of a cluster
+    bool aligned;    // x can be read 16 bytes at a time
 };
 
-// R tiles of 16 outputs, NT times 8 rows.
-template <typename T, int G, int NT, int R>
+// Shared memory: x as fragments [step][quarter of 32 inputs][n][lane] of 16 bytes, the groups' sums of x
+// [step][group][8 NT], and the warps' sums of (16 outputs, 8 NT rows): warp w's of the block's tile t is number w + t,
+// which grows along the warps' row of steps.
+template <int G, int NT>
+constexpr int x_step_bytes = 4 * NT * 512 + (step_inputs / G) * 8 * NT * 4;
+template <int NT>
+constexpr int sum_floats = 16 * 8 * NT;
+template <int NT>
+constexpr int sums_bytes = (warps + most_tiles - 1) * sum_floats<NT> * 4;
+
+template <typename T, int G, int NT>
 __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs a, const Shape shape) {
     constexpr bool half = std::is_same_v<T, __half>;
-    constexpr int groups = step_inputs / G, quarters = G / 32;  // 32 inputs each
-    constexpr int depth = R == 1 ? 4 : R == 2 ? 2 : 1;          // steps of weights in flight
+    constexpr int groups = step_inputs / G, quarters = G / 32;
+    constexpr int depth = G == 32 ? 3 : 4;  // steps of weights in flight, as the registers allow
     constexpr unsigned one = half ? 0x3c003c00u : 0x3f803f80u;
-    __shared__ float sums[warps][R][16][8 * NT];
+    extern __shared__ __align__(128) std::uint8_t shared[];
+    join_chain();
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = lane / 4, j = lane % 4;
     const cg::cluster_group cluster = cg::this_cluster();
     const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
-    const int first_tile = blockIdx.x / parts * R;
+    const int blocks = static_cast<int>(gridDim.x) / parts, block = static_cast<int>(blockIdx.x) / parts;
+    const int first_tile = static_cast<int>(static_cast<std::int64_t>(shape.tiles) * block / blocks);
+    const int tiles = static_cast<int>(static_cast<std::int64_t>(shape.tiles) * (block + 1) / blocks) - first_tile;
+    const int first_step = part * shape.part_steps;
+    const int steps = max(0, min(shape.part_steps, shape.steps - first_step));
     const std::int64_t first_row = static_cast<std::int64_t>(blockIdx.y) * (8 * NT);
-    const int stride = warps * parts, start = part * warps + warp;
-    const int count = start < shape.steps ? (shape.steps - start + stride - 1) / stride : 0;
+    uint4* const x_parts = reinterpret_cast<uint4*>(shared);
+    float* const x_sums = reinterpret_cast<float*>(shared + shape.part_steps * (4 * NT * 512));
+    float* const sums = reinterpret_cast<float*>(shared + shape.part_steps * x_step_bytes<G, NT>);
 
-    const uint4* codes[R];
-    const uint2* scales[R];
+    // ---- this warp's part of the steps of the block's tiles in a row, and its first weights ----
+    const int total = tiles * steps;
+    const int begin = total * warp / warps, end = total * (warp + 1) / warps;
+    uint4 code[depth][2];
+    uint2 pair[depth][groups];
+    const int begin_tile = steps > 0 ? begin / steps : 0;
+    const std::int64_t begin_at =
+        static_cast<std::int64_t>(first_tile + begin_tile) * shape.steps + first_step + (begin - begin_tile * steps);
+    const uint4* codes = reinterpret_cast<const uint4*>(a.codes) + begin_at * 64 + lane;
+    const uint2* scales = reinterpret_cast<const uint2*>(a.scales) + begin_at * (8 * groups) + r;
+    int to_load = end - begin, to_tile_end = steps - (begin - begin_tile * steps);
+    auto load_weights = [&](int slot) {
+        if (to_load <= 0) return;
+        code[slot][0] = __ldcs(codes);
+        code[slot][1] = __ldcs(codes + 32);
 #pragma unroll
-    for (int t = 0; t < R; ++t) {  // a tile past the last reads the last and is not stored
-        const std::int64_t at = static_cast<std::int64_t>(min(first_tile + t, shape.tiles - 1)) * shape.steps + start;
-        codes[t] = reinterpret_cast<const uint4*>(a.codes) + at * 64 + lane;
-        scales[t] = reinterpret_cast<const uint2*>(a.scales) + at * (8 * groups) + r;
-    }
-    uint4 code[depth][R][2];
-    uint2 pair[depth][R][groups];
-    auto load_weights = [&](int i, int slot) {
-        if (i >= count) return;
-#pragma unroll
-        for (int t = 0; t < R; ++t) {
-            code[slot][t][0] = __ldcs(codes[t] + static_cast<std::int64_t>(i) * stride * 64);
-            code[slot][t][1] = __ldcs(codes[t] + static_cast<std::int64_t>(i) * stride * 64 + 32);
-#pragma unroll
-            for (int g = 0; g < groups; ++g) {
-                pair[slot][t][g] = __ldg(scales[t] + static_cast<std::int64_t>(i) * stride * (8 * groups) + 8 * g);
-            }
-        }
-    };
-    const T* x[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) x[n] = static_cast<const T*>(a.x) + (first_row + 8 * n + r) * a.x_stride + 8 * j;
-    uint4 value[NT][4], value_next[NT][4];
-    auto load_x = [&](int i, uint4 (&to)[NT][4]) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int k = (start + i * stride) * step_inputs + 32 * q;
-                uint4 v = {0u, 0u, 0u, 0u};
-                if (i < count && k < a.inputs && first_row + 8 * n + r < a.rows) {
-                    if (shape.aligned) {
-                        v = __ldg(reinterpret_cast<const uint4*>(x[n] + k));
-                    } else {
-                        alignas(16) T values[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) values[e] = x[n][k + e];
-                        v = *reinterpret_cast<const uint4*>(values);
-                    }
-                }
-                to[n][q] = v;
-            }
+        for (int g = 0; g < groups; ++g) pair[slot][g] = __ldcs(scales + 8 * g);
+        codes += 64, scales += 8 * groups, --to_load;
+        if (--to_tile_end == 0) {  // over the other blocks' steps
+            to_tile_end = steps;
+            codes += (shape.steps - steps) * 64, scales += (shape.steps - steps) * (8 * groups);
         }
     };
 #pragma unroll
-    for (int s = 0; s < depth; ++s) load_weights(s, s);
-    load_x(0, value);
+    for (int s = 0; s < depth; ++s) load_weights(s);
 
-    float y[R][NT][4];
+    // ---- x to shared memory, and its groups' sums as products with ones ----
+    for (int e = threadIdx.x; e < steps * (4 * NT * 32); e += 32 * warps) {
+        const int to_lane = e % 32, n = e / 32 % NT, q = e / (32 * NT) % 4, step = e / (128 * NT);
+        const int k = (first_step + step) * step_inputs + 32 * q + to_lane % 4 * 8;
+        const std::int64_t row = first_row + 8 * n + to_lane / 4;
+        const bool inside = row < a.rows && k < a.inputs;  // inputs are a multiple of 32, so all eight are inside
+        const T* const from = static_cast<const T*>(a.x) + (inside ? row * a.x_stride + k : 0);
+        if (shape.aligned) {  // zeros outside
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                             static_cast<unsigned>(__cvta_generic_to_shared(x_parts + e))),
+                         "l"(from), "r"(inside ? 16 : 0)
+                         : "memory");
+        } else {
+            alignas(16) T values[8];
 #pragma unroll
-    for (int t = 0; t < R; ++t) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) y[t][n][0] = y[t][n][1] = y[t][n][2] = y[t][n][3] = 0.0f;
-    }
-    for (int base = 0; base < count; base += depth) {
-#pragma unroll
-        for (int s = 0; s < depth; ++s) {
-            if (base + s >= count) break;
-            load_x(base + s + 1, value_next);
-#pragma unroll
-            for (int g = 0; g < groups; ++g) {
-                float x_sum[NT][4];
-                const unsigned ones[4] = {one, one, one, one};
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    x_sum[n][0] = x_sum[n][1] = x_sum[n][2] = x_sum[n][3] = 0.0f;
-#pragma unroll
-                    for (int q = g * quarters; q < (g + 1) * quarters; ++q) {
-                        mma<T>(x_sum[n], ones, value[n][q].x, value[n][q].z);
-                        mma<T>(x_sum[n], ones, value[n][q].y, value[n][q].w);
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < R; ++t) {
-                    float even[NT][4], odd[NT][4];  // for bfloat16 all of them in `even`
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) even[n][i] = odd[n][i] = 0.0f;
-                    }
-#pragma unroll
-                    for (int q = g * quarters; q < (g + 1) * quarters; ++q) {
-                        const uint4 raw = code[s][t][q / 2];
-                        const unsigned near = q % 2 == 0 ? raw.x : raw.z, far = q % 2 == 0 ? raw.y : raw.w;
-                        unsigned front[4], back[4];
-                        if constexpr (half) {
-                            const unsigned near8 = near >> 8, far8 = far >> 8;
-                            front[0] = near & 0x000f000fu, front[1] = far & 0x000f000fu;
-                            front[2] = near8 & 0x000f000fu, front[3] = far8 & 0x000f000fu;
-                            back[0] = near & 0x00f000f0u, back[1] = far & 0x00f000f0u;
-                            back[2] = near8 & 0x00f000f0u, back[3] = far8 & 0x00f000f0u;
-                        } else {
-                            front[0] = (near & 0x000f000fu) | 0x43004300u, front[1] = (far & 0x000f000fu) | 0x43004300u;
-                            front[2] = (near >> 8 & 0x000f000fu) | 0x43004300u;
-                            front[3] = (far >> 8 & 0x000f000fu) | 0x43004300u;
-                            back[0] = (near >> 4 & 0x000f000fu) | 0x43004300u;
-                            back[1] = (far >> 4 & 0x000f000fu) | 0x43004300u;
-                            back[2] = (near >> 12 & 0x000f000fu) | 0x43004300u;
-                            back[3] = (far >> 12 & 0x000f000fu) | 0x43004300u;
-                        }
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            mma<T>(even[n], front, value[n][q].x, value[n][q].z);
-                            mma<T>(half ? odd[n] : even[n], back, value[n][q].y, value[n][q].w);
-                        }
-                    }
-                    const float2 near_pair = __half22float2(reinterpret_cast<const __half2&>(pair[s][t][g].x));
-                    const float2 far_pair = __half22float2(reinterpret_cast<const __half2&>(pair[s][t][g].y));
-                    const float near_scale = half ? near_pair.x * 0x1p24f : near_pair.x;
-                    const float far_scale = half ? far_pair.x * 0x1p24f : far_pair.x;
-                    const float near_low = half ? near_pair.y : fmaf(-128.0f, near_pair.x, near_pair.y);
-                    const float far_low = half ? far_pair.y : fmaf(-128.0f, far_pair.x, far_pair.y);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float dot = half ? fmaf(odd[n][i], 0.0625f, even[n][i]) : even[n][i];
-                            const float with_low = fmaf(i < 2 ? near_low : far_low, x_sum[n][i], y[t][n][i]);
-                            y[t][n][i] = fmaf(i < 2 ? near_scale : far_scale, dot, with_low);
-                        }
-                    }
-                }
-            }
-            load_weights(base + s + depth, s);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) value[n][q] = value_next[n][q];
-            }
+            for (int i = 0; i < 8; ++i) values[i] = inside ? from[i] : narrow<T>(0.0f);
+            x_parts[e] = *reinterpret_cast<const uint4*>(values);
         }
     }
-
-#pragma unroll
-    for (int t = 0; t < R; ++t) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    for (int e = warp; e < steps * groups; e += warps) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const unsigned ones[4] = {one, one, one, one};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sums[warp][t][r + (i & 2) * 4][8 * n + 2 * j + (i & 1)] = y[t][n][i];
+            for (int q = 0; q < quarters; ++q) {
+                const uint4 v = x_parts[((e / groups * 4 + e % groups * quarters + q) * NT + n) * 32 + lane];
+                mma<T>(sum, ones, v.x, v.z);
+                mma<T>(sum, ones, v.y, v.w);
+            }
+            if (r == 0) *reinterpret_cast<float2*>(x_sums + e * (8 * NT) + 8 * n + 2 * j) = {sum[0], sum[1]};
         }
     }
     __syncthreads();
-    constexpr int outs = R * 16 * 8 * NT;
-    for (int e = threadIdx.x; e < outs; e += 32 * warps) {
-        float* const at = &sums[0][0][0][0] + e;
-        float total = 0.0f;
+
+    // ---- the stream of weights ----
+    float y[NT][4];
 #pragma unroll
-        for (int w = 0; w < warps; ++w) total += at[w * outs];
-        *at = total;  // this thread alone reads and writes element e of every warp
-    }
-    if (parts > 1) {
-        cluster.sync();
-    } else {
-        __syncthreads();
-    }
-    if (part == 0) {
-        for (int e = threadIdx.x; e < outs; e += 32 * warps) {
-            const int output = e % (16 * R), row = e / (16 * R);  // neighbouring threads store neighbouring outputs
-            float* const at = &sums[0][output / 16][output % 16][row];
-            float total = *at;
-            for (int p = 1; p < parts; ++p) total += *cluster.map_shared_rank(at, p);
-            const int n = first_tile * 16 + output;
-            if (n < a.outputs && first_row + row < a.rows) {
-                if (a.bias != nullptr) total += widen(static_cast<const T*>(a.bias)[n]);
-                static_cast<T*>(a.y)[(first_row + row) * a.outputs + n] = narrow<T>(total);
+    for (int n = 0; n < NT; ++n) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.0f;
+    int tile = begin_tile, step = begin - tile * steps;
+    for (int base = begin; base < end; base += depth) {
+#pragma unroll
+        for (int s = 0; s < depth; ++s) {
+            if (base + s >= end) break;
+            const uint4* const x_step = x_parts + step * (4 * NT * 32) + lane;
+            const float* const x_sum_step = x_sums + step * (groups * 8 * NT) + 2 * j;
+#pragma unroll
+            for (int g = 0; g < groups; ++g) {
+                float even[NT][4], odd[NT][4];  // for bfloat16 all of them in `even`
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) even[n][i] = odd[n][i] = 0.0f;
+                }
+#pragma unroll
+                for (int q = g * quarters; q < (g + 1) * quarters; ++q) {
+                    const uint4 raw = code[s][q / 2];
+                    const unsigned near = q % 2 == 0 ? raw.x : raw.z, far = q % 2 == 0 ? raw.y : raw.w;
+                    unsigned front[4], back[4];
+                    if constexpr (half) {
+                        const unsigned near8 = near >> 8, far8 = far >> 8;
+                        front[0] = near & 0x000f000fu, front[1] = far & 0x000f000fu;
+                        front[2] = near8 & 0x000f000fu, front[3] = far8 & 0x000f000fu;
+                        back[0] = near & 0x00f000f0u, back[1] = far & 0x00f000f0u;
+                        back[2] = near8 & 0x00f000f0u, back[3] = far8 & 0x00f000f0u;
+                    } else {
+                        front[0] = (near & 0x000f000fu) | 0x43004300u, front[1] = (far & 0x000f000fu) | 0x43004300u;
+                        front[2] = (near >> 8 & 0x000f000fu) | 0x43004300u;
+                        front[3] = (far >> 8 & 0x000f000fu) | 0x43004300u;
+                        back[0] = (near >> 4 & 0x000f000fu) | 0x43004300u;
+                        back[1] = (far >> 4 & 0x000f000fu) | 0x43004300u;
+                        back[2] = (near >> 12 & 0x000f000fu) | 0x43004300u;
+                        back[3] = (far >> 12 & 0x000f000fu) | 0x43004300u;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const uint4 v = x_step[(q * NT + n) * 32];
+                        mma<T>(even[n], front, v.x, v.z);
+                        mma<T>(half ? odd[n] : even[n], back, v.y, v.w);
+                    }
+                }
+                const float2 near_pair = __half22float2(reinterpret_cast<const __half2&>(pair[s][g].x));
+                const float2 far_pair = __half22float2(reinterpret_cast<const __half2&>(pair[s][g].y));
+                const float near_scale = half ? near_pair.x * 0x1p24f : near_pair.x;
+                const float far_scale = half ? far_pair.x * 0x1p24f : far_pair.x;
+                const float near_low = half ? near_pair.y : fmaf(-128.0f, near_pair.x, near_pair.y);
+                const float far_low = half ? far_pair.y : fmaf(-128.0f, far_pair.x, far_pair.y);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float2 x_sum = *reinterpret_cast<const float2*>(x_sum_step + g * (8 * NT) + 8 * n);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float dot = half ? fmaf(odd[n][i], 0.0625f, even[n][i]) : even[n][i];
+                        const float with_low = fmaf(i < 2 ? near_low : far_low, i % 2 == 0 ? x_sum.x : x_sum.y, y[n][i]);
+                        y[n][i] = fmaf(i < 2 ? near_scale : far_scale, dot, with_low);
+                    }
+                }
+            }
+            load_weights(s);
+            ++step;
+            if (step == steps || base + s + 1 == end) {  // the tile's end, or this warp's
+                float* const to = sums + (warp + tile) * sum_floats<NT> + r;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {  // [row][output]
+                        to[(8 * n + 2 * j + (i & 1)) * 16 + (i & 2) * 4] = y[n][i];
+                        y[n][i] = 0.0f;
+                    }
+                }
+                step = 0, ++tile;
             }
         }
     }
-    if (parts > 1) cluster.sync();  // the other blocks' sums stay until they are read
+    __syncthreads();
+
+    // ---- join the warps, then the blocks of the cluster ----
+    auto warp_of = [&](int at) { return ((at + 1) * warps - 1) / total; };  // whose part holds step `at` of the row
+    const int outs = tiles * sum_floats<NT>;
+    auto joined = [&](int e) {
+        const int t = e / sum_floats<NT>, within = e % sum_floats<NT>;
+        float value = 0.0f;
+        if (total > 0) {
+            const int last = warp_of((t + 1) * steps - 1);
+            for (int w = warp_of(t * steps); w <= last; ++w) {
+                if (total * w / warps == total * (w + 1) / warps) continue;  // fewer steps than warps: this one had none
+                value += sums[(w + t) * sum_floats<NT> + within];
+            }
+        }
+        return value;
+    };
+    auto store = [&](int e, float value) {
+        const int output = (first_tile + e / sum_floats<NT>) * 16 + e % 16;
+        const std::int64_t row = first_row + e % sum_floats<NT> / 16;
+        if (output >= a.outputs || row >= a.rows) return;
+        if (a.bias != nullptr) value += widen(static_cast<const T*>(a.bias)[output]);
+        static_cast<T*>(a.y)[row * a.outputs + output] = narrow<T>(value);
+    };
+    if (parts == 1) {
+        for (int e = threadIdx.x; e < outs; e += 32 * warps) store(e, joined(e));
+        return;
+    }
+    float* const whole = reinterpret_cast<float*>(shared);  // over x (16 steps at least here), which is not read any more
+    for (int e = threadIdx.x; e < outs; e += 32 * warps) whole[e] = joined(e);
+    cluster.sync();
+    for (int e = part * 32 * warps + threadIdx.x; e < outs; e += parts * 32 * warps) {
+        float value = 0.0f;
+        for (int p = 0; p < parts; ++p) value += *cluster.map_shared_rank(whole + e, p);
+        store(e, value);
+    }
+    cluster.sync();  // the other blocks' sums stay until they are read
 }
 
-template <typename T, int G, int NT, int R>
-cudaError_t launch(const MultiplyArgs& a, const Shape& shape, cudaStream_t stream) {
-    const int blocks = (shape.tiles + R - 1) / R;
-    const unsigned row_blocks = static_cast<unsigned>((a.rows + 8 * NT - 1) / (8 * NT));
-    // Blocks of a cluster share the inputs while the SMs are not all taken and every warp keeps two steps.
-    int parts = 1;
-    while (parts < 8 && static_cast<std::int64_t>(blocks) * row_blocks * parts * 2 <= sm_count() &&
-           shape.steps >= 2 * warps * parts * 2) {
-        parts *= 2;
-    }
+// Clusters of `parts` blocks, one block an SM, that run at once (asked once: clusters keep to groups of SMs whose
+// sizes are not multiples of theirs).
+template <typename T, int G, int NT>
+int clusters_at_once(int parts) {
+    if (parts == 1) return sm_count();
+    static std::atomic<int> known[4];  // 1, 2, 4, 8 parts
+    std::atomic<int>& found = known[parts == 2 ? 1 : parts == 4 ? 2 : 3];
+    int clusters = found.load(std::memory_order_relaxed);
+    if (clusters > 0) return clusters;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(blocks * parts), row_blocks);
+    config.gridDim = dim3(static_cast<unsigned>(parts * sm_count()));
     config.blockDim = dim3(32 * warps);
-    config.stream = stream;
+    config.dynamicSmemBytes = 120 * 1024;  // one block an SM
     cudaLaunchAttribute attribute[1];
     attribute[0].id = cudaLaunchAttributeClusterDimension;
     attribute[0].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
     config.attrs = attribute;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, multiply_kernel<T, G, NT, R>, a, shape);
+    if (cudaOccupancyMaxActiveClusters(&clusters, multiply_kernel<T, G, NT>, &config) != cudaSuccess || clusters <= 0) {
+        cudaGetLastError();
+        clusters = std::max(1, sm_count() / parts);
+    }
+    found.store(clusters, std::memory_order_relaxed);
+    return clusters;
 }
 
 template <typename T, int G, int NT>
-cudaError_t launch_tiles(const MultiplyArgs& a, const Shape& shape, cudaStream_t stream) {
-    // More outputs a block read x fewer times; fewer spread a small matrix over the SMs.
-    if (shape.tiles >= 4 * sm_count()) return launch<T, G, NT, 4>(a, shape, stream);
-    if (shape.tiles >= 2 * sm_count()) return launch<T, G, NT, 2>(a, shape, stream);
-    return launch<T, G, NT, 1>(a, shape, stream);
+cudaError_t launch(const MultiplyArgs& a, Shape shape, cudaStream_t stream) {
+    constexpr int room = 226 * 1024 - sums_bytes<NT>;
+    static SharedAllowance allowance;
+    const cudaError_t allowed = allowance.allow(multiply_kernel<T, G, NT>, room + sums_bytes<NT>);
+    if (allowed != cudaSuccess) return allowed;
+    const std::int64_t row_blocks = (a.rows + 8 * NT - 1) / (8 * NT);
+    // Blocks of a cluster divide the inputs where x would not fit, and while the SMs are not all taken and every warp
+    // still has a step.
+    int parts = 1;
+    while (parts < 8 && (shape.steps + parts - 1) / parts * x_step_bytes<G, NT> > room) parts *= 2;
+    if ((shape.steps + parts - 1) / parts * x_step_bytes<G, NT> > room) {
+        if constexpr (NT == 2) return launch<T, G, 1>(a, shape, stream);  // 8 rows at a time
+        return cudaErrorInvalidValue;
+    }
+    while (parts < 8 && shape.tiles * row_blocks * parts * 2 <= sm_count() && shape.steps >= warps * parts * 2) parts *= 2;
+    shape.part_steps = (shape.steps + parts - 1) / parts;
+    const std::size_t bytes = static_cast<std::size_t>(shape.part_steps) * x_step_bytes<G, NT> + sums_bytes<NT>;
+    const int at_once = std::max<int>(1, static_cast<int>(clusters_at_once<T, G, NT>(parts) / row_blocks));
+    const int rounds = (shape.tiles + most_tiles * at_once - 1) / (most_tiles * at_once);
+    const int blocks = std::min(shape.tiles, at_once * rounds);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(blocks * parts), static_cast<unsigned>(row_blocks));
+    config.blockDim = dim3(32 * warps);
+    config.dynamicSmemBytes = bytes;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, multiply_kernel<T, G, NT>, a, static_cast<const Shape&>(shape));
 }
 
 template <typename T, int G>
 cudaError_t launch_rows(const MultiplyArgs& a, const Shape& shape, cudaStream_t stream) {
-    return a.rows <= 8 ? launch_tiles<T, G, 1>(a, shape, stream) : launch_tiles<T, G, 2>(a, shape, stream);
+    return a.rows <= 8 ? launch<T, G, 1>(a, shape, stream) : launch<T, G, 2>(a, shape, stream);
 }
 
 template <typename T>
@@ -349,7 +410,7 @@ cudaError_t pack(const std::uint8_t* codes, const std::uint16_t* scales, const s
 
 cudaError_t multiply(const MultiplyArgs& args, cudaStream_t stream) {
     if (args.rows == 0) return cudaSuccess;
-    const Shape shape{steps_of(args.inputs), tiles_of(args.outputs),
+    const Shape shape{steps_of(args.inputs), tiles_of(args.outputs), 0,
                       reinterpret_cast<std::uintptr_t>(args.x) % 16 == 0 && args.x_stride % 8 == 0};
     return args.type == Type::f16 ? launch_group<__half>(args, shape, stream)
                                   : launch_group<__nv_bfloat16>(args, shape, stream);

@@ -38,6 +38,7 @@ __device__ __forceinline__ float bias_at(const void* bias, int i) {
 template <typename T>
 __global__ void __launch_bounds__(threads) long_norm_kernel(NormArgs a) {
     __shared__ float scratch[threads / 32];
+    join_chain();
     const std::int64_t row = blockIdx.x;
     const T* block = static_cast<const T*>(a.block) + row * a.block_stride;
     const T* residual = a.residual == nullptr ? nullptr : static_cast<const T*>(a.residual) + row * a.residual_stride;
@@ -135,6 +136,7 @@ template <typename T, int VEC, int C>
 __global__ void __launch_bounds__(C == 1 ? 1024 : 512, VEC > 1 && C == 2 ? 2 : 1) norm_kernel(NormArgs a) {
     using P = Pack<T, VEC>;
     __shared__ float scratch[4][32];
+    join_chain();
     const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     if (row >= a.rows) return;  // whole warps of a block without barriers
     const int warps = blockDim.x / 32, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -239,8 +241,7 @@ cudaError_t launch_rows(const NormArgs& a, cudaStream_t stream) {
     const unsigned threads = static_cast<unsigned>((lanes + 31) / 32 * 32);
     const unsigned together = threads == 32 ? 8 : 1;  // rows of a block
     const unsigned grid = static_cast<unsigned>((a.rows + together - 1) / together);
-    norm_kernel<T, VEC, C><<<grid, dim3(threads, together), 0, stream>>>(a);
-    return cudaGetLastError();
+    return kernels::launch_overlapped(norm_kernel<T, VEC, C>, dim3(grid), dim3(threads, together), 0, stream, a);
 }
 
 template <typename T>
@@ -263,8 +264,7 @@ cudaError_t launch_type(const NormArgs& a, cudaStream_t stream) {
         if (a.width <= 8 * 512) return launch_rows<T, 1, 8>(a, stream);
         if (a.width <= 16 * 512) return launch_rows<T, 1, 16>(a, stream);
     }
-    long_norm_kernel<T><<<static_cast<unsigned>(a.rows), threads, 0, stream>>>(a);
-    return cudaGetLastError();
+    return kernels::launch_overlapped(long_norm_kernel<T>, dim3(static_cast<unsigned>(a.rows)), dim3(threads), 0, stream, a);
 }
 
 }  // namespace

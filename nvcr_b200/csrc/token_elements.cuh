@@ -2,6 +2,7 @@
 
 // Element access and warp sums shared by the token kernels.
 
+#include "launch.cuh"
 #include "token_kernels.hpp"
 
 #include <atomic>
@@ -10,6 +11,14 @@
 #include <cuda_fp16.h>
 
 namespace nvcr_sm100::token {
+
+// The first thing every kernel does: a token model's step is a chain of short
+// launches, so each starts while the one before it ends, and waits for it here,
+// before it touches memory; then the next may start the same way.
+__device__ __forceinline__ void join_chain() {
+    kernels::grid_dependency_wait();
+    kernels::launch_dependents();
+}
 
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }

@@ -658,6 +658,17 @@ def test_multiply_shapes(cuda, group, inputs, outputs):
         near(y, want, tolerance, name)
 
 
+@pytest.mark.parametrize("inputs,outputs,rows,group", [
+    (2048, 16, 1, 128), (4096, 16, 16, 64), (8192, 40, 3, 32), (8192, 1500, 16, 128), (6016, 300, 12, 32),
+    (32768, 33, 16, 64), (98304, 20, 9, 128), (98304, 20, 1, 32), (128, 40000, 2, 128), (256, 20000, 16, 32),
+])
+def test_multiply_divisions(cuda, inputs, outputs, rows, group):
+    """Inputs divided among the blocks of a cluster, rows too long for 16 at a time, many outputs a block."""
+    for name in ("float16", "bfloat16"):
+        y, want, tolerance = check_multiply(rows, inputs, outputs, group, name, bias=True)
+        near(y, want, tolerance, name)
+
+
 def test_multiply_odd_inputs(cuda):
     for inputs in (32, 96, 160, 1056):
         for name, rows in (("float16", 1), ("bfloat16", 9)):
