@@ -66,21 +66,29 @@ struct Shape {
     bool aligned;    // x can be read 16 bytes at a time
 };
 
-// Shared memory: x as fragments [step][quarter of 32 inputs][n][lane] of 16 bytes, the groups' sums of x
-// [step][group][8 NT], and the warps' sums of (16 outputs, 8 NT rows): warp w's of the block's tile t is number w + t,
-// which grows along the warps' row of steps.
+// Shared memory: x as fragments [step][quarter of 32 inputs][row][j] of 16 bytes (a lane whose row is past the last
+// reads the last: its column of the product is not stored), the groups' sums of x [step][group][8 NT], and the warps'
+// sums of (16 outputs, 8 NT rows): warp w's of the block's tile t is number w + t, which grows along the warps' row of
+// steps.
 template <int G, int NT>
-constexpr int x_step_bytes = 4 * NT * 512 + (step_inputs / G) * 8 * NT * 4;
+__host__ __device__ constexpr int x_step_bytes(int rows) { return rows * 256 + (step_inputs / G) * 8 * NT * 4; }
 template <int NT>
 constexpr int sum_floats = 16 * 8 * NT;
 template <int NT>
 constexpr int sums_bytes = (warps + most_tiles - 1) * sum_floats<NT> * 4;
+// x's part of it, which holds the block's own sums when a cluster joins them.
+template <int G, int NT>
+__host__ __device__ constexpr int x_bytes(int steps, int rows) {
+    const int x = steps * x_step_bytes<G, NT>(rows), own = most_tiles * sum_floats<NT> * 4;
+    return x > own ? x : own;
+}
 
 template <typename T, int G, int NT>
 __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs a, const Shape shape) {
     constexpr bool half = std::is_same_v<T, __half>;
     constexpr int groups = step_inputs / G, quarters = G / 32;
-    constexpr int depth = G == 32 ? 3 : 4;  // steps of weights in flight, as the registers allow
+    // steps of weights in flight, as the registers allow
+    constexpr int depth = (G == 128 ? 5 : G == 64 ? 4 : 3) + (NT == 1 ? 1 : 0);
     constexpr unsigned one = half ? 0x3c003c00u : 0x3f803f80u;
     extern __shared__ __align__(128) std::uint8_t shared[];
     join_chain();
@@ -93,9 +101,10 @@ __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs
     const int first_step = part * shape.part_steps;
     const int steps = max(0, min(shape.part_steps, shape.steps - first_step));
     const std::int64_t first_row = static_cast<std::int64_t>(blockIdx.y) * (8 * NT);
+    const int rows = static_cast<int>(min(static_cast<std::int64_t>(8 * NT), a.rows - first_row));
     uint4* const x_parts = reinterpret_cast<uint4*>(shared);
-    float* const x_sums = reinterpret_cast<float*>(shared + shape.part_steps * (4 * NT * 512));
-    float* const sums = reinterpret_cast<float*>(shared + shape.part_steps * x_step_bytes<G, NT>);
+    float* const x_sums = reinterpret_cast<float*>(shared + shape.part_steps * (rows * 256));
+    float* const sums = reinterpret_cast<float*>(shared + x_bytes<G, NT>(shape.part_steps, rows));
 
     // ---- this warp's part of the steps of the block's tiles in a row, and its first weights ----
     const int total = tiles * steps;
@@ -124,13 +133,14 @@ __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs
     for (int s = 0; s < depth; ++s) load_weights(s);
 
     // ---- x to shared memory, and its groups' sums as products with ones ----
-    for (int e = threadIdx.x; e < steps * (4 * NT * 32); e += 32 * warps) {
-        const int to_lane = e % 32, n = e / 32 % NT, q = e / (32 * NT) % 4, step = e / (128 * NT);
-        const int k = (first_step + step) * step_inputs + 32 * q + to_lane % 4 * 8;
-        const std::int64_t row = first_row + 8 * n + to_lane / 4;
-        const bool inside = row < a.rows && k < a.inputs;  // inputs are a multiple of 32, so all eight are inside
-        const T* const from = static_cast<const T*>(a.x) + (inside ? row * a.x_stride + k : 0);
-        if (shape.aligned) {  // zeros outside
+    // the fragments in a row, an octet of inputs a thread; 32 * warps / 4 (quarter, row) pairs on at a time
+    int x_row = static_cast<int>(threadIdx.x) / 4 % rows, x_quarter = static_cast<int>(threadIdx.x) / 4 / rows;
+    const int more_rows = 32 * warps / 4 % rows, more_quarters = 32 * warps / 4 / rows;
+    for (int e = threadIdx.x; e < steps * 16 * rows; e += 32 * warps) {
+        const int k = first_step * step_inputs + 32 * x_quarter + 8 * j;
+        const bool inside = k < a.inputs;  // zeros past the inputs, which are a multiple of 32
+        const T* const from = static_cast<const T*>(a.x) + (first_row + x_row) * a.x_stride + (inside ? k : 0);
+        if (shape.aligned) {
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                              static_cast<unsigned>(__cvta_generic_to_shared(x_parts + e))),
                          "l"(from), "r"(inside ? 16 : 0)
@@ -141,7 +151,12 @@ __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs
             for (int i = 0; i < 8; ++i) values[i] = inside ? from[i] : narrow<T>(0.0f);
             x_parts[e] = *reinterpret_cast<const uint4*>(values);
         }
+        x_row += more_rows, x_quarter += more_quarters;
+        if (x_row >= rows) x_row -= rows, ++x_quarter;
     }
+    int x_lane[NT];  // of this lane's row in a quarter
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x_lane[n] = min(8 * n + r, rows - 1) * 4 + j;
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     for (int e = warp; e < steps * groups; e += warps) {
@@ -151,7 +166,7 @@ __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs
             const unsigned ones[4] = {one, one, one, one};
 #pragma unroll
             for (int q = 0; q < quarters; ++q) {
-                const uint4 v = x_parts[((e / groups * 4 + e % groups * quarters + q) * NT + n) * 32 + lane];
+                const uint4 v = x_parts[(e * quarters + q) * (rows * 4) + x_lane[n]];
                 mma<T>(sum, ones, v.x, v.z);
                 mma<T>(sum, ones, v.y, v.w);
             }
@@ -169,7 +184,7 @@ __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs
 #pragma unroll
         for (int s = 0; s < depth; ++s) {
             if (base + s >= end) break;
-            const uint4* const x_step = x_parts + step * (4 * NT * 32) + lane;
+            const uint4* const x_step = x_parts + step * (rows * 16);
             const float* const x_sum_step = x_sums + step * (groups * 8 * NT) + 2 * j;
 #pragma unroll
             for (int g = 0; g < groups; ++g) {
@@ -201,7 +216,7 @@ __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs
                     }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const uint4 v = x_step[(q * NT + n) * 32];
+                        const uint4 v = x_step[q * (rows * 4) + x_lane[n]];
                         mma<T>(even[n], front, v.x, v.z);
                         mma<T>(half ? odd[n] : even[n], back, v.y, v.w);
                     }
@@ -267,7 +282,7 @@ __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs
         for (int e = threadIdx.x; e < outs; e += 32 * warps) store(e, joined(e));
         return;
     }
-    float* const whole = reinterpret_cast<float*>(shared);  // over x (16 steps at least here), which is not read any more
+    float* const whole = reinterpret_cast<float*>(shared);  // over x, which is not read any more
     for (int e = threadIdx.x; e < outs; e += 32 * warps) whole[e] = joined(e);
     cluster.sync();
     for (int e = part * 32 * warps + threadIdx.x; e < outs; e += parts * 32 * warps) {
@@ -313,15 +328,17 @@ cudaError_t launch(const MultiplyArgs& a, Shape shape, cudaStream_t stream) {
     const std::int64_t row_blocks = (a.rows + 8 * NT - 1) / (8 * NT);
     // Blocks of a cluster divide the inputs where x would not fit, and while the SMs are not all taken and every warp
     // still has a step.
+    const int step_bytes = x_step_bytes<G, NT>(static_cast<int>(std::min<std::int64_t>(a.rows, 8 * NT)));
     int parts = 1;
-    while (parts < 8 && (shape.steps + parts - 1) / parts * x_step_bytes<G, NT> > room) parts *= 2;
-    if ((shape.steps + parts - 1) / parts * x_step_bytes<G, NT> > room) {
+    while (parts < 8 && (shape.steps + parts - 1) / parts * step_bytes > room) parts *= 2;
+    if ((shape.steps + parts - 1) / parts * step_bytes > room) {
         if constexpr (NT == 2) return launch<T, G, 1>(a, shape, stream);  // 8 rows at a time
         return cudaErrorInvalidValue;
     }
     while (parts < 8 && shape.tiles * row_blocks * parts * 2 <= sm_count() && shape.steps >= warps * parts * 2) parts *= 2;
     shape.part_steps = (shape.steps + parts - 1) / parts;
-    const std::size_t bytes = static_cast<std::size_t>(shape.part_steps) * x_step_bytes<G, NT> + sums_bytes<NT>;
+    const int x_rows = static_cast<int>(std::min<std::int64_t>(a.rows, 8 * NT));
+    const std::size_t bytes = static_cast<std::size_t>(x_bytes<G, NT>(shape.part_steps, x_rows) + sums_bytes<NT>);
     const int at_once = std::max<int>(1, static_cast<int>(clusters_at_once<T, G, NT>(parts) / row_blocks));
     const int rounds = (shape.tiles + most_tiles * at_once - 1) / (most_tiles * at_once);
     const int blocks = std::min(shape.tiles, at_once * rounds);
