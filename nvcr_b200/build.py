@@ -1,4 +1,5 @@
-"""Builds libnvcr_sm100.so in-tree (nvcr_b200/_build/) for sm_100a.
+"""Builds libnvcr_sm100.so in-tree (nvcr_b200/_build/) for sm_100a, and the
+Python binding of its token operators (nvcr_tokens.so, against torch's headers).
 
 CUDA sources: nvcc -gencode arch=compute_100a,code=sm_100a -lineinfo -O3
 -fmad=false (no FP contraction; denormals kept, IEEE division) and no fast
@@ -12,12 +13,15 @@ from __future__ import annotations
 import concurrent.futures
 import os
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
 SOURCE = PACKAGE / "csrc"
 BUILD = PACKAGE / "_build"
 LIBRARY = BUILD / "libnvcr_sm100.so"
+BINDING = BUILD / "nvcr_tokens.so"
+BINDING_SOURCE = PACKAGE / "binding" / "tokens_binding.cpp"
 INCLUDE = PACKAGE.parent / "include"
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 NVCC = str(CUDA_HOME / "bin" / "nvcc")
@@ -67,7 +71,30 @@ def build(verbose: bool = False) -> Path:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{result.stdout}\n{result.stderr}")
         if verbose:
             print(f"built {LIBRARY}")
+    build_binding(verbose)
     return LIBRARY
+
+
+def build_binding(verbose: bool = False) -> Path:
+    """The token operators' extension module, linked to the library beside it."""
+    newest_dep = max(p.stat().st_mtime for p in (BINDING_SOURCE, INCLUDE / "nvcr_sm100.h"))
+    if BINDING.exists() and BINDING.stat().st_mtime >= newest_dep:
+        return BINDING
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    include = [f"-I{root / 'include'}", f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+               f"-I{sysconfig.get_paths()['include']}", f"-I{CUDA_HOME / 'include'}"]
+    cmd = ["g++", "-std=c++20", "-O2", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *include, str(BINDING_SOURCE), "-o",
+           str(BINDING), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+           f"-L{BUILD}", "-lnvcr_sm100", "-Wl,-rpath,$ORIGIN"]
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{result.stdout}\n{result.stderr}")
+    if verbose:
+        print(f"built {BINDING}")
+    return BINDING
 
 
 if __name__ == "__main__":

@@ -15,14 +15,17 @@ FP16 scale s and an FP16 minimum m, and stands for ``c * s + m``.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 
 import torch
 
+from .build import BINDING
 from .executor import ErrorCode, ExecutorError, _check, _stream_handle, library
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-_HALVES = (torch.float16, torch.bfloat16)
 _KINDS = {"rms": 0, "layer": 1}
+_module = None
 
 
 class _Cache(ctypes.Structure):
@@ -41,46 +44,29 @@ def _require(condition: bool, message: str) -> None:
         _refuse(message)
 
 
-def _stream(stream, index: int) -> int | None:
-    if stream is not None:
-        return _stream_handle(stream)
-    if index < 0:
-        _refuse("tensors must be on a CUDA device")
-    return torch._C._cuda_getCurrentRawStream(index)
+def _native():
+    """The compiled binding, loaded at its first use (raises if it is not built)."""
+    global _module
+    if _module is None:
+        if not BINDING.exists():
+            raise FileNotFoundError(f"{BINDING} is not built; run nvcr_b200.build.build()")
+        library()
+        loader = importlib.machinery.ExtensionFileLoader("nvcr_tokens", str(BINDING))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("nvcr_tokens", loader))
+        loader.exec_module(module)
+        module.bind(_refuse, _check)
+        _module = module
+    return _module
 
 
-def _channels(tensor: torch.Tensor | None, name: str, width: int, first: torch.Tensor) -> int | None:
-    """The address of an optional contiguous vector of `width`, of `first`'s type and device."""
-    if tensor is None:
-        return None
-    if tensor.dtype is not first.dtype or tensor.shape != (width,) or tensor.get_device() != first.get_device() \
-            or not tensor.is_contiguous():
-        _refuse(f"{name} must be a contiguous {first.dtype} tensor of shape {(width,)} on {first.device}")
-    return tensor.data_ptr()
-
-
-def _rows(tensor: torch.Tensor, name: str, first: torch.Tensor) -> int:
-    """The address of a [rows, width] tensor like `first` (its row stride is free)."""
-    if tensor.dtype is not first.dtype or tensor.shape != first.shape or tensor.get_device() != first.get_device() \
-            or (tensor.stride(1) != 1 and tensor.shape[1] > 1):
-        _refuse(f"{name} must be a {first.dtype} tensor of shape {tuple(first.shape)} on {first.device} "
-                "with contiguous rows")
-    return tensor.data_ptr()
+def _stream(stream) -> int | None:
+    return None if stream is None else _stream_handle(stream) or 0
 
 
 def _whole(tensor: torch.Tensor, name: str, kind: torch.dtype, shape: tuple, index: int) -> int:
     """The address of a contiguous tensor of a type and shape on CUDA device `index`."""
     if tensor.dtype is not kind or tensor.shape != shape or tensor.get_device() != index or not tensor.is_contiguous():
         _refuse(f"{name} must be a contiguous {kind} tensor of shape {tuple(shape)} on cuda:{index}")
-    return tensor.data_ptr()
-
-
-def _heads(tensor: torch.Tensor, name: str, shape: tuple, first: torch.Tensor) -> int:
-    """The address of a [tokens, heads, dim] tensor whose channels are contiguous (its other strides are free)."""
-    if tensor.dtype is not first.dtype or tensor.shape != shape or tensor.get_device() != first.get_device() \
-            or (tensor.stride(2) != 1 and tensor.numel() > 0):
-        _refuse(f"{name} must be a {first.dtype} tensor of shape {tuple(shape)} on {first.device} "
-                "with contiguous channels")
     return tensor.data_ptr()
 
 
@@ -95,35 +81,12 @@ def block_norm(block: torch.Tensor, *, residual: torch.Tensor | None = None, gat
     normed = N(hidden; pre_weight, pre_bias). N is the root-mean-square norm ("rms") or the layer norm ("layer"),
     with weights taken as weight + weight_offset. `gate` is [width] or [rows, width]. block, residual and a gate of
     rows may have any row stride. ``hidden=False`` or ``normed=False`` leaves that output out (None)."""
-    code, layer = _TYPES.get(block.dtype), _KINDS.get(kind)
-    if code is None or block.dim() != 2:
-        _refuse("block must be a [rows, width] tensor of a float type")
+    layer = _KINDS.get(kind)
     if layer is None:
         _refuse(f"kind must be one of {sorted(_KINDS)}")
-    if not (hidden or normed):
-        _refuse("neither hidden nor normed is wanted")
-    rows, width = block.shape
-    block_address, residual_address, gate_address = _rows(block, "block", block), None, None
-    residual_stride = gate_stride = 0
-    if residual is not None:
-        residual_address, residual_stride = _rows(residual, "residual", block), residual.stride(0)
-    if gate is not None:
-        if gate.dim() == 1:
-            gate_address = _channels(gate, "gate", width, block)
-        else:
-            gate_address, gate_stride = _rows(gate, "gate", block), gate.stride(0)
-    weights = (_channels(post_weight, "post_weight", width, block), _channels(post_bias, "post_bias", width, block),
-               _channels(pre_weight, "pre_weight", width, block), _channels(pre_bias, "pre_bias", width, block))
-    handle = _stream(stream, block.get_device())
-    sums = torch.empty_like(block, memory_format=torch.contiguous_format) if hidden else None
-    out = torch.empty_like(block, memory_format=torch.contiguous_format) if normed else None
-    status = library().nvcr_sm100_token_norm(
-        code, layer, post, block_address, block.stride(0), residual_address, residual_stride, gate_address, gate_stride,
-        *weights, None if sums is None else sums.data_ptr(), None if out is None else out.data_ptr(), rows, width,
-        residual_scale, weight_offset, epsilon, handle)
-    if status:
-        _check(status)
-    return sums, out
+    return (_module or _native()).norm(block, residual, gate, post, post_weight, post_bias, pre_weight, pre_bias, layer,
+                                       residual_scale, weight_offset, epsilon, hidden, normed,
+                                       None if stream is None else _stream(stream))
 
 
 class PagedCache:
@@ -171,55 +134,17 @@ class PagedCache:
         stored; else distinct). With int32 `positions`, keys are rotated before they are stored, and `queries`
         [tokens, heads, head_dim] into the tensor that is returned, by rows of the float32 tables `cosines` and
         `sines` [rows, rotary / 2]: pairs (i, i + rotary / 2), or (2 i, 2 i + 1) if `interleaved`."""
-        index = self._index
-        if keys.dim() != 3 or keys.dtype not in _HALVES or keys.get_device() != index:
-            _refuse("keys must be a float16 or bfloat16 tensor of three dimensions on the cache's device")
-        tokens = keys.shape[0]
-        shape = (tokens, self.kv_heads, self.head_dim)
-        key_address, value_address = _heads(keys, "keys", shape, keys), _heads(values, "values", shape, keys)
-        slot_address = _whole(slots, "slots", torch.int64, (tokens,), index)
-        rotated = query_address = rotated_address = position_address = cosine_address = sine_address = None
-        query_heads = query_stride = query_head_stride = table_rows = rotary = 0
-        if queries is not None:
-            if queries.dim() != 3:
-                _refuse("queries have three dimensions")
-            query_heads = queries.shape[1]
-            query_address = _heads(queries, "queries", (tokens, query_heads, self.head_dim), keys)
-            query_stride, query_head_stride = queries.stride(0), queries.stride(1)
-            rotated = torch.empty_like(queries, memory_format=torch.contiguous_format)
-            rotated_address = rotated.data_ptr()
-        if positions is not None:
-            if cosines is None or sines is None or cosines.dim() != 2:
-                _refuse("positions need rotation tables")
-            position_address = _whole(positions, "positions", torch.int32, (tokens,), index)
-            table_rows, half = table = cosines.shape
-            rotary = 2 * half
-            cosine_address = _whole(cosines, "cosines", torch.float32, table, index)
-            sine_address = _whole(sines, "sines", torch.float32, table, index)
-        status = library().nvcr_sm100_token_append(
-            self._address, _TYPES[keys.dtype], key_address, keys.stride(0), keys.stride(1), value_address,
-            values.stride(0), values.stride(1), slot_address, tokens, query_address, query_stride, query_head_stride,
-            query_heads, rotated_address, position_address, cosine_address, sine_address, table_rows, rotary,
-            interleaved, _stream(stream, index))
-        if status:
-            _check(status)
-        return rotated
+        return (_module or _native()).append(self._address, self._index, keys, values, slots, queries, positions, cosines,
+                                             sines, interleaved, None if stream is None else _stream(stream))
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16,
              stream=None) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values [n, kv_heads, head_dim] that the codes at int64 `slots` stand for (zeros outside)."""
         code = _TYPES.get(dtype)
-        if slots.dim() != 1 or code is None:
-            _refuse("slots have one dimension and dtype is a float type")
-        count = slots.shape[0]
-        slot_address = _whole(slots, "slots", torch.int64, (count,), self._index)
-        keys = torch.empty((count, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
-        values = torch.empty_like(keys)
-        status = library().nvcr_sm100_token_read(self._address, code, slot_address, count, keys.data_ptr(),
-                                                 values.data_ptr(), _stream(stream, self._index))
-        if status:
-            _check(status)
-        return keys, values
+        if code is None:
+            _refuse("dtype is a float type")
+        return (_module or _native()).read(self._address, self._index, slots, code,
+                                           None if stream is None else _stream(stream))
 
     def check(self) -> None:
         """Waits for the device and raises if a kernel met a slot, position, page number or length out of range since
@@ -265,29 +190,9 @@ class TokenContext:
         of the int32 `page_table`; its new tokens are query_offsets[b] .. query_offsets[b + 1] - 1 (int32 [batch + 1],
         at most `max_queries` each; None: token b). A token sees the places up to its own; one that sees none gives
         zeros. `scale` defaults to 1 / sqrt(head_dim)."""
-        index = cache._index
-        if queries.dim() != 3 or queries.dtype not in _HALVES or queries.get_device() != index:
-            _refuse("queries must be a float16 or bfloat16 tensor of three dimensions on the cache's device")
-        tokens, heads, dim = queries.shape
-        query_address = _heads(queries, "queries", (tokens, heads, cache.head_dim), queries)
-        if lengths.dim() != 1 or page_table.dim() != 2:
-            _refuse("lengths have one dimension and page_table two")
-        batch, columns = page_table.shape
-        if page_table.dtype is not torch.int32 or page_table.get_device() != index or lengths.shape[0] != batch \
-                or (page_table.stride(1) != 1 and columns > 1):
-            _refuse(f"page_table must be an int32 tensor of {lengths.shape[0]} rows on {cache.device} "
-                    "with contiguous rows")
-        length_address = _whole(lengths, "lengths", torch.int32, (batch,), index)
-        offset_address = None if query_offsets is None else _whole(query_offsets, "query_offsets", torch.int32,
-                                                                   (batch + 1,), index)
-        out = torch.empty_like(queries, memory_format=torch.contiguous_format)
-        status = library().nvcr_sm100_token_attend(
-            self._handle, cache._address, _TYPES[queries.dtype], query_address, queries.stride(0), queries.stride(1),
-            tokens, heads, page_table.data_ptr(), page_table.stride(0), columns, length_address, batch, offset_address,
-            max_queries, max_length, dim ** -0.5 if scale is None else scale, out.data_ptr(), _stream(stream, index))
-        if status:
-            _check(status)
-        return out
+        return (_module or _native()).attend(self._handle.value or 0, cache._address, cache._index, queries, page_table, lengths,
+                                             query_offsets, max_queries, max_length, scale,
+                                             None if stream is None else _stream(stream))
 
 
 class PackedMatrix:
@@ -310,8 +215,8 @@ class PackedMatrix:
         self.codes = torch.empty(code_bytes.value, dtype=torch.uint8, device=device)
         self.scales = torch.empty(scale_bytes.value, dtype=torch.uint8, device=device)
         self._addresses = (self.codes.data_ptr(), self.scales.data_ptr())
-        _check(library().nvcr_sm100_token_pack(*addresses, outputs, inputs, group, *self._addresses,
-                                               _stream(stream, index)))
+        handle = torch.cuda.current_stream(index).cuda_stream if stream is None else _stream(stream)
+        _check(library().nvcr_sm100_token_pack(*addresses, outputs, inputs, group, *self._addresses, handle))
 
     @classmethod
     def quantise(cls, weights: torch.Tensor, group: int = 64, stream=None) -> "PackedMatrix":
@@ -328,15 +233,5 @@ class PackedMatrix:
 
     def multiply(self, x: torch.Tensor, bias: torch.Tensor | None = None, stream=None) -> torch.Tensor:
         """x [rows, inputs] (float16 or bfloat16, any row stride) times the matrix's transpose, plus bias [outputs]."""
-        if x.dim() != 2 or x.shape[1] != self.inputs or x.dtype not in _HALVES or x.get_device() != self._index \
-                or x.stride(1) != 1:
-            _refuse(f"x must be a float16 or bfloat16 tensor of shape (rows, {self.inputs}) on {self.device} "
-                    "with contiguous rows")
-        rows = x.shape[0]
-        y = x.new_empty((rows, self.outputs))
-        status = library().nvcr_sm100_token_multiply(
-            _TYPES[x.dtype], x.data_ptr(), x.stride(0), rows, *self._addresses, self.outputs, self.inputs, self.group,
-            _channels(bias, "bias", self.outputs, x), y.data_ptr(), _stream(stream, self._index))
-        if status:
-            _check(status)
-        return y
+        return (_module or _native()).multiply(*self._addresses, self.outputs, self.inputs, self.group, self._index, x, bias,
+                                               None if stream is None else _stream(stream))
