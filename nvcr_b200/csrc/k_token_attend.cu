@@ -27,7 +27,7 @@
 // Work is cut evenly over the blocks that run at once, whatever the lengths: a
 // segment is one cache head, 8 or 16 query rows and a sequence's whole length, in
 // units of 128 keys (16 for each of eight warps); all segments' units in a row are
-// divided among the blocks. A warp streams its runs of 16 keys through a ring of
+// divided among the blocks (segments of one length alike, each among as many). A warp streams its runs of 16 keys through a ring of
 // its own in shared memory (cp.async; 16-byte chunks XOR-swizzled so that the
 // fragment reads touch every bank once) and keeps its own running maximum and
 // sum. A block joins its warps in shared memory; a segment that several blocks
@@ -44,7 +44,8 @@ constexpr int warps = 8;
 constexpr int unit = 16 * warps;  // keys
 constexpr int least_units = 4;    // of a block, on average, where segments are cut
 constexpr int join_units = 6;     // what joining a cut segment costs, in units
-constexpr int most_blocks = 512;
+constexpr int lead_units = 4;     // what starting on a segment costs
+constexpr int most_blocks = 320;
 constexpr float log2_e = 1.4426950408889634f;
 // A running maximum is raised only when a score passes it by this much (in
 // powers of two): weights stay below 2^8, and few tiles rescale their sums.
@@ -165,7 +166,6 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = lane / 4, j = lane % 4;
 
     // ---- this block's part of all the segments' units ----
-    bool whole = false;  // blocks take whole segments, each of them then one unit
     auto share_of = [&](int sequence, bool tell) {
         Share s{0, 0, 0, 0, sequence};
         int last = sequence + 1;
@@ -177,17 +177,20 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
         s.count = last - s.first;
         s.length = min(max(s.length, 0), a.max_length);
         s.blocks = (s.count * work.ratio + rows - 1) / rows;
-        s.units = whole ? 1 : max(1, (s.length + unit - 1) / unit);
+        s.units = max(1, (s.length + unit - 1) / unit);
         return s;
     };
-    const int each = (a.batch + 32 * warps - 1) / (32 * warps);  // sequences a thread counts
-    const int from = min(a.batch, static_cast<int>(threadIdx.x) * each), to = min(a.batch, from + each);
+    // Up to 32 sequences are one to a lane in every warp; more are divided among the block's threads.
+    const bool few = a.batch <= 32;
+    const int each = few ? 1 : (a.batch + 32 * warps - 1) / (32 * warps), counter = few ? lane : static_cast<int>(threadIdx.x);
+    const int from = min(a.batch, counter * each), to = min(a.batch, from + each);
+    Share own{0, 0, 0, 0, 0};  // of the last of them
     int units = 0, segments = 0, longest = 0;
     for (int b = from; b < to; ++b) {
-        const Share s = share_of(b, blockIdx.x == 0);
-        units += s.blocks * s.units * cache.kv_heads;
-        segments += s.blocks * cache.kv_heads;
-        if (s.blocks > 0) longest = max(longest, s.units);
+        own = share_of(b, blockIdx.x == 0);
+        units += own.blocks * own.units * cache.kv_heads;
+        segments += own.blocks * cache.kv_heads;
+        if (own.blocks > 0) longest = max(longest, own.units);
     }
     int units_to = units, segments_to = segments;  // become those of the threads up to this one
 #pragma unroll
@@ -197,46 +200,73 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
         if (lane >= offset) units_to += other, segments_to += others;
     }
     longest = __reduce_max_sync(0xffffffffu, longest);
-    if (lane == 31) joint_units[warp] = units_to, joint_segments[warp] = segments_to, joint_longest[warp] = longest;
-    __syncthreads();
-    int all_units = 0, all_segments = 0;
+    int all_units = __shfl_sync(0xffffffffu, units_to, 31), all_segments = __shfl_sync(0xffffffffu, segments_to, 31);
+    if (!few) {
+        if (lane == 31) joint_units[warp] = units_to, joint_segments[warp] = segments_to, joint_longest[warp] = longest;
+        __syncthreads();
+        all_units = all_segments = 0;
 #pragma unroll
-    for (int w = 0; w < warps; ++w) {
-        if (w < warp) units_to += joint_units[w], segments_to += joint_segments[w];
-        all_units += joint_units[w], all_segments += joint_segments[w];
-        longest = max(longest, joint_longest[w]);
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) units_to += joint_units[w], segments_to += joint_segments[w];
+            all_units += joint_units[w], all_segments += joint_segments[w];
+            longest = max(longest, joint_longest[w]);
+        }
     }
     // Segments are cut only where that saves more units than joining costs.
     const int grid = static_cast<int>(gridDim.x);
-    whole = (all_segments + grid - 1) / grid * longest <= max(all_units / grid, least_units) + join_units;
-    const int total = whole ? all_segments : all_units, mine = whole ? segments : units;
-    const int before = (whole ? segments_to : units_to) - mine;
-    const int blocks = max(1, min(grid, whole ? total : total / least_units));
+    const bool whole = (all_segments + grid - 1) / grid * longest <= max(all_units / grid, least_units) + join_units;
+    int blocks = max(1, min(grid, whole ? all_segments : all_units / least_units));
+    // Segments of one length are cut alike, `per` blocks each, so that none has a second piece to start on; others at
+    // any unit, the first `more` blocks having one more than `fewer`, where starting on a segment counts as `lead` units
+    // before its first. A segment that is not cut counts as one.
+    const int per = !whole && longest * all_segments == all_units && all_segments > 0 ? blocks / all_segments : 0;
+    const int lead = whole || per > 0 ? 0 : lead_units;
+    const int total = whole ? all_segments : all_units + lead * all_segments;
+    const int mine = whole ? segments : units + lead * segments;
+    const int before = (whole ? segments_to : units_to + lead * segments_to) - mine;
+    auto span_of = [&](const Share& s) { return whole ? 1 : s.units + lead; };
+    if (per > 0) blocks = per * all_segments;
     if (static_cast<int>(blockIdx.x) >= blocks) return;
-    // the first `more` blocks have one unit more than `fewer`
     const int fewer = total / blocks, more = total - fewer * blocks;
-    auto start_of = [&](int block) { return block * fewer + min(block, more); };
+    auto start_of = [&](int block) {
+        if (per > 0) return block / per * longest + block % per * longest / per;
+        return block * fewer + min(block, more);
+    };
     auto block_of = [&](int at) {
+        if (per > 0) return at / longest * per + ((at % longest + 1) * per - 1) / longest;
         const int wide = more * (fewer + 1);
         return at < wide ? at / (fewer + 1) : more + (at - wide) / fewer;
     };
     int at = start_of(blockIdx.x);
     const int stop = start_of(blockIdx.x + 1);
-    if (at >= before && at < before + mine) {
-        int start = before, b = from;
-        for (;; ++b) {
-            const Share s = share_of(b, false);
-            const int next = start + s.blocks * s.units * cache.kv_heads;
-            if (at < next) break;
-            start = next;
-        }
-        joint_sequence = b;
-        joint_before = start;
-    }
-    __syncthreads();
     if (at >= stop) return;  // no work at all
-    int sequence = joint_sequence, sequence_start = joint_before;
-    Share share = share_of(sequence, false);
+    auto share_at = [&](int sequence) {
+        if (!few) return share_of(sequence, false);
+        return Share{__shfl_sync(0xffffffffu, own.count, sequence), __shfl_sync(0xffffffffu, own.length, sequence),
+                     __shfl_sync(0xffffffffu, own.blocks, sequence), __shfl_sync(0xffffffffu, own.units, sequence),
+                     __shfl_sync(0xffffffffu, own.first, sequence)};
+    };
+    int sequence, sequence_start;
+    const bool here = at >= before && at < before + mine;
+    if (few) {
+        sequence = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+        sequence_start = __shfl_sync(0xffffffffu, before, sequence);
+    } else {
+        if (here) {
+            int start = before, b = from;
+            for (;; ++b) {
+                const Share s = share_of(b, false);
+                const int next = start + s.blocks * span_of(s) * cache.kv_heads;
+                if (at < next) break;
+                start = next;
+            }
+            joint_sequence = b;
+            joint_before = start;
+        }
+        __syncthreads();
+        sequence = joint_sequence, sequence_start = joint_before;
+    }
+    Share share = share_at(sequence);
 
     // ---- what does not change from piece to piece ----
     const unsigned ring_base = static_cast<unsigned>(__cvta_generic_to_shared(shared)) + warp * ring * run_bytes<D, G>;
@@ -268,14 +298,17 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
     const unsigned page_runs = static_cast<unsigned>(cache.page_size) / 16;
 
     while (at < stop) {
-        while (at >= sequence_start + share.blocks * share.units * cache.kv_heads) {
-            sequence_start += share.blocks * share.units * cache.kv_heads;
-            share = share_of(++sequence, false);
+        while (at >= sequence_start + share.blocks * span_of(share) * cache.kv_heads) {
+            sequence_start += share.blocks * span_of(share) * cache.kv_heads;
+            share = share_at(++sequence);
         }
-        const int segment = (at - sequence_start) / share.units;
-        const int segment_start = sequence_start + segment * share.units;
+        const int span = span_of(share), segment = (at - sequence_start) / span;
+        const int segment_start = sequence_start + segment * span;
         const int kv_head = segment / share.blocks, row_block = segment - kv_head * share.blocks;
-        const int first_unit = at - segment_start, last_unit = min(stop - segment_start, share.units);
+        const int first_unit = whole ? 0 : max(0, at - segment_start - lead);
+        const int last_unit = whole ? share.units : min(stop - segment_start, span) - lead;
+        at = segment_start + min(stop - segment_start, span);
+        if (last_unit <= first_unit) continue;  // the lead alone: the next block has the segment's first unit
         const int first = share.first, count = share.count, length = share.length;
         const int first_row = row_block * rows, total_rows = count * work.ratio;
         const int used_rows = min(rows, total_rows - first_row);
@@ -283,7 +316,29 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
         const int visible_first = max(0, length - count + static_cast<int>(divide(first_row, work.by_ratio)) + 1);
         const int visible_last =
             max(0, length - count + static_cast<int>(divide(first_row + used_rows - 1, work.by_ratio)) + 1);
-        const int end = whole ? visible_last : min(visible_last, last_unit * unit);
+        const int end = min(visible_last, last_unit * unit);
+
+        // ---- this warp's rows of the queries (w and w + 8), on their way while the pages are looked up ----
+        constexpr int per_lane = D / 32;  // channels lane * per_lane .. of a row
+        alignas(16) T query_raw[NT][per_lane];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int row = min(first_row + 8 * n + warp, total_rows - 1);
+            const int token = static_cast<int>(divide(row, work.by_ratio));
+            const T* source = static_cast<const T*>(a.queries) + static_cast<std::int64_t>(first + token) * a.query_stride +
+                static_cast<std::int64_t>(kv_head * work.ratio + row - token * work.ratio) * a.query_head_stride +
+                lane * per_lane;
+            if (!work.aligned) {
+#pragma unroll
+                for (int i = 0; i < per_lane; ++i) query_raw[n][i] = source[i];
+            } else if constexpr (per_lane == 8) {
+                *reinterpret_cast<uint4*>(query_raw[n]) = *reinterpret_cast<const uint4*>(source);
+            } else if constexpr (per_lane == 4) {
+                *reinterpret_cast<uint2*>(query_raw[n]) = *reinterpret_cast<const uint2*>(source);
+            } else {
+                *reinterpret_cast<unsigned*>(query_raw[n]) = *reinterpret_cast<const unsigned*>(source);
+            }
+        }
 
         // ---- the ring: run k of this warp holds places begin + k * unit .. + 15 ----
         const int begin = first_unit * unit + 16 * warp;
@@ -327,35 +382,12 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
         for (int s = 0; s < ring - 1; ++s) issue(s, s);
 
         // ---- the queries: warp w prepares rows w and w + 8, every warp then reads all of them as fragments ----
-        constexpr int per_lane = D / 32;  // channels lane * per_lane .. of a row
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int row = first_row + 8 * n + warp;
+            const bool used = first_row + 8 * n + warp < total_rows;
             float q[per_lane];
-            if (row < total_rows) {
-                const int token = static_cast<int>(divide(row, work.by_ratio));
-                const T* source = static_cast<const T*>(a.queries) + static_cast<std::int64_t>(first + token) * a.query_stride +
-                    static_cast<std::int64_t>(kv_head * work.ratio + row - token * work.ratio) * a.query_head_stride +
-                    lane * per_lane;
-                if (work.aligned) {
-                    alignas(16) T raw[per_lane];
-                    if constexpr (per_lane == 8) {
-                        *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(source);
-                    } else if constexpr (per_lane == 4) {
-                        *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(source);
-                    } else {
-                        *reinterpret_cast<unsigned*>(raw) = *reinterpret_cast<const unsigned*>(source);
-                    }
 #pragma unroll
-                    for (int i = 0; i < per_lane; ++i) q[i] = widen(raw[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < per_lane; ++i) q[i] = widen(source[i]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < per_lane; ++i) q[i] = 0.0f;
-            }
+            for (int i = 0; i < per_lane; ++i) q[i] = used ? widen(query_raw[n][i]) : 0.0f;
             float largest = 0.0f;
 #pragma unroll
             for (int i = 0; i < per_lane; ++i) largest = max_nan(largest, fabsf(q[i]));
@@ -694,7 +726,7 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
             *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(out);
         };
         const bool complete = first_unit == 0 && last_unit == share.units;
-        const int begin_block = complete ? 0 : block_of(segment_start);
+        const int begin_block = complete ? 0 : block_of(segment_start + lead);
         float* const part = work.partials +
             (2 * static_cast<std::int64_t>(blockIdx.x) + (static_cast<int>(blockIdx.x) == begin_block)) * partial_floats;
         const int quads = used_rows * (D / 4);
@@ -722,13 +754,16 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
 
         // ---- join the blocks of a segment: the last of them to get here ----
         if (!complete) {
-            const int pieces = block_of(segment_start + share.units - 1) - begin_block + 1;
+            const int pieces = block_of(segment_start + span - 1) - begin_block + 1;
             __syncthreads();
-            if (threadIdx.x == 0) {
-                __threadfence();
-                joint_last = atomicAdd(&work.tickets[begin_block], 1u) + 1 == static_cast<unsigned>(pieces);
+            if (threadIdx.x == 0) {  // releases the block's sums, and acquires the others'
+                unsigned before_me;
+                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
+                             : "=r"(before_me)
+                             : "l"(work.tickets + begin_block)
+                             : "memory");
+                joint_last = before_me + 1 == static_cast<unsigned>(pieces);
                 if (joint_last) work.tickets[begin_block] = 0;
-                __threadfence();
             }
             __syncthreads();
             if (joint_last) {
@@ -737,13 +772,29 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                         (2 * static_cast<std::int64_t>(begin_block + piece) + (piece == 0)) * partial_floats;
                 };
                 float* const weights = reinterpret_cast<float*>(shared);  // [piece][row]
-                float4* const sums = reinterpret_cast<float4*>(weights + most_blocks * rows);
+                float* const totals = weights + most_blocks * rows;       // [piece][row]
+                float4* const sums = reinterpret_cast<float4*>(totals + most_blocks * rows);
+                const int shares = max(1, 32 * warps / quads);  // threads that divide one quad's pieces
+                const int quad = shares > 1 ? static_cast<int>(threadIdx.x) % quads : static_cast<int>(threadIdx.x);
+                const int mine_of = shares > 1 ? static_cast<int>(threadIdx.x) / quads : 0;
+                constexpr int early = 4;  // pieces on their way before the weights are known
+                float4 first_sums[early];
+#pragma unroll
+                for (int k = 0; k < early; ++k) {
+                    const int piece = mine_of + k * shares;
+                    if (quad < quads && mine_of < shares && piece < pieces) {
+                        first_sums[k] = __ldcg(reinterpret_cast<const float4*>(part_of(piece) + quad * 4));
+                    }
+                }
                 for (int e = threadIdx.x; e < pieces * rows; e += 32 * warps) {
-                    if (e % rows < used_rows) weights[e] = __ldcg(part_of(e / rows) + rows * D + e % rows);
+                    if (e % rows < used_rows) {
+                        const float* const one = part_of(e / rows) + rows * D + e % rows;
+                        weights[e] = __ldcg(one), totals[e] = __ldcg(one + rows);
+                    }
                 }
                 __syncthreads();
                 for (int row = warp; row < used_rows; row += warps) {
-                    float most = -FLT_MAX, whole = 0.0f;
+                    float most = -FLT_MAX, whole_sum = 0.0f;
                     for (int piece = lane; piece < pieces; piece += 32) most = fmaxf(most, weights[piece * rows + row]);
 #pragma unroll
                     for (int offset = 16; offset > 0; offset /= 2) {
@@ -752,25 +803,32 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                     for (int piece = lane; piece < pieces; piece += 32) {
                         const float weight = exp2_fast(weights[piece * rows + row] - most);
                         weights[piece * rows + row] = weight;
-                        whole = fmaf(__ldcg(part_of(piece) + rows * D + rows + row), weight, whole);
+                        whole_sum = fmaf(totals[piece * rows + row], weight, whole_sum);
                     }
-                    whole = warp_sum(whole);
-                    if (lane == 0) joint_sum[0][row] = whole;
+                    whole_sum = warp_sum(whole_sum);
+                    if (lane == 0) joint_sum[0][row] = whole_sum;
                 }
                 __syncthreads();
-                const int shares = max(1, 32 * warps / quads);  // threads that divide one quad's pieces
                 for (int base = 0; base < quads; base += 32 * warps) {
-                    const int e = base + (shares > 1 ? static_cast<int>(threadIdx.x) % quads : static_cast<int>(threadIdx.x));
-                    const int mine_of = shares > 1 ? static_cast<int>(threadIdx.x) / quads : 0;
-                    const int row = e / (D / 4), d = e % (D / 4) * 4;
+                    const int e = base + quad, row = e / (D / 4), d = e % (D / 4) * 4;
                     float4 value = {0.0f, 0.0f, 0.0f, 0.0f};
+                    auto add = [&](const float4& o, int piece) {
+                        const float weight = weights[piece * rows + row];
+                        value.x = fmaf(o.x, weight, value.x), value.y = fmaf(o.y, weight, value.y);
+                        value.z = fmaf(o.z, weight, value.z), value.w = fmaf(o.w, weight, value.w);
+                    };
                     if (e < quads && mine_of < shares) {
+                        int piece = mine_of;
+                        if (base == 0) {
+#pragma unroll
+                            for (int k = 0; k < early; ++k) {
+                                if (piece < pieces) add(first_sums[k], piece);
+                                piece += shares;
+                            }
+                        }
 #pragma unroll 8
-                        for (int piece = mine_of; piece < pieces; piece += shares) {
-                            const float4 o = __ldcg(reinterpret_cast<const float4*>(part_of(piece) + row * D + d));
-                            const float weight = weights[piece * rows + row];
-                            value.x = fmaf(o.x, weight, value.x), value.y = fmaf(o.y, weight, value.y);
-                            value.z = fmaf(o.z, weight, value.z), value.w = fmaf(o.w, weight, value.w);
+                        for (; piece < pieces; piece += shares) {
+                            add(__ldcg(reinterpret_cast<const float4*>(part_of(piece) + row * D + d)), piece);
                         }
                     }
                     if (shares > 1) {
@@ -785,7 +843,6 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                 }
             }
         }
-        at = segment_start + last_unit;
         __syncthreads();  // before the next piece's copies
     }
 }
@@ -793,7 +850,7 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
 template <typename T, int D, int G, int NT>
 cudaError_t launch(Work& work, cudaStream_t stream) {
     constexpr int bytes = shared_bytes<D, G, NT>;
-    static_assert(bytes >= most_blocks * 8 * NT * 4 + 32 * warps * 16, "the blocks' join fits the ring");
+    static_assert(bytes >= 2 * most_blocks * 8 * NT * 4 + 32 * warps * 16, "the blocks' join fits the ring");
     static SharedAllowance allowance;
     const cudaError_t allowed = allowance.allow(attend_kernel<T, D, G, NT>, bytes);
     if (allowed != cudaSuccess) return allowed;
