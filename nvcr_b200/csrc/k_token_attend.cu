@@ -24,14 +24,26 @@
 // after scaling to the group's largest scale so far, as a 16-bit operand must.
 // Scores, softmax statistics and sums are FP32.
 //
-// Work is cut evenly over the blocks that run at once, whatever the lengths: a
-// segment is one cache head, 8 or 16 query rows and a sequence's whole length, in
-// units of 128 keys (16 for each of eight warps); all segments' units in a row are
-// divided among the blocks (segments of one length alike, each among as many). A warp streams its runs of 16 keys through a ring of
-// its own in shared memory (cp.async; 16-byte chunks XOR-swizzled so that the
-// fragment reads touch every bank once) and keeps its own running maximum and
-// sum. A block joins its warps in shared memory; a segment that several blocks
-// share is joined in the context's workspace by the last of them, in order.
+// Work is cut evenly over the blocks, one an SM, whatever the lengths: a segment is
+// one cache head, 8 or 16 query rows and a sequence's whole length, in units of 256
+// or 128 keys (two runs of 16, or one, for each of eight warps); all segments' units
+// in a row are divided among the blocks (segments of one length alike, each among
+// as many), or taken whole where a cut saves less than its join costs. A warp
+// streams its runs through a ring of its own in shared memory (cp.async; 16-byte
+// chunks XOR-swizzled so that the fragment reads touch every bank once) and keeps
+// its own running maximum and sum; the next piece's copies and queries are on
+// their way while a piece is joined. A block joins its warps in shared memory; a
+// segment that several blocks share is joined in the context's workspace by the
+// last of them, in order: the same bits every time.
+//
+// Measured on a B200: 131072 keys, 32 heads over 8 of 128 channels, one token
+// (142.6 MB): 47.4 us, 3.0 TB/s; 32 sequences of 1 to 4096 keys (76 MB): 35.1 us; 200
+// keys: 5.5 us. What bounds a long stream is the integer pipe that takes the
+// codes apart (168 of 327 instructions a run of 16 keys, at half rate) and the
+// warps' latency: 141 cycles a run an SM, 109 without the values' conversion. Two
+// blocks an SM with 128 registers a thread took 135 cycles a run, but twice the
+// fixed work: 6.3 us for 200 keys. Short calls are bound by the chain lengths -> page
+// table -> cache -> join, about 1 us a link.
 #include "token_elements.cuh"
 
 #include <algorithm>
@@ -41,11 +53,10 @@ namespace nvcr_sm100::token {
 namespace {
 
 constexpr int warps = 8;
-constexpr int unit = 16 * warps;  // keys
-constexpr int least_units = 4;    // of a block, on average, where segments are cut
-constexpr int join_units = 6;     // what joining a cut segment costs, in units
-constexpr int lead_units = 4;     // what starting on a segment costs
-constexpr int most_blocks = 320;
+// In keys: the least a block takes on average where segments are cut, what joining a cut segment costs, and what
+// starting on one costs.
+constexpr int least_keys = 512, join_keys = 768, lead_keys = 512;
+constexpr int most_blocks = 160;
 constexpr float log2_e = 1.4426950408889634f;
 // A running maximum is raised only when a score passes it by this much (in
 // powers of two): weights stay below 2^8, and few tiles rescale their sums.
@@ -130,16 +141,28 @@ __device__ __forceinline__ int swizzle(int t) {
 template <int D, int G>
 constexpr int run_bytes = 16 * (D + 8 * (D / G));
 
-// Runs in a warp's ring: two blocks an SM fit its shared memory.
-template <int D>
-constexpr int ring_runs = D == 64 ? 6 : D == 128 ? 5 : 3;
+// Runs of 16 keys a warp takes at once: two share a warp's control, copies and vote, where the registers allow.
+template <int D, int NT>
+constexpr int together = NT == 1 && D < 256 ? 2 : 1;
+
+// Slots of that many runs in a warp's ring.
+template <int D, int G, int NT>
+constexpr int ring_slots = together<D, NT> == 2 ? (D == 128 && G == 32 ? 2 : 3) : D == 256 ? 3 : 4;
 
 template <int D, int G, int NT>
-constexpr int shared_bytes = std::max(warps * ring_runs<D> * run_bytes<D, G>, warps * 8 * NT * (D + 4) * 4);
+constexpr int shared_bytes = warps * (ring_slots<D, G, NT> * together<D, NT> * run_bytes<D, G> + 8 * NT * (D + 4) * 4);
 
-// Blocks an SM: the sums of 16 rows of 128 channels, or 8 of 256, take the registers of one.
-template <int D, int NT>
-constexpr int resident = D * NT >= 256 ? 1 : 2;
+// What a block takes of one segment.
+struct Piece {
+    int segment_start, segment_end;  // in the row of all segments
+    int first_unit, last_unit;
+    int kv_head, first, before;      // `first` of the sequence's new tokens, which are at positions `before` and on
+    int first_row, total_rows, used_rows;
+    int visible_first, visible_last; // keys that the first and the last row see
+    int begin, end, steps;           // this warp's places
+    const std::int32_t* table;
+    bool complete;
+};
 
 // The units of one sequence: `blocks` blocks of rows times `units` of each segment.
 struct Share {
@@ -148,8 +171,11 @@ struct Share {
 };
 
 template <typename T, int D, int G, int NT>
-__global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(const Work work) {
-    constexpr int groups = D / G, rows = 8 * NT, ring = ring_runs<D>;
+__global__ void __launch_bounds__(32 * warps) attend_kernel(const Work work) {
+    constexpr int groups = D / G, rows = 8 * NT, H = together<D, NT>, ring = ring_slots<D, G, NT>;
+    constexpr int unit = 16 * H * warps, slot_bytes = H * run_bytes<D, G>;  // unit: keys
+    constexpr int least_units = (least_keys + unit - 1) / unit, join_units = (join_keys + unit - 1) / unit;
+    constexpr int lead_units = (lead_keys + unit - 1) / unit;
     constexpr int row_bytes = D / 2, chunks = row_bytes / 16;
     constexpr int words = G / 32;  // 32-bit words of codes a lane holds of a group of one key
     constexpr int tiles = G / 16;  // 16-channel tiles of a group
@@ -269,8 +295,8 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
     Share share = share_at(sequence);
 
     // ---- what does not change from piece to piece ----
-    const unsigned ring_base = static_cast<unsigned>(__cvta_generic_to_shared(shared)) + warp * ring * run_bytes<D, G>;
-    const std::uint8_t* const ring_bytes = shared + warp * ring * run_bytes<D, G>;
+    const unsigned ring_base = static_cast<unsigned>(__cvta_generic_to_shared(shared)) + warp * ring * slot_bytes;
+    const std::uint8_t* const ring_bytes = shared + warp * ring * slot_bytes;
     const int my_key = row_key(r);                // score rows my_key and my_key + 8 of a run
     const int pair_key = (j & 1) | (j & 2) << 1;  // value keys pair_key and pair_key + 2, and 8 on
     int key_offset[groups], value_offset[groups][2];
@@ -297,71 +323,63 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
     const unsigned scale_to = ring_base + 16 * D + lane * 16;
     const unsigned page_runs = static_cast<unsigned>(cache.page_size) / 16;
 
-    while (at < stop) {
-        while (at >= sequence_start + share.blocks * span_of(share) * cache.kv_heads) {
-            sequence_start += share.blocks * span_of(share) * cache.kv_heads;
-            share = share_at(++sequence);
-        }
-        const int span = span_of(share), segment = (at - sequence_start) / span;
-        const int segment_start = sequence_start + segment * span;
-        const int kv_head = segment / share.blocks, row_block = segment - kv_head * share.blocks;
-        const int first_unit = whole ? 0 : max(0, at - segment_start - lead);
-        const int last_unit = whole ? share.units : min(stop - segment_start, span) - lead;
-        at = segment_start + min(stop - segment_start, span);
-        if (last_unit <= first_unit) continue;  // the lead alone: the next block has the segment's first unit
-        const int first = share.first, count = share.count, length = share.length;
-        const int first_row = row_block * rows, total_rows = count * work.ratio;
-        const int used_rows = min(rows, total_rows - first_row);
-        // keys that the block's first and last row see
-        const int visible_first = max(0, length - count + static_cast<int>(divide(first_row, work.by_ratio)) + 1);
-        const int visible_last =
-            max(0, length - count + static_cast<int>(divide(first_row + used_rows - 1, work.by_ratio)) + 1);
-        const int end = min(visible_last, last_unit * unit);
-
-        // ---- this warp's rows of the queries (w and w + 8), on their way while the pages are looked up ----
-        constexpr int per_lane = D / 32;  // channels lane * per_lane .. of a row
-        alignas(16) T query_raw[NT][per_lane];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int row = min(first_row + 8 * n + warp, total_rows - 1);
-            const int token = static_cast<int>(divide(row, work.by_ratio));
-            const T* source = static_cast<const T*>(a.queries) + static_cast<std::int64_t>(first + token) * a.query_stride +
-                static_cast<std::int64_t>(kv_head * work.ratio + row - token * work.ratio) * a.query_head_stride +
-                lane * per_lane;
-            if (!work.aligned) {
-#pragma unroll
-                for (int i = 0; i < per_lane; ++i) query_raw[n][i] = source[i];
-            } else if constexpr (per_lane == 8) {
-                *reinterpret_cast<uint4*>(query_raw[n]) = *reinterpret_cast<const uint4*>(source);
-            } else if constexpr (per_lane == 4) {
-                *reinterpret_cast<uint2*>(query_raw[n]) = *reinterpret_cast<const uint2*>(source);
-            } else {
-                *reinterpret_cast<unsigned*>(query_raw[n]) = *reinterpret_cast<const unsigned*>(source);
+    // ---- pieces of segments: the copies and queries of the next one are on their way while one is joined ----
+    Piece feed;  // the piece whose copies go on
+    auto advance = [&] {
+        while (at < stop) {
+            while (at >= sequence_start + share.blocks * span_of(share) * cache.kv_heads) {
+                sequence_start += share.blocks * span_of(share) * cache.kv_heads;
+                share = share_at(++sequence);
             }
+            const int span = span_of(share), segment = (at - sequence_start) / span;
+            feed.segment_start = sequence_start + segment * span;
+            feed.segment_end = feed.segment_start + span;
+            feed.kv_head = segment / share.blocks;
+            feed.first_unit = whole ? 0 : max(0, at - feed.segment_start - lead);
+            feed.last_unit = whole ? share.units : min(stop - feed.segment_start, span) - lead;
+            feed.complete = feed.first_unit == 0 && feed.last_unit == share.units;
+            at = feed.segment_start + min(stop - feed.segment_start, span);
+            if (feed.last_unit <= feed.first_unit) continue;  // the lead alone: the next block has the first unit
+            feed.first = share.first, feed.before = share.length - share.count;
+            feed.first_row = (segment - feed.kv_head * share.blocks) * rows;
+            feed.total_rows = share.count * work.ratio;
+            feed.used_rows = min(rows, feed.total_rows - feed.first_row);
+            // keys that the block's first and last row see
+            feed.visible_first = max(0, feed.before + static_cast<int>(divide(feed.first_row, work.by_ratio)) + 1);
+            feed.visible_last =
+                max(0, feed.before + static_cast<int>(divide(feed.first_row + feed.used_rows - 1, work.by_ratio)) + 1);
+            feed.end = min(feed.visible_last, feed.last_unit * unit);
+            feed.begin = feed.first_unit * unit + 16 * H * warp;
+            feed.steps = feed.end > feed.begin ? (feed.end - feed.begin + unit - 1) / unit : 0;
+            feed.table = a.page_table + sequence * a.table_stride;
+            return true;
         }
-
-        // ---- the ring: run k of this warp holds places begin + k * unit .. + 15 ----
-        const int begin = first_unit * unit + 16 * warp;
-        const int runs = end > begin ? (end - begin + unit - 1) / unit : 0;
-        const std::int32_t* const table = a.page_table + sequence * a.table_stride;
-        int ahead = 0;     // lane l: where run l of the next 32 to copy lies, in runs of 16 places; -1 without a page
-        unsigned bad = 0;  // bit: a slot of the ring whose run has no page
-        auto look_ahead = [&](int run) {
-            if (run + lane >= runs) return;
-            const unsigned index = static_cast<unsigned>(begin + (run + lane) * unit) / 16;
-            const unsigned column = divide(index, work.runs_per_page);
-            const int page = table[column];
-            const bool good = page >= 0 && page < cache.pages;
-            if (!good) note(cache, status_page);
-            ahead = good ? static_cast<int>((page * cache.kv_heads + kv_head) * page_runs + (index - column * page_runs)) : -1;
-        };
-        auto issue = [&](int run, int slot) {
-            if (run < runs) {
-                if (run % 32 == 0) look_ahead(run);
-                const int place = __shfl_sync(0xffffffffu, ahead, run % 32);
-                bad = (bad & ~(1u << slot)) | static_cast<unsigned>(place < 0) << slot;
+        return false;
+    };
+    // The ring: step k of this warp takes places begin + k * unit .. + 16 H - 1, H runs of 16.
+    int ahead = 0;     // lane l: where run l of the next 32 to copy lies, in runs of 16 places; -1 without a page
+    unsigned bad = 0;  // bits: runs of the ring without a page, or past the end
+    auto look_ahead = [&](int step) {
+        const int place = feed.begin + (step + lane / H) * unit + lane % H * 16;
+        ahead = -1;
+        if (place >= feed.end) return;
+        const unsigned index = static_cast<unsigned>(place) / 16;
+        const unsigned column = divide(index, work.runs_per_page);
+        const int page = feed.table[column];
+        const bool good = page >= 0 && page < cache.pages;
+        if (!good) note(cache, status_page);
+        if (good) ahead = static_cast<int>((page * cache.kv_heads + feed.kv_head) * page_runs + (index - column * page_runs));
+    };
+    auto issue = [&](int step, int slot) {
+        if (step < feed.steps) {
+            if (step % (32 / H) == 0) look_ahead(step);
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const int place = __shfl_sync(0xffffffffu, ahead, step % (32 / H) * H + h);
+                const unsigned bit = 1u << (slot * H + h);
+                bad = place < 0 ? bad | bit : bad & ~bit;
                 if (place >= 0) {
-                    const unsigned slot_at = slot * run_bytes<D, G>;
+                    const unsigned slot_at = slot * slot_bytes + h * run_bytes<D, G>;
                     const std::uint8_t* keys = key_source + static_cast<std::int64_t>(place) * (16 * row_bytes);
                     const std::uint8_t* values = value_source + static_cast<std::int64_t>(place) * (16 * row_bytes);
 #pragma unroll
@@ -376,15 +394,44 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                     }
                 }
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    constexpr int per_lane = D / 32;  // channels lane * per_lane .. of a row of the queries
+    constexpr int own_rows = (rows + warps - 1) / warps;
+    alignas(16) T query_raw[own_rows][per_lane];  // this warp's rows, w and w + warps
+    auto start = [&] {
+#pragma unroll
+        for (int n = 0; n < own_rows; ++n) {
+            const int row = min(feed.first_row + warps * n + warp, feed.total_rows - 1);
+            const int token = static_cast<int>(divide(row, work.by_ratio));
+            const T* source = static_cast<const T*>(a.queries) + static_cast<std::int64_t>(feed.first + token) * a.query_stride +
+                static_cast<std::int64_t>(feed.kv_head * work.ratio + row - token * work.ratio) * a.query_head_stride +
+                lane * per_lane;
+            if (!work.aligned) {
+#pragma unroll
+                for (int i = 0; i < per_lane; ++i) query_raw[n][i] = source[i];
+            } else if constexpr (per_lane == 8) {
+                *reinterpret_cast<uint4*>(query_raw[n]) = *reinterpret_cast<const uint4*>(source);
+            } else if constexpr (per_lane == 4) {
+                *reinterpret_cast<uint2*>(query_raw[n]) = *reinterpret_cast<const uint2*>(source);
+            } else {
+                *reinterpret_cast<unsigned*>(query_raw[n]) = *reinterpret_cast<const unsigned*>(source);
+            }
+        }
 #pragma unroll
         for (int s = 0; s < ring - 1; ++s) issue(s, s);
-
-        // ---- the queries: warp w prepares rows w and w + 8, every warp then reads all of them as fragments ----
+    };
+    if (!advance()) return;
+    start();
+    for (;;) {
+        const Piece now = feed;
+        // ---- the queries: each warp prepares its rows, every warp then reads all of them as fragments ----
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const bool used = first_row + 8 * n + warp < total_rows;
+        for (int n = 0; n < own_rows; ++n) {
+            const int in_block = warps * n + warp;
+            if (in_block >= rows) break;
+            const bool used = now.first_row + in_block < now.total_rows;
             float q[per_lane];
 #pragma unroll
             for (int i = 0; i < per_lane; ++i) q[i] = used ? widen(query_raw[n][i]) : 0.0f;
@@ -406,15 +453,15 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                 const int channel = lane * per_lane + i, g = channel / G, in_group = channel % G;
                 const int to_j = in_group / (G / 4), w = in_group % (G / 4) / 8, at_place = in_group % 8;
                 const int odd = at_place & 1, reg = at_place >> 1 & 1, high = at_place >> 2;
-                joint_query[n][((g * words + w) * 32 + warp * 4 + to_j) * 8 + odd * 4 + reg * 2 + high] =
+                joint_query[in_block / 8][((g * words + w) * 32 + in_block % 8 * 4 + to_j) * 8 + odd * 4 + reg * 2 + high] =
                     __float2half_rn(odd ? v * 0.0625f : v);
             }
 #pragma unroll
             for (int offset = 1; offset < G / per_lane; offset *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
             // the codes' 2^-24 goes into the group's sum as well
-            if (lane % (G / per_lane) == 0) joint_query_sum[8 * n + warp][lane / (G / per_lane)] = sum * 0x1p-24f;
+            if (lane % (G / per_lane) == 0) joint_query_sum[in_block][lane / (G / per_lane)] = sum * 0x1p-24f;
             if (lane == 0) {
-                joint_factor[8 * n + warp] =
+                joint_factor[in_block] =
                     __uint_as_float(static_cast<unsigned>(exponent - 12) << 23) * 0x1p24f * (a.scale * log2_e);
             }
         }
@@ -438,10 +485,10 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 factor[n][i] = joint_factor[8 * n + 2 * j + i];
-                const int column = first_row + 8 * n + 2 * j + i;
-                visible[n][i] = column < total_rows
-                    ? length - count + static_cast<int>(divide(column, work.by_ratio)) + 1
-                    : visible_last;
+                const int column = now.first_row + 8 * n + 2 * j + i;
+                visible[n][i] = column < now.total_rows
+                    ? now.before + static_cast<int>(divide(column, work.by_ratio)) + 1
+                    : now.visible_last;
             }
         }
 
@@ -467,100 +514,120 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
             }
         }
 
-        // A run of 16 keys. `edge`: some of them are hidden from some rows, or hold nothing (`absent`: all).
-        auto process = [&](const std::uint8_t* codes, int place, bool edge, bool absent) {
-            const std::uint8_t* key_scales = codes + 16 * D;
-            const std::uint8_t* value_scales = key_scales + 64 * groups;
-            float x[NT][4];
+        // A step's H runs of 16 keys. `edge`: some keys are hidden from some rows, or hold nothing (a bit of `absent`: a
+        // whole run).
+        auto process = [&](const std::uint8_t* slot_codes, int place, bool edge, unsigned absent) {
+            float x[H][NT][4];
+            auto scores = [&](int h) {
+                const std::uint8_t* const codes = slot_codes + h * run_bytes<D, G>;
+                const std::uint8_t* const key_scales = codes + 16 * D;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+                for (int n = 0; n < NT; ++n) x[h][n][0] = x[h][n][1] = x[h][n][2] = x[h][n][3] = 0.0f;
 #pragma unroll
-            for (int g = 0; g < groups; ++g) {
-                unsigned near[words], far[words];
-                const std::uint8_t* from_key = codes + key_offset[g];
-                if constexpr (words == 4) {
-                    *reinterpret_cast<uint4*>(near) = *reinterpret_cast<const uint4*>(from_key);
-                    *reinterpret_cast<uint4*>(far) = *reinterpret_cast<const uint4*>(from_key + 8 * row_bytes);
-                } else if constexpr (words == 2) {
-                    *reinterpret_cast<uint2*>(near) = *reinterpret_cast<const uint2*>(from_key);
-                    *reinterpret_cast<uint2*>(far) = *reinterpret_cast<const uint2*>(from_key + 8 * row_bytes);
-                } else {
-                    near[0] = *reinterpret_cast<const unsigned*>(from_key);
-                    far[0] = *reinterpret_cast<const unsigned*>(from_key + 8 * row_bytes);
-                }
-                float dot[2][NT][4];  // of the even and of the odd places, two chains
+                for (int g = 0; g < groups; ++g) {
+                    unsigned near[words], far[words];
+                    const std::uint8_t* from_key = codes + key_offset[g];
+                    if constexpr (words == 4) {
+                        *reinterpret_cast<uint4*>(near) = *reinterpret_cast<const uint4*>(from_key);
+                        *reinterpret_cast<uint4*>(far) = *reinterpret_cast<const uint4*>(from_key + 8 * row_bytes);
+                    } else if constexpr (words == 2) {
+                        *reinterpret_cast<uint2*>(near) = *reinterpret_cast<const uint2*>(from_key);
+                        *reinterpret_cast<uint2*>(far) = *reinterpret_cast<const uint2*>(from_key + 8 * row_bytes);
+                    } else {
+                        near[0] = *reinterpret_cast<const unsigned*>(from_key);
+                        far[0] = *reinterpret_cast<const unsigned*>(from_key + 8 * row_bytes);
+                    }
+                    float dot[2][NT][4];  // of the even and of the odd places, two chains
 #pragma unroll
-                for (int w = 0; w < words; ++w) {
-                    const unsigned near8 = near[w] >> 8, far8 = far[w] >> 8;
-                    const unsigned even[4] = {near[w] & 0x000f000fu, far[w] & 0x000f000fu, near8 & 0x000f000fu,
-                                              far8 & 0x000f000fu};
-                    const unsigned odd[4] = {near[w] & 0x00f000f0u, far[w] & 0x00f000f0u, near8 & 0x00f000f0u,
-                                             far8 & 0x00f000f0u};
+                    for (int w = 0; w < words; ++w) {
+                        const unsigned near8 = near[w] >> 8, far8 = far[w] >> 8;
+                        const unsigned even[4] = {near[w] & 0x000f000fu, far[w] & 0x000f000fu, near8 & 0x000f000fu,
+                                                  far8 & 0x000f000fu};
+                        const unsigned odd[4] = {near[w] & 0x00f000f0u, far[w] & 0x00f000f0u, near8 & 0x00f000f0u,
+                                                 far8 & 0x00f000f0u};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            if (w == 0) {
+                                mma_from_zero(dot[0][n], even, query[g][w][0][0][n], query[g][w][0][1][n]);
+                                mma_from_zero(dot[1][n], odd, query[g][w][1][0][n], query[g][w][1][1][n]);
+                            } else {
+                                mma(dot[0][n], even, query[g][w][0][0][n], query[g][w][0][1][n]);
+                                mma(dot[1][n], odd, query[g][w][1][0][n], query[g][w][1][1][n]);
+                            }
+                        }
+                    }
+                    const float2 pair_near = pair_at(key_scales, (my_key * groups + g) * 4);
+                    const float2 pair_far = pair_at(key_scales, ((my_key + 8) * groups + g) * 4);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        if (w == 0) {
-                            mma_from_zero(dot[0][n], even, query[g][w][0][0][n], query[g][w][0][1][n]);
-                            mma_from_zero(dot[1][n], odd, query[g][w][1][0][n], query[g][w][1][1][n]);
-                        } else {
-                            mma(dot[0][n], even, query[g][w][0][0][n], query[g][w][0][1][n]);
-                            mma(dot[1][n], odd, query[g][w][1][0][n], query[g][w][1][1][n]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            x[h][n][i] = fmaf(pair_near.x, dot[0][n][i] + dot[1][n][i],
+                                              fmaf(pair_near.y, query_sum[g][n][i], x[h][n][i]));
+                            x[h][n][i + 2] = fmaf(pair_far.x, dot[0][n][i + 2] + dot[1][n][i + 2],
+                                                  fmaf(pair_far.y, query_sum[g][n][i], x[h][n][i + 2]));
                         }
                     }
                 }
-                const float2 pair_near = pair_at(key_scales, (my_key * groups + g) * 4);
-                const float2 pair_far = pair_at(key_scales, ((my_key + 8) * groups + g) * 4);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        x[n][i] = fmaf(pair_near.x, dot[0][n][i] + dot[1][n][i],
-                                       fmaf(pair_near.y, query_sum[g][n][i], x[n][i]));
-                        x[n][i + 2] = fmaf(pair_far.x, dot[0][n][i + 2] + dot[1][n][i + 2],
-                                           fmaf(pair_far.y, query_sum[g][n][i], x[n][i + 2]));
-                    }
+                    for (int i = 0; i < 4; ++i) x[h][n][i] *= factor[n][i & 1];
                 }
-            }
-            float2 value_near[groups], value_far[groups];
+            };
+#pragma unroll
+            for (int h = 0; h < H; ++h) scores(h);
+            // Values' pairs (scale, minimum) of keys my_key and my_key + 8; places past the block's last visible key are no
+            // one's, whatever they hold.
+            auto value_pair = [&](int h, int far, int g) {
+                const int key = my_key + 8 * far;
+                float2 pair = pair_at(slot_codes + h * run_bytes<D, G> + 16 * D + 64 * groups, (key * groups + g) * 4);
+                if (edge && ((absent >> h & 1u) != 0 || place + 16 * h + key >= now.end)) pair = {0.0f, 0.0f};
+                return pair;
+            };
             bool raise = false;
+            float largest[groups];
 #pragma unroll
             for (int g = 0; g < groups; ++g) {
-                value_near[g] = pair_at(value_scales, (my_key * groups + g) * 4);
-                value_far[g] = pair_at(value_scales, ((my_key + 8) * groups + g) * 4);
-            }
+                largest[g] = 0.0f;  // an infinite scale raises nothing
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+                for (int h = 0; h < H; ++h) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[n][i] *= factor[n][i & 1];
+                    for (int far = 0; far < 2; ++far) largest[g] = fmaxf(largest[g], value_pair(h, far, g).x);
+                }
+                raise |= largest[g] > value_top[g];
             }
             if (edge) {
-                const int last = absent ? 0 : end - place;  // places from here on are no one's
 #pragma unroll
-                for (int g = 0; g < groups; ++g) {
-                    if (my_key >= last) value_near[g] = {0.0f, 0.0f};
-                    if (my_key + 8 >= last) value_far[g] = {0.0f, 0.0f};
-                }
+                for (int h = 0; h < H; ++h) {
+                    const int last = (absent >> h & 1u) != 0 ? 0 : now.end - place - 16 * h;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
+                    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = my_key + (i & 2) * 4;
-                        if (key >= last || place + key >= visible[n][i & 1]) x[n][i] = -INFINITY;
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = my_key + (i & 2) * 4;
+                            if (key >= last || place + 16 * h + key >= visible[n][i & 1]) x[h][n][i] = -INFINITY;
+                        }
                     }
                 }
             }
-#pragma unroll
-            for (int g = 0; g < groups; ++g) raise |= fmaxf(value_near[g].x, value_far[g].x) > value_top[g];
+            float most_of[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) raise |= fmaxf(x[n][i], x[n][i + 2]) > limit[n][i];
+                for (int i = 0; i < 2; ++i) {
+                    most_of[n][i] = fmaxf(x[0][n][i], x[0][n][i + 2]);
+#pragma unroll
+                    for (int h = 1; h < H; ++h) most_of[n][i] = fmaxf(most_of[n][i], fmaxf(x[h][n][i], x[h][n][i + 2]));
+                    raise |= most_of[n][i] > limit[n][i];
+                }
             }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float most = fmaxf(x[n][i], x[n][i + 2]);
+                        float most = most_of[n][i];
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
@@ -578,10 +645,9 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                     }
                 }
 #pragma unroll
-                for (int g = 0; g < groups; ++g) {  // an infinite scale raises nothing
-                    float most = fmaxf(value_near[g].x < INFINITY ? value_near[g].x : 0.0f,
-                                       value_far[g].x < INFINITY ? value_far[g].x : 0.0f);
-                    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(most, 0.0f))));
+                for (int g = 0; g < groups; ++g) {
+                    const float finite = largest[g] < INFINITY ? largest[g] : 0.0f;
+                    const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(finite)));
                     if (most > value_top[g]) {  // the power of two above it becomes 2^6
                         const unsigned exponent = (__float_as_uint(most) >> 23) + 1;
                         value_top[g] = __uint_as_float(exponent << 23);
@@ -599,88 +665,95 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                     }
                 }
             }
-            float p[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) p[n][i] = exp2_fast(x[n][i] - top[n][i & 1]);
-                sum[n][0] += p[n][0] + p[n][2];
-                sum[n][1] += p[n][1] + p[n][3];
-            }
-            const std::uint8_t* values = codes + 16 * row_bytes;
-#pragma unroll
-            for (int g = 0; g < groups; ++g) {
-                unsigned b[NT][2];
-                const float near_scale = value_near[g].x * value_factor[g], far_scale = value_far[g].x * value_factor[g];
-                const float near_middle = fmaf(8.0f, value_near[g].x, value_near[g].y);
-                const float far_middle = fmaf(8.0f, value_far[g].x, value_far[g].y);
+            auto accumulate = [&](int h) {
+                const std::uint8_t* const values = slot_codes + h * run_bytes<D, G> + 16 * row_bytes;
+                float p[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float w[4], m[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        w[i] = p[n][i] * (i < 2 ? near_scale : far_scale);
-                        m[i] = i < 2 ? near_middle : far_middle;
-                    }
-                    if (edge) {  // a hidden key's weight is 0 even against a scale that is no number
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (x[n][i] == -INFINITY) w[i] = m[i] = 0.0f;
-                        }
-                    }
-                    low[g][n][0] = fmaf(p[n][0], m[0], fmaf(p[n][2], m[2], low[g][n][0]));
-                    low[g][n][1] = fmaf(p[n][1], m[1], fmaf(p[n][3], m[3], low[g][n][1]));
-                    b[n][0] = transpose8x8(pack_half(w[0], w[1]));
-                    b[n][1] = transpose8x8(pack_half(w[2], w[3]));
-                }
-                // the lane's channels of four keys: 4 codes of each (halves), 8 (a word) or 16 (two words)
-                constexpr int value_words = G == 128 ? 2 : 1;
-                unsigned code[4][value_words];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const std::uint8_t* from_value = values + value_offset[g][k & 1] + (k & 2) * 4 * row_bytes;
-                    if constexpr (G == 128) {
-                        *reinterpret_cast<uint2*>(code[k]) = *reinterpret_cast<const uint2*>(from_value);
-                    } else if constexpr (G == 64) {
-                        code[k][0] = *reinterpret_cast<const unsigned*>(from_value);
-                    } else {
-                        code[k][0] = *reinterpret_cast<const std::uint16_t*>(from_value);
-                    }
+                    for (int i = 0; i < 4; ++i) p[n][i] = exp2_fast(x[h][n][i] - top[n][i & 1]);
+                    sum[n][0] += p[n][0] + p[n][2];
+                    sum[n][1] += p[n][1] + p[n][3];
                 }
 #pragma unroll
-                for (int t = 0; t < tiles; t += 2) {
-                    const int w = t / 4;
-                    const unsigned select = t % 4 == 0 ? 0x5410u : 0x7632u;
-                    const unsigned one = __byte_perm(code[0][w], code[1][w], select);
-                    const unsigned two = __byte_perm(code[2][w], code[3][w], select);
-                    const unsigned front[4] = {even_codes(one), odd_codes(one), even_codes(two), odd_codes(two)};
-                    const unsigned back[4] = {even_codes(one >> 8), odd_codes(one >> 8), even_codes(two >> 8),
-                                              odd_codes(two >> 8)};
+                for (int g = 0; g < groups; ++g) {
+                    unsigned b[NT][2];
+                    const float2 near_pair = value_pair(h, 0, g), far_pair = value_pair(h, 1, g);
+                    const float near_scale = near_pair.x * value_factor[g], far_scale = far_pair.x * value_factor[g];
+                    const float near_middle = fmaf(8.0f, near_pair.x, near_pair.y);
+                    const float far_middle = fmaf(8.0f, far_pair.x, far_pair.y);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        mma(acc[g][t][n], front, b[n][0], b[n][1]);
-                        mma(acc[g][t + 1][n], back, b[n][0], b[n][1]);
+                        float w[4], m[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            w[i] = p[n][i] * (i < 2 ? near_scale : far_scale);
+                            m[i] = i < 2 ? near_middle : far_middle;
+                        }
+                        if (edge) {  // a hidden key's weight is 0 even against a scale that is no number
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (x[h][n][i] == -INFINITY) w[i] = m[i] = 0.0f;
+                            }
+                        }
+                        low[g][n][0] = fmaf(p[n][0], m[0], fmaf(p[n][2], m[2], low[g][n][0]));
+                        low[g][n][1] = fmaf(p[n][1], m[1], fmaf(p[n][3], m[3], low[g][n][1]));
+                        b[n][0] = transpose8x8(pack_half(w[0], w[1]));
+                        b[n][1] = transpose8x8(pack_half(w[2], w[3]));
+                    }
+                    // the lane's channels of four keys: 4 codes of each (halves), 8 (a word) or 16 (two words)
+                    constexpr int value_words = G == 128 ? 2 : 1;
+                    unsigned code[4][value_words];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const std::uint8_t* from_value = values + value_offset[g][k & 1] + (k & 2) * 4 * row_bytes;
+                        if constexpr (G == 128) {
+                            *reinterpret_cast<uint2*>(code[k]) = *reinterpret_cast<const uint2*>(from_value);
+                        } else if constexpr (G == 64) {
+                            code[k][0] = *reinterpret_cast<const unsigned*>(from_value);
+                        } else {
+                            code[k][0] = *reinterpret_cast<const std::uint16_t*>(from_value);
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < tiles; t += 2) {
+                        const int w = t / 4;
+                        const unsigned select = t % 4 == 0 ? 0x5410u : 0x7632u;
+                        const unsigned one = __byte_perm(code[0][w], code[1][w], select);
+                        const unsigned two = __byte_perm(code[2][w], code[3][w], select);
+                        const unsigned front[4] = {even_codes(one), odd_codes(one), even_codes(two), odd_codes(two)};
+                        const unsigned back[4] = {even_codes(one >> 8), odd_codes(one >> 8), even_codes(two >> 8),
+                                                  odd_codes(two >> 8)};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma(acc[g][t][n], front, b[n][0], b[n][1]);
+                            mma(acc[g][t + 1][n], back, b[n][0], b[n][1]);
+                        }
                     }
                 }
-            }
+            };
+#pragma unroll
+            for (int h = 0; h < H; ++h) accumulate(h);
         };
 
-        for (int run = 0, slot = 0; run < runs; ++run) {
+        const int edge_from = min(now.visible_first, now.end) - 16 * H;  // steps that start after it have an edge
+        for (int step = 0, slot = 0; step < now.steps; ++step) {
             asm volatile("cp.async.wait_group %0;" ::"n"(ring - 2) : "memory");
-            __syncwarp();
-            const int place = begin + run * unit;
-            const std::uint8_t* codes = ring_bytes + slot * run_bytes<D, G>;
-            const bool absent = bad >> slot & 1u;
-            process(codes, place, absent || place + 16 > min(visible_first, end), absent);
-            __syncwarp();
-            issue(run + ring - 1, slot == 0 ? ring - 1 : slot - 1);
+            __syncwarp();  // every lane's copies are here, and every lane is done with the slot before this one
+            issue(step + ring - 1, slot == 0 ? ring - 1 : slot - 1);
+            const int place = now.begin + step * unit;
+            const unsigned absent = bad >> (slot * H) & ((1u << H) - 1u);
+            process(ring_bytes + slot * slot_bytes, place, absent != 0 || place > edge_from, absent);
             slot = slot + 1 == ring ? 0 : slot + 1;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();  // every lane is done with the ring
+        const bool another = advance();
+        if (another) start();
 
         // ---- join the warps ----
         constexpr int pitch = D + 4;
-        float* const outs = reinterpret_cast<float*>(shared);  // [warp][row][pitch]
+        float* const outs = reinterpret_cast<float*>(shared + warps * ring * slot_bytes);  // [warp][row][pitch]
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -695,7 +768,6 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                 }
             }
         }
-        __syncthreads();  // every warp is done with its ring
 #pragma unroll
         for (int g = 0; g < groups; ++g) {
             const float unscale = 1.0f / value_factor[g];
@@ -717,19 +789,18 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
         }
         __syncthreads();
         auto store = [&](int row, int d, float4 value, float whole) {
-            const int at_row = first_row + row, token = static_cast<int>(divide(at_row, work.by_ratio));
+            const int at_row = now.first_row + row, token = static_cast<int>(divide(at_row, work.by_ratio));
             const float inverse = whole == 0.0f ? 0.0f : 1.0f / whole;
             T* to = static_cast<T*>(a.output) +
-                (static_cast<std::int64_t>(first + token) * a.heads + kv_head * work.ratio + at_row - token * work.ratio) * D + d;
+                (static_cast<std::int64_t>(now.first + token) * a.heads + now.kv_head * work.ratio + at_row - token * work.ratio) * D + d;
             alignas(8) T out[4] = {narrow<T>(value.x * inverse), narrow<T>(value.y * inverse), narrow<T>(value.z * inverse),
                                    narrow<T>(value.w * inverse)};
             *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(out);
         };
-        const bool complete = first_unit == 0 && last_unit == share.units;
-        const int begin_block = complete ? 0 : block_of(segment_start + lead);
+        const int begin_block = now.complete ? 0 : block_of(now.segment_start + lead);
         float* const part = work.partials +
             (2 * static_cast<std::int64_t>(blockIdx.x) + (static_cast<int>(blockIdx.x) == begin_block)) * partial_floats;
-        const int quads = used_rows * (D / 4);
+        const int quads = now.used_rows * (D / 4);
         for (int e = threadIdx.x; e < quads; e += 32 * warps) {
             const int row = e / (D / 4), d = e % (D / 4) * 4;
             float most = -FLT_MAX, whole = 0.0f;
@@ -744,7 +815,7 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                 value.x = fmaf(o.x, weight, value.x), value.y = fmaf(o.y, weight, value.y);
                 value.z = fmaf(o.z, weight, value.z), value.w = fmaf(o.w, weight, value.w);
             }
-            if (complete) {
+            if (now.complete) {
                 store(row, d, value, whole);
             } else {
                 *reinterpret_cast<float4*>(part + row * D + d) = value;
@@ -753,8 +824,8 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
         }
 
         // ---- join the blocks of a segment: the last of them to get here ----
-        if (!complete) {
-            const int pieces = block_of(segment_start + span - 1) - begin_block + 1;
+        if (!now.complete) {
+            const int pieces = block_of(now.segment_end - 1) - begin_block + 1;
             __syncthreads();
             if (threadIdx.x == 0) {  // releases the block's sums, and acquires the others'
                 unsigned before_me;
@@ -771,7 +842,7 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                     return work.partials +
                         (2 * static_cast<std::int64_t>(begin_block + piece) + (piece == 0)) * partial_floats;
                 };
-                float* const weights = reinterpret_cast<float*>(shared);  // [piece][row]
+                float* const weights = outs;                         // [piece][row]
                 float* const totals = weights + most_blocks * rows;       // [piece][row]
                 float4* const sums = reinterpret_cast<float4*>(totals + most_blocks * rows);
                 const int shares = max(1, 32 * warps / quads);  // threads that divide one quad's pieces
@@ -787,13 +858,13 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                     }
                 }
                 for (int e = threadIdx.x; e < pieces * rows; e += 32 * warps) {
-                    if (e % rows < used_rows) {
+                    if (e % rows < now.used_rows) {
                         const float* const one = part_of(e / rows) + rows * D + e % rows;
                         weights[e] = __ldcg(one), totals[e] = __ldcg(one + rows);
                     }
                 }
                 __syncthreads();
-                for (int row = warp; row < used_rows; row += warps) {
+                for (int row = warp; row < now.used_rows; row += warps) {
                     float most = -FLT_MAX, whole_sum = 0.0f;
                     for (int piece = lane; piece < pieces; piece += 32) most = fmaxf(most, weights[piece * rows + row]);
 #pragma unroll
@@ -843,23 +914,24 @@ __global__ void __launch_bounds__(32 * warps, resident<D, NT>) attend_kernel(con
                 }
             }
         }
-        __syncthreads();  // before the next piece's copies
+        if (!another) return;
     }
 }
 
 template <typename T, int D, int G, int NT>
 cudaError_t launch(Work& work, cudaStream_t stream) {
     constexpr int bytes = shared_bytes<D, G, NT>;
-    static_assert(bytes >= 2 * most_blocks * 8 * NT * 4 + 32 * warps * 16, "the blocks' join fits the ring");
+    static_assert(warps * 8 * NT * (D + 4) * 4 >= 2 * most_blocks * 8 * NT * 4 + 32 * warps * 16, "the blocks' join fits");
     static SharedAllowance allowance;
     const cudaError_t allowed = allowance.allow(attend_kernel<T, D, G, NT>, bytes);
     if (allowed != cudaSuccess) return allowed;
     // the blocks that run at once, and no more than there can be units
+    constexpr int unit = 16 * together<D, NT> * warps;
     const std::int64_t rows = static_cast<std::int64_t>(work.a.max_queries) * work.ratio;
     const std::int64_t units = static_cast<std::int64_t>(work.a.batch) * work.cache.kv_heads * ((rows + 8 * NT - 1) / (8 * NT)) *
         std::max(1, (work.a.max_length + unit - 1) / unit);
     if (units > 0x7fffffff) return cudaErrorInvalidValue;
-    const std::int64_t grid = std::min<std::int64_t>(std::min(resident<D, NT> * sm_count(), most_blocks), units);
+    const std::int64_t grid = std::min<std::int64_t>(std::min(sm_count(), most_blocks), units);
     return kernels::launch_overlapped(attend_kernel<T, D, G, NT>, dim3(static_cast<unsigned>(grid)), dim3(32 * warps), bytes,
                                       stream, static_cast<const Work&>(work));
 }
