@@ -177,127 +177,147 @@ __device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
     }
 }
 
-// Eight channels a thread, D / 8 threads a (token, run of H heads of queries,
-// keys or values): a thread reads its angles' cosines and sines once, loads all
-// its heads in 16-byte accesses before it uses any (HBM-bound: that keeps enough
-// bytes in flight), and a key's or query's rotation partner, eight channels
+// Eight channels a thread, D / 8 threads a (token, run of heads of queries, keys
+// or values): a thread reads its angles' cosines and sines once, loads H heads in
+// 16-byte accesses before it uses any (that keeps enough bytes in flight), and a key's or query's rotation partner, eight channels
 // elsewhere in the head, as a second load of a line that is in L1. Takes aligned
 // tensors and rotations of whole octets (pairs (i, i + rotary / 2): rotary a
 // multiple of 16; (2 i, 2 i + 1): of 8).
-template <typename T, int D, int H>
-__global__ void __launch_bounds__(256, 4) append_octets_kernel(Cache cache, AppendArgs a, Divisor runs_per_page) {
+template <typename T, int D, int H, bool interleaved>
+__global__ void __launch_bounds__(256, 4) append_octets_kernel(Cache cache, AppendArgs a, int run_heads,
+                                                               Divisor runs_per_page) {
     constexpr int lanes = D / 8;
     join_chain();
     const int lane = threadIdx.x % lanes, channel = 8 * lane;
     const std::int64_t token = static_cast<std::int64_t>(blockIdx.x) * (256 / lanes) + threadIdx.x / lanes;
     const bool valid = token < a.tokens;  // threads past the end stay for the shuffles
-    const int query_runs = a.queries != nullptr ? (a.query_heads + H - 1) / H : 0;
-    const int kv_runs = (cache.kv_heads + H - 1) / H;
-    int run = blockIdx.y;
-    const bool is_query = run < query_runs, is_key = !is_query && run < query_runs + kv_runs;
-    run -= is_query ? 0 : is_key ? query_runs : query_runs + kv_runs;
-    const int first = run * H, last = min(is_query ? a.query_heads : cache.kv_heads, first + H);
-    const std::int64_t head_stride = is_query ? a.query_head_stride : is_key ? a.key_head_stride : a.value_head_stride;
-    const T* const source =
-        (is_query  ? static_cast<const T*>(a.queries) + token * a.query_stride
-             : is_key ? static_cast<const T*>(a.keys) + token * a.key_stride
-                      : static_cast<const T*>(a.values) + token * a.value_stride) +
-        first * head_stride + channel;
+    const int query_runs = a.queries != nullptr ? (a.query_heads + run_heads - 1) / run_heads : 0;
+    const int kv_runs = (cache.kv_heads + run_heads - 1) / run_heads;
     const int half = a.rotary / 2;
-    const bool second = !a.interleaved && channel >= half;
-    const bool turns = a.positions != nullptr && (is_query || is_key) && channel < a.rotary;
-    const bool partners = turns && !a.interleaved;
-    uint4 raw[H], partner[H];
+    const bool second = !interleaved && channel >= half;
+
+    // One body for queries, keys and values (the kind is uniform in a block).
+    auto body = [&](auto kind_tag, int run) {
+        constexpr int kind = decltype(kind_tag)::value;
+        constexpr bool is_query = kind == 0, rotates = kind != 2;
+        int first = run * run_heads;
+        const int last = min(is_query ? a.query_heads : cache.kv_heads, first + run_heads);
+        const std::int64_t head_stride = is_query ? a.query_head_stride : kind == 1 ? a.key_head_stride : a.value_head_stride;
+        const T* source = static_cast<const T*>(is_query ? a.queries : kind == 1 ? a.keys : a.values) + channel +
+            (valid ? token * (is_query ? a.query_stride : kind == 1 ? a.key_stride : a.value_stride) + first * head_stride : 0);
+        const bool turns = rotates && a.positions != nullptr && channel < a.rotary;
+        uint4 raw[H], partner[rotates && !interleaved ? H : 1];
+        auto load = [&] {
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-        raw[h] = partner[h] = {0u, 0u, 0u, 0u};
-        if (valid && first + h < last) {
-            raw[h] = *reinterpret_cast<const uint4*>(source + h * head_stride);
-            if (partners) partner[h] = *reinterpret_cast<const uint4*>(source + h * head_stride + (second ? -half : half));
-        }
-    }
-    std::int64_t slot = -1, position = 0;
-    if (valid && !is_query) slot = a.slots[token];
-    if (valid && a.positions != nullptr) position = a.positions[token];
-    const bool placed = a.positions == nullptr || (position >= 0 && position < a.table_rows);
-    if (!placed && lane == 0) note(cache, status_position);
-    // x cos - partner sin for a pair's first element, x cos + partner sin for its second: the sign goes to the sine
-    float cosine[8], sine[8];
-    if (turns && placed && valid) {
-        const float4* cosines = reinterpret_cast<const float4*>(a.cosines + position * half);
-        const float4* sines = reinterpret_cast<const float4*>(a.sines + position * half);
-        if (a.interleaved) {
-            const float4 c = cosines[lane], s = sines[lane];
-            cosine[0] = cosine[1] = c.x, cosine[2] = cosine[3] = c.y, cosine[4] = cosine[5] = c.z, cosine[6] = cosine[7] = c.w;
-            sine[1] = s.x, sine[3] = s.y, sine[5] = s.z, sine[7] = s.w;
-            sine[0] = -s.x, sine[2] = -s.y, sine[4] = -s.z, sine[6] = -s.w;
-        } else {
-            const int at = (second ? channel - half : channel) / 4;
-            const float sign = second ? 1.0f : -1.0f;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float4 c = cosines[at + i], s = sines[at + i];
-                cosine[4 * i] = c.x, cosine[4 * i + 1] = c.y, cosine[4 * i + 2] = c.z, cosine[4 * i + 3] = c.w;
-                sine[4 * i] = sign * s.x, sine[4 * i + 1] = sign * s.y;
-                sine[4 * i + 2] = sign * s.z, sine[4 * i + 3] = sign * s.w;
+            for (int h = 0; h < H; ++h) {
+                if (first + h < last) {  // a thread past the end reads the first token and stores nothing
+                    raw[h] = *reinterpret_cast<const uint4*>(source + h * head_stride);
+                    if constexpr (rotates && !interleaved) {
+                        if (turns) partner[h] = *reinterpret_cast<const uint4*>(source + h * head_stride + (second ? -half : half));
+                    }
+                }
             }
-        }
-    }
-    T* const rotated = static_cast<T*>(a.rotated) + (token * a.query_heads + first) * D + channel;
-    const std::int64_t limit = static_cast<std::int64_t>(cache.pages) * cache.page_size;
-    const bool stored = placed && slot >= 0 && slot < limit;
-    if (slot >= limit && lane == 0) note(cache, status_slot);
-    std::int64_t place = 0;
-    if (stored) {  // slots are below 2^35, their runs of 16 below 2^31
-        const std::int64_t page = divide(static_cast<unsigned>(slot >> 4), runs_per_page);
-        place = (page * cache.kv_heads + first) * cache.page_size + (slot - page * cache.page_size);
-    }
-    const int group_lanes = cache.group / 8;
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-        if (first + h >= last) break;
-        float x[8];
-        unpack8<T>(raw[h], x);
-        if (turns && placed) {
-            float turned[8];
-            if (a.interleaved) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) turned[i] = __fadd_rn(__fmul_rn(x[i], cosine[i]), __fmul_rn(x[i ^ 1], sine[i]));
+        };
+        load();
+        std::int64_t slot = -1, position = 0;
+        if (valid && !is_query) slot = a.slots[token];
+        if (valid && a.positions != nullptr) position = a.positions[token];
+        const bool placed = a.positions == nullptr || (position >= 0 && position < a.table_rows);
+        if (!placed && lane == 0) note(cache, status_position);
+        const bool turned = turns && placed;
+        // x cos - partner sin for a pair's first element, x cos + partner sin for its second: the sign goes to the sine
+        float cosine[8], sine[8];
+        if (rotates && turned) {
+            const float4* cosines = reinterpret_cast<const float4*>(a.cosines + position * half);
+            const float4* sines = reinterpret_cast<const float4*>(a.sines + position * half);
+            if constexpr (interleaved) {
+                const float4 c = cosines[lane], s = sines[lane];
+                cosine[0] = cosine[1] = c.x, cosine[2] = cosine[3] = c.y;
+                cosine[4] = cosine[5] = c.z, cosine[6] = cosine[7] = c.w;
+                sine[1] = s.x, sine[3] = s.y, sine[5] = s.z, sine[7] = s.w;
+                sine[0] = -s.x, sine[2] = -s.y, sine[4] = -s.z, sine[6] = -s.w;
             } else {
-                float other[8];
-                unpack8<T>(partner[h], other);
+                const int at = (second ? channel - half : channel) / 4;
+                const float sign = second ? 1.0f : -1.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) turned[i] = __fadd_rn(__fmul_rn(x[i], cosine[i]), __fmul_rn(other[i], sine[i]));
+                for (int i = 0; i < 2; ++i) {
+                    const float4 c = cosines[at + i], s = sines[at + i];
+                    cosine[4 * i] = c.x, cosine[4 * i + 1] = c.y, cosine[4 * i + 2] = c.z, cosine[4 * i + 3] = c.w;
+                    sine[4 * i] = sign * s.x, sine[4 * i + 1] = sign * s.y;
+                    sine[4 * i + 2] = sign * s.z, sine[4 * i + 3] = sign * s.w;
+                }
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = turned[i];
         }
-        if (is_query) {
-            if (!placed) {
+        const std::int64_t limit = static_cast<std::int64_t>(cache.pages) * cache.page_size;
+        const bool stored = !is_query && placed && slot >= 0 && slot < limit;
+        if (slot >= limit && lane == 0) note(cache, status_slot);
+        std::int64_t place = 0;
+        if (stored) {  // slots are below 2^35, their runs of 16 below 2^31
+            const std::int64_t page = divide(static_cast<unsigned>(slot >> 4), runs_per_page);
+            place = (page * cache.kv_heads + first) * cache.page_size + (slot - page * cache.page_size);
+        }
+        const int group_lanes = cache.group / 8, group_shift = 31 - __clz(group_lanes);  // 4, 8 or 16
+        unsigned* const codes_to = reinterpret_cast<unsigned*>(kind == 1 ? cache.key_codes : cache.value_codes) + lane;
+        unsigned* const pairs_to =
+            reinterpret_cast<unsigned*>(kind == 1 ? cache.key_scales : cache.value_scales) + (lane >> group_shift);
+        T* rotated = static_cast<T*>(a.rotated) + (is_query && valid ? (token * a.query_heads + first) * D + channel : 0);
+        for (;;) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = NAN;
+            for (int h = 0; h < H; ++h) {
+                if (first + h >= last) break;
+                float x[8];
+                unpack8<T>(raw[h], x);
+                if (rotates && turned) {
+                    float other[8], result[8];
+                    if constexpr (interleaved) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) other[i] = x[i ^ 1];
+                    } else {
+                        unpack8<T>(partner[rotates && !interleaved ? h : 0], other);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) result[i] = __fadd_rn(__fmul_rn(x[i], cosine[i]), __fmul_rn(other[i], sine[i]));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = result[i];
+                }
+                if constexpr (is_query) {
+                    if (!placed) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] = NAN;
+                    }
+                    if (valid) store8(rotated + h * D, x);
+                } else {
+                    float low = x[0], high = x[0];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) low = min_nan(low, x[i]), high = max_nan(high, x[i]);
+#pragma unroll
+                    for (int offset = 1; offset < 16; offset *= 2) {
+                        if (offset >= group_lanes) break;
+                        low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, offset));
+                        high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, offset));
+                    }
+                    if (stored) {
+                        const GroupForm form(low, high);
+                        const std::int64_t at = place + h * cache.page_size;
+                        codes_to[at * lanes] = form.codes(x);
+                        if ((lane & (group_lanes - 1)) == 0) pairs_to[at * (lanes >> group_shift)] = form.bits();
+                    }
+                }
             }
-            if (valid) store8(rotated + h * D, x);
-            continue;
+            first += H;
+            if (first >= last) return;
+            source += H * head_stride, rotated += is_query ? H * D : 0;
+            place += static_cast<std::int64_t>(H) * cache.page_size;
+            load();
         }
-        float low = x[0], high = x[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) low = min_nan(low, x[i]), high = max_nan(high, x[i]);
-#pragma unroll
-        for (int offset = 1; offset < 16; offset *= 2) {
-            if (offset >= group_lanes) break;
-            low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, offset));
-            high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, offset));
-        }
-        if (!stored) continue;
-        const GroupForm form(low, high);
-        const unsigned codes = form.codes(x);
-        const std::int64_t at = place + h * cache.page_size;
-        reinterpret_cast<unsigned*>(is_key ? cache.key_codes : cache.value_codes)[at * lanes + lane] = codes;
-        if (lane % group_lanes == 0) {
-            reinterpret_cast<unsigned*>(is_key ? cache.key_scales : cache.value_scales)[at * (lanes / group_lanes) +
-                                                                                       lane / group_lanes] = form.bits();
-        }
+    };
+    const int run = blockIdx.y;
+    if (run < query_runs) {
+        body(std::integral_constant<int, 0>{}, run);
+    } else if (run < query_runs + kv_runs) {
+        body(std::integral_constant<int, 1>{}, run - query_runs);
+    } else {
+        body(std::integral_constant<int, 2>{}, run - query_runs - kv_runs);
     }
 }
 
@@ -317,8 +337,8 @@ __global__ void __launch_bounds__(256) read_kernel(Cache cache, const std::int64
     if (slot >= 0 && slot < static_cast<std::int64_t>(cache.pages) * cache.page_size) {
         const std::int64_t page = divide(static_cast<unsigned>(slot >> 4), runs_per_page);
         const std::int64_t at = (page * cache.kv_heads + head) * cache.page_size + slot - page * cache.page_size;
-        const int group_lanes = cache.group / 8;
-        const std::int64_t code_at = at * lanes + lane, pair_at = at * (lanes / group_lanes) + lane / group_lanes;
+        const int group_shift = 28 - __clz(cache.group);  // of the lanes of a group: 4, 8 or 16
+        const std::int64_t code_at = at * lanes + lane, pair_at = at * (lanes >> group_shift) + (lane >> group_shift);
         codes[0] = reinterpret_cast<const unsigned*>(cache.key_codes)[code_at];
         codes[1] = reinterpret_cast<const unsigned*>(cache.value_codes)[code_at];
         pairs[0] = reinterpret_cast<const unsigned*>(cache.key_scales)[pair_at];
@@ -359,15 +379,18 @@ cudaError_t append_shape(const Cache& cache, const AppendArgs& a, cudaStream_t s
     if (octets) {
         constexpr int tokens_each = 256 / (D / 8);
         const std::int64_t token_blocks = (a.tokens + tokens_each - 1) / tokens_each;
-        // Four heads a thread share the angles and are in flight together; one keeps a few tokens' threads many.
-        const int each = token_blocks * heads >= 16 * static_cast<std::int64_t>(sm_count()) ? 4 : 1;
-        const int query_heads = a.queries != nullptr ? a.query_heads : 0;
-        const std::int64_t runs = (query_heads + each - 1) / each + 2 * ((cache.kv_heads + each - 1) / each);
+        // Many tokens: eight heads a thread share its angles and addresses, four of them in flight together. A few: one,
+        // which makes their threads many.
+        const bool many = token_blocks * heads >= 16 * static_cast<std::int64_t>(sm_count());
+        const int run_heads = many ? 8 : 1, query_heads = a.queries != nullptr ? a.query_heads : 0;
+        const std::int64_t runs = (query_heads + run_heads - 1) / run_heads + 2 * ((cache.kv_heads + run_heads - 1) / run_heads);
         if (runs > 65535) return cudaErrorInvalidValue;
         const dim3 grid(static_cast<unsigned>(token_blocks), static_cast<unsigned>(runs));
         const Divisor runs_per_page = divisor(static_cast<unsigned>(cache.page_size / 16));
-        return kernels::launch_overlapped(each == 4 ? append_octets_kernel<T, D, 4> : append_octets_kernel<T, D, 1>, grid,
-                                          dim3(256), 0, stream, cache, a, runs_per_page);
+        const auto kernel = a.interleaved
+            ? many ? append_octets_kernel<T, D, 4, true> : append_octets_kernel<T, D, 1, true>
+            : many ? append_octets_kernel<T, D, 4, false> : append_octets_kernel<T, D, 1, false>;
+        return kernels::launch_overlapped(kernel, grid, dim3(256), 0, stream, cache, a, run_heads, runs_per_page);
     }
     const std::int64_t blocks = (a.tokens * heads + 7) / 8;
     if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
