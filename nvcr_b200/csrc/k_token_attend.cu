@@ -37,12 +37,12 @@
 // last of them, in order: the same bits every time.
 //
 // Measured on a B200: 131072 keys, 32 heads over 8 of 128 channels, one token
-// (142.6 MB): 47.4 us, 3.0 TB/s; 32 sequences of 1 to 4096 keys (76 MB): 35.1 us; 200
+// (142.6 MB): 47.3 us, 3.0 TB/s; 32 sequences of 1 to 4096 keys (76 MB): 35.0 us; 200
 // keys: 5.5 us. What bounds a long stream is the integer pipe that takes the
 // codes apart (168 of 327 instructions a run of 16 keys, at half rate) and the
-// warps' latency: 141 cycles a run an SM, 109 without the values' conversion. Two
-// blocks an SM with 128 registers a thread took 135 cycles a run, but twice the
-// fixed work: 6.3 us for 200 keys. Short calls are bound by the chain lengths -> page
+// warps' latency: 141 cycles a run an SM. Two blocks an SM with 128 registers a
+// thread took 135 cycles a run (109 with the values' conversion left out), but twice
+// the fixed work: 6.3 us for 200 keys. Short calls are bound by the chain lengths -> page
 // table -> cache -> join, about 1 us a link.
 #include "token_elements.cuh"
 
@@ -170,8 +170,10 @@ struct Share {
     int first;  // of its new tokens
 };
 
+// One block an SM, said to the compiler: it then takes 222 registers for FP16 heads of 128 in groups of 128, and 168
+// without (131072 keys: 47.3 us, 51.7 us).
 template <typename T, int D, int G, int NT>
-__global__ void __launch_bounds__(32 * warps) attend_kernel(const Work work) {
+__global__ void __launch_bounds__(32 * warps, 1) attend_kernel(const Work work) {
     constexpr int groups = D / G, rows = 8 * NT, H = together<D, NT>, ring = ring_slots<D, G, NT>;
     constexpr int unit = 16 * H * warps, slot_bytes = H * run_bytes<D, G>;  // unit: keys
     constexpr int least_units = (least_keys + unit - 1) / unit, join_units = (join_keys + unit - 1) / unit;
