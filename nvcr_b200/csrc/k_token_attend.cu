@@ -940,10 +940,15 @@ cudaError_t launch(Work& work, cudaStream_t stream) {
 
 template <typename T, int D, int G>
 cudaError_t launch_rows(Work& work, cudaStream_t stream) {
-    // 16 rows a block read the cache once for twice the rows; one block of 8 has half the registers. With heads of
-    // 256 channels 16 rows' sums do not fit the registers.
+    // Segments of 16 rows read the cache once for twice the rows, of 8 rows take two runs at a time and have a shorter
+    // chain: 8 while each such segment has an SM of its own. Heads of 128, 8 cache heads, 16 rows each, 1024 keys, us
+    // with 16 rows and with 8: one sequence (16 segments of 8) 14.7, 10.1; 8 sequences (128) 15.1, 10.3; 12 (192) 15.2,
+    // 18.1; 32 (512) 28.2, 33.9. 4096 keys: 15.4, 11.9; 28.5, 27.7; 44.2, 41.9; 84.2, 97.9. The rule's worst: 2 cache
+    // heads, 12 sequences of 4096 keys (48) 23.0, 28.0. With heads of 256 channels 16 rows' sums do not fit the registers.
     if constexpr (D < 256) {
-        if (static_cast<std::int64_t>(work.a.max_queries) * work.ratio > 8) return launch<T, D, G, 2>(work, stream);
+        const std::int64_t rows = static_cast<std::int64_t>(work.a.max_queries) * work.ratio;
+        const std::int64_t eights = static_cast<std::int64_t>(work.a.batch) * work.cache.kv_heads * ((rows + 7) / 8);
+        if (rows > 8 && eights > sm_count()) return launch<T, D, G, 2>(work, stream);
     }
     return launch<T, D, G, 1>(work, stream);
 }

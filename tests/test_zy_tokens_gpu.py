@@ -521,6 +521,17 @@ def test_attend_several_new_tokens(cuda):
     assert torch.count_nonzero(out[:2]) == 0 and torch.count_nonzero(out[5:7]) == 0
 
 
+@pytest.mark.parametrize("name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 128)])
+def test_attend_many_rows_of_many_sequences(cuda, dim, group, name):
+    """More segments of 8 rows than SMs, with rows that do not fill 16, whole and cut among blocks."""
+    counts = [5, 1, 4, 5, 0, 3, 2, 5, 1, 5] * 3
+    lengths = [5, 1, 70, 129, 0, 257, 31, 200, 16, 64] * 3
+    attend(Sequences(lengths, dim, group, 2, 16), counts, 12, name)
+    lengths[3], lengths[17] = 3001, 1500
+    attend(Sequences(lengths, dim, group, 2, 48), counts, 10, name)
+
+
 @pytest.mark.parametrize("length", [1000, 4095, 20000])
 def test_attend_long(cuda, length):
     """Work that is split over the length and joined."""
@@ -667,6 +678,16 @@ def test_multiply_divisions(cuda, inputs, outputs, rows, group):
     for name in ("float16", "bfloat16"):
         y, want, tolerance = check_multiply(rows, inputs, outputs, group, name, bias=True)
         near(y, want, tolerance, name)
+
+
+@pytest.mark.parametrize("name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("inputs,outputs,rows", [(4224, 1001, 9), (1152, 4000, 16), (16384, 300, 12), (98304, 50, 16),
+                                                 (512, 100, 40), (2048, 2048, 32), (2048, 2049, 31)])
+def test_multiply_sixteen_rows(cuda, inputs, outputs, rows, group, name):
+    """16 rows at a time on both sides of where they begin, with clusters, and too long for that."""
+    y, want, tolerance = check_multiply(rows, inputs, outputs, group, name, bias=True)
+    near(y, want, tolerance, name)
 
 
 def test_multiply_odd_inputs(cuda):
