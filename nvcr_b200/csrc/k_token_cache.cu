@@ -9,6 +9,10 @@
 // want them in one 32-bit word; groups beyond the FP16 range (or holding a NaN
 // or infinity) stand for non-finite values. The rotation is FP32, each product
 // rounded by itself, and keys are quantised from the unrounded rotation.
+//
+// Measured on a B200, 32 query heads, 8 cache heads of 128, all rotated: 8192 tokens
+// appended and read back (225 MB) 49.5 us, 4.5 TB/s, bound by instruction issue
+// and HBM (24 million warp instructions); one token 3.4 us for the two launches.
 #include "token_elements.cuh"
 
 #include <algorithm>
@@ -179,8 +183,9 @@ __device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
 
 // Eight channels a thread, D / 8 threads a (token, run of heads of queries, keys
 // or values): a thread reads its angles' cosines and sines once, loads H heads in
-// 16-byte accesses before it uses any (that keeps enough bytes in flight), and a key's or query's rotation partner, eight channels
-// elsewhere in the head, as a second load of a line that is in L1. Takes aligned
+// 16-byte accesses before it uses any (that keeps enough bytes in flight), and a
+// key's or query's rotation partner, eight channels elsewhere in the head, as a
+// second load of a line that is in L1. Takes aligned
 // tensors and rotations of whole octets (pairs (i, i + rotary / 2): rotary a
 // multiple of 16; (2 i, 2 i + 1): of 8).
 template <typename T, int D, int H, bool interleaved>
@@ -380,10 +385,17 @@ cudaError_t append_shape(const Cache& cache, const AppendArgs& a, cudaStream_t s
         constexpr int tokens_each = 256 / (D / 8);
         const std::int64_t token_blocks = (a.tokens + tokens_each - 1) / tokens_each;
         // Many tokens: eight heads a thread share its angles and addresses, four of them in flight together. A few: one,
-        // which makes their threads many.
-        const bool many = token_blocks * heads >= 16 * static_cast<std::int64_t>(sm_count());
-        const int run_heads = many ? 8 : 1, query_heads = a.queries != nullptr ? a.query_heads : 0;
-        const std::int64_t runs = (query_heads + run_heads - 1) / run_heads + 2 * ((cache.kv_heads + run_heads - 1) / run_heads);
+        // which makes their threads many. us with one and with eight, 32 query heads and 8 cache heads of 128: 512
+        // tokens (192 blocks of eight heads) 6.2, 7.2; 640 (240) 7.6, 7.3; 2048 19.8, 13.7; 8192 84, 41. 16 and 2: 768
+        // tokens (192) 4.6, 3.8; 1536 (384) 7.2, 5.6. No queries, 8 cache heads: 1536 (192) 7.0, 7.6. The general kernel
+        // takes 2.6 us for one token (2.0 here) and 147 us for 8192.
+        const int query_heads = a.queries != nullptr ? a.query_heads : 0;
+        const auto runs_of = [&](int n) {
+            return static_cast<std::int64_t>((query_heads + n - 1) / n) + 2 * ((cache.kv_heads + n - 1) / n);
+        };
+        const bool many = 2 * token_blocks * runs_of(8) >= 3 * static_cast<std::int64_t>(sm_count());
+        const int run_heads = many ? 8 : 1;
+        const std::int64_t runs = runs_of(run_heads);
         if (runs > 65535) return cudaErrorInvalidValue;
         const dim3 grid(static_cast<unsigned>(token_blocks), static_cast<unsigned>(runs));
         const Divisor runs_per_page = divisor(static_cast<unsigned>(cache.page_size / 16));
