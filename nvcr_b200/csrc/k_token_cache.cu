@@ -10,9 +10,10 @@
 // or infinity) stand for non-finite values. The rotation is FP32, each product
 // rounded by itself, and keys are quantised from the unrounded rotation.
 //
-// Measured on a B200, 32 query heads, 8 cache heads of 128, all rotated: 8192 tokens
-// appended and read back (225 MB) 49.5 us, 4.5 TB/s, bound by instruction issue
-// and HBM (24 million warp instructions); one token 3.4 us for the two launches.
+// Measured on a B200, 32 query heads, 8 cache heads of 128: 8192 BF16 tokens, 64
+// channels rotated, groups of 32, appended and read back (225 MB) 49.5 us, 4.5 TB/s,
+// bound by instruction issue and HBM (the append is 24 million warp instructions);
+// one FP16 token, all channels rotated, groups of 64, 3.4 us for the two launches.
 #include "token_elements.cuh"
 
 #include <algorithm>
@@ -386,7 +387,7 @@ cudaError_t append_shape(const Cache& cache, const AppendArgs& a, cudaStream_t s
         const std::int64_t token_blocks = (a.tokens + tokens_each - 1) / tokens_each;
         // Many tokens: eight heads a thread share its angles and addresses, four of them in flight together. A few: one,
         // which makes their threads many. us with one and with eight, 32 query heads and 8 cache heads of 128: 512
-        // tokens (192 blocks of eight heads) 6.2, 7.2; 640 (240) 7.6, 7.3; 2048 19.8, 13.7; 8192 84, 41. 16 and 2: 768
+        // tokens (192 blocks of eight heads) 6.2, 7.2; 640 (240) 7.6, 7.4; 2048 19.8, 13.7; 8192 84, 41. 16 and 2: 768
         // tokens (192) 4.6, 3.8; 1536 (384) 7.2, 5.6. No queries, 8 cache heads: 1536 (192) 7.0, 7.6. The general kernel
         // takes 2.6 us for one token (2.0 here) and 147 us for 8192.
         const int query_heads = a.queries != nullptr ? a.query_heads : 0;
