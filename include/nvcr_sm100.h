@@ -402,9 +402,9 @@ int nvcr_sm100_token_norm(int type, int layer, int post, const void* block, int6
  * of page p. The buffers are the caller's. head_dim is 64, 128 or 256, group
  * 32, 64 or 128 with 1, 2 or 4 groups a head, page_size a multiple of 16.
  * Kernels OR into *status (may be NULL) what they find wrong in device data,
- * and leave the token or page concerned out: 1 a slot past the end, 2 a
- * position outside the rotation table, 4 a page number outside the cache, 8 a
- * length or an offset outside what the call said. */
+ * and leave the token, page or sequence concerned out: 1 a slot past the end,
+ * 2 a position outside the rotation table, 4 a page number outside the cache,
+ * 8 a sequence whose length or offsets are outside what the call said. */
 typedef struct nvcr_sm100_token_cache {
     uint8_t* key_codes;    /* [pages][kv_heads][page_size][head_dim / 2] */
     uint16_t* key_scales;  /* [pages][kv_heads][page_size][head_dim / group][2]: FP16 scale, minimum */
@@ -456,7 +456,9 @@ void nvcr_sm100_token_context_destroy(nvcr_sm100_token_context* context);
  * and page_table has table_pages columns. A token sees the places up to its
  * own. Query head h reads cache head h / (heads / kv_heads). Scores are scaled
  * by `scale`; output [tokens][heads][head_dim] of `type` (F16 or BF16), 16-byte
- * aligned, zeros for a token that sees nothing. FP32 softmax and sums. */
+ * aligned, zeros for a token that sees nothing, that belongs to no sequence
+ * (the offsets need not begin at 0 nor end at `tokens`), or whose sequence is
+ * left out. FP32 softmax and sums. */
 int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_token_cache* cache, int type,
                             const void* queries, int64_t query_stride, int64_t query_head_stride, int64_t tokens,
                             int32_t heads, const int32_t* page_table, int64_t table_stride, int32_t table_pages,

@@ -248,8 +248,8 @@ int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_
             return refuse("max_length needs more pages than page_table has");
         }
         if (!std::isfinite(scale)) return refuse("scale must be finite");
-        if (tokens > 0 && batch > 0 &&
-            (queries == nullptr || page_table == nullptr || lengths == nullptr || output == nullptr)) {
+        if (tokens > 0 &&
+            (output == nullptr || (batch > 0 && (queries == nullptr || page_table == nullptr || lengths == nullptr)))) {
             return refuse("null queries, page_table, lengths or output");
         }
         if (reinterpret_cast<std::uintptr_t>(output) % 16 != 0) return refuse("output must be 16-byte aligned");

@@ -1,7 +1,8 @@
 // Attention of new tokens over the paged 4-bit cache. Token i of a sequence's
 // count new ones is at position length - count + i and sees the keys up to its
-// own position; one that sees none gives zeros. Grouped heads: query head h
-// reads cache head h / (heads / kv_heads).
+// own position; one that sees none gives zeros, as does a token that belongs to
+// no sequence, or to one whose offsets or length are out of range. Grouped heads:
+// query head h reads cache head h / (heads / kv_heads).
 //
 // The codes are never expanded to values. With s, m a group's scale and minimum,
 //   score = sum_g s_g (q_g . c_g) + m_g sum(q_g),
@@ -167,8 +168,46 @@ struct Piece {
 // The units of one sequence: `blocks` blocks of rows times `units` of each segment.
 struct Share {
     int count, length, blocks, units;
-    int first;  // of its new tokens
+    int first;  // of its new tokens; -1: out of range, and left out
 };
+
+// A sequence's tokens and length; false where they are out of range, and the sequence is left out.
+__device__ __forceinline__ bool extent_of(const std::int32_t* offsets, const std::int32_t* lengths, int max_queries,
+                                          int max_length, std::int64_t tokens, int sequence, int& first, int& last,
+                                          int& length) {
+    first = sequence, last = sequence + 1;
+    if (offsets != nullptr) first = offsets[sequence], last = offsets[sequence + 1];
+    length = lengths[sequence];
+    return first >= 0 && last <= tokens && last >= first && last - first <= max_queries && length >= 0 && length <= max_length;
+}
+
+// Zeros for the tokens of no sequence, a warp each. Not inlined: the kernel's registers are for its stream of keys.
+__device__ __noinline__ void clear_left_out(const std::int32_t* offsets, const std::int32_t* lengths, int batch,
+                                            int max_queries, int max_length, std::int64_t tokens, uint4* output,
+                                            int row_chunks) {
+    const int lane = threadIdx.x % 32;
+    int first, last, length;
+    bool all_good = true;  // then the sequences' tokens lie in a row
+    for (int b = lane; b < batch; b += 32) {
+        all_good = all_good && extent_of(offsets, lengths, max_queries, max_length, tokens, b, first, last, length);
+    }
+    all_good = __all_sync(0xffffffffu, all_good);
+    for (std::int64_t token = static_cast<std::int64_t>(blockIdx.x) * warps + threadIdx.x / 32; token < tokens;
+         token += static_cast<std::int64_t>(gridDim.x) * warps) {
+        bool inside = false;
+        if (all_good) {
+            inside = offsets == nullptr || (token >= offsets[0] && token < offsets[batch]);
+        } else {
+            for (int b = lane; b < batch; b += 32) {
+                const bool good = extent_of(offsets, lengths, max_queries, max_length, tokens, b, first, last, length);
+                inside = inside || (good && token >= first && token < last);
+            }
+            inside = __any_sync(0xffffffffu, inside);
+        }
+        if (inside) continue;
+        for (int i = lane; i < row_chunks; i += 32) output[token * row_chunks + i] = {0u, 0u, 0u, 0u};
+    }
+}
 
 // One block an SM, said to the compiler: it then takes 222 registers for FP16 heads of 128 in groups of 128, and 168
 // without (131072 keys: 47.3 us, 51.7 us).
@@ -195,15 +234,12 @@ __global__ void __launch_bounds__(32 * warps, 1) attend_kernel(const Work work) 
 
     // ---- this block's part of all the segments' units ----
     auto share_of = [&](int sequence, bool tell) {
-        Share s{0, 0, 0, 0, sequence};
-        int last = sequence + 1;
-        if (a.query_offsets != nullptr) s.first = a.query_offsets[sequence], last = a.query_offsets[sequence + 1];
-        s.length = a.lengths[sequence];
-        const bool good = s.first >= 0 && last <= a.tokens && last >= s.first && last - s.first <= a.max_queries;
-        if (tell && (!good || s.length < 0 || s.length > a.max_length)) note(cache, status_length);
-        if (!good) return s;
-        s.count = last - s.first;
-        s.length = min(max(s.length, 0), a.max_length);
+        int first, last, length;
+        if (!extent_of(a.query_offsets, a.lengths, a.max_queries, a.max_length, a.tokens, sequence, first, last, length)) {
+            if (tell) note(cache, status_length);
+            return Share{0, 0, 0, 0, -1};
+        }
+        Share s{last - first, length, 0, 0, first};
         s.blocks = (s.count * work.ratio + rows - 1) / rows;
         s.units = max(1, (s.length + unit - 1) / unit);
         return s;
@@ -214,8 +250,11 @@ __global__ void __launch_bounds__(32 * warps, 1) attend_kernel(const Work work) 
     const int from = min(a.batch, counter * each), to = min(a.batch, from + each);
     Share own{0, 0, 0, 0, 0};  // of the last of them
     int units = 0, segments = 0, longest = 0;
+    // Every token is some sequence's: each sequence's begin where the last one's end.
+    bool covered = true;
     for (int b = from; b < to; ++b) {
         own = share_of(b, blockIdx.x == 0);
+        covered = covered && own.first >= 0 && (b > 0 || own.first == 0) && (b < a.batch - 1 || own.first + own.count == a.tokens);
         units += own.blocks * own.units * cache.kv_heads;
         segments += own.blocks * cache.kv_heads;
         if (own.blocks > 0) longest = max(longest, own.units);
@@ -231,7 +270,7 @@ __global__ void __launch_bounds__(32 * warps, 1) attend_kernel(const Work work) 
     int all_units = __shfl_sync(0xffffffffu, units_to, 31), all_segments = __shfl_sync(0xffffffffu, segments_to, 31);
     if (!few) {
         if (lane == 31) joint_units[warp] = units_to, joint_segments[warp] = segments_to, joint_longest[warp] = longest;
-        __syncthreads();
+        covered = __syncthreads_and(covered);
         all_units = all_segments = 0;
 #pragma unroll
         for (int w = 0; w < warps; ++w) {
@@ -239,6 +278,10 @@ __global__ void __launch_bounds__(32 * warps, 1) attend_kernel(const Work work) 
             all_units += joint_units[w], all_segments += joint_segments[w];
             longest = max(longest, joint_longest[w]);
         }
+    }
+    if (__any_sync(0xffffffffu, !covered)) {
+        clear_left_out(a.query_offsets, a.lengths, a.batch, a.max_queries, a.max_length, a.tokens,
+                       static_cast<uint4*>(a.output), a.heads * (D / 8));
     }
     // Segments are cut only where that saves more units than joining costs.
     const int grid = static_cast<int>(gridDim.x);
@@ -974,7 +1017,12 @@ std::size_t attend_partial_bytes() {
 std::size_t attend_ticket_bytes() { return most_blocks * sizeof(unsigned); }
 
 cudaError_t attend(const Cache& cache, const AttendArgs& args, const AttendWorkspace& workspace, cudaStream_t stream) {
-    if (args.tokens == 0 || args.batch == 0) return cudaSuccess;
+    if (args.tokens == 0) return cudaSuccess;
+    if (args.batch == 0) {
+        const std::size_t values = static_cast<std::size_t>(args.tokens) * static_cast<std::size_t>(args.heads) *
+            static_cast<std::size_t>(cache.head_dim);
+        return cudaMemsetAsync(args.output, 0, values * 2, stream);
+    }
     Work work{};
     work.cache = cache;
     work.a = args;

@@ -26,7 +26,7 @@ enum class Type : int { f16 = 0, bf16 = 1, f32 = 2 };
 constexpr unsigned status_slot = 1;      // a slot past the cache's end
 constexpr unsigned status_position = 2;  // a position outside the rotation table
 constexpr unsigned status_page = 4;      // a page number outside the cache
-constexpr unsigned status_length = 8;    // a length or an offset outside what the call said
+constexpr unsigned status_length = 8;    // a sequence's length or offsets outside what the call said
 
 // Rows of one batch of vectors whose last dimension is contiguous; strides in elements.
 struct NormArgs {

@@ -188,8 +188,9 @@ class TokenContext:
         """Attention of queries [tokens, heads, head_dim] over the cache, the new tokens' own keys and values already
         appended. int32 `lengths` [batch] (at most `max_length`) count the new tokens; sequence b's pages are row b
         of the int32 `page_table`; its new tokens are query_offsets[b] .. query_offsets[b + 1] - 1 (int32 [batch + 1],
-        at most `max_queries` each; None: token b). A token sees the places up to its own; one that sees none gives
-        zeros. `scale` defaults to 1 / sqrt(head_dim)."""
+        at most `max_queries` each; None: token b). A token sees the places up to its own; one that sees none, or is
+        in no sequence, or in one whose length or offsets are out of range, gives zeros. `scale` defaults to
+        1 / sqrt(head_dim)."""
         return (_module or _native()).attend(self._handle.value or 0, cache._address, cache._index, queries, page_table, lengths,
                                              query_offsets, max_queries, max_length, scale,
                                              None if stream is None else _stream(stream))

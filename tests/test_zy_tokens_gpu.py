@@ -624,6 +624,76 @@ def test_attend_device_data_out_of_range(cuda):
         assert empty.shape == (0, 4, 64)
 
 
+def attend_into(out, context, seqs, queries, lengths, offsets, max_queries, max_length):
+    """Attention through the C ABI into a buffer of the caller's (FP16)."""
+    import ctypes
+
+    from nvcr_b200.executor import _check, library
+
+    table = seqs.table
+    _check(library().nvcr_sm100_token_attend(
+        context._handle, ctypes.addressof(seqs.cache._struct), 0, queries.data_ptr(), queries.stride(0),
+        queries.stride(1), queries.shape[0], queries.shape[1], table.data_ptr(), table.stride(0), table.shape[1],
+        lengths.data_ptr(), lengths.shape[0], None if offsets is None else offsets.data_ptr(), max_queries, max_length,
+        queries.shape[2] ** -0.5, out.data_ptr(), None))
+
+
+@pytest.mark.parametrize("repeat", [1, 40])
+def test_attend_tokens_of_no_sequence_are_zeros(cuda, repeat):
+    """Every row is written: tokens before the first sequence, after the last, and of sequences that are left out.
+    40 repeats of the sequences are more than one to a lane."""
+    import torch
+
+    from nvcr_b200.executor import ExecutorError
+    from nvcr_b200.tokens import TokenContext
+
+    lengths, counts = [60, 33, 5] * repeat, [3, 1, 2] * repeat
+    seqs, tokens = Sequences(lengths, 64, 32, 2, 16), sum(counts) + 6
+    queries = normal((tokens, 4, 64), 5).half()
+    starts = [2 + sum(counts[:i]) for i in range(len(counts) + 1)]
+    on_device = lambda values: torch.tensor(values, dtype=torch.int32, device="cuda")  # noqa: E731
+    with TokenContext() as context:
+        def call(lengths, offsets, max_queries=3, queries=queries):
+            out = torch.full((queries.shape[0], 4, 64), float("nan"), dtype=torch.float16, device="cuda")
+            attend_into(out, context, seqs, queries, lengths, offsets, max_queries, 60)
+            torch.cuda.synchronize()
+            return out
+
+        def told():
+            with pytest.raises(ExecutorError, match="length or offset"):
+                seqs.cache.check()
+
+        whole = call(seqs.lengths_on_device, on_device(starts))
+        seqs.cache.check()  # tokens around the sequences' are padding, and no fault
+        assert torch.count_nonzero(whole[:2]) == 0 and torch.count_nonzero(whole[-4:]) == 0
+        seqs.check(queries[2:-4], counts, whole[2:-4], 64 ** -0.5, "float16")
+
+        def left_out(lengths, offsets, gone, max_queries=3):
+            out = call(lengths, offsets, max_queries)
+            told()
+            kept = torch.ones(tokens, dtype=torch.bool, device="cuda")
+            kept[gone] = False
+            assert torch.count_nonzero(out[~kept]) == 0 and torch.equal(out[kept], whole[kept])
+
+        first = slice(starts[0], starts[1])
+        for bad in (61, -1):
+            left_out(on_device([bad] + lengths[1:]), on_device(starts), first)
+        # a sequence of more tokens than the call said; one past the tokens' end; ends before starts, and so overlaps
+        left_out(seqs.lengths_on_device, on_device([0] + starts[1:]), first, 4)
+        last = slice(starts[-2], starts[-1])
+        left_out(seqs.lengths_on_device, on_device(starts[:-1] + [tokens + 1]), last)
+        left_out(seqs.lengths_on_device, on_device([-3] + starts[1:]), first)
+        left_out(seqs.lengths_on_device, on_device(starts[:-1] + [starts[-2] - 1]), last)
+
+        one = normal((len(lengths), 4, 64), 6).half()
+        good = call(seqs.lengths_on_device, None, 1, one)
+        out = call(on_device(lengths[:-1] + [1000]), None, 1, one)
+        told()
+        assert torch.count_nonzero(out[-1]) == 0 and torch.equal(out[:-1], good[:-1])
+        none = call(seqs.lengths_on_device[:0], on_device([0]))
+        assert torch.count_nonzero(none) == 0
+
+
 # ---- products ----
 
 def check_multiply(rows, inputs, outputs, group, name, bias=False, spread=1.0, x=None):
