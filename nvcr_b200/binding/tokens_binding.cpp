@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -87,6 +88,17 @@ int type_of(const at::Tensor& t) {
     case at::kBFloat16: return NVCR_SM100_TOKEN_BF16;
     case at::kFloat: return NVCR_SM100_TOKEN_F32;
     default: return -1;
+    }
+}
+
+// The library launches on the current device, and the default stream's handle is the same for all of them. (Asking
+// which one is current takes 0.15 us: not where there is only one.)
+void require_current(int device) {
+    static const int devices = c10::cuda::device_count();
+    if (devices == 1 && device == 0) return;
+    c10::DeviceIndex current = -1;
+    if (c10::cuda::GetDevice(&current) != cudaSuccess || current != device) {
+        throw Refusal{"the tensors are on cuda:" + std::to_string(device) + ", which is not the current CUDA device"};
     }
 }
 
@@ -185,6 +197,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
         require(block.is_cuda(), "tensors must be on a CUDA device");
         const at::ScalarType kind = block.scalar_type();
         const int device = block.get_device();
+        require_current(device);
         const at::IntArrayRef shape = block.sizes();
         const std::int64_t rows = shape[0], width = shape[1];
         const void* const from = strided(block, "block", kind, shape, device);
@@ -227,6 +240,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return guarded(count, 11, [&] {
         const auto* cache = static_cast<const nvcr_sm100_token_cache*>(address(args[0]));
         const int device = small(args[1], "device");
+        require_current(device);
         const at::Tensor& keys = tensor(args[2], "keys");
         const at::Tensor& values = tensor(args[3], "values");
         require(keys.dim() == 3 && is_half(keys), "keys must be a float16 or bfloat16 tensor of three dimensions");
@@ -277,6 +291,7 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return guarded(count, 5, [&] {
         const auto* cache = static_cast<const nvcr_sm100_token_cache*>(address(args[0]));
         const int device = small(args[1], "device"), type = small(args[3], "dtype");
+        require_current(device);
         const at::Tensor& slots = tensor(args[2], "slots");
         require(slots.dim() == 1, "slots have one dimension");
         const std::int64_t tokens = slots.size(0);
@@ -299,6 +314,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
         auto* context = static_cast<nvcr_sm100_token_context*>(address(args[0]));
         const auto* cache = static_cast<const nvcr_sm100_token_cache*>(address(args[1]));
         const int device = small(args[2], "device");
+        require_current(device);
         const at::Tensor& queries = tensor(args[3], "queries");
         const at::Tensor& table = tensor(args[4], "page_table");
         const at::Tensor& lengths = tensor(args[5], "lengths");
@@ -331,6 +347,7 @@ PyObject* multiply(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return guarded(count, 9, [&] {
         const int outputs = small(args[2], "outputs"), inputs = small(args[3], "inputs"), group = small(args[4], "group");
         const int device = small(args[5], "device");
+        require_current(device);
         const at::Tensor& x = tensor(args[6], "x");
         require(x.dim() == 2 && is_half(x), "x must be a float16 or bfloat16 tensor of two dimensions");
         const std::int64_t rows = x.size(0);
@@ -341,6 +358,14 @@ PyObject* multiply(PyObject*, PyObject* const* args, Py_ssize_t count) {
         check(nvcr_sm100_token_multiply(type_of(x), from, x.stride(0), rows, address(args[0]), address(args[1]), outputs,
                                         inputs, group, bias, y.data_ptr(), stream_of(args[8], device)));
         return wrapped(y);
+    });
+}
+
+// on_current(device): refuses another device than the current one.
+PyObject* on_current(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    return guarded(count, 1, [&]() -> PyObject* {
+        require_current(small(args[0], "device"));
+        Py_RETURN_NONE;
     });
 }
 
@@ -357,7 +382,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t count) {
 
 #define TOKEN_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {TOKEN_METHOD(norm),     TOKEN_METHOD(append), TOKEN_METHOD(read), TOKEN_METHOD(attend),
-                         TOKEN_METHOD(multiply), TOKEN_METHOD(bind),   {nullptr, nullptr, 0, nullptr}};
+                         TOKEN_METHOD(multiply), TOKEN_METHOD(on_current), TOKEN_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "nvcr_tokens", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -4,9 +4,10 @@
 ``PagedCache`` holds keys and values in 4 bits, rotated on the way in;
 ``TokenContext.attend`` is attention over such a cache; ``PackedMatrix`` is a
 4-bit weight matrix with group scales. Tensors are torch tensors on the current
-CUDA device; work is enqueued on torch's current stream unless ``stream`` names
-another (then the caller orders the two, and keeps the tensors alive). What the
-operators refuse raises ``ExecutorError``; there is no CPU fallback.
+CUDA device (another one's are refused); work is enqueued on torch's current
+stream unless ``stream`` names another (then the caller orders the two, and keeps
+the tensors alive). What the operators refuse raises ``ExecutorError``; there is
+no CPU fallback.
 
 The 4-bit group form, of caches and weights alike: a group of consecutive values
 is held as codes c in 0..15, two a byte with the even index in the low half, an
@@ -206,6 +207,7 @@ class PackedMatrix:
         outputs, inputs, groups = codes.shape[0], 2 * codes.shape[1], scales.shape[1]
         _require(groups > 0 and inputs % groups == 0, "scales hold a whole number of groups")
         device, index, group = codes.device, codes.get_device(), inputs // groups
+        (_module or _native()).on_current(index)
         addresses = (_whole(codes, "codes", torch.uint8, (outputs, inputs // 2), index),
                      _whole(scales, "scales", torch.float16, (outputs, groups), index),
                      _whole(minimums, "minimums", torch.float16, (outputs, groups), index))

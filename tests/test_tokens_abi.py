@@ -150,3 +150,34 @@ def test_wrappers_refuse_host_tensors(built_library):
         with pytest.raises(ExecutorError) as error:
             call()
         assert error.value.code == ErrorCode.invalid_argument
+
+
+def test_tensors_of_another_device_are_refused(built_library, room):
+    """Fake tensors stand for another device's; each call refuses before it takes an address from one or launches."""
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from nvcr_b200 import tokens
+    from nvcr_b200.executor import ErrorCode, ExecutorError
+
+    def there(*shape, dtype=torch.float16):
+        with FakeTensorMode():
+            return torch.empty(shape, dtype=dtype, device="cuda:1")
+
+    keeper = cache(room)
+    at, native = ctypes.addressof(keeper), tokens._native()
+    keys, slots = there(1, 2, 128), there(1, dtype=torch.int64)
+    assert keys.is_cuda and keys.get_device() == 1
+    refused = [
+        lambda: tokens.block_norm(there(2, 8)),
+        lambda: native.append(at, 1, keys, keys, slots, None, None, None, None, False, None),
+        lambda: native.read(at, 1, slots, 0, None),
+        lambda: native.attend(room, at, 1, there(1, 4, 128), there(1, 4, dtype=torch.int32), there(1, dtype=torch.int32),
+                              None, 1, 64, None, None),
+        lambda: native.multiply(room, room, 4, 64, 64, 1, there(1, 64), None, None),
+        lambda: tokens.PackedMatrix(there(4, 32, dtype=torch.uint8), there(4, 1), there(4, 1)),
+    ]
+    for call in refused:
+        with pytest.raises(ExecutorError, match="not the current CUDA device") as error:
+            call()
+        assert error.value.code == ErrorCode.invalid_argument
