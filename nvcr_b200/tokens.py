@@ -15,6 +15,7 @@ FP16 scale s and an FP16 minimum m, and stands for ``c * s + m``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib.machinery
 import importlib.util
@@ -62,6 +63,16 @@ def _native():
 
 def _stream(stream) -> int | None:
     return None if stream is None else _stream_handle(stream) or 0
+
+
+def _on(stream, device: torch.device):
+    """torch's own operations on a stream given as the operators take one (None: the current stream)."""
+    if stream is None:
+        return contextlib.nullcontext()
+    if isinstance(stream, torch.cuda.Stream):
+        return torch.cuda.stream(stream)
+    handle = _stream(stream)
+    return torch.cuda.stream(torch.cuda.ExternalStream(handle, device) if handle else torch.cuda.default_stream(device))
 
 
 def _whole(tensor: torch.Tensor, name: str, kind: torch.dtype, shape: tuple, index: int) -> int:
@@ -226,13 +237,17 @@ class PackedMatrix:
         """From a float matrix [outputs, inputs], each group by its own range."""
         _require(weights.dim() == 2 and group > 0 and weights.shape[1] % group == 0,
                  "weights have two dimensions and inputs are a multiple of group")
-        parts = weights.float().unflatten(1, (-1, group))
-        low, high = parts.amin(-1), parts.amax(-1)
-        minimums, scales = low.half(), ((high - low) / 15).half()
-        steps = scales.float().unsqueeze(-1)
-        codes = torch.where(steps > 0, torch.round((parts - minimums.float().unsqueeze(-1)) / steps), 0.0)
-        codes = codes.clamp(0, 15).to(torch.uint8).flatten(1)
-        return cls(codes[:, 0::2] | codes[:, 1::2] << 4, scales, minimums, stream)
+        _require(weights.is_cuda, "weights are on a CUDA device")
+        # all of it on one stream, whose allocator takes the codes back when this returns
+        with _on(stream, weights.device):
+            parts = weights.float().unflatten(1, (-1, group))
+            low, high = parts.amin(-1), parts.amax(-1)
+            minimums, scales = low.half(), ((high - low) / 15).half()
+            steps = scales.float().unsqueeze(-1)
+            codes = torch.where(steps > 0, torch.round((parts - minimums.float().unsqueeze(-1)) / steps), 0.0)
+            codes = codes.clamp(0, 15).to(torch.uint8).flatten(1)
+            codes = codes[:, 0::2] | codes[:, 1::2] << 4
+        return cls(codes, scales, minimums, stream)
 
     def multiply(self, x: torch.Tensor, bias: torch.Tensor | None = None, stream=None) -> torch.Tensor:
         """x [rows, inputs] (float16 or bfloat16, any row stride) times the matrix's transpose, plus bias [outputs]."""

@@ -812,6 +812,29 @@ def test_quantised_matrix(cuda):
 
 # ---- streams and graphs ----
 
+@pytest.mark.parametrize("as_handle", [False, True])
+def test_quantised_on_another_stream(cuda, as_handle):
+    """Weights that a busy stream is still writing, quantised on it: nothing of the call runs ahead of that, and what it
+    releases is not reused before that stream has read it."""
+    import torch
+
+    from nvcr_b200.tokens import PackedMatrix
+
+    weights, side = normal((512, 2048), 3, 0.05), torch.cuda.Stream()
+    want = PackedMatrix.quantise(weights, 64)
+    late, product = torch.zeros_like(weights), torch.zeros((4096, 4096), device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):  # milliseconds of work
+            product = product @ product
+        late.copy_(weights)
+    matrix = PackedMatrix.quantise(late, 64, stream=side.cuda_stream if as_handle else side)
+    for _ in range(8):  # takes what this stream's allocator has of the temporaries' sizes, and writes it
+        [torch.full(shape, 255, dtype=torch.uint8, device="cuda") for shape in ((512, 1024), (512, 32, 2), (512, 2048, 4))]
+    torch.cuda.synchronize()
+    assert torch.equal(matrix.codes, want.codes) and torch.equal(matrix.scales, want.scales)
+
+
 def test_another_stream_and_a_graph(cuda):
     """The operators run on torch's current stream, on a named one, and inside a captured graph with new inputs."""
     import torch
