@@ -159,11 +159,13 @@ class PagedCache:
                                            None if stream is None else _stream(stream))
 
     def check(self) -> None:
-        """Waits for the device and raises if a kernel met a slot, position, page number or length out of range since
-        the last check (the token or page was left out)."""
+        """Waits for all streams of the device and raises if a kernel met a slot, position, page number, length or
+        offset out of range since the last check (the token, page or sequence was left out)."""
+        torch.cuda.synchronize(self.device)
         found = int(self.status.item())
         if found:
-            self.status.zero_()
+            self.status.bitwise_and_(~found)  # not the bits of calls that another thread makes meanwhile
+            torch.cuda.current_stream(self.device).synchronize()  # before any stream's next call
             names = [name for bit, name in ((1, "slot"), (2, "position"), (4, "page number"), (8, "length or offset"))
                      if found & bit]
             _refuse(f"out of range on the device: {', '.join(names)}")

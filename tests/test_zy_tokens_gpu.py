@@ -812,6 +812,30 @@ def test_quantised_matrix(cuda):
 
 # ---- streams and graphs ----
 
+def test_check_waits_for_other_streams(cuda):
+    """What a kernel still to run on another stream finds is told by this check, and once."""
+    import torch
+
+    from nvcr_b200.executor import ExecutorError
+    from nvcr_b200.tokens import PagedCache
+
+    cache, side = PagedCache.empty(2, 2, 16, 64, 32), torch.cuda.Stream()
+    x, slots = normal((3, 2, 64), 1).half(), torch.tensor([32, 33, 1], device="cuda")
+    product, others = torch.zeros((4096, 4096), device="cuda"), slots - 30
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        product @ product
+    cache.append(x, x, others, stream=side)  # loading a kernel would wait for the device
+    cache.check()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            product = product @ product
+    cache.append(x, x, slots, stream=side)
+    with pytest.raises(ExecutorError, match="slot"):
+        cache.check()
+    cache.check()
+
+
 @pytest.mark.parametrize("as_handle", [False, True])
 def test_quantised_on_another_stream(cuda, as_handle):
     """Weights that a busy stream is still writing, quantised on it: nothing of the call runs ahead of that, and what it
