@@ -443,7 +443,11 @@ int nvcr_sm100_token_read(const nvcr_sm100_token_cache* cache, int type, const i
                           void* keys, void* values, void* stream);
 
 /* Working memory of nvcr_sm100_token_attend on the current device. A context
- * serves one call at a time: calls that share it belong on one stream. */
+ * serves one call at a time: calls that share it, replays of a graph that
+ * captured one among them, belong on one stream. Creating one may wait for the
+ * device, so it comes before a capture. Destroying one waits for nothing, and
+ * its memory goes to the next context; that of one whose calls were captured is
+ * kept for the graph, for good. */
 typedef struct nvcr_sm100_token_context nvcr_sm100_token_context;
 int nvcr_sm100_token_context_create(nvcr_sm100_token_context** context);
 void nvcr_sm100_token_context_destroy(nvcr_sm100_token_context* context);

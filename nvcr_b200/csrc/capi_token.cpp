@@ -19,6 +19,7 @@
 struct nvcr_sm100_token_context {
     int device = 0;
     nvcr_sm100::token::AttendWorkspace workspace{};
+    bool captured = false;  // a graph holds the workspace's address
 };
 
 int nvcr_sm100::token::sm_count() {
@@ -42,9 +43,10 @@ using nvcr_sm100::report_error;
 using nvcr_sm100::report_ok;
 namespace token = nvcr_sm100::token;
 
-// Workspaces of destroyed contexts, ready for the next ones: their tickets are
-// zero between calls. `contexts` counts those made, so `spares` never grows
-// past its reservation.
+// Workspaces of destroyed contexts for the next ones, which wait for the calls
+// that may still use them; a captured one is nobody's again, as its graph may be
+// replayed. `contexts` counts those made, so `spares` never grows past its
+// reservation.
 std::mutex spare_lock;
 std::vector<std::unique_ptr<nvcr_sm100_token_context>> spares;
 std::size_t contexts = 0;
@@ -186,17 +188,30 @@ int nvcr_sm100_token_context_create(nvcr_sm100_token_context** context) {
         int device = 0;
         cudaError_t status = cudaGetDevice(&device);
         if (status != cudaSuccess) return launched(status);
-        std::lock_guard<std::mutex> guard(spare_lock);
-        auto spare = std::find_if(spares.begin(), spares.end(), [&](const auto& c) { return c->device == device; });
-        if (spare != spares.end()) {
-            *context = spare->release();
-            spares.erase(spare);
-            return report_ok();
+        const std::size_t ticket_bytes = (token::attend_ticket_bytes() + 255) / 256 * 256;
+        {
+            std::unique_lock<std::mutex> guard(spare_lock);
+            auto spare = std::find_if(spares.begin(), spares.end(),
+                                      [&](const auto& c) { return c->device == device && !c->captured; });
+            if (spare != spares.end()) {
+                std::unique_ptr<nvcr_sm100_token_context> found = std::move(*spare);
+                spares.erase(spare);
+                guard.unlock();
+                status = cudaDeviceSynchronize();  // the destroyed context's calls
+                if (status == cudaSuccess) status = cudaMemset(found->workspace.tickets, 0, ticket_bytes);
+                if (status == cudaSuccess) status = cudaStreamSynchronize(nullptr);
+                if (status != cudaSuccess) {
+                    guard.lock();
+                    spares.push_back(std::move(found));
+                    return launched(status);
+                }
+                *context = found.release();
+                return report_ok();
+            }
+            spares.reserve(++contexts);  // so that destroying one needs no memory
         }
-        spares.reserve(++contexts);  // so that destroying one needs no memory
         auto made = std::make_unique<nvcr_sm100_token_context>();
         made->device = device;
-        const std::size_t ticket_bytes = (token::attend_ticket_bytes() + 255) / 256 * 256;
         unsigned char* memory = nullptr;
         status = cudaMalloc(&memory, ticket_bytes + token::attend_partial_bytes());
         if (status == cudaErrorMemoryAllocation) {
@@ -218,12 +233,7 @@ int nvcr_sm100_token_context_create(nvcr_sm100_token_context** context) {
 
 void nvcr_sm100_token_context_destroy(nvcr_sm100_token_context* context) {
     if (context == nullptr) return;
-    // Waits for the calls that use the workspace, as freeing it would, then keeps it for the next context.
-    int current = 0;
-    const bool switched = cudaGetDevice(&current) == cudaSuccess && current != context->device &&
-        cudaSetDevice(context->device) == cudaSuccess;
-    cudaDeviceSynchronize();
-    if (switched) cudaSetDevice(current);
+    // No CUDA call: this may come at any time, in the middle of a capture or of the calls that use the workspace.
     std::lock_guard<std::mutex> guard(spare_lock);
     spares.emplace_back(context);
 }
@@ -259,6 +269,12 @@ int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_
         if (device != context->device) {
             return report_error(Error{Code::invalid_state, "the context belongs to device " +
                                                                std::to_string(context->device)});
+        }
+        if (!context->captured) {
+            cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+            const cudaError_t asked = cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture);
+            if (asked != cudaSuccess) return launched(asked);
+            context->captured = capture != cudaStreamCaptureStatusNone;
         }
         return launched(token::attend(cache_of(*cache),
                                       {static_cast<token::Type>(type), queries, query_stride, query_head_stride, tokens,

@@ -172,7 +172,8 @@ class PagedCache:
 
 
 class TokenContext:
-    """Working memory of attention on the current device; calls that share one belong on one stream."""
+    """Working memory of attention on the current device; calls that share one, replays of graphs that captured one among
+    them, belong on one stream. Make it before a capture; closing it waits for nothing, at any time."""
 
     def __init__(self) -> None:
         handle = ctypes.c_void_p()

@@ -900,3 +900,39 @@ def test_another_stream_and_a_graph(cuda):
         replayed = captured.clone()
         assert torch.equal(step(), replayed)
     context.close()
+
+
+def test_contexts_closed_around_captures(cuda):
+    """Closing a context does not disturb a capture; one that a graph holds is not handed out again, others are."""
+    import torch
+
+    from nvcr_b200.tokens import TokenContext
+
+    seqs = Sequences([20000], 128, 64, 2, 64)  # cut among blocks, which join in the context's memory
+    queries = [normal((1, 8, 128), seed).half() for seed in (1, 2)]
+    call = lambda context, q: context.attend(q, seqs.cache, seqs.table, seqs.lengths_on_device,  # noqa: E731
+                                             max_length=20000)
+    held, other = TokenContext(), TokenContext()
+    want = [call(held, q) for q in queries]
+    graph, holder = torch.cuda.CUDAGraph(), held._handle.value
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = call(held, queries[0])
+        other.close()
+        held.close()
+    with TokenContext() as context:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(20):  # the graph and another context at once
+            graph.replay()
+            with torch.cuda.stream(side):
+                out = call(context, queries[1])
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want[0]) and torch.equal(out, want[1])
+        ordinary = context._handle.value
+    several = [TokenContext() for _ in range(24)]
+    handles = {context._handle.value for context in several}
+    assert ordinary in handles and holder not in handles
+    for context in several:
+        assert torch.equal(call(context, queries[0]), want[0])
+        context.close()
