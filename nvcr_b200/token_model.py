@@ -80,19 +80,22 @@ class TokenModel:
         self.cosines, self.sines = angles.cos().float(), angles.sin().float()
         # every sequence may use any page: they are handed out in an order that is nobody's own
         order = torch.randperm(batch * self.columns, generator=make, device="cuda")
-        self.table = order.view(batch, self.columns).to(torch.int32)
+        # the last column's page is none of a cache's: of the places past a sequence's end
+        self.pages = torch.full((batch, self.columns + 1), batch * self.columns, dtype=torch.int32, device="cuda")
+        self.pages[:, :-1] = order.view(batch, self.columns)
+        self.table = self.pages[:, :-1]
         self.lengths = torch.zeros((batch,), dtype=torch.int32, device="cuda")
 
     def advance(self, symbols: torch.Tensor) -> torch.Tensor:
         """Appends int64 symbols [batch, count] to the sequences and returns the logits [batch, count, symbols] of what
-        follows each. Nothing waits for the host, so that a step can be captured in a CUDA graph."""
+        follows each. Nothing waits for the host, so that a step can be captured in a CUDA graph; symbols past
+        max_length are not stored, their sequence attends to nothing from then on, and `check` tells."""
         config = self.config
         batch, count = symbols.shape
         nth = torch.arange(count, device="cuda", dtype=torch.int32)
         places = (self.lengths[:, None] + nth).flatten()
         self.lengths += count
-        pages = self.table.gather(1, (places.view(batch, count) // self.page_size).long()).flatten()
-        slots = pages.long() * self.page_size + places % self.page_size
+        slots = self._slots(self.pages, places.view(batch, count), self.page_size)
         offsets = torch.arange(0, batch * count + 1, count, device="cuda", dtype=torch.int32)
         hidden, delta = self.embedding[symbols.flatten()], None
         heads = config.heads, config.kv_heads, config.kv_heads
@@ -111,6 +114,12 @@ class TokenModel:
             after, gate = layer.after[1], layer.gates[1]
         _, normed = self._between(hidden, delta, after, gate, self.last_norm)
         return self.head.multiply(normed).view(batch, count, -1)
+
+    @staticmethod
+    def _slots(pages: torch.Tensor, places: torch.Tensor, page_size: int) -> torch.Tensor:
+        """The slots of places [batch, count]; past the table's end all are the first one past the cache's."""
+        places = places.clamp(max=(pages.shape[1] - 1) * page_size)
+        return (pages.gather(1, (places // page_size).long()).long() * page_size + places % page_size).flatten()
 
     @staticmethod
     def _between(hidden, delta, after, gate, before):

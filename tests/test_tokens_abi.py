@@ -181,3 +181,16 @@ def test_tensors_of_another_device_are_refused(built_library, room):
         with pytest.raises(ExecutorError, match="not the current CUDA device") as error:
             call()
         assert error.value.code == ErrorCode.invalid_argument
+
+
+def test_places_past_the_page_table_become_no_slot():
+    """The model's slots on the CPU, where an index out of range raises (on the device it would end the process)."""
+    import torch
+
+    from nvcr_b200.token_model import TokenModel
+
+    pages = torch.tensor([[2, 0, 4], [3, 1, 4]], dtype=torch.int32)  # two columns, and one of no page
+    places = torch.tensor([[0, 17, 31, 32, 33], [15, 16, 47, 48, 1 << 30]], dtype=torch.int32)
+    slots = TokenModel._slots(pages, places, 16)
+    assert slots.dtype == torch.int64
+    assert slots.tolist() == [32, 1, 15, 64, 64, 63, 16, 64, 64, 64]

@@ -119,3 +119,32 @@ def test_the_command_runs(cuda, capsys, monkeypatch):
     monkeypatch.setattr(sys, "argv", ["token_model", "--batch", "2", "--prompt", "5", "--steps", "3", "--layers", "1"])
     token_model.main()
     assert "us a step" in capsys.readouterr().out
+
+
+def test_steps_past_the_longest_sequence_are_told(cuda):
+    """Symbols past max_length are left out and told, by a prompt and step by step; nothing stored changes."""
+    import torch
+
+    from nvcr_b200.executor import ExecutorError
+    from nvcr_b200.token_model import TokenModel, TokenModelConfig
+
+    config = TokenModelConfig(layers=1, width=128, heads=2, kv_heads=1, head_dim=64, inner=128, symbols=32)
+    for counts in ((20, 12, 1, 1, 30), (20, 5, 9, 1)):
+        model = TokenModel(config, batch=2, max_length=32)
+        make = torch.Generator(device="cuda").manual_seed(1)
+        prompt = torch.randint(0, config.symbols, (2, counts[0]), generator=make, device="cuda")
+        model.advance(prompt)
+        at = counts[0]
+        for count in counts[1:]:
+            before = [t.clone() for t in model.caches[0].tensors]
+            logits = model.advance(prompt[:, :1].expand(2, count).contiguous())
+            at += count
+            assert logits.shape == (2, count, config.symbols) and torch.isfinite(logits).all()
+            if at <= 32:
+                model.check()
+                continue
+            with pytest.raises(ExecutorError, match="slot, length or offset"):
+                model.check()
+            if at - count >= 32:
+                for t, old in zip(model.caches[0].tensors, before):
+                    assert torch.equal(t, old)
