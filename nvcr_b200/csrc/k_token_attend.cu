@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(32 * warps, 1) attend_kernel(const Work work) 
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
 #pragma unroll
-                    for (int far = 0; far < 2; ++far) largest[g] = fmaxf(largest[g], value_pair(h, far, g).x);
+                    for (int far = 0; far < 2; ++far) largest[g] = fmaxf(largest[g], fabsf(value_pair(h, far, g).x));
                 }
                 raise |= largest[g] > value_top[g];
             }

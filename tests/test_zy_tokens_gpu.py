@@ -552,6 +552,25 @@ def test_attend_scores_of_every_size(cuda):
     attend(seqs, [2], 4, "float16")
 
 
+@pytest.mark.parametrize("factor,lengths,spread", [(2.0 ** -17, [40, 23], 1.0), (1.0, [700, 90], 1.0),
+                                                   (2.0 ** 14, [3000, 500], 6.0)])
+@pytest.mark.parametrize("share", [0.5, 1.0])
+def test_attend_negative_scales(cuda, factor, lengths, spread, share):
+    """Groups of keys and values whose scale is negative, some or all of them: values whose weights are float16's smallest
+    numbers unless they are scaled, ordinary ones, and ones whose weights pass float16 with a rising maximum."""
+    import torch
+
+    seqs = Sequences(lengths, 128, 32, 1, 16)
+    make = torch.Generator(device="cuda").manual_seed(9)
+    for which, by in ((1, 1.0), (3, factor)):
+        pairs = seqs.cache.tensors[which]
+        turned = torch.rand(pairs.shape[:-1], generator=make, device="cuda") < share
+        scales, minimums = pairs[..., 0].float() * by, pairs[..., 1].float() * by
+        pairs[..., 0] = torch.where(turned, -scales, scales).half()
+        pairs[..., 1] = torch.where(turned, minimums + 15.0 * scales, minimums).half()  # nearly the same values' range
+    attend(seqs, [2, 1], 4, "bfloat16", spread=spread)
+
+
 def test_attend_large_queries(cuda):
     """bfloat16 queries past FP16's range, and float16 ones at its ends."""
     attend(Sequences([90, 40], 128, 64, 1, 16), [1, 1], 8, "bfloat16", spread=1e6, scale=1e-7)
