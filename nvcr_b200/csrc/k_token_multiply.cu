@@ -88,6 +88,32 @@ __host__ __device__ constexpr int x_bytes(int steps, int rows) {
     return x > own ? x : own;
 }
 
+// One output of one row, value by value in the order of the inputs: an output that is no finite number is taken again
+// here, as an infinite x times codes and minimums apart is no number where x times their values is an infinity (and 128
+// times a bfloat16 sum may overflow). A row of 4096 inputs with an infinity takes 120 us to 4096 outputs; a NaN ends the
+// loop.
+template <typename T, int G>
+__device__ __noinline__ float product_of_values(const T* x, const unsigned* codes, const unsigned* pairs, int inputs,
+                                                int steps, int output) {
+    constexpr int groups = step_inputs / G;
+    const int row = output % 16, r = row % 8, far = row / 8;
+    const std::int64_t first = static_cast<std::int64_t>(output / 16) * steps;
+    float sum = 0.0f;
+    for (int octet = 0; octet < inputs / 8 && sum == sum; ++octet) {
+        const std::int64_t step = first + octet / 16;
+        const int part = octet / 8 % 2, word = octet / 4 % 2 * 2 + far;
+        const unsigned code = codes[step * 256 + part * 128 + (r * 4 + octet % 4) * 4 + word];
+        const unsigned pair = pairs[(step * groups + octet % 16 * 8 / G) * 16 + r * 2 + far];
+        const float scale = half_bits(static_cast<std::uint16_t>(pair));
+        const float minimum = half_bits(static_cast<std::uint16_t>(pair >> 16));
+        for (int i = 0; i < 8; ++i) {
+            const float c = static_cast<float>(code >> (4 * (i / 2 + i % 2 * 4)) & 15u);
+            sum = fmaf(widen(x[octet * 8 + i]), fmaf(c, scale, minimum), sum);
+        }
+    }
+    return sum;
+}
+
 template <typename T, int G, int NT>
 __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs a, const Shape shape) {
     constexpr bool half = std::is_same_v<T, __half>;
@@ -280,6 +306,11 @@ __global__ void __launch_bounds__(32 * warps) multiply_kernel(const MultiplyArgs
         const int output = (first_tile + e / sum_floats<NT>) * 16 + e % 16;
         const std::int64_t row = first_row + e % sum_floats<NT> / 16;
         if (output >= a.outputs || row >= a.rows) return;
+        if (!(fabsf(value) < INFINITY)) {
+            value = product_of_values<T, G>(static_cast<const T*>(a.x) + row * a.x_stride,
+                                            reinterpret_cast<const unsigned*>(a.codes),
+                                            reinterpret_cast<const unsigned*>(a.scales), a.inputs, shape.steps, output);
+        }
         if (a.bias != nullptr) value += widen(static_cast<const T*>(a.bias)[output]);
         static_cast<T*>(a.y)[row * a.outputs + output] = narrow<T>(value);
     };

@@ -803,6 +803,37 @@ def test_multiply_values_of_every_size(cuda):
     near(y[[0, 2, 4]], want[[0, 2, 4]], tolerance[[0, 2, 4]], "float16")
 
 
+@pytest.mark.parametrize("name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("inputs,outputs,rows", [(512, 100, 7), (4096, 16, 16), (8192, 1500, 9), (384, 2500, 3)])
+def test_multiply_infinities(cuda, inputs, outputs, rows, group, name):
+    """An infinity times a weight has the weight's sign, opposite ones and zero weights give NaN; other rows are as ever."""
+    import torch
+
+    make = torch.Generator(device="cuda").manual_seed(inputs + rows)
+    x = normal((rows, inputs), 5).to(kind_of(name))
+    at = torch.randint(0, inputs, (rows,), generator=make, device="cuda")
+    for row in range(0, rows, 2):
+        x[row, at[row]] = math.inf if row % 4 == 0 else -math.inf
+    x[rows - 1, at[0]], x[rows - 1, at[rows - 1]] = math.inf, -math.inf
+    y, want, tolerance = check_multiply(rows, inputs, outputs, group, name, x=x)
+    near(y, want, tolerance, name)
+    infinite = want.isinf()
+    assert infinite.any() and torch.equal(y.double()[infinite], want[infinite])
+    assert want[rows - 1].isnan().any() or at[0] == at[rows - 1]  # the row with both
+
+
+def test_multiply_sums_past_a_row_of_codes(cuda):
+    """bfloat16 rows whose products are finite while 128 times a group's sum is not."""
+    import torch
+
+    x = torch.full((2, 256), 2.0 ** 120, dtype=torch.bfloat16, device="cuda")
+    x[1, ::2] = -(2.0 ** 120)
+    y, want, tolerance = check_multiply(2, 256, 40, 128, "bfloat16", x=x)
+    assert torch.isfinite(want).all() and float(want.abs().max()) < 3e38
+    near(y, want, tolerance, "bfloat16")
+
+
 def test_multiply_unaligned_rows(cuda):
     import torch
 
