@@ -237,7 +237,9 @@ class PackedMatrix:
 
     @classmethod
     def quantise(cls, weights: torch.Tensor, group: int = 64, stream=None) -> "PackedMatrix":
-        """From a float matrix [outputs, inputs], each group by its own range."""
+        """From a float matrix [outputs, inputs], each group by its own range, as `PagedCache.append` stores one:
+        m = fp16(min), s = fp16((max - min) * (1 / 15)), or 2^-24 where that is 0 and the range is not, and
+        c = clamp(rint((x - m) / s), 0, 15), from FP32."""
         _require(weights.dim() == 2 and group > 0 and weights.shape[1] % group == 0,
                  "weights have two dimensions and inputs are a multiple of group")
         _require(weights.is_cuda, "weights are on a CUDA device")
@@ -245,7 +247,9 @@ class PackedMatrix:
         with _on(stream, weights.device):
             parts = weights.float().unflatten(1, (-1, group))
             low, high = parts.amin(-1), parts.amax(-1)
-            minimums, scales = low.half(), ((high - low) / 15).half()
+            fifteenth = torch.tensor(1.0 / 15.0, dtype=torch.float32)  # a number of the host's: no copy, and FP32
+            minimums, scales = low.half(), ((high - low) * fifteenth).half()
+            scales = torch.where((scales == 0) & (high > low), 2.0 ** -24, scales)
             steps = scales.float().unsqueeze(-1)
             codes = torch.where(steps > 0, torch.round((parts - minimums.float().unsqueeze(-1)) / steps), 0.0)
             codes = codes.clamp(0, 15).to(torch.uint8).flatten(1)

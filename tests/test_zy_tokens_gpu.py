@@ -860,6 +860,25 @@ def test_quantised_matrix(cuda):
     assert ((back.unflatten(1, (-1, 32)) - parts).abs() <= limit).all()
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantised_matrix_is_the_header_s_form(cuda, group):
+    """The same codes, scales and minimums as the formula in FP32 on the host, ranges too small for a float16 step too."""
+    import torch
+
+    from nvcr_b200.tokens import PackedMatrix
+
+    weights = normal((48, 512), 4, 0.05, 0.01)
+    weights[::3] *= 1e-6  # steps among float16's smallest numbers, and below them
+    weights[1::3] = weights[1::3] * 1e-8 + 2.0 ** -20
+    weights[5] = 0.25
+    weights[6] = 0.0
+    codes, scales, minimums = quantised_fp32(weights.cpu().numpy(), group)
+    assert (scales == 2.0 ** -24).any() and (scales == 0).any()
+    on_device = [torch.from_numpy(a).cuda() for a in (codes[:, 0::2] | codes[:, 1::2] << 4, scales, minimums)]
+    want, got = PackedMatrix(*on_device), PackedMatrix.quantise(weights, group)
+    assert torch.equal(got.scales, want.scales) and torch.equal(got.codes, want.codes)
+
+
 # ---- streams and graphs ----
 
 def test_check_waits_for_other_streams(cuda):
