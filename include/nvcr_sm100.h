@@ -386,7 +386,8 @@ int nvcr_sm100_dcvc_ycbcr_padded_to_yuv420p8(const uint16_t* input, int32_t batc
  *   hidden = residual_scale * residual + gate * p
  *   normed = N(hidden; pre_weight, pre_bias)
  * N(v) = v / sqrt(mean(v^2) + epsilon) * (weight + weight_offset) + bias, of
- * v - mean(v) when `layer` is not 0. `rows` rows of `width` values of `type`;
+ * v - mean(v) when `layer` is not 0. `rows` rows of `width` (at most 2^30) values
+ * of `type`;
  * residual and gate may be NULL (no term; one), a gate_stride of 0 gives every
  * row the same gate; NULL weights are one and NULL biases zero; hidden and
  * normed are contiguous and either may be NULL. FP32 inside; normed is taken
@@ -456,7 +457,7 @@ void nvcr_sm100_token_context_destroy(nvcr_sm100_token_context* context);
  * and values (the new tokens' own already appended). Sequence b's new tokens
  * are query_offsets[b] .. query_offsets[b + 1] - 1 (NULL: token b), at most
  * max_queries of them; its length, new tokens included, is lengths[b], at most
- * max_length; place t is on page page_table[b * table_stride + t / page_size],
+ * max_length, which is at most 2^30; place t is on page page_table[b * table_stride + t / page_size],
  * and page_table has table_pages columns. A token sees the places up to its
  * own. Query head h reads cache head h / (heads / kv_heads). Scores are scaled
  * by `scale`; output [tokens][heads][head_dim] of `type` (F16 or BF16), 16-byte

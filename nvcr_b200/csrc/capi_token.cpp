@@ -76,6 +76,8 @@ bool half_type(int type) { return type == NVCR_SM100_TOKEN_F16 || type == NVCR_S
 bool any_type(int type) { return half_type(type) || type == NVCR_SM100_TOKEN_F32; }
 
 constexpr std::int64_t most_rows = std::numeric_limits<std::int32_t>::max();
+// Kernels walk a row, or look ahead in a sequence, in steps that pass its end: 32-bit places stay clear of 2^31.
+constexpr std::int32_t most_places = 1 << 30;
 
 // Null when the cache's shape and buffers can be used, else why not.
 const char* cache_refusal(const nvcr_sm100_token_cache* cache) {
@@ -110,7 +112,7 @@ token::Cache cache_of(const nvcr_sm100_token_cache& cache) {
 
 // 8 rows of 98304 inputs fit the shared memory of a cluster of eight blocks.
 bool matrix_shape(std::int32_t outputs, std::int32_t inputs, std::int32_t group) {
-    return outputs > 0 && inputs > 0 && inputs <= 98304 && (group == 32 || group == 64 || group == 128) && inputs % group == 0;
+    return outputs > 0 && outputs <= most_rows - 15 && inputs > 0 && inputs <= 98304 && (group == 32 || group == 64 || group == 128) && inputs % group == 0;
 }
 
 }  // namespace
@@ -124,7 +126,7 @@ int nvcr_sm100_token_norm(int type, int layer, int post, const void* block, int6
                           float epsilon, void* stream) {
     return guarded([&] {
         if (!any_type(type)) return refuse("unknown type");
-        if (rows < 0 || rows > most_rows || width <= 0) return refuse("rows or width out of range");
+        if (rows < 0 || rows > most_rows || width <= 0 || width > most_places) return refuse("rows or width out of range");
         if (rows > 0 && hidden == nullptr && normed == nullptr) return refuse("neither hidden nor normed is wanted");
         if (rows > 0 && block == nullptr) return refuse("null block");
         if (!(epsilon >= 0.0f)) return refuse("epsilon must not be negative");
@@ -253,6 +255,7 @@ int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_
         }
         if (max_queries <= 0 || max_queries > 65535) return refuse("max_queries out of range");
         if (query_offsets == nullptr && tokens != batch) return refuse("without query_offsets there is one token a sequence");
+        if (max_length > most_places) return refuse("max_length is at most 2^30");
         if (max_length < 0 || table_pages < 0 ||
             max_length > static_cast<std::int64_t>(table_pages) * cache->page_size) {
             return refuse("max_length needs more pages than page_table has");

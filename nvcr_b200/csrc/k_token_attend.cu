@@ -973,9 +973,11 @@ cudaError_t launch(Work& work, cudaStream_t stream) {
     // the blocks that run at once, and no more than there can be units
     constexpr int unit = 16 * together<D, NT> * warps;
     const std::int64_t rows = static_cast<std::int64_t>(work.a.max_queries) * work.ratio;
-    const std::int64_t units = static_cast<std::int64_t>(work.a.batch) * work.cache.kv_heads * ((rows + 8 * NT - 1) / (8 * NT)) *
-        std::max(1, (work.a.max_length + unit - 1) / unit);
-    if (units > 0x7fffffff) return cudaErrorInvalidValue;
+    const std::int64_t segments = static_cast<std::int64_t>(work.a.batch) * work.cache.kv_heads * ((rows + 8 * NT - 1) / (8 * NT));
+    const std::int64_t most = 0x7fffffff, each = std::max(1, (work.a.max_length + unit - 1) / unit);  // the kernel's are 32 bits
+    constexpr int lead_units = (lead_keys + unit - 1) / unit;
+    if (segments > most || segments * (each + lead_units) > most) return cudaErrorInvalidValue;
+    const std::int64_t units = segments * each;
     const std::int64_t grid = std::min<std::int64_t>(std::min(sm_count(), most_blocks), units);
     return kernels::launch_overlapped(attend_kernel<T, D, G, NT>, dim3(static_cast<unsigned>(grid)), dim3(32 * warps), bytes,
                                       stream, static_cast<const Work&>(work));

@@ -194,3 +194,21 @@ def test_places_past_the_page_table_become_no_slot():
     slots = TokenModel._slots(pages, places, 16)
     assert slots.dtype == torch.int64
     assert slots.tolist() == [32, 1, 15, 64, 64, 63, 16, 64, 64, 64]
+
+
+def test_sizes_past_32_bit_places_are_refused(lib, room):
+    """A row, a sequence or a matrix whose last places' 32-bit successors would overflow."""
+    last = (1 << 31) - 1
+    sizes = [ctypes.byref(ctypes.c_size_t(0)) for _ in range(2)]
+    for outputs in (last, last - 14):
+        assert lib.nvcr_sm100_token_packed_bytes(outputs, 32, 32, *sizes) == INVALID
+        assert lib.nvcr_sm100_token_multiply(0, room, 32, 1, room, room, outputs, 32, 32, None, room, None) == INVALID
+    assert lib.nvcr_sm100_token_packed_bytes(last - 15, 32, 32, *sizes) == 0
+    for width in (last, (1 << 30) + 1):
+        assert lib.nvcr_sm100_token_norm(0, 0, 0, room, width, None, 0, None, 0, None, None, None, None, room, None, 2,
+                                         width, 1.0, 0.0, 1e-6, None) == INVALID
+    at = ctypes.addressof(keeper := cache(room))
+    for length in (last, (1 << 30) + 1):
+        changes = dict(max_length=length, columns=1 << 27)
+        assert lib.nvcr_sm100_token_attend(room, at, *attend_args(room, **changes)) == INVALID
+    del keeper

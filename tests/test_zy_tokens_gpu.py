@@ -713,6 +713,24 @@ def test_attend_tokens_of_no_sequence_are_zeros(cuda, repeat):
         assert torch.count_nonzero(none) == 0
 
 
+def test_attend_refuses_more_work_than_it_can_count(cuda):
+    """Upper bounds of the schedule past 32 bits, and past 64."""
+    import torch
+
+    from nvcr_b200.executor import ErrorCode, ExecutorError
+    from nvcr_b200.tokens import PagedCache, TokenContext
+
+    cache, queries = PagedCache.empty(1, 1, 16, 64, 32), torch.zeros((1, 64, 64), dtype=torch.float16, device="cuda")
+    lengths = torch.zeros((65535,), dtype=torch.int32, device="cuda")
+    offsets = torch.zeros((65536,), dtype=torch.int32, device="cuda")
+    with TokenContext() as context:
+        for columns, length, most in ((1, 16, 65535), (1 << 23, 1 << 27, 65535), (1 << 23, 1 << 27, 1)):
+            table = torch.zeros((1, columns), dtype=torch.int32, device="cuda").expand(65535, columns)
+            with pytest.raises(ExecutorError) as error:
+                context.attend(queries, cache, table, lengths, query_offsets=offsets, max_queries=most, max_length=length)
+            assert error.value.code == ErrorCode.invalid_argument
+
+
 # ---- products ----
 
 def check_multiply(rows, inputs, outputs, group, name, bias=False, spread=1.0, x=None):
