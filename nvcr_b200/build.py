@@ -1,5 +1,6 @@
 """Builds libnvcr_sm100.so in-tree (nvcr_b200/_build/) for sm_100a, and the
-Python binding of its token operators (nvcr_tokens.so, against torch's headers).
+Python binding of its token operators (nvcr_tokens.so, against the headers of
+the torch that is installed; without one there is no binding, nor a use for it).
 
 CUDA sources: nvcc -gencode arch=compute_100a,code=sm_100a -lineinfo -O3
 -fmad=false (no FP contraction; denormals kept, IEEE division) and no fast
@@ -11,6 +12,8 @@ machine without a GPU driver (symbols can be listed; compute calls fail).
 from __future__ import annotations
 
 import concurrent.futures
+import importlib.metadata
+import importlib.util
 import os
 import subprocess
 import sysconfig
@@ -75,10 +78,23 @@ def build(verbose: bool = False) -> Path:
     return LIBRARY
 
 
-def build_binding(verbose: bool = False) -> Path:
-    """The token operators' extension module, linked to the library beside it."""
+def _torch_identity() -> str | None:
+    """Version and place of the torch that is installed, without importing it; None where there is none."""
+    spec = importlib.util.find_spec("torch")
+    return None if spec is None else f"{importlib.metadata.version('torch')} {spec.origin}"
+
+
+def build_binding(verbose: bool = False) -> Path | None:
+    """The token operators' extension module, linked to the library beside it; built anew when torch is another one.
+    None without torch."""
+    identity, stamp = _torch_identity(), BINDING.with_suffix(".torch")
+    if identity is None:
+        if verbose:
+            print("no torch: the token operators' binding is not built")
+        return None
     newest_dep = max(p.stat().st_mtime for p in (BINDING_SOURCE, INCLUDE / "nvcr_sm100.h"))
-    if BINDING.exists() and BINDING.stat().st_mtime >= newest_dep:
+    if (BINDING.exists() and BINDING.stat().st_mtime >= newest_dep and stamp.exists()
+            and stamp.read_text() == identity):
         return BINDING
     import torch
 
@@ -92,6 +108,7 @@ def build_binding(verbose: bool = False) -> Path:
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{result.stdout}\n{result.stderr}")
+    stamp.write_text(identity)
     if verbose:
         print(f"built {BINDING}")
     return BINDING

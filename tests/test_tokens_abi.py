@@ -212,3 +212,22 @@ def test_sizes_past_32_bit_places_are_refused(lib, room):
         changes = dict(max_length=length, columns=1 << 27)
         assert lib.nvcr_sm100_token_attend(room, at, *attend_args(room, **changes)) == INVALID
     del keeper
+
+
+def test_binding_follows_torch(built_library, monkeypatch):
+    """Built anew for another torch, not for the same one; without torch the library alone is built."""
+    from nvcr_b200 import build
+
+    class Compiled(Exception):
+        pass
+
+    def compiler(*_args, **_options):
+        raise Compiled
+
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    assert build.build() == build.LIBRARY and build.build_binding() == build.BINDING
+    monkeypatch.setattr(build.importlib.metadata, "version", lambda _name: "0.0.1")
+    with pytest.raises(Compiled):
+        build.build_binding()
+    monkeypatch.setattr(build.importlib.util, "find_spec", lambda _name: None)
+    assert build.build_binding() is None and build.build() == build.LIBRARY
