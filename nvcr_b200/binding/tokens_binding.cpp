@@ -13,6 +13,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -174,8 +175,8 @@ PyObject* guarded(Py_ssize_t given, Py_ssize_t wanted, F&& body) {
         raised = PyObject_CallFunction(check_function, "i", failure.status);
     } catch (const Raised&) {
         return nullptr;
-    } catch (const std::exception& exception) {
-        PyErr_SetString(PyExc_RuntimeError, exception.what());
+    } catch (...) {  // torch's own exceptions as torch raises them
+        torch::translate_exception_to_python(std::current_exception());
         return nullptr;
     }
     if (raised != nullptr) {  // neither returns without raising

@@ -1023,3 +1023,21 @@ def test_contexts_closed_around_captures(cuda):
     for context in several:
         assert torch.equal(call(context, queries[0]), want[0])
         context.close()
+
+
+def test_output_that_does_not_fit_raises_torch_s_error(cuda):
+    """The allocator's refusal arrives as what a program around torch catches, and the next call runs."""
+    import torch
+
+    from nvcr_b200 import tokens
+
+    block = torch.zeros((1, 1 << 20), dtype=torch.float16, device="cuda")
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.01)  # torch's own bound: no memory is taken
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            tokens.block_norm(block.expand(2000, 1 << 20))
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    hidden, _ = tokens.block_norm(block)
+    assert torch.equal(hidden, block)
