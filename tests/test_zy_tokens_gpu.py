@@ -532,6 +532,14 @@ def test_attend_many_rows_of_many_sequences(cuda, dim, group, name):
     attend(Sequences(lengths, dim, group, 2, 48), counts, 10, name)
 
 
+@pytest.mark.parametrize("name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim,group,kv_heads,heads", [(64, 32, 2, 8), (128, 64, 1, 5), (128, 128, 2, 4), (256, 64, 1, 4)])
+def test_attend_prompts(cuda, dim, group, kv_heads, heads, name):
+    """Prompts of hundreds of tokens, alone and packed, some behind tokens that are cached already."""
+    attend(Sequences([611], dim, group, kv_heads, 16), [611], heads, name)
+    attend(Sequences([400, 1, 333, 900], dim, group, kv_heads, 48), [400, 1, 130, 257], heads, name)
+
+
 @pytest.mark.parametrize("length", [1000, 4095, 20000])
 def test_attend_long(cuda, length):
     """Work that is split over the length and joined."""
