@@ -367,12 +367,17 @@ int nvcr_sm100_dcvc_ycbcr_padded_to_yuv420p8(const uint16_t* input, int32_t batc
                                              int32_t width, int32_t visible_width, int32_t visible_height,
                                              uint8_t* output, void* stream);
 
-/* Token operators: one step of a token model in low-bit form (an autoregressive
- * context model over a codec's symbols, or a language model beside the codec).
- * No counterpart in the reference. All tensors are in device memory, strides
- * are in elements, last dimensions are contiguous, and every call enqueues on
- * `stream` (a cudaStream_t; NULL for the default stream) and returns; a refused
- * call (NVCR_SM100_INVALID_ARGUMENT) enqueues nothing.
+/* Token operators: one step of a language model in low-bit form, beside the
+ * codec. No counterpart in the reference. All tensors are in the current
+ * device's memory, strides are in elements, last dimensions are contiguous, and
+ * every call enqueues on `stream` (a cudaStream_t; NULL for the default stream)
+ * and returns; a refused call (NVCR_SM100_INVALID_ARGUMENT) enqueues nothing.
+ *
+ * The same call on the same kind of GPU gives the same bits. A token's bits may
+ * change with the rest of its call (the number of rows, the other sequences)
+ * and with the number of SMs, as those decide the order of sums: a prompt and
+ * its single steps agree to rounding, not to the bit, so an entropy coder's
+ * two sides must not depend on these functions.
  *
  * The 4-bit group form: `group` consecutive values (32, 64 or 128) are held as
  * codes c in 0..15, two a byte with the even index in the low half, an FP16
@@ -390,8 +395,8 @@ int nvcr_sm100_dcvc_ycbcr_padded_to_yuv420p8(const uint16_t* input, int32_t batc
  * of `type`;
  * residual and gate may be NULL (no term; one), a gate_stride of 0 gives every
  * row the same gate; NULL weights are one and NULL biases zero; hidden and
- * normed are contiguous and either may be NULL. FP32 inside; normed is taken
- * from the unrounded sum. hidden may be residual's buffer and normed block's
+ * normed are contiguous and either may be NULL. FP32 inside (a row whose squares sum
+ * past its range has no norm); normed is taken from the unrounded sum. hidden may be residual's buffer and normed block's
  * (same rows and strides); no other overlap. */
 int nvcr_sm100_token_norm(int type, int layer, int post, const void* block, int64_t block_stride, const void* residual,
                           int64_t residual_stride, const void* gate, int64_t gate_stride, const void* post_weight,
@@ -400,7 +405,8 @@ int nvcr_sm100_token_norm(int type, int layer, int post, const void* block, int6
                           float epsilon, void* stream);
 
 /* A paged cache of keys and values in 4 bits; slot p * page_size + i is place i
- * of page p. The buffers are the caller's. head_dim is 64, 128 or 256, group
+ * of page p. The buffers are the caller's. kv_heads is at most 65535, head_dim
+ * 64, 128 or 256, group
  * 32, 64 or 128 with 1, 2 or 4 groups a head, page_size a multiple of 16.
  * Kernels OR into *status (may be NULL) what they find wrong in device data,
  * and leave the token, page or sequence concerned out: 1 a slot past the end,
@@ -463,7 +469,10 @@ void nvcr_sm100_token_context_destroy(nvcr_sm100_token_context* context);
  * by `scale`; output [tokens][heads][head_dim] of `type` (F16 or BF16), 16-byte
  * aligned, zeros for a token that sees nothing, that belongs to no sequence
  * (the offsets need not begin at 0 nor end at `tokens`), or whose sequence is
- * left out. FP32 softmax and sums. */
+ * left out. Scores, softmax and sums are FP32; a softmax weight times a group's
+ * scale is rounded to FP16 (2^-11 of itself, the group's largest magnitude so
+ * far scaled to 2^5 .. 2^6), as the tensor cores take it. batch, heads and
+ * max_queries are at most 65535. */
 int nvcr_sm100_token_attend(nvcr_sm100_token_context* context, const nvcr_sm100_token_cache* cache, int type,
                             const void* queries, int64_t query_stride, int64_t query_head_stride, int64_t tokens,
                             int32_t heads, const int32_t* page_table, int64_t table_stride, int32_t table_pages,
@@ -477,9 +486,11 @@ int nvcr_sm100_token_packed_bytes(int32_t outputs, int32_t inputs, int32_t group
                                   size_t* scale_bytes);
 int nvcr_sm100_token_pack(const uint8_t* codes, const uint16_t* scales, const uint16_t* minimums, int32_t outputs,
                           int32_t inputs, int32_t group, void* packed_codes, void* packed_scales, void* stream);
-/* y[r][n] = sum_k x[r][k] w[n][k] + bias[n] for `rows` rows of x (F16 or BF16);
- * bias may be NULL; y is contiguous. Made for a few rows: each 16 rows read
- * the weights once. FP32 sums. */
+/* y[r][n] = sum_k x[r][k] w[n][k] + bias[n] for `rows` (at most 65535) rows of
+ * x (F16 or BF16); bias may be NULL; y is contiguous. Made for a few rows: each
+ * 8 or 16 rows read the weights once. FP32 sums, of x times the codes (for BF16
+ * times 128 + c, whose 128 is taken out again: a group's rounding is that of
+ * numbers about ten times as large) and of x alone. */
 int nvcr_sm100_token_multiply(int type, const void* x, int64_t x_stride, int64_t rows, const void* packed_codes,
                               const void* packed_scales, int32_t outputs, int32_t inputs, int32_t group,
                               const void* bias, void* y, void* stream);

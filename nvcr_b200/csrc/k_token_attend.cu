@@ -38,12 +38,12 @@
 // last of them, in order: the same bits every time.
 //
 // Measured on a B200: 131072 keys, 32 heads over 8 of 128 channels, one token
-// (142.6 MB): 47.3 us, 3.0 TB/s; 32 sequences of 1 to 4096 keys (76 MB): 35.0 us; 200
+// (142.6 MB): 47.4 us, 3.0 TB/s; 32 sequences of 1 to 4096 keys (76 MB): 35.5 us; 200
 // keys: 5.5 us. What bounds a long stream is the integer pipe that takes the
-// codes apart (168 of 327 instructions a run of 16 keys, at half rate) and the
-// warps' latency: 141 cycles a run an SM. Two blocks an SM with 128 registers a
-// thread took 135 cycles a run (109 with the values' conversion left out), but twice
-// the fixed work: 6.3 us for 200 keys. Short calls are bound by the chain lengths -> page
+// codes apart (174 of a launch's 348 instructions for each run of 16 keys, at half
+// rate) and the warps' latency: 171 cycles a run while an SM is active. Two blocks an
+// SM with 128 registers a thread streamed as fast (47.2 us), but had twice the fixed
+// work: 6.3 us for 200 keys. Short calls are bound by the chain lengths -> page
 // table -> cache -> join, about 1 us a link.
 #include "token_elements.cuh"
 
@@ -92,7 +92,7 @@ __device__ __forceinline__ unsigned transpose8x8(unsigned v) {
 }
 
 // Nibbles 0 and 4 (even) or 1 and 5 (odd) of a word as the FP16 pair c - 8: under the exponent of 1024 they read
-// 1024 + c and 1024 + 16 c.
+// 1024 + c and 1024 + 16 c. (Published for 4-bit weights by Kim, Henry, Fahim and Awadalla, 2022, arXiv 2211.10017.)
 __device__ __forceinline__ unsigned even_codes(unsigned v) {
     unsigned codes;
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(codes) : "r"((v & 0x000f000fu) | 0x64006400u), "r"(0x64086408u));

@@ -22,10 +22,11 @@
 // cluster divide the inputs and are summed over distributed shared memory. All
 // sums are in a fixed order: no atomics, no workspace, one launch.
 //
-// Measured on a B200: one FP16 row, 4096 -> 4096 (8.9 MB): 5.4 us, 1.7 TB/s, bound by
-// latency (4.4 us with the arithmetic left out); 16 BF16 rows, 4096 -> 16384 (38
-// MB): 19.8 us, 1.9 TB/s, bound by the conversion and the sums (12.3 us without
-// arithmetic); 5 rows, 1088 -> 1001 with a bias: 3.8 us.
+// Measured on a B200, weights from HBM: one FP16 row, 4096 -> 4096 (8.9 MB): 6.2 us,
+// 1.4 TB/s, bound by latency (5.0 us with the arithmetic left out; 5.4 with weights
+// that are in L2); 16 BF16 rows, 4096 -> 16384 (38 MB): 20.1 us, 1.9 TB/s, bound by
+// the conversion and the sums (13.2 us without arithmetic); 5 rows, 1088 -> 1001 with
+// a bias: 3.9 us.
 #include "token_elements.cuh"
 
 #include <algorithm>

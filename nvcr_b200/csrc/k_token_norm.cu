@@ -6,9 +6,11 @@
 // are FP32; `normed` comes from the unrounded sum. Each input is read once and
 // each output written once.
 //
-// Measured on a B200: 4096 x 4096 BF16, five tensors of rows (168 MB): 32 us, 5.2
-// TB/s, bound by HBM. One row of 2048 FP16: 2.1 to 2.3 us, bound by the launch and two sums
-// across a block. 77 x 1111 FP32, element by element: 2.8 us. Rows held in
+// Measured on a B200: 4096 x 4096 BF16, five tensors of rows (168 MB): 32 us, 5.3
+// TB/s, bound by HBM; FP32 (336 MB) 56.5 us, 5.9 TB/s. One row of 2048 FP16: 2.1 to 2.2
+// us, bound by the launch and two sums across a block. Element by element: 77 x 1111
+// FP32 2.7 us, 2048 x 4097 BF16 69 us (1.2 TB/s). Rows past the registers, 512 x 20000
+// FP32: 138 us (1.5 TB/s). Rows held in
 // registers, with every load issued before the first sum, took the first from 82
 // us (the row re-read for each pass) to 47, and 64 registers a thread, which lets
 // twice as many rows be in flight, to 32.

@@ -1,6 +1,6 @@
-"""A small token model over the token operators: what a step of an autoregressive
-context model (over a codec's latent symbols, say) or of a language model looks
-like with 4-bit weights and a 4-bit cache, together as they are used.
+"""A small token model over the token operators: what a step of a language model
+looks like with 4-bit weights and a 4-bit cache, together as they are used. A
+prompt and its single steps agree to rounding, not to the bit.
 
 A layer is two blocks, each with a norm before and after it and a gate on the way
 back to the residual stream::

@@ -1,4 +1,4 @@
-"""The token operators through the C ABI: one step of a token model in low-bit form.
+"""The token operators through the C ABI: one step of a language model in low-bit form.
 
 ``block_norm`` is the norms after and before a block with its gate and residual;
 ``PagedCache`` holds keys and values in 4 bits, rotated on the way in;
@@ -7,7 +7,11 @@
 CUDA device (another one's are refused); work is enqueued on torch's current
 stream unless ``stream`` names another (then the caller orders the two, and keeps
 the tensors alive). What the operators refuse raises ``ExecutorError``; there is
-no CPU fallback.
+no CPU fallback. They are forward operators: an output has no gradient, whether or
+not an input requires one.
+
+The same call on the same kind of GPU gives the same bits; a token's may change
+with the rest of its call, as the other rows and sequences decide the order of sums.
 
 The 4-bit group form, of caches and weights alike: a group of consecutive values
 is held as codes c in 0..15, two a byte with the even index in the low half, an
