@@ -251,7 +251,7 @@ class PackedMatrix:
         with _on(stream, weights.device):
             parts = weights.float().unflatten(1, (-1, group))
             low, high = parts.amin(-1), parts.amax(-1)
-            fifteenth = torch.tensor(1.0 / 15.0, dtype=torch.float32)  # a number of the host's: no copy, and FP32
+            fifteenth = torch.tensor(1.0 / 15.0, dtype=torch.float32, device="cpu")  # no copy, and a product in FP32
             minimums, scales = low.half(), ((high - low) * fifteenth).half()
             scales = torch.where((scales == 0) & (high > low), 2.0 ** -24, scales)
             steps = scales.float().unsqueeze(-1)
