@@ -495,6 +495,73 @@ int nvcr_sm100_token_multiply(int type, const void* x, int64_t x_stride, int64_t
                               const void* packed_scales, int32_t outputs, int32_t inputs, int32_t group,
                               const void* bias, void* y, void* stream);
 
+/* Weights in 8 bits, laid out once for nvcr_sm100_token_bytes_multiply and
+ * nvcr_sm100_token_experts_multiply: codes [matrices][outputs][inputs], one
+ * matrix or an expert's each; inputs at most 131072 and outputs at most 2^24.
+ * The packed buffer's size in bytes comes first; it is 16-byte aligned. */
+int nvcr_sm100_token_bytes_packed(int64_t matrices, int32_t outputs, int32_t inputs, size_t* bytes);
+int nvcr_sm100_token_bytes_pack(const int8_t* codes, int64_t matrices, int32_t outputs, int32_t inputs, void* packed,
+                                void* stream);
+/* y[r][n] = (sum_k q[r][k] codes[n][k]) * scales[n] * s[r] + bias[n] for rows
+ * of x (F16, BF16 or F32): the sum in integers, exact; the rest in FP32, each
+ * step rounded. A row is taken as s = max(max|x| * (1 / 127), 2^-126) and
+ * q = rint(x * (1 / s)), from FP32; one that holds a NaN or an infinity gives
+ * NaNs. scales are FP32, bias (may be NULL) is of x's type, y is contiguous.
+ * The workspace (its size first; 16-byte aligned) is the call's own until it
+ * has run. Every wait in the kernel is bounded: one that runs out sets bit 0 of
+ * *status (may be NULL), and the outputs concerned are not written. */
+int nvcr_sm100_token_bytes_workspace(int64_t rows, int32_t outputs, int32_t inputs, size_t* bytes);
+int nvcr_sm100_token_bytes_multiply(int type, const void* x, int64_t x_stride, int64_t rows, const void* packed,
+                                    const float* scales, int32_t outputs, int32_t inputs, const void* bias, void* y,
+                                    void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
+/* The same product by experts (at most 1024): token t's j-th row is multiplied
+ * with the matrix of expert choices[t][j], j < chosen. x is [tokens][inputs], or
+ * with `rows_each` not 0 [tokens][chosen][inputs]; scales are [experts][outputs].
+ * Without weights (NULL) y is [tokens][chosen][outputs]; with them, y[t] =
+ * sum_j weights[t][j] * product, [tokens][outputs], added in FP32 in the order
+ * of j and rounded once. A choice outside 0 .. experts - 1 has no product: zeros,
+ * and nothing in the sum. choices and weights (FP32) are contiguous. */
+int nvcr_sm100_token_experts_workspace(int64_t tokens, int32_t chosen, int weighted, int32_t experts, int32_t outputs,
+                                       int32_t inputs, size_t* bytes);
+int nvcr_sm100_token_experts_multiply(int type, const void* x, int64_t x_stride, int64_t x_row_stride, int rows_each,
+                                      int64_t tokens, const int32_t* choices, int32_t chosen, const float* weights,
+                                      const void* packed, const float* scales, int32_t experts, int32_t outputs,
+                                      int32_t inputs, void* y, void* workspace, size_t workspace_bytes,
+                                      uint32_t* status, void* stream);
+
+/* Routing of tokens to experts (at most 1024) by scores [tokens][experts] (F16,
+ * BF16 or F32): s = softmax of a token's scores, or their sigmoid when `sigmoid`
+ * is not 0; b = s + bias (FP32 [experts], may be NULL). The experts are `groups`
+ * runs of equal size; the kept_groups with the largest sums of their two largest
+ * b stay, and of their experts the `count` with the largest b, in falling order,
+ * are choices [tokens][count]; equal ones in the order of their indexes. weights
+ * [tokens][count] (FP32) are their s, divided by the sum of them when
+ * `renormalise` is not 0 (a sum of zero leaves zeros), times scale. An expert
+ * whose score is -infinity or NaN, or whose b is, is never chosen; choices that
+ * are left over are -1, with weight 0. FP64 inside. */
+int nvcr_sm100_token_route(int type, const void* scores, int64_t stride, int64_t tokens, int32_t experts,
+                           int32_t count, int sigmoid, const float* bias, int32_t groups, int32_t kept_groups,
+                           int renormalise, float scale, int32_t* choices, float* weights, void* stream);
+
+/* A symbol of each row of logits [rows][symbols] (F16, BF16 or F32; at most 2^20
+ * symbols), by the row's uniform number u. w = exp((l - max l) / temperature), in
+ * FP64; in the order of falling logits, equal ones by index, are kept: the first
+ * top_k symbols (all, when top_k is 0 or less); of them the shortest prefix that
+ * has at least top_p of their weight (all, from 1 on or for a NaN; one at least);
+ * of these the symbols with w >= min_p (at least the first; all, when min_p is 0
+ * or less or NaN). Chosen is the first kept one, in the order of indexes, at
+ * which the running sum of w is above u times the whole; u below 0 or NaN counts
+ * as 0, from 1 on the last one with a weight is chosen. probabilities (FP32): its
+ * share of the kept weight. A temperature that is not above 0 takes the largest
+ * logit, the first of equal ones. Logits of -infinity and NaN are left out; a
+ * row of nothing else gives -1 and 0. Weights are summed in multiples of 2^-43:
+ * smaller ones are never chosen. temperatures, top_ks, top_ps and min_ps hold a
+ * value a row; where one is NULL, every row has the value after it. */
+int nvcr_sm100_token_sample(int type, const void* logits, int64_t stride, int64_t rows, int32_t symbols,
+                            const float* uniforms, const float* temperatures, float temperature,
+                            const int32_t* top_ks, int32_t top_k, const float* top_ps, float top_p, const float* min_ps,
+                            float min_p, int64_t* chosen, float* probabilities, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

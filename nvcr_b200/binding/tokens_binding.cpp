@@ -12,6 +12,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -20,7 +21,9 @@
 #include <cstdint>
 #include <exception>
 #include <initializer_list>
+#include <optional>
 #include <string>
+#include <type_traits>
 
 #include "../../include/nvcr_sm100.h"
 
@@ -362,6 +365,149 @@ PyObject* multiply(PyObject*, PyObject* const* args, Py_ssize_t count) {
     });
 }
 
+// Working memory of one call, of the call's own stream: its allocator hands it on to that stream's later work only.
+at::Tensor workspace(std::size_t bytes, int device, PyObject* stream) {
+    std::optional<c10::cuda::CUDAStreamGuard> guard;
+    if (stream != Py_None) {
+        const auto index = static_cast<c10::DeviceIndex>(device);
+        auto handle = static_cast<cudaStream_t>(address(stream));
+        guard.emplace(handle == nullptr ? c10::cuda::getDefaultCUDAStream(index)
+                                        : c10::cuda::getStreamFromExternal(handle, index));
+    }
+    return at::empty({static_cast<std::int64_t>(bytes)},
+                     at::TensorOptions().dtype(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+}
+
+// bytes_multiply(packed, scales, outputs, inputs, status, device, x, bias, stream) -> y
+PyObject* bytes_multiply(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    return guarded(count, 9, [&] {
+        const int outputs = small(args[2], "outputs"), inputs = small(args[3], "inputs");
+        const int device = small(args[5], "device");
+        require_current(device);
+        const at::Tensor& x = tensor(args[6], "x");
+        const int type = type_of(x);
+        require(x.dim() == 2 && type >= 0, "x must be a tensor of a float type of two dimensions");
+        const std::int64_t rows = x.size(0);
+        const std::int64_t shape[2] = {rows, inputs};
+        const void* const from = strided(x, "x", x.scalar_type(), shape, device);
+        const void* const bias = plain_or_null(args[7], "bias", x.scalar_type(), {outputs}, device);
+        std::size_t bytes = 0;
+        check(nvcr_sm100_token_bytes_workspace(rows, outputs, inputs, &bytes));
+        const at::Tensor y = at::empty({rows, outputs}, x.options());
+        const at::Tensor room = workspace(bytes, device, args[8]);
+        check(nvcr_sm100_token_bytes_multiply(type, from, x.stride(0), rows, address(args[0]),
+                                              static_cast<const float*>(address(args[1])), outputs, inputs, bias,
+                                              y.data_ptr(), room.data_ptr(), bytes,
+                                              static_cast<std::uint32_t*>(address(args[4])), stream_of(args[8], device)));
+        return wrapped(y);
+    });
+}
+
+// experts_multiply(packed, scales, experts, outputs, inputs, status, device, x, choices, weights, stream) -> y
+PyObject* experts_multiply(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    return guarded(count, 11, [&] {
+        const int experts = small(args[2], "experts"), outputs = small(args[3], "outputs"), inputs = small(args[4], "inputs");
+        const int device = small(args[6], "device");
+        require_current(device);
+        const at::Tensor& x = tensor(args[7], "x");
+        const at::Tensor& choices = tensor(args[8], "choices");
+        const int type = type_of(x);
+        require((x.dim() == 2 || x.dim() == 3) && type >= 0, "x must be a tensor of a float type of two or three dimensions");
+        require(choices.dim() == 2, "choices have two dimensions");
+        const std::int64_t tokens = choices.size(0), chosen = choices.size(1);
+        require(chosen <= INT32_MAX, "choices are out of range");
+        const bool rows_each = x.dim() == 3;
+        const std::int64_t flat[2] = {tokens, inputs}, deep[3] = {tokens, chosen, inputs};
+        const void* const from =
+            strided(x, "x", x.scalar_type(), rows_each ? at::IntArrayRef(deep) : at::IntArrayRef(flat), device);
+        const void* const which = plain(choices, "choices", at::kInt, {tokens, chosen}, device);
+        const void* const weights = plain_or_null(args[9], "weights", at::kFloat, {tokens, chosen}, device);
+        std::size_t bytes = 0;
+        check(nvcr_sm100_token_experts_workspace(tokens, static_cast<std::int32_t>(chosen), weights != nullptr, experts,
+                                                 outputs, inputs, &bytes));
+        const at::Tensor y = weights != nullptr ? at::empty({tokens, outputs}, x.options())
+                                                : at::empty({tokens, chosen, outputs}, x.options());
+        const at::Tensor room = workspace(bytes, device, args[10]);
+        check(nvcr_sm100_token_experts_multiply(
+            type, from, x.stride(0), rows_each ? x.stride(1) : 0, rows_each, tokens,
+            static_cast<const std::int32_t*>(which), static_cast<std::int32_t>(chosen),
+            static_cast<const float*>(weights), address(args[0]), static_cast<const float*>(address(args[1])), experts,
+            outputs, inputs, y.data_ptr(), room.data_ptr(), bytes, static_cast<std::uint32_t*>(address(args[5])),
+            stream_of(args[10], device)));
+        return wrapped(y);
+    });
+}
+
+// route(scores, count, sigmoid, bias, groups, kept_groups, renormalise, scale, stream) -> (choices, weights)
+PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    return guarded(count, 9, [&] {
+        const at::Tensor& scores = tensor(args[0], "scores");
+        const int type = type_of(scores);
+        require(type >= 0 && scores.dim() == 2, "scores must be a [tokens, experts] tensor of a float type");
+        require(scores.is_cuda(), "tensors must be on a CUDA device");
+        const int device = scores.get_device();
+        require_current(device);
+        const std::int64_t tokens = scores.size(0), experts = scores.size(1);
+        require(experts <= INT32_MAX, "scores have too many experts");
+        const int chosen = small(args[1], "count");
+        require(chosen > 0 && chosen <= experts, "count must be 1 to the number of experts");
+        const void* const from = strided(scores, "scores", scores.scalar_type(), scores.sizes(), device);
+        const void* const bias = plain_or_null(args[3], "bias", at::kFloat, {experts}, device);
+        const at::Tensor choices = at::empty({tokens, chosen}, scores.options().dtype(at::kInt));
+        const at::Tensor weights = at::empty({tokens, chosen}, scores.options().dtype(at::kFloat));
+        check(nvcr_sm100_token_route(type, from, scores.stride(0), tokens, static_cast<std::int32_t>(experts), chosen,
+                                     truth(args[2]), static_cast<const float*>(bias), small(args[4], "groups"),
+                                     small(args[5], "kept_groups"), truth(args[6]), static_cast<float>(real(args[7])),
+                                     choices.data_ptr<std::int32_t>(), weights.data_ptr<float>(),
+                                     stream_of(args[8], device)));
+        return pair(choices, weights);
+    });
+}
+
+// A number for every row, or a tensor with one for each.
+template <typename T>
+struct EachRow {
+    const T* values = nullptr;
+    T value{};
+    EachRow(PyObject* object, const char* what, at::ScalarType type, std::int64_t rows, int device) {
+        if (THPVariable_Check(object)) {
+            values = static_cast<const T*>(plain(tensor(object, what), what, type, {rows}, device));
+        } else if constexpr (std::is_same_v<T, float>) {
+            value = static_cast<float>(real(object));
+        } else {
+            value = small(object, what);
+        }
+    }
+};
+
+// sample(logits, uniforms, temperature, top_k, top_p, min_p, stream) -> (symbols, probabilities)
+PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    return guarded(count, 7, [&] {
+        const at::Tensor& logits = tensor(args[0], "logits");
+        const int type = type_of(logits);
+        require(type >= 0 && logits.dim() == 2, "logits must be a [rows, symbols] tensor of a float type");
+        require(logits.is_cuda(), "tensors must be on a CUDA device");
+        const int device = logits.get_device();
+        require_current(device);
+        const std::int64_t rows = logits.size(0), symbols = logits.size(1);
+        require(symbols <= INT32_MAX, "logits have too many symbols");
+        const void* const from = strided(logits, "logits", logits.scalar_type(), logits.sizes(), device);
+        const void* const uniforms = plain(tensor(args[1], "uniforms"), "uniforms", at::kFloat, {rows}, device);
+        const EachRow<float> temperature(args[2], "temperature", at::kFloat, rows, device);
+        const EachRow<std::int32_t> top_k(args[3], "top_k", at::kInt, rows, device);
+        const EachRow<float> top_p(args[4], "top_p", at::kFloat, rows, device);
+        const EachRow<float> min_p(args[5], "min_p", at::kFloat, rows, device);
+        const at::Tensor chosen = at::empty({rows}, logits.options().dtype(at::kLong));
+        const at::Tensor probabilities = at::empty({rows}, logits.options().dtype(at::kFloat));
+        check(nvcr_sm100_token_sample(type, from, logits.stride(0), rows, static_cast<std::int32_t>(symbols),
+                                      static_cast<const float*>(uniforms), temperature.values, temperature.value,
+                                      top_k.values, top_k.value, top_p.values, top_p.value, min_p.values, min_p.value,
+                                      chosen.data_ptr<std::int64_t>(), probabilities.data_ptr<float>(),
+                                      stream_of(args[6], device)));
+        return pair(chosen, probabilities);
+    });
+}
+
 // on_current(device): refuses another device than the current one.
 PyObject* on_current(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return guarded(count, 1, [&]() -> PyObject* {
@@ -383,7 +529,9 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t count) {
 
 #define TOKEN_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {TOKEN_METHOD(norm),     TOKEN_METHOD(append), TOKEN_METHOD(read), TOKEN_METHOD(attend),
-                         TOKEN_METHOD(multiply), TOKEN_METHOD(on_current), TOKEN_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+                         TOKEN_METHOD(multiply), TOKEN_METHOD(bytes_multiply), TOKEN_METHOD(experts_multiply),
+                         TOKEN_METHOD(route),    TOKEN_METHOD(sample), TOKEN_METHOD(on_current), TOKEN_METHOD(bind),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "nvcr_tokens", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

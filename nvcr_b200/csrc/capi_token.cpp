@@ -115,6 +115,39 @@ bool matrix_shape(std::int32_t outputs, std::int32_t inputs, std::int32_t group)
     return outputs > 0 && outputs <= most_rows - 15 && inputs > 0 && inputs <= 98304 && (group == 32 || group == 64 || group == 128) && inputs % group == 0;
 }
 
+// 131072 products of -128 and 127 stay below 2^31.
+bool byte_matrix_shape(std::int64_t matrices, std::int32_t outputs, std::int32_t inputs) {
+    return matrices > 0 && matrices <= most_rows && outputs > 0 && outputs <= 1 << 24 && inputs > 0 && inputs <= 131072;
+}
+constexpr const char* byte_matrix_reason = "a matrix has 1 to 2^24 outputs and 1 to 131072 inputs";
+
+bool aligned(const void* buffer) { return reinterpret_cast<std::uintptr_t>(buffer) % 16 == 0; }
+
+// Null when the experts' call can be made, else why not. Rows of experts are padded by up to 15, and counted in 32 bits.
+const char* experts_refusal(std::int64_t tokens, std::int32_t chosen, std::int32_t experts, std::int32_t outputs,
+                            std::int32_t inputs) {
+    if (experts <= 0 || experts > token::most_experts) return "experts must be 1 to 1024";
+    if (!byte_matrix_shape(experts, outputs, inputs)) return byte_matrix_reason;
+    if (chosen <= 0 || tokens < 0 || tokens > most_places / chosen) return "tokens or chosen out of range";
+    return nullptr;
+}
+
+token::BytesArgs experts_args(std::int64_t tokens, std::int32_t chosen, const std::int32_t* choices, const float* weights,
+                              std::int32_t experts, std::int32_t outputs, std::int32_t inputs) {
+    token::BytesArgs args{};
+    args.tokens = tokens, args.chosen = chosen, args.inner = 1;
+    args.choices = choices, args.weights = weights;
+    args.experts = experts, args.outputs = outputs, args.inputs = inputs;
+    return args;
+}
+
+token::BytesArgs matrix_args(std::int64_t rows, std::int32_t outputs, std::int32_t inputs) {
+    token::BytesArgs args{};
+    args.tokens = rows, args.inner = args.chosen = args.experts = 1;
+    args.outputs = outputs, args.inputs = inputs;
+    return args;
+}
+
 }  // namespace
 
 extern "C" {
@@ -335,6 +368,133 @@ int nvcr_sm100_token_multiply(int type, const void* x, int64_t x_stride, int64_t
                                          static_cast<const std::uint16_t*>(packed_scales), outputs, inputs, group, bias,
                                          y},
                                         static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_bytes_packed(int64_t matrices, int32_t outputs, int32_t inputs, size_t* bytes) {
+    return guarded([&] {
+        if (bytes == nullptr) return refuse("null argument");
+        if (!byte_matrix_shape(matrices, outputs, inputs)) return refuse(byte_matrix_reason);
+        *bytes = token::byte_matrix_bytes(matrices, outputs, inputs);
+        return report_ok();
+    });
+}
+
+int nvcr_sm100_token_bytes_pack(const int8_t* codes, int64_t matrices, int32_t outputs, int32_t inputs, void* packed,
+                                void* stream) {
+    return guarded([&] {
+        if (!byte_matrix_shape(matrices, outputs, inputs)) return refuse(byte_matrix_reason);
+        if (codes == nullptr || packed == nullptr) return refuse("null argument");
+        if (!aligned(packed)) return refuse("packed buffers must be 16-byte aligned");
+        return launched(token::pack_bytes(codes, matrices, outputs, inputs, packed, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_bytes_workspace(int64_t rows, int32_t outputs, int32_t inputs, size_t* bytes) {
+    return guarded([&] {
+        if (bytes == nullptr) return refuse("null argument");
+        if (!byte_matrix_shape(1, outputs, inputs)) return refuse(byte_matrix_reason);
+        if (rows < 0 || rows > most_places) return refuse("rows out of range");
+        *bytes = token::bytes_workspace(matrix_args(rows, outputs, inputs));
+        return report_ok();
+    });
+}
+
+int nvcr_sm100_token_bytes_multiply(int type, const void* x, int64_t x_stride, int64_t rows, const void* packed,
+                                    const float* scales, int32_t outputs, int32_t inputs, const void* bias, void* y,
+                                    void* workspace, size_t workspace_bytes, uint32_t* status, void* stream) {
+    return guarded([&] {
+        if (!any_type(type)) return refuse("unknown type");
+        if (!byte_matrix_shape(1, outputs, inputs)) return refuse(byte_matrix_reason);
+        if (rows < 0 || rows > most_places) return refuse("rows out of range");
+        if (packed == nullptr || scales == nullptr ||
+            (rows > 0 && (x == nullptr || y == nullptr || workspace == nullptr))) {
+            return refuse("null argument");
+        }
+        if (!aligned(packed) || !aligned(workspace)) return refuse("packed and workspace buffers must be 16-byte aligned");
+        token::BytesArgs args = matrix_args(rows, outputs, inputs);
+        if (workspace_bytes < token::bytes_workspace(args)) return refuse("the workspace is too small");
+        args.type = static_cast<token::Type>(type);
+        args.x = x, args.x_stride = x_stride;
+        args.packed = packed, args.scales = scales, args.bias = bias, args.y = y;
+        args.workspace = workspace, args.status = status;
+        return launched(token::multiply_bytes(args, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_experts_workspace(int64_t tokens, int32_t chosen, int weighted, int32_t experts, int32_t outputs,
+                                       int32_t inputs, size_t* bytes) {
+    return guarded([&] {
+        if (bytes == nullptr) return refuse("null argument");
+        if (const char* reason = experts_refusal(tokens, chosen, experts, outputs, inputs)) return refuse(reason);
+        // the size goes by whether there are choices and weights, not by what they are
+        const std::int32_t choices = 0;
+        const float weights = 0.0f;
+        *bytes = token::bytes_workspace(
+            experts_args(tokens, chosen, &choices, weighted != 0 ? &weights : nullptr, experts, outputs, inputs));
+        return report_ok();
+    });
+}
+
+int nvcr_sm100_token_experts_multiply(int type, const void* x, int64_t x_stride, int64_t x_row_stride, int rows_each,
+                                      int64_t tokens, const int32_t* choices, int32_t chosen, const float* weights,
+                                      const void* packed, const float* scales, int32_t experts, int32_t outputs,
+                                      int32_t inputs, void* y, void* workspace, size_t workspace_bytes,
+                                      uint32_t* status, void* stream) {
+    return guarded([&] {
+        if (!any_type(type)) return refuse("unknown type");
+        if (const char* reason = experts_refusal(tokens, chosen, experts, outputs, inputs)) return refuse(reason);
+        if (packed == nullptr || scales == nullptr ||
+            (tokens > 0 && (x == nullptr || choices == nullptr || y == nullptr || workspace == nullptr))) {
+            return refuse("null argument");
+        }
+        if (!aligned(packed) || !aligned(workspace)) return refuse("packed and workspace buffers must be 16-byte aligned");
+        if (tokens == 0) return report_ok();
+        token::BytesArgs args = experts_args(tokens, chosen, choices, weights, experts, outputs, inputs);
+        if (workspace_bytes < token::bytes_workspace(args)) return refuse("the workspace is too small");
+        args.type = static_cast<token::Type>(type);
+        args.x = x, args.x_stride = x_stride;
+        if (rows_each != 0) args.inner = chosen, args.x_inner_stride = x_row_stride;
+        args.packed = packed, args.scales = scales, args.y = y;
+        args.workspace = workspace, args.status = status;
+        return launched(token::multiply_bytes(args, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_route(int type, const void* scores, int64_t stride, int64_t tokens, int32_t experts,
+                           int32_t count, int sigmoid, const float* bias, int32_t groups, int32_t kept_groups,
+                           int renormalise, float scale, int32_t* choices, float* weights, void* stream) {
+    return guarded([&] {
+        if (!any_type(type)) return refuse("unknown type");
+        if (tokens < 0 || tokens > most_rows) return refuse("tokens out of range");
+        if (experts <= 0 || experts > token::most_experts) return refuse("experts must be 1 to 1024");
+        if (count <= 0 || count > experts) return refuse("count must be 1 to the number of experts");
+        if (groups <= 0 || experts % groups != 0) return refuse("experts must be a multiple of groups");
+        if (kept_groups <= 0 || kept_groups > groups) return refuse("kept_groups must be 1 to groups");
+        if (!std::isfinite(scale)) return refuse("scale must be finite");
+        if (tokens > 0 && (scores == nullptr || choices == nullptr || weights == nullptr)) {
+            return refuse("null scores, choices or weights");
+        }
+        return launched(token::route({static_cast<token::Type>(type), scores, stride, tokens, experts, count, sigmoid != 0,
+                                      bias, groups, kept_groups, renormalise != 0, scale, choices, weights},
+                                     static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_sample(int type, const void* logits, int64_t stride, int64_t rows, int32_t symbols,
+                            const float* uniforms, const float* temperatures, float temperature,
+                            const int32_t* top_ks, int32_t top_k, const float* top_ps, float top_p, const float* min_ps,
+                            float min_p, int64_t* chosen, float* probabilities, void* stream) {
+    return guarded([&] {
+        if (!any_type(type)) return refuse("unknown type");
+        if (rows < 0 || rows > most_rows) return refuse("rows out of range");
+        if (symbols <= 0 || symbols > token::most_symbols) return refuse("symbols must be 1 to 2^20");
+        if (rows > 0 && (logits == nullptr || uniforms == nullptr || chosen == nullptr || probabilities == nullptr)) {
+            return refuse("null logits, uniforms, chosen or probabilities");
+        }
+        return launched(token::sample({static_cast<token::Type>(type), logits, stride, rows, symbols, uniforms, temperatures,
+                                       top_ks, top_ps, min_ps, temperature, top_k, top_p, min_p, chosen, probabilities},
+                                      static_cast<cudaStream_t>(stream)));
     });
 }
 

@@ -1,0 +1,738 @@
+// Products in 8-bit integers: y[t][n] = (sum_k q[t][k] w[n][k]) * scale[n] * s[t] + bias[n], the rows of x taken as
+// codes q = rint(x / s) with a scale s of their own, one matrix for all rows or the matrix of the expert that each
+// row has chosen. The sums are exact in int32, so their order, and a split of them, change no bit.
+//
+// Three launches at most: where the rows of each expert go (`arrange`), the rows as codes (`quantise`), the product.
+// Both operands lie in memory as the tensor cores read them from shared memory, in the 128-byte swizzle: weights as
+// blocks of 128 outputs by 128 inputs, rows as [128 inputs][row][128 bytes]. So every tile is one contiguous copy,
+// with neither a tensor map nor an alignment that a caller has to keep.
+#include "tcgen05.cuh"
+#include "token_elements.cuh"
+
+#include <algorithm>
+
+namespace nvcr_sm100::token {
+namespace {
+
+using namespace kernels;
+
+constexpr int block_rows = 128;    // outputs of a weight block: the MMA's M
+constexpr int block_bytes = 128;   // inputs of a block: a swizzled row
+constexpr int weight_block = block_rows * block_bytes;
+constexpr int step_rows = 16;      // rows of x are padded to the MMA's step of N
+constexpr int most_tile = 256;     // rows of x a tile
+
+int blocks_of(int inputs) { return (inputs + block_bytes - 1) / block_bytes; }
+int tiles_of(int outputs) { return (outputs + block_rows - 1) / block_rows; }
+std::int64_t padded(std::int64_t rows) { return (rows + step_rows - 1) / step_rows * step_rows; }
+std::size_t aligned(std::size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// ---- weights: [matrix][tile of outputs][block of inputs][128][128], zeros past the edges, laid out once ----
+
+__global__ void __launch_bounds__(256) pack_kernel(const std::int8_t* codes, std::int64_t blocks, int outputs, int inputs,
+                                                   int tiles, int k_blocks, uint4* packed) {
+    // a thread a 16-byte piece: piece c of row r lies at piece c ^ (r % 8)
+    for (std::int64_t i = blockIdx.x * 256ll + threadIdx.x; i < blocks * (weight_block / 16);
+         i += static_cast<std::int64_t>(gridDim.x) * 256) {
+        const std::int64_t block = i / (weight_block / 16);
+        const int row = static_cast<int>(i / 8 % block_rows), piece = static_cast<int>(i % 8) ^ (row & 7);
+        const int k = static_cast<int>(block % k_blocks) * block_bytes + piece * 16;
+        const int output = static_cast<int>(block / k_blocks % tiles) * block_rows + row;
+        const std::int64_t matrix = block / k_blocks / tiles;
+        unsigned words[4] = {0, 0, 0, 0};
+        if (output < outputs) {
+            const std::int8_t* from = codes + (matrix * outputs + output) * inputs + k;
+            for (int b = 0; b < 16; ++b) {
+                if (k + b < inputs) words[b / 4] |= static_cast<unsigned>(static_cast<std::uint8_t>(from[b])) << (b % 4 * 8);
+            }
+        }
+        packed[i] = {words[0], words[1], words[2], words[3]};
+    }
+}
+
+// ---- where the rows of each expert go ----
+
+constexpr int arrange_threads = 1024;
+
+struct Arranged {
+    int* place;       // [pairs]: the row of a pair, or -1
+    int* pair;        // [rows]: the pair of a row
+    int4* tiles;      // expert, first row, rows
+    int* tile_count;
+};
+
+// One block. Which of an expert's rows a pair gets is decided by atomics, and changes no output: rows are independent
+// and their sums exact.
+__global__ void __launch_bounds__(arrange_threads) arrange_kernel(const std::int32_t* choices, std::int64_t pairs, int experts,
+                                                                  int tile_rows, Arranged out) {
+    extern __shared__ int shared[];
+    int* counts = shared;             // [experts], then the next row of each
+    int* scratch = shared + experts;  // two sums of each warp
+    join_chain();
+    const int thread = threadIdx.x, lane = thread % 32, warp = thread / 32;
+    for (int e = thread; e < experts; e += arrange_threads) counts[e] = 0;
+    __syncthreads();
+    for (std::int64_t i = thread; i < pairs; i += arrange_threads) {
+        const int e = choices[i];
+        if (e >= 0 && e < experts) atomicAdd(&counts[e], 1);
+    }
+    __syncthreads();
+    int first_row = 0, first_tile = 0;
+    for (int from = 0; from < experts; from += arrange_threads) {
+        const int e = from + thread;
+        const int count = e < experts ? counts[e] : 0;
+        const int rows = (count + step_rows - 1) / step_rows * step_rows;
+        const int tiles = (count + tile_rows - 1) / tile_rows;
+        int row = rows, tile = tiles;
+        for (int o = 1; o < 32; o *= 2) {
+            const int r = __shfl_up_sync(0xffffffffu, row, o), t = __shfl_up_sync(0xffffffffu, tile, o);
+            if (lane >= o) row += r, tile += t;
+        }
+        if (lane == 31) scratch[warp] = row, scratch[32 + warp] = tile;
+        __syncthreads();
+        int rows_before = 0, tiles_before = 0, all_rows = 0, all_tiles = 0;
+        for (int w = 0; w < arrange_threads / 32; ++w) {
+            if (w < warp) rows_before += scratch[w], tiles_before += scratch[32 + w];
+            all_rows += scratch[w], all_tiles += scratch[32 + w];
+        }
+        row += first_row + rows_before - rows, tile += first_tile + tiles_before - tiles;
+        for (int t = 0; t < tiles; ++t) {
+            out.tiles[tile + t] = {e, row + t * tile_rows, min(tile_rows, count - t * tile_rows), 0};
+        }
+        if (e < experts) counts[e] = row;
+        first_row += all_rows, first_tile += all_tiles;
+        __syncthreads();
+    }
+    if (thread == 0) *out.tile_count = first_tile;
+    for (std::int64_t i = thread; i < pairs; i += arrange_threads) {
+        const int e = choices[i];
+        int row = -1;
+        if (e >= 0 && e < experts) {
+            row = atomicAdd(&counts[e], 1);
+            out.pair[row] = static_cast<int>(i);
+        }
+        out.place[i] = row;
+    }
+}
+
+// ---- rows as codes ----
+
+struct QuantiseArgs {
+    const void* x;
+    std::int64_t stride, inner_stride;  // of a token, and of a row within a token
+    int inner;                          // rows a token
+    std::int64_t rows;
+    int inputs, k_blocks;
+    bool vector;          // rows begin on 16-byte boundaries
+    const int* place;     // null: row r goes to row r; else to rows place[r * fan ..]
+    int fan;
+    std::int64_t out_rows;
+    std::uint8_t* codes;  // [k_blocks][out_rows][128], swizzled
+    float* scales;        // [out_rows]
+    void* zeros;          // null, or the output whose rows without a place are zeros
+    int outputs;
+};
+
+template <typename T>
+__device__ __forceinline__ void load_sixteen(const T* row, int at, int inputs, bool vector, float (&v)[16]) {
+    if (vector && at + 16 <= inputs) {
+        constexpr int each = 16 / sizeof(T);
+#pragma unroll
+        for (int part = 0; part < 16 / each; ++part) {
+            const uint4 words = *reinterpret_cast<const uint4*>(row + at + part * each);
+            const unsigned word[4] = {words.x, words.y, words.z, words.w};
+#pragma unroll
+            for (int i = 0; i < each; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    v[part * each + i] = __uint_as_float(word[i]);
+                } else {
+                    const std::uint16_t bits = static_cast<std::uint16_t>(word[i / 2] >> (i % 2 * 16));
+                    v[part * each + i] = widen(reinterpret_cast<const T&>(bits));
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = at + i < inputs ? widen(row[at + i]) : 0.0f;
+    }
+}
+
+// Warps warps a row, a thread 16 values at a time, of which the first `held` stay in registers between the row's
+// maximum and its codes; longer rows are read again.
+template <typename T, int Warps>
+__global__ void __launch_bounds__(256) quantise_kernel(QuantiseArgs a) {
+    constexpr int threads = Warps * 32, held = 2;
+    __shared__ float largest[8];
+    join_chain();
+    const int part = threadIdx.x % threads;
+    const std::int64_t row = blockIdx.x * static_cast<std::int64_t>(8 / Warps) + threadIdx.x / threads;
+    const bool there = row < a.rows;
+    const T* x = static_cast<const T*>(a.x);
+    if (there) x += row / a.inner * a.stride + row % a.inner * a.inner_stride;
+    const int pieces = a.k_blocks * (block_bytes / 16);
+    float kept[held][16];
+    float most = 0.0f;
+#pragma unroll
+    for (int h = 0; h < held; ++h) {
+        const int piece = part + h * threads;
+        if (there && piece < pieces) {
+            load_sixteen(x, piece * 16, a.inputs, a.vector, kept[h]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = max_nan(most, fabsf(kept[h][i]));
+        }
+    }
+    for (int piece = part + held * threads; there && piece < pieces; piece += threads) {
+        float v[16];
+        load_sixteen(x, piece * 16, a.inputs, a.vector, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = max_nan(most, fabsf(v[i]));
+    }
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, offset));
+    if constexpr (Warps > 1) {
+        if (threadIdx.x % 32 == 0) largest[threadIdx.x / 32] = most;
+        __syncthreads();
+        const int first = threadIdx.x / threads * Warps;
+#pragma unroll
+        for (int w = 0; w < Warps; ++w) most = max_nan(most, largest[first + w]);
+    }
+    if (!there) return;
+    // 2^-126: the inverse of a smaller scale would overflow
+    const float scale = fmaxf(__fmul_rn(most, 1.0f / 127.0f), 1.17549435e-38f);
+    const float inverse = __frcp_rn(scale);
+    const bool finite = most <= 3.40282347e38f;
+    auto store = [&](const float (&v)[16], int piece) {
+        unsigned words[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            unsigned byte[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                // within 127.5 of zero: adding 1.5 * 2^23 rounds to a whole number, whose low byte is the code
+                byte[b] = __float_as_uint(__fadd_rn(__fmul_rn(v[4 * w + b], inverse), 12582912.0f));
+            }
+            words[w] = __byte_perm(__byte_perm(byte[0], byte[1], 0x0040), __byte_perm(byte[2], byte[3], 0x0040), 0x5410);
+        }
+        for (int f = 0; f < a.fan; ++f) {
+            const std::int64_t to = a.place == nullptr ? row : a.place[row * a.fan + f];
+            if (to < 0) continue;
+            uint4* at = reinterpret_cast<uint4*>(a.codes + (piece / 8 * a.out_rows + to) * block_bytes);
+            at[(piece % 8) ^ static_cast<int>(to & 7)] = {words[0], words[1], words[2], words[3]};
+        }
+    };
+#pragma unroll
+    for (int h = 0; h < held; ++h) {
+        if (part + h * threads < pieces) store(kept[h], part + h * threads);
+    }
+    for (int piece = part + held * threads; piece < pieces; piece += threads) {
+        float v[16];
+        load_sixteen(x, piece * 16, a.inputs, a.vector, v);
+        store(v, piece);
+    }
+    for (int f = part; f < a.fan; f += threads) {
+        const std::int64_t to = a.place == nullptr ? row : a.place[row * a.fan + f];
+        if (to >= 0) a.scales[to] = finite ? scale : __int_as_float(0x7fffffff);  // such a row's outputs are no numbers
+    }
+    if (a.zeros != nullptr) {
+        for (int f = 0; f < a.fan; ++f) {
+            if (a.place[row * a.fan + f] >= 0) continue;
+            T* out = static_cast<T*>(a.zeros) + (row * a.fan + f) * a.outputs;
+            for (int i = part; i < a.outputs; i += threads) out[i] = narrow<T>(0.0f);
+        }
+    }
+}
+
+// ---- the product ----
+
+constexpr int epilogue_warps = 8;
+constexpr int weight_warp = 8, row_warp = 9, mma_warp = 10;
+constexpr int product_threads = 32 * 11;
+constexpr int most_stages = 12;
+
+struct ProductArgs {
+    const std::uint8_t* weights;
+    const float* scales;
+    const void* bias;
+    const std::uint8_t* codes;
+    const float* row_scales;
+    Arranged arranged;  // tiles null: rows 0 .. rows - 1 of one matrix
+    std::int64_t rows, out_rows;
+    int outputs, tiles, k_blocks;
+    int tile_rows, stages, splits;
+    unsigned tmem_columns;
+    void* y;
+    unsigned* status;
+};
+
+struct ProductTail {
+    std::uint64_t full[most_stages], empty[most_stages], tmem_full[2], tmem_empty[2], drain;
+    std::uint32_t tmem;
+    unsigned status;  // of waits: told to the caller's at the end
+    int abort;
+};
+
+__device__ __forceinline__ void bulk_load(std::uint32_t to, const void* from, std::uint32_t bytes, std::uint32_t barrier) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+                 "l"(__cvta_generic_to_global(from)), "r"(bytes), "r"(barrier)
+                 : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ int peer_load(std::uint32_t address, int rank) {
+    int v;
+    asm volatile(
+        "{\n\t.reg .b32 there;\n\tmapa.shared::cluster.u32 there, %1, %2;\n\tld.shared::cluster.b32 %0, [there];\n\t}"
+        : "=r"(v)
+        : "r"(address), "r"(rank)
+        : "memory");
+    return v;
+}
+
+struct Tile {
+    int expert, output;          // output: first of the tile
+    std::int64_t row;            // first row of the codes
+    int rows, columns;           // columns: rows padded to the MMA's step
+};
+
+template <bool Experts>
+__device__ __forceinline__ Tile tile_at(const ProductArgs& a, std::int64_t item) {
+    const std::int64_t nth = item / a.tiles;
+    Tile t;
+    t.output = static_cast<int>(item - nth * a.tiles) * block_rows;
+    if constexpr (Experts) {
+        const int4 found = a.arranged.tiles[nth];
+        t.expert = found.x, t.row = found.y, t.rows = found.z;
+    } else {
+        t.expert = 0, t.row = nth * a.tile_rows;
+        t.rows = static_cast<int>(min(static_cast<std::int64_t>(a.tile_rows), a.rows - t.row));
+    }
+    t.columns = (t.rows + step_rows - 1) / step_rows * step_rows;
+    return t;
+}
+
+// A block takes tiles of 128 outputs by tile_rows rows one after another: two warps copy blocks of weights and rows
+// into a ring, a thread issues the MMAs into one of two accumulators, eight warps scale and store the other. With
+// `splits` > 1 a cluster of that many blocks has one tile, each block a part of its inputs, and the sums are added over
+// the cluster's shared memory.
+template <typename T, bool Experts>
+__global__ void __launch_bounds__(product_threads, 1) product_kernel(const ProductArgs a) {
+    extern __shared__ std::uint8_t dynamic[];
+    __shared__ ProductTail tail;
+    const std::uint32_t raw = smem_address(dynamic);
+    const std::uint32_t ring = (raw + 1023u) & ~1023u;
+    const std::uint32_t row_bytes = static_cast<std::uint32_t>(a.tile_rows) * block_bytes;
+    const std::uint32_t rows_ring = ring + static_cast<std::uint32_t>(a.stages) * weight_block;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int splits = a.splits;
+    const int rank = static_cast<int>(blockIdx.x) % splits;
+    const std::int64_t first_item = blockIdx.x / splits, item_step = gridDim.x / splits;
+    const int k_from = static_cast<int>(static_cast<std::int64_t>(a.k_blocks) * rank / splits);
+    const int k_to = static_cast<int>(static_cast<std::int64_t>(a.k_blocks) * (rank + 1) / splits);
+
+    if (warp == mma_warp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&tail.tmem)),
+                     "r"(a.tmem_columns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == weight_warp && lane == 0) {
+        for (int s = 0; s < a.stages; ++s) {
+            barrier_init(smem_address(&tail.full[s]), 2);
+            barrier_init(smem_address(&tail.empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            barrier_init(smem_address(&tail.tmem_full[b]), 1);
+            barrier_init(smem_address(&tail.tmem_empty[b]), epilogue_warps * 32);
+        }
+        barrier_init(smem_address(&tail.drain), 1);
+        tail.status = 0;
+        tail.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async_shared();
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const std::uint32_t tmem = tail.tmem;
+    volatile int* abort = &tail.abort;
+    unsigned* waits = &tail.status;
+    launch_dependents();
+    // The kernel before this one waits for all before it and only then lets this one start, so the weights are
+    // written when one matrix's are loaded; which expert's, its tiles say.
+    if (Experts || warp != weight_warp) grid_dependency_wait();
+    const std::int64_t row_tiles = Experts ? *a.arranged.tile_count : (a.rows + a.tile_rows - 1) / a.tile_rows;
+    const std::int64_t items = row_tiles * a.tiles;
+
+    if (warp == weight_warp || warp == row_warp) {
+        if (lane == 0) {
+            const bool weights = warp == weight_warp;
+            int slot = 0, issued = 0;
+            std::uint32_t phase = 0;
+            for (std::int64_t item = first_item; item < items && !*abort; item += item_step) {
+                const Tile t = tile_at<Experts>(a, item);
+                const std::uint32_t bytes = weights ? weight_block : static_cast<std::uint32_t>(t.columns) * block_bytes;
+                const std::int64_t matrix_tile = static_cast<std::int64_t>(t.expert) * a.tiles + t.output / block_rows;
+                const std::uint8_t* from = weights ? a.weights + matrix_tile * a.k_blocks * weight_block
+                                                   : a.codes + t.row * block_bytes;
+                const std::int64_t step = weights ? weight_block : a.out_rows * block_bytes;
+                for (int k = k_from; k < k_to; ++k) {
+                    if (!barrier_wait(smem_address(&tail.empty[slot]), phase ^ 1u, waits)) {
+                        *abort = 1;
+                        break;
+                    }
+                    const std::uint32_t full = smem_address(&tail.full[slot]);
+                    barrier_expect_bytes(full, bytes);
+                    bulk_load(weights ? ring + slot * weight_block : rows_ring + slot * row_bytes, from + k * step, bytes, full);
+                    ++issued;
+                    if (++slot == a.stages) slot = 0, phase ^= 1u;
+                }
+            }
+            if (*abort) {  // the copies under way
+                for (int s = 0; s < a.stages && s < issued; ++s) {
+                    if (--slot < 0) slot = a.stages - 1, phase ^= 1u;
+                    barrier_wait(smem_address(&tail.full[slot]), phase, waits);
+                }
+            }
+        }
+    } else if (warp == mma_warp) {
+        if (lane == 0) {
+            int slot = 0, buffer = 0;
+            std::uint32_t phase = 0, pass = 0;
+            for (std::int64_t item = first_item; item < items && !*abort; item += item_step) {
+                const Tile t = tile_at<Experts>(a, item);
+                const std::uint32_t instruction = i8_instruction(t.columns);
+                if (!barrier_wait(smem_address(&tail.tmem_empty[buffer]), pass ^ 1u, waits)) *abort = 1;
+                tmem_fence_after();
+                const std::uint32_t sums = tmem + static_cast<std::uint32_t>(buffer * a.tile_rows);
+                for (int k = k_from; k < k_to && !*abort; ++k) {
+                    if (!barrier_wait(smem_address(&tail.full[slot]), phase, waits)) {
+                        *abort = 1;
+                        break;
+                    }
+                    tmem_fence_after();
+                    const std::uint64_t w = sw128_descriptor(ring + slot * weight_block);
+                    const std::uint64_t x = sw128_descriptor(rows_ring + slot * row_bytes);
+#pragma unroll
+                    for (int step = 0; step < block_bytes / 32; ++step) {
+                        mma_i8(sums, w + 2 * step, x + 2 * step, instruction, k > k_from || step > 0);
+                    }
+                    mma_commit(smem_address(&tail.empty[slot]));
+                    if (++slot == a.stages) slot = 0, phase ^= 1u;
+                }
+                if (!*abort) mma_commit(smem_address(&tail.tmem_full[buffer]));
+                if (++buffer == 2) buffer = 0, pass ^= 1u;
+            }
+            if (*abort) {  // the MMAs under way
+                mma_commit(smem_address(&tail.drain));
+                barrier_wait(smem_address(&tail.drain), 0, waits);
+            }
+        }
+    } else {
+        const int quarter = warp % 4, half = warp / 4;
+        int buffer = 0;
+        std::uint32_t pass = 0;
+        for (std::int64_t item = first_item; item < items && !*abort; item += item_step) {
+            const Tile t = tile_at<Experts>(a, item);
+            if (!barrier_wait(smem_address(&tail.tmem_full[buffer]), pass, waits)) {
+                *abort = 1;
+                break;
+            }
+            tmem_fence_after();
+            const std::uint32_t sums = tmem + static_cast<std::uint32_t>(buffer * a.tile_rows) +
+                (static_cast<std::uint32_t>(quarter * 32) << 16);
+            const int output = t.output + quarter * 32 + lane;
+            if (splits == 1) {
+                const bool inside = output < a.outputs;
+                const std::int64_t channel = static_cast<std::int64_t>(t.expert) * a.outputs + output;
+                const float scale = inside ? a.scales[channel] : 0.0f;
+                const float bias = inside && a.bias != nullptr ? widen(static_cast<const T*>(a.bias)[channel]) : 0.0f;
+                T* y = static_cast<T*>(a.y) + output;
+                for (int column = half * 16; column < t.columns; column += 32) {
+                    int acc[16];
+                    tmem_load16(sums + static_cast<std::uint32_t>(column), acc);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (inside && column + i < t.rows) {
+                            const std::int64_t row = t.row + column + i;
+                            float v = __fmul_rn(__fmul_rn(__int2float_rn(acc[i]), scale), a.row_scales[row]);
+                            if (a.bias != nullptr) v = __fadd_rn(v, bias);
+                            const std::int64_t to = Experts ? a.arranged.pair[row] : row;
+                            y[to * a.outputs] = narrow<T>(v);
+                        }
+                    }
+                }
+            } else {  // the ring is free: every copy has been read
+                for (int column = half * 16; column < t.columns; column += 32) {
+                    int acc[16];
+                    tmem_load16(sums + static_cast<std::uint32_t>(column), acc);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(
+                                         ring + static_cast<std::uint32_t>((column + i) * block_rows + quarter * 32 + lane) * 4),
+                                     "r"(acc[i])
+                                     : "memory");
+                    }
+                }
+            }
+            tmem_fence_before();
+            barrier_arrive(smem_address(&tail.tmem_empty[buffer]));
+            if (++buffer == 2) buffer = 0, pass ^= 1u;
+        }
+    }
+    __syncwarp();
+
+    if (splits > 1) {
+        cluster_sync();
+        if (first_item < items && !*abort) {
+            const Tile t = tile_at<Experts>(a, first_item);
+            const int mine = block_rows / splits;  // outputs of the tile that this block adds up and stores
+            for (int i = threadIdx.x; i < mine * t.rows; i += product_threads) {
+                const int column = i / mine, channel_in = rank * mine + i % mine;
+                const int output = t.output + channel_in;
+                if (output >= a.outputs) continue;
+                const std::uint32_t at = ring + static_cast<std::uint32_t>(column * block_rows + channel_in) * 4;
+                int sum = 0;
+                for (int r = 0; r < splits; ++r) sum += peer_load(at, r);
+                const std::int64_t channel = static_cast<std::int64_t>(t.expert) * a.outputs + output;
+                const std::int64_t row = t.row + column;
+                float v = __fmul_rn(__fmul_rn(__int2float_rn(sum), a.scales[channel]), a.row_scales[row]);
+                if (a.bias != nullptr) v = __fadd_rn(v, widen(static_cast<const T*>(a.bias)[channel]));
+                const std::int64_t to = Experts ? a.arranged.pair[row] : row;
+                static_cast<T*>(a.y)[to * a.outputs + output] = narrow<T>(v);
+            }
+        }
+        cluster_sync();  // the others may still be reading
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == mma_warp) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_columns) : "memory");
+        if (lane == 0 && tail.status != 0 && a.status != nullptr) atomicOr(a.status, tail.status);
+    }
+}
+
+// ---- y[t] = sum_j weights[t][j] * products[t][j], in the order of j ----
+
+template <typename T>
+__global__ void __launch_bounds__(256) combine_kernel(const float* products, const std::int32_t* choices, const float* weights,
+                                                      int chosen, int experts, int outputs, T* y) {
+    join_chain();
+    const std::int64_t token = blockIdx.x;
+    const int output = static_cast<int>(blockIdx.y * 256 + threadIdx.x);
+    if (output >= outputs) return;
+    float sum = 0.0f;
+    for (int j = 0; j < chosen; ++j) {
+        const std::int64_t pair = token * chosen + j;
+        const int e = choices[pair];
+        if (e >= 0 && e < experts) sum = fmaf(weights[pair], products[pair * outputs + output], sum);
+    }
+    y[token * outputs + output] = narrow<T>(sum);
+}
+
+// ---- launches ----
+
+template <typename T, int Warps>
+cudaError_t quantise_rows(const QuantiseArgs& a, cudaStream_t stream) {
+    const std::int64_t blocks = (a.rows + 8 / Warps - 1) / (8 / Warps);
+    return launch_overlapped(quantise_kernel<T, Warps>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
+}
+
+template <typename T>
+cudaError_t quantise(const QuantiseArgs& a, cudaStream_t stream) {
+    if (a.inputs <= 1024) return quantise_rows<T, 1>(a, stream);
+    if (a.inputs <= 2048) return quantise_rows<T, 2>(a, stream);
+    return quantise_rows<T, 8>(a, stream);
+}
+
+cudaError_t quantise(Type type, const QuantiseArgs& a, cudaStream_t stream) {
+    switch (type) {
+    case Type::f16: return quantise<__half>(a, stream);
+    case Type::bf16: return quantise<__nv_bfloat16>(a, stream);
+    default: return quantise<float>(a, stream);
+    }
+}
+
+template <typename T, bool Experts>
+cudaError_t product(ProductArgs a, std::int64_t most_items, cudaStream_t stream) {
+    static SharedAllowance allowance;
+    constexpr int room = 208 * 1024;
+    const int stage = weight_block + a.tile_rows * block_bytes;
+    a.stages = std::min(most_stages, room / stage);
+    a.tmem_columns = 32;
+    while (a.tmem_columns < 2u * static_cast<unsigned>(a.tile_rows)) a.tmem_columns *= 2;
+    const int bytes = a.stages * stage + 1024;
+    cudaError_t status = allowance.allow(product_kernel<T, Experts>, 227 * 1024 - 1024);
+    if (status != cudaSuccess) return status;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(a.splits > 1 ? most_items * a.splits
+                                                             : std::min<std::int64_t>(most_items, sm_count())));
+    config.blockDim = dim3(product_threads);
+    config.dynamicSmemBytes = static_cast<std::size_t>(bytes);
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = static_cast<unsigned>(a.splits);
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = a.splits > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&config, product_kernel<T, Experts>, a);
+}
+
+template <bool Experts>
+cudaError_t product(Type type, const ProductArgs& a, std::int64_t most_items, cudaStream_t stream) {
+    switch (type) {
+    case Type::f16: return product<__half, Experts>(a, most_items, stream);
+    case Type::bf16: return product<__nv_bfloat16, Experts>(a, most_items, stream);
+    default: return product<float, Experts>(a, most_items, stream);
+    }
+}
+
+// Rows a tile: what loads the fewest bytes over the turns that the tiles take on all SMs.
+int rows_a_tile(std::int64_t rows, int tiles) {
+    int best = step_rows;
+    std::int64_t least = -1;
+    for (int n = step_rows; n <= most_tile; n += step_rows) {
+        const std::int64_t turns = ((rows + n - 1) / n * tiles + sm_count() - 1) / sm_count();
+        const std::int64_t cost = turns * (weight_block + n * block_bytes);
+        if (least < 0 || cost < least) least = cost, best = n;
+        if (n >= rows) break;
+    }
+    return best;
+}
+
+// Blocks that share a tile's inputs: while they all run at once and each has two blocks of them.
+int splits_of(std::int64_t items, int k_blocks) {
+    int splits = 1;
+    while (splits < 8 && items * splits * 2 <= sm_count() && k_blocks >= splits * 4) splits *= 2;
+    return splits;
+}
+
+struct Plan {
+    int tile_rows;
+    std::int64_t out_rows, tiles;
+    std::size_t codes, scales, place, pair, table, count, products, bytes;
+};
+
+Plan plan_of(const BytesArgs& a) {
+    Plan p{};
+    const std::int64_t pairs = a.tokens * a.chosen;
+    std::size_t at = 0;
+    auto take = [&](std::size_t bytes) {
+        const std::size_t here = at;
+        at += aligned(bytes);
+        return here;
+    };
+    if (a.choices == nullptr) {
+        p.tile_rows = rows_a_tile(std::max<std::int64_t>(a.tokens, 1), tiles_of(a.outputs));
+        p.out_rows = padded(a.tokens);
+        p.tiles = (a.tokens + p.tile_rows - 1) / p.tile_rows;
+    } else {
+        const std::int64_t groups = std::min<std::int64_t>(a.experts, pairs);
+        p.tile_rows = static_cast<int>(std::clamp<std::int64_t>(padded(2 * pairs / std::max<std::int64_t>(groups, 1)),
+                                                                step_rows, most_tile));
+        p.out_rows = padded(pairs + groups * (step_rows - 1));
+        p.tiles = pairs / p.tile_rows + groups;
+    }
+    p.codes = take(static_cast<std::size_t>(blocks_of(a.inputs)) * p.out_rows * block_bytes);
+    p.scales = take(p.out_rows * sizeof(float));
+    if (a.choices != nullptr) {
+        p.place = take(pairs * sizeof(int));
+        p.pair = take(p.out_rows * sizeof(int));
+        p.table = take(p.tiles * sizeof(int4));
+        p.count = take(sizeof(int));
+        if (a.weights != nullptr) p.products = take(static_cast<std::size_t>(pairs) * a.outputs * sizeof(float));
+    }
+    p.bytes = at;
+    return p;
+}
+
+template <typename T>
+cudaError_t combine(const BytesArgs& a, const float* products, cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>((a.outputs + 255) / 256));
+    return launch_overlapped(combine_kernel<T>, grid, dim3(256), 0, stream, products, a.choices, a.weights, a.chosen,
+                             a.experts, a.outputs, static_cast<T*>(a.y));
+}
+
+}  // namespace
+
+std::size_t byte_matrix_bytes(std::int64_t matrices, int outputs, int inputs) {
+    return static_cast<std::size_t>(matrices) * tiles_of(outputs) * blocks_of(inputs) * weight_block;
+}
+
+cudaError_t pack_bytes(const std::int8_t* codes, std::int64_t matrices, int outputs, int inputs, void* packed,
+                       cudaStream_t stream) {
+    const std::int64_t blocks = matrices * tiles_of(outputs) * blocks_of(inputs);
+    const std::int64_t grid = std::min<std::int64_t>((blocks * (weight_block / 16) + 255) / 256, 16ll * sm_count());
+    pack_kernel<<<static_cast<unsigned>(grid), 256, 0, stream>>>(codes, blocks, outputs, inputs, tiles_of(outputs),
+                                                                  blocks_of(inputs), static_cast<uint4*>(packed));
+    return cudaGetLastError();
+}
+
+std::size_t bytes_workspace(const BytesArgs& a) { return plan_of(a).bytes; }
+
+cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
+    if (a.tokens == 0) return cudaSuccess;
+    const Plan p = plan_of(a);
+    auto* memory = static_cast<std::uint8_t*>(a.workspace);
+    const std::int64_t pairs = a.tokens * a.chosen;
+    const int elements = a.type == Type::f32 ? 4 : 2;
+    Arranged arranged{};
+    if (a.choices != nullptr) {
+        arranged = {reinterpret_cast<int*>(memory + p.place), reinterpret_cast<int*>(memory + p.pair),
+                    reinterpret_cast<int4*>(memory + p.table), reinterpret_cast<int*>(memory + p.count)};
+        const cudaError_t status = launch_overlapped(arrange_kernel, dim3(1), dim3(arrange_threads),
+                                                     (a.experts + 64) * sizeof(int), stream, a.choices, pairs, a.experts,
+                                                     p.tile_rows, arranged);
+        if (status != cudaSuccess) return status;
+    }
+    QuantiseArgs q{};
+    q.x = a.x, q.stride = a.x_stride, q.inner_stride = a.x_inner_stride;
+    q.inner = a.inner;
+    q.rows = a.tokens * q.inner;
+    q.inputs = a.inputs, q.k_blocks = blocks_of(a.inputs);
+    q.vector = reinterpret_cast<std::uintptr_t>(a.x) % 16 == 0 && a.x_stride * elements % 16 == 0 &&
+        a.x_inner_stride * elements % 16 == 0;
+    q.place = arranged.place, q.fan = a.chosen / q.inner;
+    q.out_rows = p.out_rows;
+    q.codes = memory + p.codes, q.scales = reinterpret_cast<float*>(memory + p.scales);
+    q.zeros = a.choices != nullptr && a.weights == nullptr ? a.y : nullptr, q.outputs = a.outputs;
+    cudaError_t status = quantise(a.type, q, stream);
+    if (status != cudaSuccess) return status;
+
+    ProductArgs r{};
+    r.weights = static_cast<const std::uint8_t*>(a.packed), r.scales = a.scales, r.bias = a.bias;
+    r.codes = q.codes, r.row_scales = q.scales, r.arranged = arranged;
+    r.rows = a.tokens, r.out_rows = p.out_rows;
+    r.outputs = a.outputs, r.tiles = tiles_of(a.outputs), r.k_blocks = q.k_blocks;
+    r.tile_rows = p.tile_rows;
+    const std::int64_t items = p.tiles * r.tiles;
+    r.splits = splits_of(items, r.k_blocks);
+    r.status = a.status;
+    if (a.choices == nullptr) {
+        r.y = a.y;
+        return product<false>(a.type, r, items, stream);
+    }
+    if (a.weights == nullptr) {
+        r.y = a.y;
+        return product<true>(a.type, r, items, stream);
+    }
+    auto* products = reinterpret_cast<float*>(memory + p.products);
+    r.y = products;
+    // FP32 products, so that a token's sum is rounded once
+    status = product<true>(Type::f32, r, items, stream);
+    if (status != cudaSuccess) return status;
+    switch (a.type) {
+    case Type::f16: return combine<__half>(a, products, stream);
+    case Type::bf16: return combine<__nv_bfloat16>(a, products, stream);
+    default: return combine<float>(a, products, stream);
+    }
+}
+
+}  // namespace nvcr_sm100::token

@@ -137,4 +137,71 @@ cudaError_t pack(const std::uint8_t* codes, const std::uint16_t* scales, const s
                  int inputs, int group, std::uint8_t* packed_codes, std::uint16_t* packed_scales, cudaStream_t stream);
 cudaError_t multiply(const MultiplyArgs& args, cudaStream_t stream);
 
+// Products in 8 bits: one matrix for all rows, or (choices not null) for each row of a token's `chosen` ones that of
+// an expert.
+struct BytesArgs {
+    Type type;
+    const void* x;  // [tokens][inner][inputs]
+    std::int64_t x_stride, x_inner_stride;
+    std::int64_t tokens;
+    int inner;   // rows of x a token: 1, or chosen
+    int chosen;  // rows of products a token
+    const std::int32_t* choices;  // [tokens][chosen]; null: one matrix, and chosen is 1
+    const float* weights;         // [tokens][chosen], or null: products are not summed
+    const void* packed;
+    const float* scales;  // [experts][outputs]
+    int experts;
+    int outputs;
+    int inputs;
+    const void* bias;  // [outputs], or null; null with choices
+    void* y;           // [tokens][chosen][outputs], or with weights [tokens][outputs]
+    void* workspace;
+    unsigned* status;  // null: not wanted
+};
+std::size_t byte_matrix_bytes(std::int64_t matrices, int outputs, int inputs);
+cudaError_t pack_bytes(const std::int8_t* codes, std::int64_t matrices, int outputs, int inputs, void* packed,
+                       cudaStream_t stream);
+std::size_t bytes_workspace(const BytesArgs& args);
+cudaError_t multiply_bytes(const BytesArgs& args, cudaStream_t stream);
+
+struct RouteArgs {
+    Type type;
+    const void* scores;
+    std::int64_t stride;
+    std::int64_t tokens;
+    int experts;
+    int count;
+    bool sigmoid;
+    const float* bias;  // null: none
+    int groups;
+    int kept_groups;
+    bool renormalise;
+    float scale;
+    std::int32_t* choices;  // [tokens][count]
+    float* weights;
+};
+constexpr int most_experts = 1024;
+cudaError_t route(const RouteArgs& args, cudaStream_t stream);
+
+struct SampleArgs {
+    Type type;
+    const void* logits;
+    std::int64_t stride;
+    std::int64_t rows;
+    int symbols;
+    const float* uniforms;
+    const float* temperatures;  // null: `temperature` for every row; the same of the others
+    const std::int32_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    float temperature;
+    int top_k;
+    float top_p;
+    float min_p;
+    std::int64_t* chosen;
+    float* probabilities;
+};
+constexpr int most_symbols = 1 << 20;
+cudaError_t sample(const SampleArgs& args, cudaStream_t stream);
+
 }  // namespace nvcr_sm100::token

@@ -87,6 +87,9 @@ EXPORTS = [
     "nvcr_sm100_dcvc_ycbcr_padded_to_yuv420p8", "nvcr_sm100_token_norm", "nvcr_sm100_token_append",
     "nvcr_sm100_token_read", "nvcr_sm100_token_context_create", "nvcr_sm100_token_context_destroy",
     "nvcr_sm100_token_attend", "nvcr_sm100_token_packed_bytes", "nvcr_sm100_token_pack", "nvcr_sm100_token_multiply",
+    "nvcr_sm100_token_bytes_packed", "nvcr_sm100_token_bytes_pack", "nvcr_sm100_token_bytes_workspace",
+    "nvcr_sm100_token_bytes_multiply", "nvcr_sm100_token_experts_workspace", "nvcr_sm100_token_experts_multiply",
+    "nvcr_sm100_token_route", "nvcr_sm100_token_sample",
 ]
 
 _lib: ctypes.CDLL | None = None
@@ -193,6 +196,21 @@ def library() -> ctypes.CDLL:
         "nvcr_sm100_token_pack": (ctypes.c_int, [vp] * 3 + [ctypes.c_int32] * 3 + [vp] * 3),
         "nvcr_sm100_token_multiply": (ctypes.c_int, [ctypes.c_int, vp, i64, i64, vp, vp] + [ctypes.c_int32] * 3 +
                                       [vp] * 3),
+        "nvcr_sm100_token_bytes_packed": (ctypes.c_int, [i64, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(sz)]),
+        "nvcr_sm100_token_bytes_pack": (ctypes.c_int, [vp, i64, ctypes.c_int32, ctypes.c_int32, vp, vp]),
+        "nvcr_sm100_token_bytes_workspace": (ctypes.c_int, [i64, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(sz)]),
+        "nvcr_sm100_token_bytes_multiply": (ctypes.c_int, [ctypes.c_int, vp, i64, i64, vp, vp] + [ctypes.c_int32] * 2 +
+                                            [vp] * 3 + [sz, vp, vp]),
+        "nvcr_sm100_token_experts_workspace": (ctypes.c_int, [i64, ctypes.c_int32, ctypes.c_int] + [ctypes.c_int32] * 3 +
+                                               [ctypes.POINTER(sz)]),
+        "nvcr_sm100_token_experts_multiply": (ctypes.c_int, [ctypes.c_int, vp, i64, i64, ctypes.c_int, i64, vp,
+                                                             ctypes.c_int32, vp, vp, vp] + [ctypes.c_int32] * 3 +
+                                              [vp, vp, sz, vp, vp]),
+        "nvcr_sm100_token_route": (ctypes.c_int, [ctypes.c_int, vp, i64, i64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int,
+                                                  vp, ctypes.c_int32, ctypes.c_int32, ctypes.c_int, ctypes.c_float, vp,
+                                                  vp, vp]),
+        "nvcr_sm100_token_sample": (ctypes.c_int, [ctypes.c_int, vp, i64, i64, ctypes.c_int32, vp, vp, ctypes.c_float, vp,
+                                                   ctypes.c_int32, vp, ctypes.c_float, vp, ctypes.c_float, vp, vp, vp]),
     }
     for name, (restype, argtypes) in signatures.items():
         function = getattr(lib, name)

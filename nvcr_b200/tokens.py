@@ -3,7 +3,9 @@
 ``block_norm`` is the norms after and before a block with its gate and residual;
 ``PagedCache`` holds keys and values in 4 bits, rotated on the way in;
 ``TokenContext.attend`` is attention over such a cache; ``PackedMatrix`` is a
-4-bit weight matrix with group scales. Tensors are torch tensors on the current
+4-bit weight matrix with group scales, for a few rows; ``ByteMatrix`` and
+``ByteExperts`` are weights in 8 bits, for one row to a prompt's; ``route``
+chooses a token's experts and ``sample`` the next symbol. Tensors are torch tensors on the current
 CUDA device (another one's are refused); work is enqueued on torch's current
 stream unless ``stream`` names another (then the caller orders the two, and keeps
 the tensors alive). What the operators refuse raises ``ExecutorError``; there is
@@ -264,3 +266,130 @@ class PackedMatrix:
         """x [rows, inputs] (float16 or bfloat16, any row stride) times the matrix's transpose, plus bias [outputs]."""
         return (_module or _native()).multiply(*self._addresses, self.outputs, self.inputs, self.group, self._index, x, bias,
                                                None if stream is None else _stream(stream))
+
+
+class _Bytes:
+    """Weights in 8 bits [matrices, outputs, inputs] with a scale an output, laid out once."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, matrices: int, stream) -> None:
+        _require(codes.is_cuda, "weights are on a CUDA device")
+        outputs, inputs = codes.shape[-2:]
+        device, index = codes.device, codes.get_device()
+        (_module or _native()).on_current(index)
+        code_address = _whole(codes, "codes", torch.int8, codes.shape, index)
+        _whole(scales, "scales", torch.float32, codes.shape[:-1], index)
+        size = ctypes.c_size_t(0)
+        _check(library().nvcr_sm100_token_bytes_packed(matrices, outputs, inputs, ctypes.byref(size)))
+        self.outputs, self.inputs, self.device, self._index = outputs, inputs, device, index
+        with _on(stream, device):
+            self.codes = torch.empty(size.value, dtype=torch.uint8, device=device)
+            self.scales = scales.clone()
+            self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self._addresses = (self.codes.data_ptr(), self.scales.data_ptr())
+        handle = torch.cuda.current_stream(index).cuda_stream if stream is None else _stream(stream)
+        _check(library().nvcr_sm100_token_bytes_pack(code_address, matrices, outputs, inputs, self._addresses[0], handle))
+
+    @staticmethod
+    def _quantised(weights: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        parts = weights.float()
+        largest = parts.abs().amax(-1)
+        part = torch.tensor(1.0 / 127.0, dtype=torch.float32, device="cpu")  # a product in FP32
+        scales = (largest * part).clamp(min=2.0 ** -126)
+        codes = torch.round(parts * scales.reciprocal().unsqueeze(-1)).nan_to_num(0.0).clamp(-127, 127).to(torch.int8)
+        # a row that holds no finite values has no finite scale: its outputs are no numbers
+        return codes, torch.where(torch.isfinite(largest), scales, torch.nan)
+
+    def check(self) -> None:
+        """Waits for all streams of the device and raises if a wait in a kernel ran out since the last check."""
+        torch.cuda.synchronize(self.device)
+        found = int(self.status.item())
+        if found:
+            self.status.bitwise_and_(~found)
+            torch.cuda.current_stream(self.device).synchronize()
+            raise ExecutorError(ErrorCode.backend_error, "a wait in a product of 8-bit weights ran out")
+
+
+class ByteMatrix(_Bytes):
+    """An 8-bit weight matrix [outputs, inputs] with a scale an output, laid out once: codes int8 and scales float32
+    [outputs]. At most 131072 inputs."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, stream=None) -> None:
+        _require(codes.dim() == 2, "codes have two dimensions")
+        super().__init__(codes, scales, 1, stream)
+
+    @classmethod
+    def quantise(cls, weights: torch.Tensor, stream=None) -> "ByteMatrix":
+        """From a float matrix [outputs, inputs], each row by its largest magnitude, as `multiply` takes a row of x."""
+        _require(weights.dim() == 2, "weights have two dimensions")
+        _require(weights.is_cuda, "weights are on a CUDA device")
+        with _on(stream, weights.device):  # whose allocator takes the codes back when this returns
+            codes, scales = cls._quantised(weights)
+        return cls(codes, scales, stream)
+
+    def multiply(self, x: torch.Tensor, bias: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """x [rows, inputs] (float16, bfloat16 or float32, any row stride) times the matrix's transpose, plus bias
+        [outputs]: (sum of codes) * the output's scale * the row's, where a row of x is taken as codes rint(x / s) with
+        s = max|x| / 127. The sums are exact; a row that holds a NaN or an infinity gives NaNs."""
+        return (_module or _native()).bytes_multiply(*self._addresses, self.outputs, self.inputs, self.status.data_ptr(),
+                                                     self._index, x, bias, None if stream is None else _stream(stream))
+
+
+class ByteExperts(_Bytes):
+    """The 8-bit weight matrices of up to 1024 experts: codes int8 [experts, outputs, inputs] and scales float32
+    [experts, outputs], as `ByteMatrix`'s."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, stream=None) -> None:
+        _require(codes.dim() == 3, "codes have three dimensions")
+        self.experts = codes.shape[0]
+        super().__init__(codes, scales, self.experts, stream)
+
+    @classmethod
+    def quantise(cls, weights: torch.Tensor, stream=None) -> "ByteExperts":
+        """From float matrices [experts, outputs, inputs]."""
+        _require(weights.dim() == 3, "weights have three dimensions")
+        _require(weights.is_cuda, "weights are on a CUDA device")
+        with _on(stream, weights.device):
+            codes, scales = cls._quantised(weights)
+        return cls(codes, scales, stream)
+
+    def multiply(self, x: torch.Tensor, choices: torch.Tensor, weights: torch.Tensor | None = None,
+                 stream=None) -> torch.Tensor:
+        """Each token's rows times the matrices of the experts it chose: int32 `choices` [tokens, chosen], as `route`
+        gives them; x [tokens, inputs], or [tokens, chosen, inputs] with a row for each choice. Without `weights`
+        [tokens, chosen, outputs]; with them (float32 [tokens, chosen]) the weighted sum over a token's choices,
+        [tokens, outputs]. A choice of no expert (-1) gives zeros and is left out of the sum."""
+        return (_module or _native()).experts_multiply(*self._addresses, self.experts, self.outputs, self.inputs,
+                                                       self.status.data_ptr(), self._index, x, choices, weights,
+                                                       None if stream is None else _stream(stream))
+
+
+def route(scores: torch.Tensor, count: int, *, kind: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
+          kept_groups: int | None = None, renormalise: bool = False, scale: float = 1.0,
+          stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(choices, weights)`` of tokens' scores [tokens, experts], int32 and float32 [tokens, count]: the `count` experts
+    with the largest s + bias, in falling order (equal ones by index), s the "softmax" of a token's scores or their
+    "sigmoid", and their weights s, without the bias (float32 [experts]). With `groups` equal runs of experts, only those
+    in the `kept_groups` runs count whose two largest s + bias sum to the most. `renormalise` divides a token's weights
+    by their sum; then they are multiplied by `scale`. Experts with a score of -infinity or NaN are never chosen; where
+    fewer than `count` are left, the last choices are -1 with weight 0."""
+    if kind not in ("softmax", "sigmoid"):
+        _refuse("kind must be one of ['sigmoid', 'softmax']")
+    return (_module or _native()).route(scores, count, kind == "sigmoid", bias, groups,
+                                        groups if kept_groups is None else kept_groups, renormalise, scale,
+                                        None if stream is None else _stream(stream))
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: float | torch.Tensor = 1.0,
+           top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
+           stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(symbols, probabilities)``, int64 and float32 [rows]: a symbol of each row of logits [rows, symbols] by its
+    uniform number in [0, 1) (float32 [rows]), and that symbol's probability among those kept.
+
+    In the order of falling logits, equal ones by index, are kept: the first `top_k` symbols (0: all), of these the
+    shortest prefix with `top_p` of their weight exp(l / temperature), of these those with at least `min_p` times the
+    largest weight. The chosen one is the first, in the order of indexes, at which the running sum of the kept weights
+    is above the uniform number times the whole. A temperature of 0 takes the largest logit. Each setting is a number,
+    or a tensor [rows] (float32; int32 for `top_k`). Logits of -infinity and NaN are left out; a row of nothing else
+    gives -1 and 0."""
+    return (_module or _native()).sample(logits, uniforms, temperature, top_k, top_p, min_p,
+                                         None if stream is None else _stream(stream))
