@@ -5,21 +5,36 @@
 //
 // Every filter keeps a prefix of that order, so what is kept is told by a threshold: all logits above one, and the
 // first few equal to it. Weights are FP64 and summed as whole multiples of 2^-43 of the largest, so that no order of
-// sums changes a choice.
+// sums changes a choice, and which symbol is chosen does not hang on a rounding to FP32.
+//
+// A cluster of up to eight blocks has a row in its registers, read once (`cluster_kernel`):
+// * Where the symbols that can be kept are few (`candidates`: by min_p, top_k or ten octaves below the largest), they go
+//   to the first block, which sorts them and ends the row (`finish`). The rest is summed in FP32 for top_p's whole; a
+//   choice that hangs on that sum's error is made again by `row_by_block`, exactly.
+// * Where they are many, a histogram of weights or counts over the cluster says between which logits the threshold lies,
+//   and these are sorted (`find`); the choice is found by sums of each warp's runs (`locate`).
+// Longer rows and infinite logits take `row_by_block`, which finds the threshold's bits from memory
+// with one block.
 #include "token_elements.cuh"
 
+#include <climits>
 #include <cmath>
 
 namespace nvcr_sm100::token {
 namespace {
 
-constexpr int sample_threads = 1024;
+constexpr int threads = 512;
+constexpr int warps = threads / 32;
 constexpr int bins = 2048;
+constexpr int most_blocks = 8;
+constexpr int most_candidates = 2048;
+constexpr int most_vectors = 16;  // a thread
+constexpr int cut_bins = 256;     // of `cut`, so many an octave:
+constexpr float cut_steps = 5.5f;
 
 // The order of logits as that of unsigned integers; 0: left out (-infinity, NaN). -0 and +0 are equal.
-template <typename T>
-__device__ __forceinline__ unsigned key_of(T logit) {
-    const float v = widen(logit) + 0.0f;
+__device__ __forceinline__ unsigned key_of(float logit) {
+    const float v = logit + 0.0f;
     if (!(v > -INFINITY)) return 0;
     const unsigned bits = __float_as_uint(v);
     return bits >> 31 ? ~bits : bits | 0x80000000u;
@@ -28,31 +43,89 @@ __device__ __forceinline__ float logit_of(unsigned key) {
     return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
 }
 
+using Weight = unsigned long long;
+constexpr double unit = 8796093022208.0;  // 2^43: 2^20 weights stay below 2^63
+constexpr int table_size = 64;
+
 struct Row {
-    unsigned top;        // the largest key
-    double temperature;  // 0: the largest alone
+    unsigned top;         // the largest key
+    double temperature;   // 0: the largest alone
+    double least;         // of a kept share
+    double factor;        // steps of 2^(1/64) a logit
+    const double* table;  // unit * 2^(i / 64)
 };
 
+// A logit's share of the largest one's weight, in units. With y = 64 log2(e) (l - max) / temperature = n + f, |f| <= 1/2:
+// 2^(n / 64) from the table and its exponent, e^(f ln(2) / 64) by Taylor's polynomial, whose fifth term is below 4e-14.
 __device__ __forceinline__ double share_of(unsigned key, const Row& row) {
-    if (key == 0) return 0.0;
-    if (key == row.top) return 1.0;  // infinite ones too
-    if (row.temperature == 0.0) return 0.0;
-    return exp((static_cast<double>(logit_of(key)) - static_cast<double>(logit_of(row.top))) / row.temperature);
+    const double y = (static_cast<double>(logit_of(key)) - static_cast<double>(logit_of(row.top))) * row.factor;
+    const double whole = y + 6755399441055744.0;  // 1.5 * 2^52: rounds to a whole number, in the low word
+    const int n = __double2loint(whole);
+    const double f = y - (whole - 6755399441055744.0);
+    constexpr double c = 0.69314718055994530942 / table_size;
+    const double p = fma(f, fma(f, fma(f, fma(f, c * c * c * c / 24.0, c * c * c / 6.0), c * c / 2.0), c), 1.0);
+    const double w = row.table[n & (table_size - 1)] * p;
+    const double found = __hiloint2double(__double2hiint(w) + (n >> 6) * (1 << 20), __double2loint(w));
+    // below 2^-46, less than half a unit: none; so are symbols that are left out, and all but the largest at temperature 0
+    return key == row.top ? unit : key != 0 && y > -46.0 * table_size ? found : 0.0;
 }
-using Weight = unsigned long long;
-__device__ __forceinline__ Weight weight_of(double share) { return static_cast<Weight>(__double2ull_rn(share * 8796093022208.0)); }
+// Rounded to whole units: below 2^52 the sum's low bits.
+__device__ __forceinline__ Weight weight_of(double share) {
+    return static_cast<Weight>(__double_as_longlong(share + 4503599627370496.0)) & 0xfffffffffffffull;
+}
+__device__ __forceinline__ float probability_of(double share, Weight all) {
+    return static_cast<float>(share / static_cast<double>(all));
+}
+
+// What is kept: keys above `key`, and the first `ties` equal to it.
+struct Threshold {
+    unsigned key;
+    unsigned ties;
+};
+__device__ __forceinline__ Threshold stricter(Threshold a, Threshold b) {
+    return a.key > b.key || (a.key == b.key && a.ties < b.ties) ? a : b;
+}
+
+// The least weight that holds top_p of all.
+__device__ __forceinline__ Weight part_of(float top_p, Weight all) {
+    const double part = ceil(static_cast<double>(fmaxf(top_p, 0.0f)) * static_cast<double>(all));
+    return max(static_cast<Weight>(1), static_cast<Weight>(part));
+}
+
+// u times the whole, rounded down: below the whole. u is 0 for a NaN and below, the last symbol from 1 on.
+__device__ __forceinline__ Weight part_of_uniform(float uniform, Weight all) {
+    const unsigned long long u = !(uniform > 0.0f) ? 0ull
+        : uniform >= 1.0f                          ? ~0ull
+                                                   : static_cast<unsigned long long>(static_cast<double>(uniform) * 18446744073709551616.0);
+    return __umul64hi(u, all);
+}
+
+struct Settings {
+    float temperature, top_p, min_p, uniform;
+    int top_k;
+};
+__device__ __forceinline__ Settings settings_of(const SampleArgs& a, std::int64_t r) {
+    return {a.temperatures == nullptr ? a.temperature : a.temperatures[r], a.top_ps == nullptr ? a.top_p : a.top_ps[r],
+            a.min_ps == nullptr ? a.min_p : a.min_ps[r], a.uniforms[r], a.top_ks == nullptr ? a.top_k : a.top_ks[r]};
+}
+__device__ __forceinline__ Row row_of(unsigned top, const Settings& s, const double* table) {
+    const double temperature = s.temperature > 0.0f ? static_cast<double>(s.temperature) : 0.0;
+    return {top, temperature, s.min_p > 0.0f ? static_cast<double>(fminf(s.min_p, 1.0f)) * unit : 0.0,
+            table_size * 1.4426950408889634074 / temperature, table};
+}
+// By the block's first threads; the caller synchronises.
+__device__ __forceinline__ void make_table(double* table) {
+    if (threadIdx.x < table_size) table[threadIdx.x] = unit * exp2(threadIdx.x / static_cast<double>(table_size));
+}
 
 struct Sums {
-    unsigned counts[bins];
-    unsigned low[bins], high[bins];  // halves of the weights' sums
-    Weight warp_weight[32];
-    unsigned warp_count[32];
+    unsigned low[bins], high[bins];  // counts in low, or halves of the weights' sums
+    Weight scratch[warps];
     Weight found_weight;
-    unsigned found_count;
     int found;
 };
 
-// The sums of a block's threads before each of them, and of all.
+// The sum of the block's threads before this one, and of all.
 __device__ __forceinline__ Weight before(Weight mine, Weight* scratch, Weight& all) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     Weight sum = mine;
@@ -65,68 +138,65 @@ __device__ __forceinline__ Weight before(Weight mine, Weight* scratch, Weight& a
     __syncthreads();
     Weight earlier = 0;
     all = 0;
-    for (int w = 0; w < sample_threads / 32; ++w) {
+    for (int w = 0; w < warps; ++w) {
         if (w < warp) earlier += scratch[w];
         all += scratch[w];
     }
     return earlier + sum - mine;
 }
 
-// What is kept: keys above `key`, and the first `ties` equal to it.
-struct Threshold {
-    unsigned key;
-    unsigned ties;
-};
+__device__ __forceinline__ void add(Sums& sums, unsigned bin, Weight w) {
+    const unsigned low = static_cast<unsigned>(w), old = atomicAdd(&sums.low[bin], low);
+    atomicAdd(&sums.high[bin], static_cast<unsigned>(w >> 32) + (old + low < old ? 1u : 0u));
+}
 
-// The threshold of the shortest prefix that holds `wanted` of the counts (by_weight: of the weights), among what `kept`
-// keeps: the key's bits from the top down, each level a histogram of the keys that agree with those found.
+// The bin, from the top down, at which the sums pass `wanted`, and what lies above it. found stays -1 where they do not.
+template <typename Of>
+__device__ __forceinline__ void pass(Sums& sums, Weight above, Weight wanted, Of&& of) {
+    constexpr int each = bins / threads;
+    const int first = bins - 1 - each * static_cast<int>(threadIdx.x);
+    Weight mine[each], sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < each; ++i) sum += mine[i] = of(first - i);
+    Weight earlier = above + before(sum, sums.scratch, all);
+#pragma unroll
+    for (int i = 0; i < each; ++i) {
+        if (earlier < wanted && earlier + mine[i] >= wanted) sums.found = first - i, sums.found_weight = earlier;
+        earlier += mine[i];
+    }
+}
+
+// ---- a block a row, from memory: any row, exactly ----
+
 template <typename T>
-__device__ Threshold find(const T* logits, int symbols, const Row& row, bool by_weight, Weight wanted, Threshold kept,
-                          Sums& sums) {
+__device__ Threshold find_by_block(const T* logits, int symbols, const Row& row, bool by_weight, Weight wanted, Threshold kept,
+                                   Sums& sums) {
     unsigned prefix = 0;
     int shift = 32;
     Weight above = 0;  // of keys above the prefix's
     for (const int width : {11, 11, 10}) {
         const int next = shift - width;
         __syncthreads();
-        for (int i = threadIdx.x; i < bins; i += sample_threads) sums.counts[i] = sums.low[i] = sums.high[i] = 0;
+        for (int i = threadIdx.x; i < bins; i += threads) sums.low[i] = sums.high[i] = 0;
         if (threadIdx.x == 0) sums.found = -1;
         __syncthreads();
-        for (int i = threadIdx.x; i < symbols; i += sample_threads) {
-            const unsigned key = key_of(logits[i]);
+        for (int i = threadIdx.x; i < symbols; i += threads) {
+            const unsigned key = key_of(widen(logits[i]));
             if (key < kept.key || key == 0 || (shift < 32 && key >> shift != prefix)) continue;
             const unsigned bin = key >> next & ((1u << width) - 1);
             if (!by_weight) {
-                atomicAdd(&sums.counts[bin], 1u);
-                continue;
+                atomicAdd(&sums.low[bin], 1u);
+            } else if (key != kept.key) {  // those are added below
+                const Weight w = weight_of(share_of(key, row));
+                if (w != 0) add(sums, bin, w);
             }
-            if (key == kept.key) continue;  // counted below
-            const Weight w = weight_of(share_of(key, row));
-            if (w == 0) continue;
-            const unsigned low = static_cast<unsigned>(w), old = atomicAdd(&sums.low[bin], low);
-            atomicAdd(&sums.high[bin], static_cast<unsigned>(w >> 32) + (old + low < old ? 1u : 0u));
         }
         __syncthreads();
         if (by_weight && threadIdx.x == 0 && kept.key != 0 && (shift == 32 || kept.key >> shift == prefix)) {
-            const unsigned bin = kept.key >> next & ((1u << width) - 1);
-            const Weight w = (static_cast<Weight>(sums.high[bin]) << 32 | sums.low[bin]) +
-                kept.ties * weight_of(share_of(kept.key, row));
-            sums.low[bin] = static_cast<unsigned>(w), sums.high[bin] = static_cast<unsigned>(w >> 32);
+            add(sums, kept.key >> next & ((1u << width) - 1), kept.ties * weight_of(share_of(kept.key, row)));
         }
         __syncthreads();
-        // from the top bin down: thread t has bins - 1 - 2 t and the one below it
-        const int first = bins - 1 - 2 * static_cast<int>(threadIdx.x);
-        auto of = [&](int bin) {
-            return by_weight ? static_cast<Weight>(sums.high[bin]) << 32 | sums.low[bin] : static_cast<Weight>(sums.counts[bin]);
-        };
-        Weight all;
-        const Weight one = of(first), two = of(first - 1);
-        const Weight earlier = above + before(one + two, sums.warp_weight, all);
-        if (earlier < wanted && earlier + one + two >= wanted) {
-            const bool upper = earlier + one >= wanted;
-            sums.found = upper ? first : first - 1;
-            sums.found_weight = upper ? earlier : earlier + one;
-        }
+        pass(sums, above, wanted, [&](int bin) { return static_cast<Weight>(sums.high[bin]) << 32 | sums.low[bin]; });
         __syncthreads();
         if (sums.found < 0) return kept;  // there is less than wanted: all of it
         prefix = prefix << width | static_cast<unsigned>(sums.found);
@@ -135,71 +205,55 @@ __device__ Threshold find(const T* logits, int symbols, const Row& row, bool by_
     }
     __syncthreads();
     const Weight each = by_weight ? weight_of(share_of(prefix, row)) : 1;
-    const Weight ties = (wanted - above + each - 1) / each;
-    return {prefix, static_cast<unsigned>(ties)};
-}
-
-__device__ __forceinline__ Threshold stricter(Threshold a, Threshold b) {
-    return a.key > b.key || (a.key == b.key && a.ties < b.ties) ? a : b;
+    return {prefix, static_cast<unsigned>((wanted - above + each - 1) / each)};
 }
 
 template <typename T>
-__global__ void __launch_bounds__(sample_threads) sample_kernel(SampleArgs a) {
-    __shared__ Sums sums;
-    join_chain();
-    const std::int64_t r = blockIdx.x;
+__device__ __noinline__ void row_by_block(const SampleArgs& a, std::int64_t r, Sums& sums, const double* table) {
     const T* logits = static_cast<const T*>(a.logits) + r * a.stride;
     const int symbols = a.symbols, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const float temperature = a.temperatures == nullptr ? a.temperature : a.temperatures[r];
-    const float top_p = a.top_ps == nullptr ? a.top_p : a.top_ps[r];
-    const float min_p = a.min_ps == nullptr ? a.min_p : a.min_ps[r];
-    const int top_k = a.top_ks == nullptr ? a.top_k : a.top_ks[r];
-    const float uniform = a.uniforms[r];
-
+    const Settings s = settings_of(a, r);
     unsigned top = 0;
-    for (int i = threadIdx.x; i < symbols; i += sample_threads) top = max(top, key_of(logits[i]));
+    for (int i = threadIdx.x; i < symbols; i += threads) top = max(top, key_of(widen(logits[i])));
     top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) sums.warp_count[warp] = top;
     __syncthreads();
-    for (int w = 0; w < sample_threads / 32; ++w) top = max(top, sums.warp_count[w]);
+    if (lane == 0) sums.scratch[warp] = top;
+    __syncthreads();
+    for (int w = 0; w < warps; ++w) top = max(top, static_cast<unsigned>(sums.scratch[w]));
     if (top == 0) {  // nothing to choose
         if (threadIdx.x == 0) a.chosen[r] = -1, a.probabilities[r] = 0.0f;
         return;
     }
-    const Row row{top, temperature > 0.0f ? static_cast<double>(temperature) : 0.0};
+    const Row row = row_of(top, s, table);
     Threshold kept{0, 0};
     if (row.temperature == 0.0) {
         kept = {top, 1};
     } else {
-        if (top_k > 0 && top_k < symbols) kept = find(logits, symbols, row, false, top_k, kept, sums);
-        if (top_p < 1.0f) {
+        if (s.top_k > 0 && s.top_k < symbols) kept = find_by_block(logits, symbols, row, false, s.top_k, kept, sums);
+        if (s.top_p < 1.0f) {
             Weight mine = 0, all;
-            for (int i = threadIdx.x; i < symbols; i += sample_threads) {
-                const unsigned key = key_of(logits[i]);
+            for (int i = threadIdx.x; i < symbols; i += threads) {
+                const unsigned key = key_of(widen(logits[i]));
                 if (key > kept.key) mine += weight_of(share_of(key, row));
             }
-            before(mine, sums.warp_weight, all);
+            before(mine, sums.scratch, all);
             if (kept.key != 0) all += kept.ties * weight_of(share_of(kept.key, row));
-            const double part = ceil(static_cast<double>(fmaxf(top_p, 0.0f)) * static_cast<double>(all));
-            const Weight wanted = max(static_cast<Weight>(1), static_cast<Weight>(part));
-            kept = stricter(kept, find(logits, symbols, row, true, wanted, kept, sums));
+            kept = stricter(kept, find_by_block(logits, symbols, row, true, part_of(s.top_p, all), kept, sums));
         }
     }
-    const double least = min_p > 0.0f ? static_cast<double>(fminf(min_p, 1.0f)) : 0.0;
-
     // a thread a run of symbols, in the order of their indexes
-    const int each = (symbols + sample_threads - 1) / sample_threads;
+    const int each = (symbols + threads - 1) / threads;
     const int from = min(symbols, static_cast<int>(threadIdx.x) * each), to = min(symbols, from + each);
     Weight ties = 0, all_ties;
-    for (int i = from; i < to; ++i) ties += key_of(logits[i]) == kept.key;
-    const Weight earlier_ties = before(ties, sums.warp_weight, all_ties);
+    for (int i = from; i < to; ++i) ties += key_of(widen(logits[i])) == kept.key;
+    const Weight earlier_ties = before(ties, sums.scratch, all_ties);
     auto walk = [&](auto&& visit) {
         Weight nth = earlier_ties;
         for (int i = from; i < to; ++i) {
-            const unsigned key = key_of(logits[i]);
+            const unsigned key = key_of(widen(logits[i]));
             if (key == 0 || key < kept.key || (key == kept.key && nth++ >= kept.ties)) continue;
             const double share = share_of(key, row);
-            if (share >= least && !visit(i, share)) return;
+            if (share >= row.least && !visit(i, share)) return;
         }
     };
     Weight mine = 0, all;
@@ -207,26 +261,880 @@ __global__ void __launch_bounds__(sample_threads) sample_kernel(SampleArgs a) {
         mine += weight_of(share);
         return true;
     });
-    Weight sum = before(mine, sums.warp_weight, all);
-    // u in units of 2^-64; 0 for a NaN and below, the last symbol from 1 on
-    const unsigned long long u = !(uniform > 0.0f) ? 0ull
-        : uniform >= 1.0f                          ? ~0ull
-                                                   : static_cast<unsigned long long>(static_cast<double>(uniform) * 18446744073709551616.0);
-    const Weight wanted = __umul64hi(u, all);  // below `all`
+    Weight sum = before(mine, sums.scratch, all);
+    const Weight wanted = part_of_uniform(s.uniform, all);
     if (wanted >= sum && wanted < sum + mine) {
         walk([&](int i, double share) {
             sum += weight_of(share);
             if (sum <= wanted) return true;
             a.chosen[r] = i;
-            a.probabilities[r] = static_cast<float>(share * 8796093022208.0 / static_cast<double>(all));
+            a.probabilities[r] = probability_of(share, all);
             return false;
         });
     }
 }
 
 template <typename T>
+__global__ void __launch_bounds__(threads) block_kernel(SampleArgs a) {
+    __shared__ Sums sums;
+    __shared__ double table[table_size];
+    make_table(table);
+    join_chain();
+    __syncthreads();
+    row_by_block<T>(a, blockIdx.x, sums, table);
+}
+
+// ---- a cluster a row, from registers ----
+
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ std::uint32_t at_block(const void* here, int rank) {
+    std::uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(there)
+                 : "r"(static_cast<std::uint32_t>(__cvta_generic_to_shared(here))), "r"(rank));
+    return there;
+}
+__device__ __forceinline__ void put(const void* here, int rank, unsigned long long v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at_block(here, rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ unsigned get(const unsigned* here, int rank) {
+    unsigned v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at_block(here, rank)) : "memory");
+    return v;
+}
+
+struct Shared {
+    Sums sums;
+    unsigned long long gathered[most_candidates];  // the first block's: a part for each block
+    alignas(16) unsigned long long sorted[most_candidates];
+    Weight weights[most_candidates];  // running sums
+    Weight cells[most_vectors * warps];
+    double table[table_size];
+    unsigned long long maxima[most_blocks], totals[most_blocks], counts[2][most_blocks], sums_of[2][most_blocks];
+    unsigned long long told[2];  // the first block to all
+    float parts[2][warps];
+    unsigned count, queued;
+    unsigned kept, low, high;
+    int cut;
+};
+
+template <typename T>
+struct Elements {
+    static constexpr int each = 16 / sizeof(T);
+    static __device__ __forceinline__ float get(const uint4& v, int i) {
+        const unsigned words[4] = {v.x, v.y, v.z, v.w};
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(words[i]);
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            return __uint_as_float(i % 2 == 0 ? words[i / 2] << 16 : words[i / 2] & 0xffff0000u);
+        } else {
+            return half_bits(static_cast<std::uint16_t>(words[i / 2] >> (i % 2 * 16)));
+        }
+    }
+    static __device__ __forceinline__ float pick(const uint4& v, int i) {  // i known at run time only
+        const int at = i / (each / 4);
+        const unsigned word = at == 0 ? v.x : at == 1 ? v.y : at == 2 ? v.z : v.w;
+        const uint4 found{word, word, word, word};
+        return sizeof(T) == 4 || i % 2 == 0 ? get(found, 0) : get(found, 1);
+    }
+    static __device__ __forceinline__ float largest(const uint4& v) {  // no NaN, unless all are
+        if constexpr (sizeof(T) == 4) {
+            return fmaxf(fmaxf(get(v, 0), get(v, 1)), fmaxf(get(v, 2), get(v, 3)));
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            const auto pair = [](const unsigned& w) { return reinterpret_cast<const __nv_bfloat162&>(w); };
+            const __nv_bfloat162 most = __hmax2(__hmax2(pair(v.x), pair(v.y)), __hmax2(pair(v.z), pair(v.w)));
+            return fmaxf(__low2float(most), __high2float(most));
+        } else {
+            const auto pair = [](const unsigned& w) { return reinterpret_cast<const __half2&>(w); };
+            const __half2 most = __hmax2(__hmax2(pair(v.x), pair(v.y)), __hmax2(pair(v.z), pair(v.w)));
+            return fmaxf(__low2float(most), __high2float(most));
+        }
+    }
+    // -infinity in every place
+    static __device__ __forceinline__ uint4 none() {
+        const unsigned w = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __nv_bfloat16> ? 0xff80ff80u : 0xfc00fc00u;
+        return {w, w, w, w};
+    }
+};
+
+// What a cluster keeps: keys above `key`, and those equal to it up to index `last`.
+struct Kept {
+    unsigned key;
+    int last;
+    __device__ __forceinline__ bool holds(unsigned k, int index) const { return k > key || (k == key && k != 0 && index <= last); }
+};
+
+// 2048 in falling order, by 512 threads: four neighbours a thread, so that only exchanges over 128 places and more pass
+// through shared memory.
+__device__ __forceinline__ void sort(unsigned long long* shared) {
+    static_assert(most_candidates == 4 * threads);
+    unsigned long long v[4];
+    const int base = 4 * static_cast<int>(threadIdx.x);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = shared[base + i];
+    auto order = [](unsigned long long& a, unsigned long long& b, bool falling) {
+        if ((a < b) == falling) {
+            const unsigned long long t = a;
+            a = b, b = t;
+        }
+    };
+#pragma unroll 1
+    for (int size = 2; size <= most_candidates; size *= 2) {
+        int apart = size / 2;
+        if (apart >= 128) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) shared[base + i] = v[i];
+#pragma unroll 1
+            for (; apart >= 128; apart /= 2) {
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < most_candidates / 2 / threads; ++k) {
+                    const int p = static_cast<int>(threadIdx.x) + k * threads, at = 2 * p - (p & (apart - 1));
+                    unsigned long long a = shared[at], b = shared[at + apart];
+                    order(a, b, (at & size) == 0);
+                    shared[at] = a, shared[at + apart] = b;
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = shared[base + i];
+        }
+#pragma unroll 1
+        for (; apart >= 4; apart /= 2) {
+            const bool lower = (base & apart) == 0, falling = ((base & size) == 0) == lower;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned long long other = __shfl_xor_sync(0xffffffffu, v[i], apart / 4);
+                v[i] = falling ? max(v[i], other) : min(v[i], other);
+            }
+        }
+        if (size >= 4) {
+            const bool falling = (base & size) == 0;
+            order(v[0], v[2], falling), order(v[1], v[3], falling);
+            order(v[0], v[1], falling), order(v[2], v[3], falling);
+        } else {
+            order(v[0], v[1], true), order(v[2], v[3], false);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) shared[base + i] = v[i];
+    __syncthreads();
+}
+
+// FP32 sums of weights that are not candidates, as a share of them: three roundings of 2^-24 of an exponent of at most 46,
+// and two of largest * factor, times ln 2; ex2.approx's error (2^-22) and up to 160 additions.
+__device__ __forceinline__ double bulk_error(float largest, float factor) {
+    return 3e-5 + 2e-7 * fabs(static_cast<double>(largest) * static_cast<double>(factor));
+}
+
+template <typename T>
+struct ClusterRow {
+    using Of = Elements<T>;
+    static constexpr int each = Of::each;
+    const SampleArgs& a;
+    Shared& shared;
+    std::int64_t r;
+    int rank, blocks;
+    int vectors;  // of this thread
+    int first;    // index of this thread's first element: of its n-th vector first + n * threads * each
+
+    // A vector, with -infinity outside the row.
+    __device__ __forceinline__ uint4 load(int n) const {
+        const T* logits = static_cast<const T*>(a.logits) + r * a.stride;
+        const int at = first + n * threads * each;
+        uint4 v = Of::none();
+        if (at >= 0 && at + each <= a.symbols) {
+            v = *reinterpret_cast<const uint4*>(logits + at);
+        } else if (at + each > 0 && at < a.symbols) {
+            unsigned words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < each; ++i) {
+                if (at + i < 0 || at + i >= a.symbols) continue;
+                if constexpr (sizeof(T) == 4) {
+                    words[i] = __float_as_uint(logits[at + i]);
+                } else {
+                    const unsigned bits = reinterpret_cast<const std::uint16_t*>(logits)[at + i];
+                    words[i / 2] = i % 2 == 0 ? (words[i / 2] & 0xffff0000u) | bits : (words[i / 2] & 0xffffu) | bits << 16;
+                }
+            }
+            v = {words[0], words[1], words[2], words[3]};
+        }
+        return v;
+    }
+
+    // body(n, vector) for each, four loads at a time under way.
+    template <typename Body>
+    __device__ __forceinline__ void for_vectors(Body&& body) const {
+        for (int n = 0; n < vectors; n += 4) {
+            uint4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = n + i < vectors ? load(n + i) : Of::none();
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                if (n + i >= vectors) break;
+                const uint4 one = i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3];
+                body(n + i, one);
+            }
+        }
+    }
+
+    // Where the running sum of amounts, in the order of indexes, first exceeds wanted(their whole): visit(index, key, whole)
+    // there, by one thread of the cluster.
+    template <typename Amount, typename Wanted, typename Visit>
+    __device__ __forceinline__ void locate(Amount&& amount, Wanted&& wanted_of, Visit&& visit) {
+        __syncthreads();
+        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+        for_vectors([&](int n, const uint4& v) {
+            Weight sum = 0;
+#pragma unroll
+            for (int i = 0; i < each; ++i) sum += amount(first + n * threads * each + i, key_of(Of::get(v, i)));
+#pragma unroll
+            for (int o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) shared.cells[n * warps + warp] = sum;
+        });
+        __syncthreads();
+        Weight block_sum = 0;
+        if (warp == 0) {
+            for (int c = lane; c < vectors * warps; c += 32) block_sum += shared.cells[c];
+#pragma unroll
+            for (int o = 16; o > 0; o /= 2) block_sum += __shfl_xor_sync(0xffffffffu, block_sum, o);
+            if (lane < blocks) put(&shared.totals[rank], lane, block_sum);
+        }
+        cluster_sync();
+        Weight earlier = 0, all = 0;
+        for (int b = 0; b < blocks; ++b) {
+            if (b < rank) earlier += shared.totals[b];
+            all += shared.totals[b];
+        }
+        const Weight wanted = wanted_of(all);
+        if (earlier > wanted || earlier + shared.totals[rank] <= wanted) return;
+        int cell = 0;
+        while (earlier + shared.cells[cell] <= wanted) earlier += shared.cells[cell++];
+        if (cell % warps != warp) return;
+const int n = cell / warps;
+        const uint4 v = load(n);
+        Weight sum = 0;
+#pragma unroll
+        for (int i = 0; i < each; ++i) sum += amount(first + n * threads * each + i, key_of(Of::get(v, i)));
+        Weight to = sum;
+        for (int o = 1; o < 32; o *= 2) {
+            const Weight u = __shfl_up_sync(0xffffffffu, to, o);
+            if (lane >= o) to += u;
+        }
+        Weight from = earlier + to - sum;
+        if (wanted < from || wanted >= earlier + to) return;
+#pragma unroll
+        for (int i = 0; i < each; ++i) {
+            const int index = first + n * threads * each + i;
+            const unsigned key = key_of(Of::get(v, i));
+            const Weight w = amount(index, key);
+            if (wanted >= from && wanted < from + w) visit(index, key, all);
+            from += w;
+        }
+    }
+
+    // The gathered symbols of all blocks, sorted; how many there are. Up to a block's threads each one's place is counted,
+    // by a group of threads: 64 take 1.0 us less than the sort's 21 exchanges with a barrier each.
+    __device__ __forceinline__ int collect(const unsigned long long* counts, int part) {
+        unsigned long long* from = shared.gathered;
+        int n = 0;
+        for (int b = 0; b < blocks; ++b) n += static_cast<int>(counts[b]);
+        unsigned long long* to = n <= threads ? shared.weights : shared.sorted;
+        n = 0;
+        for (int b = 0; b < blocks; ++b) {
+            const int count = static_cast<int>(counts[b]);
+            for (int i = threadIdx.x; i < count; i += threads) to[n + i] = from[b * part + i];
+            n += count;
+        }
+        if (n <= threads) {
+            __syncthreads();
+            const int group = group_of(n), i = static_cast<int>(threadIdx.x) / group;
+            const unsigned long long mine = i < n ? to[i] : 0;
+            int place = 0;
+            for (int k = static_cast<int>(threadIdx.x) % group; k < n; k += group) place += to[k] > mine;
+            for (int o = group / 2; o > 0; o /= 2) place += __shfl_xor_sync(0xffffffffu, place, o);
+            if (i < n && threadIdx.x % group == 0) shared.sorted[place] = mine;
+            __syncthreads();
+            return n;
+        }
+        for (int i = n + threadIdx.x; i < most_candidates; i += threads) shared.sorted[i] = 0;
+        sort(shared.sorted);
+        return n;
+    }
+    // Threads for each of n, a power of two.
+    static __device__ __forceinline__ int group_of(int n) {
+        int group = 32;
+        while (group > 1 && group * n > threads) group /= 2;
+        return group;
+    }
+
+    __device__ __forceinline__ void gather(unsigned key, int index, int part) {
+        const unsigned nth = atomicAdd(&shared.count, 1u);
+        if (nth < static_cast<unsigned>(part)) {
+            put(&shared.gathered[rank * part + nth], 0, static_cast<unsigned long long>(key) << 32 | ~static_cast<unsigned>(index));
+        }
+    }
+
+    // A histogram of the symbols that bin_of(logit, key) puts in a bin, the largest logits in the first, by counts or
+    // weights: the bin in which wanted_of(whole) is reached, or -1, and what of it is wanted there.
+    template <typename BinOf, typename WantedOf>
+    __device__ __forceinline__ int reach(const Row& row, bool by_weight, const Kept& kept, BinOf&& bin_of, WantedOf&& wanted_of,
+                                         Weight& wanted) {
+        Sums& sums = shared.sums;
+        __syncthreads();
+        for (int i = threadIdx.x; i < bins; i += threads) sums.low[i] = sums.high[i] = 0;
+        if (threadIdx.x == 0) sums.found = -1;
+        __syncthreads();
+        for_vectors([&](int n, const uint4& v) {
+            int bin[each];
+            Weight w[each];
+#pragma unroll
+            for (int i = 0; i < each; ++i) {
+                const float l = Of::get(v, i);
+                const unsigned key = key_of(l);
+                bin[i] = bin_of(l, key);
+                if (!kept.holds(key, first + n * threads * each + i)) bin[i] = -1;
+                if (by_weight) w[i] = weight_of(share_of(key, row));
+            }
+#pragma unroll
+            for (int i = 0; i < each; ++i) {
+                if (bin[i] < 0) continue;
+                if (!by_weight) {
+                    atomicAdd(&sums.low[bin[i]], 1u);
+                } else if (w[i] != 0) {
+                    add(sums, static_cast<unsigned>(bin[i]), w[i]);
+                }
+            }
+        });
+        cluster_sync();
+        if (rank == 0) {
+            constexpr int run = bins / threads;
+            Weight mine[run], all = 0, sum = 0;
+#pragma unroll
+            for (int i = 0; i < run; ++i) {
+                const int bin = run * static_cast<int>(threadIdx.x) + i;
+                mine[i] = 0;
+                for (int b = 0; b < blocks; ++b) {
+                    mine[i] += static_cast<Weight>(get(&sums.high[bin], b)) << 32 | get(&sums.low[bin], b);
+                }
+                sum += mine[i];
+            }
+            Weight earlier = before(sum, sums.scratch, all);
+            const Weight want = wanted_of(all);
+#pragma unroll
+            for (int i = 0; i < run; ++i) {
+                if (earlier < want && earlier + mine[i] >= want) {
+                    sums.found = run * static_cast<int>(threadIdx.x) + i, sums.found_weight = want - earlier;
+                }
+                earlier += mine[i];
+            }
+            __syncthreads();
+            if (threadIdx.x < static_cast<unsigned>(blocks)) {
+                put(&shared.told[0], static_cast<int>(threadIdx.x), static_cast<unsigned long long>(sums.found));
+                put(&shared.told[1], static_cast<int>(threadIdx.x), sums.found_weight);
+            }
+        }
+        cluster_sync();
+        wanted = shared.told[1];
+        return static_cast<int>(shared.told[0]);
+    }
+
+    // What the shortest prefix of the symbols kept so far that holds top_k of them (by_weight: top_p of their weight) ends
+    // with: a histogram over 46 octaves, of which bins hold equal steps, then the symbols of the bin that it ends in, in
+    // order. A bin with too many of them is divided by keys, down to one key, whose symbols go by their indexes.
+    __device__ __noinline__ Kept find(const Row& row, const Settings& s, bool by_weight, float largest, float factor, Kept kept) {
+        const int part = most_candidates / blocks;
+        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+        auto octave_bin = [&](float l) {
+            const float x = __fmul_rn(__fsub_rn(l, largest), -44.0f * factor);
+            return x < static_cast<float>(bins) ? static_cast<int>(x) : -1;  // a NaN is in none
+        };
+        Weight wanted;
+        const int octave = reach(
+            row, by_weight, kept, [&](float l, unsigned) { return octave_bin(l); },
+            [&](Weight all) { return by_weight ? part_of(s.top_p, all) : static_cast<Weight>(s.top_k); }, wanted);
+        if (octave < 0) return kept;  // there is less than wanted: all of it
+        unsigned low = 0, high = 0;   // the keys looked at, once they are known
+        for (int turn = 0;; ++turn) {
+            if (threadIdx.x == 0) shared.count = 0;
+            __syncthreads();
+            unsigned least = 0xffffffffu, most = 0;
+            for_vectors([&](int n, const uint4& v) {
+#pragma unroll
+                for (int i = 0; i < each; ++i) {
+                    const float l = Of::get(v, i);
+                    const unsigned key = key_of(l);
+                    const int index = first + n * threads * each + i;
+                    if (turn == 0 ? octave_bin(l) != octave : key < low || key > high) continue;
+                    if (!kept.holds(key, index)) continue;
+                    least = min(least, key), most = max(most, key);
+                    gather(key, index, part);
+                }
+            });
+            least = __reduce_min_sync(0xffffffffu, least), most = __reduce_max_sync(0xffffffffu, most);
+            if (lane == 0) shared.sums.scratch[warp] = static_cast<Weight>(least) << 32 | most;
+            __syncthreads();
+            for (int w = 0; w < warps; ++w) {
+                least = min(least, static_cast<unsigned>(shared.sums.scratch[w] >> 32));
+                most = max(most, static_cast<unsigned>(shared.sums.scratch[w]));
+            }
+            if (threadIdx.x < static_cast<unsigned>(blocks)) {
+                put(&shared.counts[0][rank], static_cast<int>(threadIdx.x), shared.count);
+                put(&shared.sums_of[0][rank], static_cast<int>(threadIdx.x), static_cast<unsigned long long>(least) << 32 | most);
+            }
+            cluster_sync();
+            bool fits = true;
+            low = 0xffffffffu, high = 0;
+            for (int b = 0; b < blocks; ++b) {
+                fits = fits && shared.counts[0][b] <= static_cast<unsigned>(part);
+                low = min(low, static_cast<unsigned>(shared.sums_of[0][b] >> 32));
+                high = max(high, static_cast<unsigned>(shared.sums_of[0][b]));
+            }
+            if (fits) {
+                if (rank == 0) {
+                    const int n = collect(shared.counts[0], part);
+                    constexpr int most_each = most_candidates / threads;
+                    const int run = (n + threads - 1) / threads, from = static_cast<int>(threadIdx.x) * run;
+                    Weight mine[most_each], sum = 0, all;
+#pragma unroll
+                    for (int i = 0; i < most_each; ++i) {
+                        mine[i] = i >= run || from + i >= n ? 0
+                            : by_weight ? weight_of(share_of(static_cast<unsigned>(shared.sorted[from + i] >> 32), row)) : 1;
+                        sum += mine[i];
+                    }
+                    Weight earlier = before(sum, shared.sums.scratch, all);
+#pragma unroll
+                    for (int i = 0; i < most_each; ++i) {
+                        if (mine[i] != 0 && earlier < wanted && earlier + mine[i] >= wanted) {
+                            for (int b = 0; b < blocks; ++b) put(&shared.told[0], b, shared.sorted[from + i]);
+                        }
+                        earlier += mine[i];
+                    }
+                }
+                break;
+            }
+            if (low == high) {
+                const Weight one = by_weight ? weight_of(share_of(low, row)) : 1;
+                locate(
+                    [&](int index, unsigned key) { return static_cast<Weight>(key == low && kept.holds(key, index)); },
+                    [&](Weight) { return (wanted + one - 1) / one - 1; },
+                    [&](int index, unsigned key, Weight) {
+                        for (int b = 0; b < blocks; ++b) {
+                            put(&shared.told[0], b, static_cast<unsigned long long>(key) << 32 | ~static_cast<unsigned>(index));
+                        }
+                    });
+                break;
+            }
+            const int shift = max(0, 32 - __clz(high - low) - 11);
+            const Weight still = wanted;
+            const unsigned from = low, to = high;
+            const int found = reach(
+                row, by_weight, kept,
+                [&](float, unsigned key) { return key >= from && key <= to ? static_cast<int>((to - key) >> shift) : -1; },
+                [&](Weight) { return still; }, wanted);
+            high = to - (static_cast<unsigned>(found) << shift);
+            low = high - min(high - from, (1u << shift) - 1);
+        }
+        cluster_sync();
+        const unsigned long long end = shared.told[0];
+        __syncthreads();
+        return {static_cast<unsigned>(end >> 32), static_cast<int>(~static_cast<unsigned>(end))};
+    }
+
+    // Any row of finite logits, exactly.
+    __device__ __forceinline__ void whole(const Row& row, const Settings& s, float largest, float factor) {
+        Kept kept{0, 0};
+        if (row.temperature == 0.0) {
+            kept = {row.top, INT_MAX};
+        } else {
+            if (s.top_k > 0 && s.top_k < a.symbols) kept = find(row, s, false, largest, factor, kept);
+            if (s.top_p < 1.0f) kept = find(row, s, true, largest, factor, kept);
+        }
+        // with a temperature of 0, u is taken as 0: the first of the largest
+        locate(
+            [&](int index, unsigned key) -> Weight {
+                if (!kept.holds(key, index)) return 0;
+                const double share = share_of(key, row);
+                return share >= row.least ? weight_of(share) : 0;
+            },
+            [&](Weight all) { return row.temperature == 0.0 ? 0 : part_of_uniform(s.uniform, all); },
+            [&](int index, unsigned key, Weight all) {
+                a.chosen[r] = index;
+                a.probabilities[r] = row.temperature == 0.0 ? 1.0f : probability_of(share_of(key, row), all);
+            });
+    }
+
+    // As `finish`, for at most 64 symbols, by one warp: a fraction of the latency of a block's barriers.
+    __device__ __forceinline__ bool finish_few(const Row& row, const Settings& s, const unsigned long long* counts, int part, int all_count,
+                                               double bulk, double slack) {
+        const int lane = threadIdx.x % 32;
+        int filled = 0;
+        for (int b = 0; b < blocks; ++b) {
+            const int count = static_cast<int>(counts[b]);
+            for (int i = lane; i < count; i += 32) shared.weights[filled + i] = shared.gathered[b * part + i];
+            filled += count;
+        }
+        for (int i = all_count + lane; i < 64; i += 32) shared.weights[i] = 0;
+        __syncwarp();
+        const unsigned long long one = shared.weights[lane], two = shared.weights[lane + 32];
+        int place_one = 0, place_two = 0;
+#pragma unroll 4
+        for (int k = 0; k < all_count; ++k) {
+            const unsigned long long other = shared.weights[k];
+            place_one += other > one, place_two += other > two;
+        }
+        if (lane < all_count) shared.sorted[place_one] = one;
+        if (lane + 32 < all_count) shared.sorted[place_two] = two;
+        __syncwarp();
+        int n = s.top_k > 0 ? min(all_count, s.top_k) : all_count;
+        // a lane has two neighbours
+        unsigned long long entry[2];
+        Weight w[2], to[2], all = 0;
+        unsigned kept = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool there = 2 * lane + i < n;
+            entry[i] = there ? shared.sorted[2 * lane + i] : 0;
+            const double share = there ? share_of(static_cast<unsigned>(entry[i] >> 32), row) : 0.0;
+            w[i] = weight_of(share);
+            kept += there && share >= row.least;
+        }
+        Weight sum = w[0] + w[1];
+        for (int o = 1; o < 32; o *= 2) {
+            const Weight v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        all = __shfl_sync(0xffffffffu, sum, 31);
+        to[1] = sum, to[0] = sum - w[1];
+        n = min(n, static_cast<int>(__reduce_add_sync(0xffffffffu, kept)));
+        if (s.top_p < 1.0f) {
+            const double p = static_cast<double>(fmaxf(s.top_p, 0.0f));
+            const double least_part = p * (static_cast<double>(all) + bulk - slack), most_part = p * (static_cast<double>(all) + bulk + slack);
+            unsigned low = 0, high = 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                low += 2 * lane + i < n && static_cast<double>(to[i]) < least_part;
+                high += 2 * lane + i < n && static_cast<double>(to[i]) < most_part;
+            }
+            low = __reduce_add_sync(0xffffffffu, low), high = __reduce_add_sync(0xffffffffu, high);
+            if (min(n, 1 + static_cast<int>(low)) != min(n, 1 + static_cast<int>(high))) return false;
+            n = min(n, 1 + static_cast<int>(low));
+        }
+        const Weight last = __shfl_sync(0xffffffffu, (n - 1) % 2 == 0 ? to[0] : to[1], (n - 1) / 2);
+        const Weight wanted = part_of_uniform(s.uniform, last);
+        shared.weights[2 * lane] = w[0], shared.weights[2 * lane + 1] = w[1];
+        __syncwarp();
+        Weight lower[2] = {0, 0};  // of those with lower indexes, whose complements are larger
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            const unsigned other = static_cast<unsigned>(shared.sorted[k]);
+            const Weight weight = shared.weights[k];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) lower[i] += other > static_cast<unsigned>(entry[i]) ? weight : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (2 * lane + i < n && wanted >= lower[i] && wanted < lower[i] + w[i]) {
+                a.chosen[r] = static_cast<std::int64_t>(~static_cast<unsigned>(entry[i]));
+                a.probabilities[r] = probability_of(share_of(static_cast<unsigned>(entry[i] >> 32), row), last);
+            }
+        }
+        return true;
+    }
+
+    // The first block: the symbols in `gathered` are all that can be kept. False where the choice hangs on the error of
+    // `bulk`, the weight of the others.
+    __device__ __forceinline__ bool finish(const Row& row, const Settings& s, const unsigned long long* counts, int part, double bulk,
+                                           double slack) {
+        if (threadIdx.x == 0) shared.kept = shared.low = shared.high = 0;
+        int n = collect(counts, part);
+        if (s.top_k > 0) n = min(n, s.top_k);
+        constexpr int most_each = most_candidates / threads;
+        const int run = (n + threads - 1) / threads, from = static_cast<int>(threadIdx.x) * run;
+        Weight mine[most_each], sum = 0, all;
+        unsigned kept = 0;
+#pragma unroll
+        for (int i = 0; i < most_each; ++i) {
+            mine[i] = 0;
+            if (i < run && from + i < n) {
+                const double share = share_of(static_cast<unsigned>(shared.sorted[from + i] >> 32), row);
+                mine[i] = weight_of(share);
+                kept += share >= row.least;
+            }
+            sum += mine[i];
+        }
+        Weight to = before(sum, shared.sums.scratch, all);
+        double least_part = 0.0, most_part = 0.0;
+        if (s.top_p < 1.0f) {
+            const double p = static_cast<double>(fmaxf(s.top_p, 0.0f));
+            least_part = p * (static_cast<double>(all) + bulk - slack), most_part = p * (static_cast<double>(all) + bulk + slack);
+        }
+        unsigned low = 0, high = 0;
+#pragma unroll
+        for (int i = 0; i < most_each; ++i) {
+            if (i < run && from + i < n) {
+                to += mine[i];
+                shared.weights[from + i] = to;
+                low += static_cast<double>(to) < least_part;
+                high += static_cast<double>(to) < most_part;
+            }
+        }
+        kept = __reduce_add_sync(0xffffffffu, kept);
+        low = __reduce_add_sync(0xffffffffu, low), high = __reduce_add_sync(0xffffffffu, high);
+        if (threadIdx.x % 32 == 0) {
+            atomicAdd(&shared.kept, kept);
+            atomicAdd(&shared.low, low);
+            atomicAdd(&shared.high, high);
+        }
+        __syncthreads();
+        n = min(n, static_cast<int>(shared.kept));
+        if (s.top_p < 1.0f) {
+            if (min(n, 1 + static_cast<int>(shared.low)) != min(n, 1 + static_cast<int>(shared.high))) return false;
+            n = min(n, 1 + static_cast<int>(shared.low));
+        }
+        const Weight whole_kept = shared.weights[n - 1];
+        const Weight wanted = part_of_uniform(s.uniform, whole_kept);
+        auto choose = [&](unsigned long long entry) {
+            a.chosen[r] = static_cast<std::int64_t>(~static_cast<unsigned>(entry));
+            a.probabilities[r] = probability_of(share_of(static_cast<unsigned>(entry >> 32), row), whole_kept);
+        };
+        auto weight_at = [&](int i) { return shared.weights[i] - (i == 0 ? 0 : shared.weights[i - 1]); };
+        if (n <= threads) {  // the weight of those with lower indexes, for each
+            const int group = group_of(n), i = static_cast<int>(threadIdx.x) / group;
+            const unsigned index = i < n ? static_cast<unsigned>(shared.sorted[i]) : 0;  // its complement
+            Weight lower = 0;
+            for (int k = static_cast<int>(threadIdx.x) % group; k < n; k += group) {
+                lower += static_cast<unsigned>(shared.sorted[k]) > index ? weight_at(k) : 0;
+            }
+            for (int o = group / 2; o > 0; o /= 2) lower += __shfl_xor_sync(0xffffffffu, lower, o);
+            if (i < n && threadIdx.x % group == 0 && wanted >= lower && wanted < lower + weight_at(i)) choose(shared.sorted[i]);
+            return true;
+        }
+        // in the order of indexes: the largest complement first
+        for (int i = threadIdx.x; i < most_candidates; i += threads) {
+            shared.gathered[i] = i < n ? (shared.sorted[i] & 0xffffffffull) << 32 | static_cast<unsigned>(i) : 0ull;
+        }
+        sort(shared.gathered);
+        const int start = static_cast<int>(threadIdx.x) * most_each;
+        sum = 0;
+#pragma unroll
+        for (int i = 0; i < most_each; ++i) {
+            mine[i] = start + i < n ? weight_at(static_cast<int>(shared.gathered[start + i] & 0xffffffffull)) : 0;
+            sum += mine[i];
+        }
+        to = before(sum, shared.sums.scratch, all);
+#pragma unroll
+        for (int i = 0; i < most_each; ++i) {
+            if (start + i < n && wanted >= to && wanted < to + mine[i]) {
+                choose(shared.sorted[static_cast<unsigned>(shared.gathered[start + i])]);
+            }
+            to += mine[i];
+        }
+        return true;
+    }
+};
+
+template <typename T, int Vectors>
+__global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(SampleArgs a, int blocks) {
+    extern __shared__ unsigned char memory[];
+    using Of = Elements<T>;
+    constexpr int each = Of::each;
+    auto& shared = *reinterpret_cast<Shared*>(memory);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int rank = static_cast<int>(blockIdx.x) % blocks;
+    const std::int64_t r = blockIdx.x / blocks;
+    make_table(shared.table);
+    join_chain();
+    const T* logits = static_cast<const T*>(a.logits) + r * a.stride;
+    // Vectors begin on 16-byte boundaries, the first one up to 15 bytes before the row; this block has a run of them.
+    const int skew = static_cast<int>(reinterpret_cast<std::uintptr_t>(logits) % 16 / sizeof(T));
+    const int all_vectors = (a.symbols + skew + each - 1) / each;
+    const int share = (all_vectors + blocks * threads - 1) / (blocks * threads);  // vectors a thread
+    const int first = (rank * share * threads + static_cast<int>(threadIdx.x)) * each - skew;
+    ClusterRow<T> of_cluster{a, shared, r, rank, blocks, share, first};
+    uint4 v[Vectors];
+    float most = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < Vectors; ++k) v[k] = k < share ? of_cluster.load(k) : Of::none();
+    const Settings s = settings_of(a, r);
+#pragma unroll
+    for (int k = 0; k < Vectors; ++k) most = fmaxf(most, Of::largest(v[k]));
+    unsigned top = __reduce_max_sync(0xffffffffu, key_of(most));
+    if (threadIdx.x == 0) shared.count = shared.queued = 0;
+    if (lane == 0) shared.sums.scratch[warp] = top;
+    __syncthreads();
+    for (int w = 0; w < warps; ++w) top = max(top, static_cast<unsigned>(shared.sums.scratch[w]));
+    if (threadIdx.x < static_cast<unsigned>(blocks)) put(&shared.maxima[rank], static_cast<int>(threadIdx.x), top);
+    cluster_sync();
+    for (int b = 0; b < blocks; ++b) top = max(top, static_cast<unsigned>(shared.maxima[b]));
+    if (top == 0) {  // nothing to choose
+        if (rank == 0 && threadIdx.x == 0) a.chosen[r] = -1, a.probabilities[r] = 0.0f;
+        return;
+    }
+    const Row row = row_of(top, s, shared.table);
+    const bool by_count = s.top_k > 0 && s.top_k < a.symbols;
+    const bool by_part = s.top_p < 1.0f;
+    const float largest = logit_of(top);
+    const float factor = 1.44269504f / s.temperature;  // octaves a logit
+    const bool greedy = row.temperature == 0.0;
+    if (!greedy && !(largest < INFINITY && factor < 1e30f && factor > 1e-30f)) {  // FP32 exponents
+        if (rank == 0) row_by_block<T>(a, r, shared.sums, shared.table);
+        return;
+    }
+    if (!greedy && (by_count || by_part || row.least > 0.0) && (!by_count || s.top_k <= most_candidates / 2) &&
+        fabsf(largest * factor) < 1e4f) {
+        // candidates: octaves from `cut` up; below -46 a weight rounds to none
+        const int part = most_candidates / blocks;
+        const bool sum_rest = by_part && !by_count;
+        const float base = -largest * factor;
+        auto exponent = [&](float l) { return fmaf(l, factor, base); };
+        const double error = bulk_error(largest, factor);
+        auto* queue = reinterpret_cast<uint4*>(shared.sorted);  // vectors with a candidate, in sorted and weights
+        auto* places = reinterpret_cast<int*>(shared.sums.high);
+        float cut = -10.0f;
+        if (row.least > 0.0) {
+            cut = fmaxf(log2f(fminf(s.min_p, 1.0f)) - 0.01f, -46.0f);
+        } else if (by_count) {
+            // at which top_k vectors have their largest logits above: so many candidates at least, and seldom many more
+            for (int i = threadIdx.x; i < cut_bins; i += threads) shared.sums.low[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < Vectors; ++k) {
+                const float x = exponent(Of::largest(v[k])) * -cut_steps;
+                if (x < static_cast<float>(cut_bins)) atomicAdd(&shared.sums.low[static_cast<int>(x)], 1u);
+            }
+            if (threadIdx.x == 0) shared.cut = cut_bins;
+            cluster_sync();
+            Weight mine = 0, all;
+            if (threadIdx.x < cut_bins) {
+                for (int b = 0; b < blocks; ++b) mine += get(&shared.sums.low[threadIdx.x], b);
+            }
+            const Weight earlier = before(mine, shared.sums.scratch, all), wanted = static_cast<Weight>(s.top_k);
+            if (earlier < wanted && earlier + mine >= wanted) shared.cut = static_cast<int>(threadIdx.x) + 1;
+            __syncthreads();
+            cut = static_cast<float>(shared.cut) * (-1.0f / cut_steps) - 0.001f;
+        }
+        for (int turn = 0;; ++turn) {
+            float held = 0.0f, rest = 0.0f;  // weights of candidates and of the others
+#pragma unroll
+            for (int k = 0; k < Vectors; ++k) {
+                if (exponent(Of::largest(v[k])) >= cut) {  // looked at below, by all threads
+                    const unsigned nth = atomicAdd(&shared.queued, 1u);
+                    if (nth < static_cast<unsigned>(part)) queue[nth] = v[k], places[nth] = first + k * threads * each;
+                } else if (sum_rest) {
+#pragma unroll
+                    for (int i = 0; i < each; ++i) rest += exp2_fast(exponent(Of::get(v[k], i)));
+                }
+            }
+            __syncthreads();
+            const int queued = static_cast<int>(shared.queued);
+            for (int e = threadIdx.x; e < min(queued, part) * each; e += threads) {
+                const float l = Of::pick(queue[e / each], e % each), x = exponent(l);
+                if (x >= cut) {
+                    of_cluster.gather(key_of(l), places[e / each] + e % each, part);
+                    held += exp2_fast(x);
+                } else if (l == l) {
+                    rest += exp2_fast(x);
+                }
+            }
+            held = warp_sum(held), rest = warp_sum(rest);
+            if (lane == 0) shared.parts[0][warp] = held, shared.parts[1][warp] = rest;
+            __syncthreads();
+            held = rest = 0.0f;
+            for (int w = 0; w < warps; ++w) held += shared.parts[0][w], rest += shared.parts[1][w];
+            const int parity = turn & 1;
+            if (threadIdx.x < static_cast<unsigned>(blocks)) {
+                put(&shared.counts[parity][rank], static_cast<int>(threadIdx.x), max(shared.count, shared.queued));
+                put(&shared.sums_of[parity][rank], static_cast<int>(threadIdx.x),
+                    static_cast<unsigned long long>(__float_as_uint(held)) << 32 | __float_as_uint(rest));
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) shared.count = shared.queued = 0;
+            cluster_sync();
+            int count = 0;
+            bool fits = true;
+            double all_held = 0.0, bulk = 0.0;
+            for (int b = 0; b < blocks; ++b) {
+                const int some = static_cast<int>(shared.counts[parity][b]);
+                fits = fits && some <= part;
+                count += some;
+                const unsigned long long both = shared.sums_of[parity][b];
+                all_held += __uint_as_float(static_cast<unsigned>(both >> 32)), bulk += __uint_as_float(static_cast<unsigned>(both));
+            }
+            if (!fits || !(bulk <= 1e30)) break;  // a NaN among the sums too
+            const bool complete = cut <= -46.0f;  // what is left out has no weight
+            const bool enough = complete || (row.least > 0.0 && !(by_count && by_part)) ||
+                (by_count ? count >= s.top_k
+                          : all_held * (1.0 - error) >= static_cast<double>(fmaxf(s.top_p, 0.0f)) *
+                                 ((all_held + bulk) * (1.0 + error) + a.symbols / unit));
+            if (enough) {
+                if (rank != 0) return;
+                const double others = sum_rest ? bulk * unit : 0.0, slack = sum_rest ? others * error + a.symbols : 0.0;
+                bool done;
+                if (count <= 64) {
+                    if (warp == 0) {
+                        done = of_cluster.finish_few(row, s, shared.counts[parity], part, count, others, slack);
+                        if (lane == 0) shared.queued = done;
+                    }
+                    __syncthreads();
+                    done = shared.queued != 0;
+                } else {
+                    done = of_cluster.finish(row, s, shared.counts[parity], part, others, slack);
+                    __syncthreads();
+                }
+                if (!done) row_by_block<T>(a, r, shared.sums, shared.table);
+                return;
+            }
+            if (cut < -14.0f) break;
+            cut = -14.5f;
+        }
+    }
+    of_cluster.whole(row, s, largest, factor);
+    cluster_sync();  // no block ends while another one reads its memory
+}
+
+template <typename T, int Vectors>
+cudaError_t launch_cluster(const SampleArgs& a, int blocks, cudaStream_t stream) {
+    static SharedAllowance allowance;
+    const cudaError_t status = allowance.allow(cluster_kernel<T, Vectors>, sizeof(Shared));
+    if (status != cudaSuccess) return status;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(a.rows * blocks));
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = sizeof(Shared);
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = static_cast<unsigned>(blocks);
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, cluster_kernel<T, Vectors>, a, blocks);
+}
+
+template <typename T>
 cudaError_t launch(const SampleArgs& a, cudaStream_t stream) {
-    return kernels::launch_overlapped(sample_kernel<T>, dim3(static_cast<unsigned>(a.rows)), dim3(sample_threads), 0, stream, a);
+    constexpr int each = 16 / sizeof(T);
+    const bool aligned = reinterpret_cast<std::uintptr_t>(a.logits) % 16 == 0 && (a.rows == 1 || a.stride % each == 0);
+    const int vectors = (a.symbols + each - 1) / each + (aligned ? 0 : 1);  // a row may begin within one
+    auto fits = [&](int blocks, int held) { return vectors <= blocks * threads * held; };
+    int blocks = 1;
+    while (blocks < most_blocks && !fits(blocks, 8)) blocks *= 2;
+    // few rows: while all blocks run at once and each has two vectors a thread
+    while (blocks < most_blocks && a.rows * blocks * 2 <= sm_count() && vectors > blocks * threads * 2) blocks *= 2;
+
+    if (a.rows > INT_MAX / most_blocks) blocks = 0;  // more blocks than a grid holds
+    if (fits(blocks, 8)) return launch_cluster<T, 8>(a, blocks, stream);
+    if (fits(blocks, 16)) return launch_cluster<T, 16>(a, blocks, stream);
+    return kernels::launch_overlapped(block_kernel<T>, dim3(static_cast<unsigned>(a.rows)), dim3(threads), 0, stream, a);
 }
 
 }  // namespace
