@@ -2,8 +2,10 @@
 // sums of their two largest b; of their experts the `count` with the largest b, ties to the lowest index; weights s,
 // divided by their sum if asked for, times a scale.
 //
-// s, b and the sums are FP64: which expert is chosen hangs on differences of b, and FP32 would decide some of them by
-// its rounding.
+// s, b and the sums are FP64 by definition: which expert is chosen hangs on differences of b, and FP32 would decide some of
+// them by its rounding. But FP32 says of most tokens that no difference is that small: `route_kernel` chooses in FP32, and
+// takes a token whose choices differ by less than that arithmetic's error again in FP64 (`exactly`), unless scores and
+// biases are equal. The weights are FP64 in either.
 #include "token_elements.cuh"
 
 #include <cmath>
@@ -38,14 +40,11 @@ __device__ __forceinline__ Best warp_best(unsigned long long key, int index) {
     return {best, best == 0 ? -1 : static_cast<int>(at)};
 }
 
-// A warp a token; lane l has experts l, l + 32, ... Key 0 stands for an expert that is left out.
+// A token by a warp in FP64; lane l has experts l, l + 32, ... Key 0 stands for an expert that is left out. `keys`: room
+// for as many as there are experts.
 template <typename T, int Each>
-__global__ void __launch_bounds__(route_warps * 32) route_kernel(RouteArgs a) {
-    extern __shared__ unsigned long long keys_of[];
-    join_chain();
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const std::int64_t token = blockIdx.x * static_cast<std::int64_t>(route_warps) + warp;
-    if (token >= a.tokens) return;
+__device__ __noinline__ void exactly(const RouteArgs& a, std::int64_t token, unsigned long long* keys) {
+    const int lane = threadIdx.x % 32;
     const T* row = static_cast<const T*>(a.scores) + token * a.stride;
     float score[Each];
     float most = -INFINITY;
@@ -88,7 +87,6 @@ __global__ void __launch_bounds__(route_warps * 32) route_kernel(RouteArgs a) {
     }
 
     if (a.kept_groups < a.groups) {
-        unsigned long long* keys = keys_of + warp * a.experts;
 #pragma unroll
         for (int i = 0; i < Each; ++i) {
             if (i * 32 + lane < a.experts) keys[i * 32 + lane] = key[i];
@@ -181,11 +179,224 @@ __global__ void __launch_bounds__(route_warps * 32) route_kernel(RouteArgs a) {
 }
 
 template <typename T, int Each>
+__global__ void __launch_bounds__(route_warps * 32) exact_kernel(RouteArgs a) {
+    extern __shared__ unsigned long long keys_of[];
+    join_chain();
+    const int warp = threadIdx.x / 32;
+    const std::int64_t token = blockIdx.x * static_cast<std::int64_t>(route_warps) + warp;
+    if (token < a.tokens) exactly<T, Each>(a, token, keys_of + warp * a.experts);
+}
+
+// The order of floats that are no NaN, as that of unsigned integers above 0.
+__device__ __forceinline__ unsigned ordered(float v) {
+    const unsigned bits = __float_as_uint(v + 0.0f);
+    return bits >> 31 ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned key) { return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
+
+__device__ __forceinline__ float reciprocal(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Shared memory of a warp, in words of 8 bytes: 32 candidates with three values each, or a key an expert.
+__host__ __device__ __forceinline__ int room_of(const RouteArgs& a) { return a.experts > 96 ? (a.experts + 1) / 2 * 2 : 96; }
+
+// Up to 256 experts, of which up to 31 are chosen.
+template <typename T, int Each>
+__global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a) {
+    extern __shared__ __align__(16) unsigned long long keys_of[];
+    join_chain();
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const std::int64_t token = blockIdx.x * static_cast<std::int64_t>(route_warps) + warp;
+    if (token >= a.tokens) return;
+    const T* row = static_cast<const T*>(a.scores) + token * a.stride;
+    float score[Each], bias[Each];
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < Each; ++i) {
+        const int e = i * 32 + lane;
+        score[i] = e < a.experts ? widen(row[e]) : -INFINITY;
+        bias[i] = a.bias != nullptr && e < a.experts ? a.bias[e] : 0.0f;
+        most = fmaxf(most, score[i]);
+    }
+    constexpr float log2e = 1.44269504f;
+    float share[Each];
+    bool certain = true;
+    if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < Each; ++i) share[i] = reciprocal(1.0f + exp2_fast(score[i] * -log2e));
+    } else {
+#pragma unroll
+        for (int offset = 16; offset > 0; offset /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
+        certain = most < INFINITY;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Each; ++i) {
+            share[i] = score[i] > -INFINITY ? exp2_fast((score[i] - most) * log2e) : 0.0f;
+            sum += share[i];
+        }
+        const float inverse = reciprocal(token::warp_sum(sum));
+#pragma unroll
+        for (int i = 0; i < Each; ++i) share[i] *= inverse;
+    }
+    // How far a share s and its sum b with the bias may be off: of exponents up to 128, rounded twice or three times to 2^-24
+    // of themselves, a factor of 1e-5 or 1.6e-5, which a sigmoid has times 1 - s; ex2, rcp and sums 4e-7, a softmax's sum
+    // 2e-6; b 2^-24 of itself; and what is flushed to zero.
+    auto error = [&](float s, float b) {
+        return s * (a.sigmoid ? 4e-7f + (1.0f - s) * 1e-5f : 2e-5f) + 1.2e-7f * fabsf(b) + 1e-37f;
+    };
+    unsigned key[Each];
+    float furthest = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Each; ++i) {
+        const float b = share[i] + bias[i];
+        const bool there = score[i] > -INFINITY && b > -INFINITY;  // a NaN is left out
+        key[i] = there ? ordered(b) : 0;
+        furthest = fmaxf(furthest, there ? fabsf(b) : 0.0f);
+    }
+    certain = certain && furthest <= 1e30f;
+    auto* keys = reinterpret_cast<unsigned*>(keys_of + warp * room_of(a));
+    if (a.kept_groups < a.groups) {
+        const int size = a.experts / a.groups;
+        // lane g has group g's value: a group is one register's lanes, or is read from shared memory
+        unsigned first = 0, second = 0;
+        if (size == 32) {
+#pragma unroll
+            for (int i = 0; i < Each; ++i) {
+                const unsigned top = __reduce_max_sync(0xffffffffu, key[i]);
+                const unsigned winners = __ballot_sync(0xffffffffu, key[i] == top);
+                const unsigned next = __reduce_max_sync(0xffffffffu, lane == __ffs(winners) - 1 ? 0u : key[i]);
+                if (lane == i) first = top, second = next;
+            }
+        } else {
+            certain = certain && a.groups <= 32;
+#pragma unroll
+            for (int i = 0; i < Each; ++i) {
+                if (i * 32 + lane < a.experts) keys[i * 32 + lane] = key[i];
+            }
+            __syncwarp();
+            for (int j = 0; lane < a.groups && j < size; ++j) {
+                const unsigned k = keys[lane * size + j];
+                second = max(second, min(first, k));
+                first = max(first, k);
+            }
+            __syncwarp();
+        }
+        const bool some = lane < a.groups && first != 0;
+        const float value = some ? value_of(first) + (second == 0 ? 0.0f : value_of(second)) : -INFINITY;
+        // two shares' errors, at most: a softmax's sum to one, a sigmoid's have s (1 - s) <= 1/4
+        const float off = (a.sigmoid ? 7e-6f : 2.2e-5f) +
+            3.6e-7f * (some ? fabsf(value_of(first)) + (second == 0 ? 0.0f : fabsf(value_of(second))) : 0.0f);
+        int place = 0;
+        for (int g = 0; g < min(a.groups, 32); ++g) {
+            const float other = __shfl_sync(0xffffffffu, value, g);
+            place += other > value || (other == value && g < lane);
+        }
+        const bool stays = lane < a.groups && place < a.kept_groups;
+        const unsigned kept = __ballot_sync(0xffffffffu, stays);
+        // the least that a group that stays may have, and the most of the others (groups without an expert are of no matter)
+        const unsigned least = __reduce_min_sync(0xffffffffu, stays && some ? ordered(value - off) : 0xffffffffu);
+        const unsigned most_out = __reduce_max_sync(0xffffffffu, !stays && some ? ordered(value + off) : 0u);
+        certain = certain && least > most_out;
+#pragma unroll
+        for (int i = 0; i < Each; ++i) {
+            const int g = size == 32 ? i : (i * 32 + lane) / size;
+            if (g >= 32 || !(kept >> g & 1u)) key[i] = 0;
+        }
+    }
+
+    // Of the lanes' largest keys the (count + 1)-th bounds the (count + 1)-th of all; those above it, few more, are put in
+    // order, a lane each.
+    unsigned bound = 0;
+#pragma unroll
+    for (int i = 0; i < Each; ++i) bound = max(bound, key[i]);
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+        for (int apart = size / 2; apart > 0; apart /= 2) {
+            const unsigned other = __shfl_xor_sync(0xffffffffu, bound, apart);
+            bound = ((lane & apart) == 0) == ((lane & size) == 0) ? max(bound, other) : min(bound, other);
+        }
+    }
+    bound = max(1u, __shfl_sync(0xffffffffu, bound, min(a.count, 31)));
+    auto* entries = reinterpret_cast<unsigned long long*>(keys);
+    int candidates = 0;
+#pragma unroll
+    for (int i = 0; i < Each; ++i) {
+        const unsigned holders = __ballot_sync(0xffffffffu, key[i] >= bound);
+        const int at = candidates + __popc(holders & ((1u << lane) - 1));
+        if (key[i] >= bound && at < 32) {
+            entries[at] = static_cast<unsigned long long>(key[i]) << 32 | ~static_cast<unsigned>(i * 32 + lane);
+            auto* values = reinterpret_cast<float*>(entries + 32) + at * 4;
+            values[0] = share[i], values[1] = score[i], values[2] = bias[i];
+        }
+        candidates += __popc(holders);
+    }
+    __syncwarp();
+    certain = certain && candidates <= 32;
+    const int n = min(candidates, 32);
+    const unsigned long long entry = lane < n ? entries[lane] : 0;
+    int place = 0;
+    for (int k = 0; k < n; ++k) place += entries[k] > entry;
+    if (lane >= n) place = lane;
+    const float4 mine_here = reinterpret_cast<const float4*>(entries + 32)[min(lane, max(n, 1) - 1)];
+    __syncwarp();
+    // lane l takes the candidate whose place is l
+    auto* slots = reinterpret_cast<int*>(entries);
+    slots[place] = lane;
+    __syncwarp();
+    const int from = slots[lane];
+    const int chosen = static_cast<int>(~static_cast<unsigned>(__shfl_sync(0xffffffffu, entry, from)));
+    const float v = value_of(static_cast<unsigned>(__shfl_sync(0xffffffffu, entry, from) >> 32));
+    const float s = __shfl_sync(0xffffffffu, mine_here.x, from), mine = __shfl_sync(0xffffffffu, mine_here.y, from),
+                b = __shfl_sync(0xffffffffu, mine_here.z, from);
+    {
+        const float after = __shfl_down_sync(0xffffffffu, v, 1), after_s = __shfl_down_sync(0xffffffffu, s, 1),
+                    after_l = __shfl_down_sync(0xffffffffu, mine, 1), after_b = __shfl_down_sync(0xffffffffu, b, 1);
+        const bool near = v - after <= error(s, v) + error(after_s, after) && !(mine == after_l && b == after_b);
+        if (lane < a.count && lane + 1 < n && near) certain = false;
+    }
+    certain = __all_sync(0xffffffffu, certain);
+    if (!certain) {
+        exactly<T, Each>(a, token, keys_of + warp * room_of(a));
+        return;
+    }
+    const bool there = lane < min(a.count, n);
+    double weight = 0.0;
+    if (a.sigmoid) {
+        if (there) weight = 1.0 / (1.0 + exp(-static_cast<double>(mine)));
+    } else {
+        if (there) weight = exp(static_cast<double>(mine) - static_cast<double>(most));
+        if (!a.renormalise) {
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < Each; ++i) {
+                if (score[i] > -INFINITY) sum += exp(static_cast<double>(score[i]) - static_cast<double>(most));
+            }
+            weight /= warp_sum(sum);
+        }
+    }
+    if (a.renormalise) {
+        const double sum = warp_sum(weight);
+        weight = sum > 0.0 ? weight / sum : 0.0;
+    }
+    if (lane < a.count) {
+        a.choices[token * a.count + lane] = there ? chosen : -1;
+        a.weights[token * a.count + lane] = there ? static_cast<float>(weight * static_cast<double>(a.scale)) : 0.0f;
+    }
+}
+
+template <typename T, int Each>
 cudaError_t launch(const RouteArgs& a, cudaStream_t stream) {
     const std::int64_t blocks = (a.tokens + route_warps - 1) / route_warps;
-    const std::size_t shared = a.kept_groups < a.groups ? static_cast<std::size_t>(route_warps) * a.experts * 8 : 0;
-    return kernels::launch_overlapped(route_kernel<T, Each>, dim3(static_cast<unsigned>(blocks)), dim3(route_warps * 32), shared,
-                                      stream, a);
+    std::size_t shared = a.kept_groups < a.groups ? static_cast<std::size_t>(route_warps) * a.experts * 8 : 0;
+    auto kernel = exact_kernel<T, Each>;
+    if constexpr (Each <= 8) {
+        if (a.count < 32) kernel = route_kernel<T, Each>, shared = static_cast<std::size_t>(route_warps) * room_of(a) * 8;
+    }
+    return kernels::launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), dim3(route_warps * 32), shared, stream, a);
 }
 
 template <typename T>
