@@ -7,23 +7,19 @@
 // blocks of 128 outputs by 128 inputs, rows as [128 inputs][row][128 bytes]. So every tile is one contiguous copy,
 // with neither a tensor map nor an alignment that a caller has to keep.
 #include "tcgen05.cuh"
-#include "token_elements.cuh"
+#include "token_bytes.cuh"
 
 #include <algorithm>
+#include <cmath>
 
 namespace nvcr_sm100::token {
 namespace {
 
 using namespace kernels;
 
-constexpr int block_rows = 128;    // outputs of a weight block: the MMA's M
-constexpr int block_bytes = 128;   // inputs of a block: a swizzled row
-constexpr int weight_block = block_rows * block_bytes;
 constexpr int step_rows = 16;      // rows of x are padded to the MMA's step of N
 constexpr int most_tile = 256;     // rows of x a tile
 
-int blocks_of(int inputs) { return (inputs + block_bytes - 1) / block_bytes; }
-int tiles_of(int outputs) { return (outputs + block_rows - 1) / block_rows; }
 std::int64_t padded(std::int64_t rows) { return (rows + step_rows - 1) / step_rows * step_rows; }
 std::size_t aligned(std::size_t bytes) { return (bytes + 255) / 256 * 256; }
 
@@ -133,30 +129,6 @@ struct QuantiseArgs {
     int outputs;
 };
 
-template <typename T>
-__device__ __forceinline__ void load_sixteen(const T* row, int at, int inputs, bool vector, float (&v)[16]) {
-    if (vector && at + 16 <= inputs) {
-        constexpr int each = 16 / sizeof(T);
-#pragma unroll
-        for (int part = 0; part < 16 / each; ++part) {
-            const uint4 words = *reinterpret_cast<const uint4*>(row + at + part * each);
-            const unsigned word[4] = {words.x, words.y, words.z, words.w};
-#pragma unroll
-            for (int i = 0; i < each; ++i) {
-                if constexpr (sizeof(T) == 4) {
-                    v[part * each + i] = __uint_as_float(word[i]);
-                } else {
-                    const std::uint16_t bits = static_cast<std::uint16_t>(word[i / 2] >> (i % 2 * 16));
-                    v[part * each + i] = widen(reinterpret_cast<const T&>(bits));
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = at + i < inputs ? widen(row[at + i]) : 0.0f;
-    }
-}
-
 // Warps warps a row, a thread 16 values at a time, of which the first `held` stay in registers between the row's
 // maximum and its codes; longer rows are read again.
 template <typename T, int Warps>
@@ -197,27 +169,14 @@ __global__ void __launch_bounds__(256) quantise_kernel(QuantiseArgs a) {
         for (int w = 0; w < Warps; ++w) most = max_nan(most, largest[first + w]);
     }
     if (!there) return;
-    // 2^-126: the inverse of a smaller scale would overflow
-    const float scale = fmaxf(__fmul_rn(most, 1.0f / 127.0f), 1.17549435e-38f);
-    const float inverse = __frcp_rn(scale);
-    const bool finite = most <= 3.40282347e38f;
+    const RowScale scale(most);
     auto store = [&](const float (&v)[16], int piece) {
-        unsigned words[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            unsigned byte[4];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                // within 127.5 of zero: adding 1.5 * 2^23 rounds to a whole number, whose low byte is the code
-                byte[b] = __float_as_uint(__fadd_rn(__fmul_rn(v[4 * w + b], inverse), 12582912.0f));
-            }
-            words[w] = __byte_perm(__byte_perm(byte[0], byte[1], 0x0040), __byte_perm(byte[2], byte[3], 0x0040), 0x5410);
-        }
+        const uint4 words = scale.codes(v);
         for (int f = 0; f < a.fan; ++f) {
             const std::int64_t to = a.place == nullptr ? row : a.place[row * a.fan + f];
             if (to < 0) continue;
             uint4* at = reinterpret_cast<uint4*>(a.codes + (piece / 8 * a.out_rows + to) * block_bytes);
-            at[(piece % 8) ^ static_cast<int>(to & 7)] = {words[0], words[1], words[2], words[3]};
+            at[(piece % 8) ^ static_cast<int>(to & 7)] = words;
         }
     };
 #pragma unroll
@@ -231,7 +190,7 @@ __global__ void __launch_bounds__(256) quantise_kernel(QuantiseArgs a) {
     }
     for (int f = part; f < a.fan; f += threads) {
         const std::int64_t to = a.place == nullptr ? row : a.place[row * a.fan + f];
-        if (to >= 0) a.scales[to] = finite ? scale : __int_as_float(0x7fffffff);  // such a row's outputs are no numbers
+        if (to >= 0) a.scales[to] = scale.told();
     }
     if (a.zeros != nullptr) {
         for (int f = 0; f < a.fan; ++f) {
@@ -245,8 +204,8 @@ __global__ void __launch_bounds__(256) quantise_kernel(QuantiseArgs a) {
 // ---- the product ----
 
 constexpr int epilogue_warps = 8;
-constexpr int weight_warp = 8, row_warp = 9, mma_warp = 10;
-constexpr int product_threads = 32 * 11;
+constexpr int copy_warp = 8, copy_warps = 4, mma_warp = 12;
+constexpr int product_threads = 32 * 13;
 constexpr int most_stages = 12;
 
 struct ProductArgs {
@@ -265,6 +224,9 @@ struct ProductArgs {
 };
 
 struct ProductTail {
+    // of the tile's columns: the rows' scales, and the rows of y; by turns, as one tile's stores overlap the next one's loads
+    alignas(16) float row_scales[2][most_tile];
+    alignas(16) int rows[2][most_tile];
     std::uint64_t full[most_stages], empty[most_stages], tmem_full[2], tmem_empty[2], drain;
     std::uint32_t tmem;
     unsigned status;  // of waits: told to the caller's at the end
@@ -277,18 +239,30 @@ __device__ __forceinline__ void bulk_load(std::uint32_t to, const void* from, st
                  : "memory");
 }
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+__device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ int peer_load(std::uint32_t address, int rank) {
-    int v;
+__device__ __forceinline__ void peer_store(std::uint32_t address, int rank, int v) {
+    asm volatile("{\n\t.reg .b32 there;\n\tmapa.shared::cluster.u32 there, %0, %1;\n\tst.shared::cluster.b32 [there], %2;\n\t}" ::"r"(address),
+                 "r"(rank), "r"(v)
+                 : "memory");
+}
+
+// A barrier of the epilogue's threads: whether any of them says so.
+__device__ __forceinline__ bool epilogue_any(bool mine) {
+    int any;
     asm volatile(
-        "{\n\t.reg .b32 there;\n\tmapa.shared::cluster.u32 there, %1, %2;\n\tld.shared::cluster.b32 %0, [there];\n\t}"
-        : "=r"(v)
-        : "r"(address), "r"(rank)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(static_cast<int>(mine))
         : "memory");
-    return v;
+    return any != 0;
 }
 
 struct Tile {
@@ -313,10 +287,12 @@ __device__ __forceinline__ Tile tile_at(const ProductArgs& a, std::int64_t item)
     return t;
 }
 
-// A block takes tiles of 128 outputs by tile_rows rows one after another: two warps copy blocks of weights and rows
-// into a ring, a thread issues the MMAs into one of two accumulators, eight warps scale and store the other. With
-// `splits` > 1 a cluster of that many blocks has one tile, each block a part of its inputs, and the sums are added over
-// the cluster's shared memory.
+// A block takes tiles of 128 outputs by tile_rows rows one after another: four warps copy blocks of weights and rows into a
+// ring, a thread issues the MMAs into one of two accumulators, eight warps scale and store the other. A copy holds up the
+// warp that issues it for some 800 cycles, but takes as many lanes' copies as there are: one warp that copied the two
+// operands of each block, for which the MMAs of 256 rows take 512 cycles, had set the pace (880 cycles a block). With
+// `splits` > 1 a cluster of that many blocks has one tile, each block a part of its inputs; each sends its sums of an
+// output to the block that adds up and stores that output.
 template <typename T, bool Experts>
 __global__ void __launch_bounds__(product_threads, 1) product_kernel(const ProductArgs a) {
     extern __shared__ std::uint8_t dynamic[];
@@ -325,6 +301,7 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
     const std::uint32_t ring = (raw + 1023u) & ~1023u;
     const std::uint32_t row_bytes = static_cast<std::uint32_t>(a.tile_rows) * block_bytes;
     const std::uint32_t rows_ring = ring + static_cast<std::uint32_t>(a.stages) * weight_block;
+    const std::uint32_t exchange = rows_ring + static_cast<std::uint32_t>(a.stages) * row_bytes;  // [block][column][output]
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int splits = a.splits;
     const int rank = static_cast<int>(blockIdx.x) % splits;
@@ -332,15 +309,9 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
     const int k_from = static_cast<int>(static_cast<std::int64_t>(a.k_blocks) * rank / splits);
     const int k_to = static_cast<int>(static_cast<std::int64_t>(a.k_blocks) * (rank + 1) / splits);
 
-    if (warp == mma_warp) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&tail.tmem)),
-                     "r"(a.tmem_columns)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    if (warp == weight_warp && lane == 0) {
+    if (warp == copy_warp && lane == 0) {
         for (int s = 0; s < a.stages; ++s) {
-            barrier_init(smem_address(&tail.full[s]), 2);
+            barrier_init(smem_address(&tail.full[s]), 1);
             barrier_init(smem_address(&tail.empty[s]), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -353,47 +324,89 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async_shared();
     }
+    if (warp == mma_warp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&tail.tmem)),
+                     "r"(a.tmem_columns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     const std::uint32_t tmem = tail.tmem;
+    if (splits > 1) cluster_arrive();  // the others' memory is there once all have
     volatile int* abort = &tail.abort;
     unsigned* waits = &tail.status;
     launch_dependents();
-    // The kernel before this one waits for all before it and only then lets this one start, so the weights are
-    // written when one matrix's are loaded; which expert's, its tiles say.
-    if (Experts || warp != weight_warp) grid_dependency_wait();
-    const std::int64_t row_tiles = Experts ? *a.arranged.tile_count : (a.rows + a.tile_rows - 1) / a.tile_rows;
-    const std::int64_t items = row_tiles * a.tiles;
+    if (Experts || warp < copy_warp || warp >= copy_warp + copy_warps) grid_dependency_wait();
+    std::int64_t items = 0;
+    if (Experts) {
+        items = *a.arranged.tile_count * static_cast<std::int64_t>(a.tiles);
+    } else {
+        items = (a.rows + a.tile_rows - 1) / a.tile_rows * a.tiles;
+    }
 
-    if (warp == weight_warp || warp == row_warp) {
-        if (lane == 0) {
-            const bool weights = warp == weight_warp;
-            int slot = 0, issued = 0;
-            std::uint32_t phase = 0;
-            for (std::int64_t item = first_item; item < items && !*abort; item += item_step) {
-                const Tile t = tile_at<Experts>(a, item);
-                const std::uint32_t bytes = weights ? weight_block : static_cast<std::uint32_t>(t.columns) * block_bytes;
-                const std::int64_t matrix_tile = static_cast<std::int64_t>(t.expert) * a.tiles + t.output / block_rows;
-                const std::uint8_t* from = weights ? a.weights + matrix_tile * a.k_blocks * weight_block
-                                                   : a.codes + t.row * block_bytes;
-                const std::int64_t step = weights ? weight_block : a.out_rows * block_bytes;
-                for (int k = k_from; k < k_to; ++k) {
-                    if (!barrier_wait(smem_address(&tail.empty[slot]), phase ^ 1u, waits)) {
-                        *abort = 1;
-                        break;
-                    }
-                    const std::uint32_t full = smem_address(&tail.full[slot]);
-                    barrier_expect_bytes(full, bytes);
-                    bulk_load(weights ? ring + slot * weight_block : rows_ring + slot * row_bytes, from + k * step, bytes, full);
-                    ++issued;
-                    if (++slot == a.stages) slot = 0, phase ^= 1u;
+    if (warp >= copy_warp && warp < copy_warp + copy_warps) {
+        // The block's copies are numbered q = 0, 1, ..., a block of inputs each, tile after tile; this warp has every
+        // fourth one. Those that fill the ring go out a lane each, the later ones a lane an operand.
+        const int blocks = k_to - k_from;
+        const std::int64_t mine = first_item < items ? (items - first_item + item_step - 1) / item_step * blocks : 0;
+        auto of = [&](std::int64_t q, std::uint32_t& bytes, const std::uint8_t*& weights, const std::uint8_t*& rows) {
+            const std::int64_t nth = q / blocks;
+            const int k = k_from + static_cast<int>(q - nth * blocks);
+            const Tile t = tile_at<Experts>(a, first_item + nth * item_step);
+            bytes = static_cast<std::uint32_t>(t.columns) * block_bytes;
+            weights = a.weights + ((static_cast<std::int64_t>(t.expert) * a.tiles + t.output / block_rows) * a.k_blocks + k) * weight_block;
+            rows = a.codes + (t.row + k * a.out_rows) * block_bytes;
+        };
+        const int own = lane * copy_warps + warp - copy_warp;
+        const bool filling = own < a.stages && own < mine;
+        const std::uint32_t own_full = smem_address(&tail.full[filling ? own : 0]);
+        std::uint32_t bytes = 0;
+        const std::uint8_t *weights = nullptr, *rows = nullptr;
+        if (filling) {
+            of(own, bytes, weights, rows);
+            barrier_expect_bytes(own_full, weight_block + bytes);
+            // The kernel before this one lets it start when all before that one have ended, and weights are written by
+            // kernels that let nothing start early: one matrix's need not wait. Which expert's, the tiles have said.
+            bulk_load(ring + own * weight_block, weights, weight_block, own_full);
+        }
+        __syncwarp();
+        if (!Experts) grid_dependency_wait();
+        if (filling) bulk_load(rows_ring + own * row_bytes, rows, bytes, own_full);
+        __syncwarp();
+        std::int64_t q = warp - copy_warp;
+        while (q < a.stages) q += copy_warps;
+        if (lane < 2) {
+            std::int64_t nth = q / blocks;
+            int k = static_cast<int>(q - nth * blocks), slot = static_cast<int>(q) % a.stages;
+            std::uint32_t pass = static_cast<std::uint32_t>(q) / static_cast<std::uint32_t>(a.stages);
+            bool moved = true;  // to another tile
+            const std::uint8_t* from = nullptr;
+            const std::int64_t step = lane == 0 ? weight_block : a.out_rows * block_bytes;
+            for (; q < mine; q += copy_warps) {
+                if (moved) {
+                    of(nth * blocks, bytes, weights, rows);
+                    from = lane == 0 ? weights : rows;
+                    moved = false;
                 }
+                bool free = true;
+                if (lane == 0) free = !*abort && barrier_wait(smem_address(&tail.empty[slot]), (pass & 1u) ^ 1u, waits);
+                if (!__shfl_sync(3u, free, 0)) {
+                    *abort = 1;
+                    break;
+                }
+                const std::uint32_t full = smem_address(&tail.full[slot]);
+                if (lane == 0) barrier_expect_bytes(full, weight_block + bytes);
+                __syncwarp(3u);
+                bulk_load(lane == 0 ? ring + slot * weight_block : rows_ring + slot * row_bytes, from + k * step,
+                          lane == 0 ? weight_block : bytes, full);
+                for (slot += copy_warps; slot >= a.stages; slot -= a.stages) ++pass;
+                for (k += copy_warps; k >= blocks; k -= blocks) ++nth, moved = true;
             }
-            if (*abort) {  // the copies under way
-                for (int s = 0; s < a.stages && s < issued; ++s) {
-                    if (--slot < 0) slot = a.stages - 1, phase ^= 1u;
-                    barrier_wait(smem_address(&tail.full[slot]), phase, waits);
+            if (*abort && lane == 0) {  // the copies under way: of q - 4, q - 8, ...
+                for (std::int64_t last = q - copy_warps; last >= 0 && last > q - copy_warps - a.stages; last -= copy_warps) {
+                    if (last < mine) barrier_wait(smem_address(&tail.full[last % a.stages]), last / a.stages & 1, waits);
                 }
             }
         }
@@ -434,11 +447,20 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
         const int quarter = warp % 4, half = warp / 4;
         int buffer = 0;
         std::uint32_t pass = 0;
-        for (std::int64_t item = first_item; item < items && !*abort; item += item_step) {
+        if (splits > 1) cluster_wait();
+        for (std::int64_t item = first_item; item < items; item += item_step) {
             const Tile t = tile_at<Experts>(a, item);
+            if (splits == 1) {
+                const int column = static_cast<int>(threadIdx.x);
+                if (column < t.rows) {
+                    tail.row_scales[buffer][column] = a.row_scales[t.row + column];
+                    if constexpr (Experts) tail.rows[buffer][column] = a.arranged.pair[t.row + column];
+                }
+            }
+            if (epilogue_any(*abort != 0)) break;  // all of them, as the next ones wait for one another here
             if (!barrier_wait(smem_address(&tail.tmem_full[buffer]), pass, waits)) {
                 *abort = 1;
-                break;
+                continue;
             }
             tmem_fence_after();
             const std::uint32_t sums = tmem + static_cast<std::uint32_t>(buffer * a.tile_rows) +
@@ -450,33 +472,41 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
                 const float scale = inside ? a.scales[channel] : 0.0f;
                 const float bias = inside && a.bias != nullptr ? widen(static_cast<const T*>(a.bias)[channel]) : 0.0f;
                 T* y = static_cast<T*>(a.y) + output;
+                if constexpr (!Experts) y += t.row * a.outputs;
                 for (int column = half * 16; column < t.columns; column += 32) {
                     int acc[16];
                     tmem_load16(sums + static_cast<std::uint32_t>(column), acc);
-                    tmem_load_wait();
+                    float row_scale[16];
+                    int row[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (inside && column + i < t.rows) {
-                            const std::int64_t row = t.row + column + i;
-                            float v = __fmul_rn(__fmul_rn(__int2float_rn(acc[i]), scale), a.row_scales[row]);
-                            if (a.bias != nullptr) v = __fadd_rn(v, bias);
-                            const std::int64_t to = Experts ? a.arranged.pair[row] : row;
-                            y[to * a.outputs] = narrow<T>(v);
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 v = reinterpret_cast<const float4*>(tail.row_scales[buffer])[column / 4 + i];
+                        row_scale[4 * i] = v.x, row_scale[4 * i + 1] = v.y, row_scale[4 * i + 2] = v.z, row_scale[4 * i + 3] = v.w;
+                        if constexpr (Experts) {
+                            const int4 r = reinterpret_cast<const int4*>(tail.rows[buffer])[column / 4 + i];
+                            row[4 * i] = r.x, row[4 * i + 1] = r.y, row[4 * i + 2] = r.z, row[4 * i + 3] = r.w;
                         }
                     }
+                    tmem_load_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (!inside || column + i >= t.rows) continue;
+                        float v = __fmul_rn(__fmul_rn(__int2float_rn(acc[i]), scale), row_scale[i]);
+                        if (a.bias != nullptr) v = __fadd_rn(v, bias);
+                        const int to = Experts ? row[i] : column + i;
+                        y[static_cast<std::int64_t>(to) * a.outputs] = narrow<T>(v);
+                    }
                 }
-            } else {  // the ring is free: every copy has been read
+            } else {
+                const int mine = block_rows / splits;  // outputs that a block adds up
+                const int channel = quarter * 32 + lane;
+                const std::uint32_t to = exchange + static_cast<std::uint32_t>(rank * a.tile_rows * mine + channel % mine) * 4;
                 for (int column = half * 16; column < t.columns; column += 32) {
                     int acc[16];
                     tmem_load16(sums + static_cast<std::uint32_t>(column), acc);
                     tmem_load_wait();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(
-                                         ring + static_cast<std::uint32_t>((column + i) * block_rows + quarter * 32 + lane) * 4),
-                                     "r"(acc[i])
-                                     : "memory");
-                    }
+                    for (int i = 0; i < 16; ++i) peer_store(to + static_cast<std::uint32_t>((column + i) * mine) * 4, channel / mine, acc[i]);
                 }
             }
             tmem_fence_before();
@@ -487,17 +517,19 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
     __syncwarp();
 
     if (splits > 1) {
-        cluster_sync();
+        if (warp >= epilogue_warps) cluster_wait();
+        cluster_arrive();
+        cluster_wait();
         if (first_item < items && !*abort) {
             const Tile t = tile_at<Experts>(a, first_item);
-            const int mine = block_rows / splits;  // outputs of the tile that this block adds up and stores
+            const int mine = block_rows / splits;
+            const int* sums = reinterpret_cast<const int*>(dynamic + (exchange - raw));
             for (int i = threadIdx.x; i < mine * t.rows; i += product_threads) {
-                const int column = i / mine, channel_in = rank * mine + i % mine;
-                const int output = t.output + channel_in;
+                const int column = i / mine, output = t.output + rank * mine + i % mine;
                 if (output >= a.outputs) continue;
-                const std::uint32_t at = ring + static_cast<std::uint32_t>(column * block_rows + channel_in) * 4;
                 int sum = 0;
-                for (int r = 0; r < splits; ++r) sum += peer_load(at, r);
+#pragma unroll 8
+                for (int r = 0; r < splits; ++r) sum += sums[r * a.tile_rows * mine + i];
                 const std::int64_t channel = static_cast<std::int64_t>(t.expert) * a.outputs + output;
                 const std::int64_t row = t.row + column;
                 float v = __fmul_rn(__fmul_rn(__int2float_rn(sum), a.scales[channel]), a.row_scales[row]);
@@ -506,7 +538,6 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
                 static_cast<T*>(a.y)[to * a.outputs + output] = narrow<T>(v);
             }
         }
-        cluster_sync();  // the others may still be reading
     }
     tmem_fence_before();
     __syncthreads();
@@ -560,13 +591,14 @@ cudaError_t quantise(Type type, const QuantiseArgs& a, cudaStream_t stream) {
 template <typename T, bool Experts>
 cudaError_t product(ProductArgs a, std::int64_t most_items, cudaStream_t stream) {
     static SharedAllowance allowance;
-    constexpr int room = 208 * 1024;
+    const int exchange = a.splits > 1 ? block_rows * a.tile_rows * 4 : 0;
+    const int room = 208 * 1024 - exchange;
     const int stage = weight_block + a.tile_rows * block_bytes;
     a.stages = std::min(most_stages, room / stage);
     a.tmem_columns = 32;
     while (a.tmem_columns < 2u * static_cast<unsigned>(a.tile_rows)) a.tmem_columns *= 2;
-    const int bytes = a.stages * stage + 1024;
-    cudaError_t status = allowance.allow(product_kernel<T, Experts>, 227 * 1024 - 1024);
+    const int bytes = a.stages * stage + exchange + 1024;
+    cudaError_t status = allowance.allow(product_kernel<T, Experts>, 210 * 1024);
     if (status != cudaSuccess) return status;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(a.splits > 1 ? most_items * a.splits
@@ -594,24 +626,32 @@ cudaError_t product(Type type, const ProductArgs& a, std::int64_t most_items, cu
     }
 }
 
-// Rows a tile: what loads the fewest bytes over the turns that the tiles take on all SMs.
-int rows_a_tile(std::int64_t rows, int tiles) {
-    int best = step_rows;
-    std::int64_t least = -1;
-    for (int n = step_rows; n <= most_tile; n += step_rows) {
-        const std::int64_t turns = ((rows + n - 1) / n * tiles + sm_count() - 1) / sm_count();
-        const std::int64_t cost = turns * (weight_block + n * block_bytes);
-        if (least < 0 || cost < least) least = cost, best = n;
-        if (n >= rows) break;
-    }
-    return best;
-}
+constexpr int most_split_tile = 64;  // rows of a tile that a cluster shares: its sums have a place of their own
 
 // Blocks that share a tile's inputs: while they all run at once and each has two blocks of them.
-int splits_of(std::int64_t items, int k_blocks) {
+int splits_of(std::int64_t items, int tile_rows, int k_blocks) {
     int splits = 1;
-    while (splits < 8 && items * splits * 2 <= sm_count() && k_blocks >= splits * 4) splits *= 2;
+    while (tile_rows <= most_split_tile && splits < 8 && items * splits * 2 <= sm_count() && k_blocks >= splits * 4) splits *= 2;
     return splits;
+}
+
+// Rows a tile: what takes the fewest cycles by a model of the kernel, whose constants fit its times within a fifth. A
+// block of inputs is loaded at 40 bytes a cycle or multiplied at two cycles a row (at least 240); a tile's stores, which
+// overlap the next tile's products, take 24 cycles a row.
+int rows_a_tile(double groups, double rows, int tiles, int k_blocks) {
+    int best = step_rows;
+    double least = -1.0;
+    for (int n = step_rows; n <= most_tile; n += step_rows) {
+        // rows of a group are spread around their mean, so beyond one tile the last is half full
+        const double items = groups * tiles * (groups == 1.0 ? std::ceil(rows / n) : std::max(1.0, rows / n + 0.5));
+        const int splits = splits_of(static_cast<std::int64_t>(items), n, k_blocks);
+        const double block = std::max({(weight_block + n * block_bytes) / 40.0, 2.0 * n, 240.0});
+        const double product = std::ceil(static_cast<double>(k_blocks) / splits) * block, stores = 600.0 + 24.0 * n;
+        const double cost = std::ceil(items * splits / sm_count()) * std::max(product, stores) + stores + (splits > 1 ? 1500.0 : 0.0);
+        if (least < 0.0 || cost < least) least = cost, best = n;
+        if (n >= rows && groups == 1.0) break;
+    }
+    return best;
 }
 
 struct Plan {
@@ -630,13 +670,14 @@ Plan plan_of(const BytesArgs& a) {
         return here;
     };
     if (a.choices == nullptr) {
-        p.tile_rows = rows_a_tile(std::max<std::int64_t>(a.tokens, 1), tiles_of(a.outputs));
+        p.tile_rows = rows_a_tile(1.0, static_cast<double>(std::max<std::int64_t>(a.tokens, 1)), tiles_of(a.outputs), blocks_of(a.inputs));
         p.out_rows = padded(a.tokens);
         p.tiles = (a.tokens + p.tile_rows - 1) / p.tile_rows;
     } else {
         const std::int64_t groups = std::min<std::int64_t>(a.experts, pairs);
-        p.tile_rows = static_cast<int>(std::clamp<std::int64_t>(padded(2 * pairs / std::max<std::int64_t>(groups, 1)),
-                                                                step_rows, most_tile));
+        p.tile_rows = rows_a_tile(static_cast<double>(std::max<std::int64_t>(groups, 1)),
+                                  static_cast<double>(pairs) / static_cast<double>(std::max<std::int64_t>(groups, 1)), tiles_of(a.outputs),
+                                  blocks_of(a.inputs));
         p.out_rows = padded(pairs + groups * (step_rows - 1));
         p.tiles = pairs / p.tile_rows + groups;
     }
@@ -679,6 +720,7 @@ std::size_t bytes_workspace(const BytesArgs& a) { return plan_of(a).bytes; }
 
 cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
     if (a.tokens == 0) return cudaSuccess;
+    if (few_rows(a)) return multiply_few(a, stream);
     const Plan p = plan_of(a);
     auto* memory = static_cast<std::uint8_t*>(a.workspace);
     const std::int64_t pairs = a.tokens * a.chosen;
@@ -713,7 +755,7 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
     r.outputs = a.outputs, r.tiles = tiles_of(a.outputs), r.k_blocks = q.k_blocks;
     r.tile_rows = p.tile_rows;
     const std::int64_t items = p.tiles * r.tiles;
-    r.splits = splits_of(items, r.k_blocks);
+    r.splits = splits_of(items, r.tile_rows, r.k_blocks);
     r.status = a.status;
     if (a.choices == nullptr) {
         r.y = a.y;

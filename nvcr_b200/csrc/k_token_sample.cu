@@ -286,9 +286,17 @@ __global__ void __launch_bounds__(threads) block_kernel(SampleArgs a) {
 
 // ---- a cluster a row, from registers ----
 
-__device__ __forceinline__ void cluster_sync() {
+__device__ __forceinline__ void cluster_arrive() {
     __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    cluster_arrive();
+    cluster_wait();
 }
 __device__ __forceinline__ std::uint32_t at_block(const void* here, int rank) {
     std::uint32_t there;
@@ -949,6 +957,7 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int rank = static_cast<int>(blockIdx.x) % blocks;
     const std::int64_t r = blockIdx.x / blocks;
+    cluster_arrive();  // the others' memory is there once all have
     make_table(shared.table);
     join_chain();
     const T* logits = static_cast<const T*>(a.logits) + r * a.stride;
@@ -970,6 +979,7 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
     if (lane == 0) shared.sums.scratch[warp] = top;
     __syncthreads();
     for (int w = 0; w < warps; ++w) top = max(top, static_cast<unsigned>(shared.sums.scratch[w]));
+    cluster_wait();
     if (threadIdx.x < static_cast<unsigned>(blocks)) put(&shared.maxima[rank], static_cast<int>(threadIdx.x), top);
     cluster_sync();
     for (int b = 0; b < blocks; ++b) top = max(top, static_cast<unsigned>(shared.maxima[b]));
