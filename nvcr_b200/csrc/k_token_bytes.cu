@@ -18,6 +18,7 @@ namespace {
 using namespace kernels;
 
 constexpr int step_rows = 16;      // rows of x are padded to the MMA's step of N
+constexpr int pair_step_rows = 32; // with two blocks a tile
 constexpr int most_tile = 256;     // rows of x a tile
 
 std::int64_t padded(std::int64_t rows) { return (rows + step_rows - 1) / step_rows * step_rows; }
@@ -216,7 +217,7 @@ struct ProductArgs {
     const float* row_scales;
     Arranged arranged;  // tiles null: rows 0 .. rows - 1 of one matrix
     std::int64_t rows, out_rows;
-    int outputs, tiles, k_blocks;
+    int experts, outputs, tiles, k_blocks;
     int tile_rows, stages, splits;
     unsigned tmem_columns;
     void* y;
@@ -271,11 +272,13 @@ struct Tile {
     int rows, columns;           // columns: rows padded to the MMA's step
 };
 
-template <bool Experts>
+// Tiles of one group of rows after another; with Pair the outputs are those of two blocks.
+template <bool Experts, bool Pair = false>
 __device__ __forceinline__ Tile tile_at(const ProductArgs& a, std::int64_t item) {
-    const std::int64_t nth = item / a.tiles;
+    const int tiles = Pair ? (a.tiles + 1) / 2 : a.tiles;
+    const std::int64_t nth = item / tiles;
     Tile t;
-    t.output = static_cast<int>(item - nth * a.tiles) * block_rows;
+    t.output = static_cast<int>(item - nth * tiles) * (Pair ? 2 * block_rows : block_rows);
     if constexpr (Experts) {
         const int4 found = a.arranged.tiles[nth];
         t.expert = found.x, t.row = found.y, t.rows = found.z;
@@ -283,8 +286,69 @@ __device__ __forceinline__ Tile tile_at(const ProductArgs& a, std::int64_t item)
         t.expert = 0, t.row = nth * a.tile_rows;
         t.rows = static_cast<int>(min(static_cast<std::int64_t>(a.tile_rows), a.rows - t.row));
     }
-    t.columns = (t.rows + step_rows - 1) / step_rows * step_rows;
+    constexpr int step = Pair ? pair_step_rows : step_rows;
+    t.columns = (t.rows + step - 1) / step * step;
     return t;
+}
+
+// What a tile's stores need of its rows, by a thread a row; the caller synchronises.
+template <bool Experts>
+__device__ __forceinline__ void stage_rows(const ProductArgs& a, const Tile& t, ProductTail& tail, int buffer) {
+    const int column = static_cast<int>(threadIdx.x);
+    if (column >= t.rows) return;
+    tail.row_scales[buffer][column] = a.row_scales[t.row + column];
+    if constexpr (Experts) tail.rows[buffer][column] = a.arranged.pair[t.row + column];
+}
+
+// An epilogue warp's part of a tile, scaled and stored: 32 outputs from `first` on, half of the columns.
+template <typename T, bool Experts>
+__device__ __forceinline__ void store_tile(const ProductArgs& a, const Tile& t, const ProductTail& tail, int buffer, int first,
+                                           std::uint32_t sums, int half) {
+    const int output = first + static_cast<int>(threadIdx.x) % 32;
+    const bool inside = output < a.outputs;
+    const std::int64_t channel = static_cast<std::int64_t>(t.expert) * a.outputs + output;
+    const float scale = inside ? a.scales[channel] : 0.0f;
+    const float bias = inside && a.bias != nullptr ? widen(static_cast<const T*>(a.bias)[channel]) : 0.0f;
+    T* y = static_cast<T*>(a.y) + output;
+    if constexpr (!Experts) y += t.row * a.outputs;
+    for (int column = half * 16; column < t.columns; column += 32) {
+        int acc[16];
+        tmem_load16(sums + static_cast<std::uint32_t>(column), acc);
+        float row_scale[16];
+        int row[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 v = reinterpret_cast<const float4*>(tail.row_scales[buffer])[column / 4 + i];
+            row_scale[4 * i] = v.x, row_scale[4 * i + 1] = v.y, row_scale[4 * i + 2] = v.z, row_scale[4 * i + 3] = v.w;
+            if constexpr (Experts) {
+                const int4 r = reinterpret_cast<const int4*>(tail.rows[buffer])[column / 4 + i];
+                row[4 * i] = r.x, row[4 * i + 1] = r.y, row[4 * i + 2] = r.z, row[4 * i + 3] = r.w;
+            }
+        }
+        tmem_load_wait();
+        if (!inside) continue;
+        T* to = y + static_cast<std::int64_t>(column) * a.outputs;
+        auto value = [&](int i) {
+            const float v = __fmul_rn(__fmul_rn(__int2float_rn(acc[i]), scale), row_scale[i]);
+            return narrow<T>(a.bias != nullptr ? __fadd_rn(v, bias) : v);
+        };
+        if (column + 16 <= t.rows) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if constexpr (Experts) {
+                    y[static_cast<std::int64_t>(row[i]) * a.outputs] = value(i);
+                } else {
+                    *to = value(i);
+                    to += a.outputs;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (column + i < t.rows) y[static_cast<std::int64_t>(Experts ? row[i] : column + i) * a.outputs] = value(i);
+            }
+        }
+    }
 }
 
 // A block takes tiles of 128 outputs by tile_rows rows one after another: four warps copy blocks of weights and rows into a
@@ -450,13 +514,7 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
         if (splits > 1) cluster_wait();
         for (std::int64_t item = first_item; item < items; item += item_step) {
             const Tile t = tile_at<Experts>(a, item);
-            if (splits == 1) {
-                const int column = static_cast<int>(threadIdx.x);
-                if (column < t.rows) {
-                    tail.row_scales[buffer][column] = a.row_scales[t.row + column];
-                    if constexpr (Experts) tail.rows[buffer][column] = a.arranged.pair[t.row + column];
-                }
-            }
+            if (splits == 1) stage_rows<Experts>(a, t, tail, buffer);
             if (epilogue_any(*abort != 0)) break;  // all of them, as the next ones wait for one another here
             if (!barrier_wait(smem_address(&tail.tmem_full[buffer]), pass, waits)) {
                 *abort = 1;
@@ -465,38 +523,8 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
             tmem_fence_after();
             const std::uint32_t sums = tmem + static_cast<std::uint32_t>(buffer * a.tile_rows) +
                 (static_cast<std::uint32_t>(quarter * 32) << 16);
-            const int output = t.output + quarter * 32 + lane;
             if (splits == 1) {
-                const bool inside = output < a.outputs;
-                const std::int64_t channel = static_cast<std::int64_t>(t.expert) * a.outputs + output;
-                const float scale = inside ? a.scales[channel] : 0.0f;
-                const float bias = inside && a.bias != nullptr ? widen(static_cast<const T*>(a.bias)[channel]) : 0.0f;
-                T* y = static_cast<T*>(a.y) + output;
-                if constexpr (!Experts) y += t.row * a.outputs;
-                for (int column = half * 16; column < t.columns; column += 32) {
-                    int acc[16];
-                    tmem_load16(sums + static_cast<std::uint32_t>(column), acc);
-                    float row_scale[16];
-                    int row[16];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4 v = reinterpret_cast<const float4*>(tail.row_scales[buffer])[column / 4 + i];
-                        row_scale[4 * i] = v.x, row_scale[4 * i + 1] = v.y, row_scale[4 * i + 2] = v.z, row_scale[4 * i + 3] = v.w;
-                        if constexpr (Experts) {
-                            const int4 r = reinterpret_cast<const int4*>(tail.rows[buffer])[column / 4 + i];
-                            row[4 * i] = r.x, row[4 * i + 1] = r.y, row[4 * i + 2] = r.z, row[4 * i + 3] = r.w;
-                        }
-                    }
-                    tmem_load_wait();
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (!inside || column + i >= t.rows) continue;
-                        float v = __fmul_rn(__fmul_rn(__int2float_rn(acc[i]), scale), row_scale[i]);
-                        if (a.bias != nullptr) v = __fadd_rn(v, bias);
-                        const int to = Experts ? row[i] : column + i;
-                        y[static_cast<std::int64_t>(to) * a.outputs] = narrow<T>(v);
-                    }
-                }
+                store_tile<T, Experts>(a, t, tail, buffer, t.output + quarter * 32, sums, half);
             } else {
                 const int mine = block_rows / splits;  // outputs that a block adds up
                 const int channel = quarter * 32 + lane;
@@ -543,6 +571,163 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
     __syncthreads();
     if (warp == mma_warp) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_columns) : "memory");
+        if (lane == 0 && tail.status != 0 && a.status != nullptr) atomicOr(a.status, tail.status);
+    }
+}
+
+// Large products: two blocks of a cluster have a tile of 256 outputs, each with half of its outputs' weights and half of its
+// rows in its shared memory, which the tensor cores of both read. A block of 128 inputs so takes 32 KB a block in place of
+// 48, where 128 x 256 tiles loaded 66 bytes a cycle and SM, which is all that L2 gave. The copies of both blocks count on
+// the first one's barriers, whose thread issues the MMAs: a thread that told it of the second one's, by an arrival with
+// release, took 1300 cycles a block of inputs.
+template <typename T, bool Experts>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) pair_kernel(
+    const __grid_constant__ CUtensorMap weights_map, const __grid_constant__ CUtensorMap codes_map, const ProductArgs a) {
+    extern __shared__ std::uint8_t dynamic[];
+    __shared__ ProductTail tail;
+    const std::uint32_t ring = (smem_address(dynamic) + 1023u) & ~1023u;
+    const std::uint32_t row_bytes = static_cast<std::uint32_t>(a.tile_rows) / 2 * block_bytes;
+    const std::uint32_t rows_ring = ring + static_cast<std::uint32_t>(a.stages) * weight_block;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int rank = static_cast<int>(blockIdx.x) % 2;
+    const std::int64_t first_item = blockIdx.x / 2, item_step = gridDim.x / 2;
+    const int blocks = a.k_blocks;
+
+    if (warp == copy_warp && lane == 0) {
+        for (int s = 0; s < a.stages; ++s) {
+            barrier_init(smem_address(&tail.full[s]), 1);
+            barrier_init(smem_address(&tail.empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            barrier_init(smem_address(&tail.tmem_full[b]), 1);
+            barrier_init(smem_address(&tail.tmem_empty[b]), 2 * epilogue_warps);
+        }
+        barrier_init(smem_address(&tail.drain), 1);
+        tail.status = 0;
+        tail.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async_shared();
+    }
+    if (warp == mma_warp) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&tail.tmem)),
+                     "r"(a.tmem_columns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tmem_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    tmem_fence_after();
+    const std::uint32_t tmem = tail.tmem;
+    volatile int* abort = &tail.abort;
+    unsigned* waits = &tail.status;
+    launch_dependents();
+    grid_dependency_wait();
+    const std::int64_t row_tiles = Experts ? *a.arranged.tile_count : (a.rows + a.tile_rows - 1) / a.tile_rows;
+    const std::int64_t items = row_tiles * ((a.tiles + 1) / 2);
+
+    if (warp >= copy_warp && warp < copy_warp + copy_warps) {
+        const std::int64_t mine = first_item < items ? (items - first_item + item_step - 1) / item_step * blocks : 0;
+        if (lane < 2) {
+            std::int64_t nth = (warp - copy_warp) / blocks;
+            int k = (warp - copy_warp) % blocks, slot = (warp - copy_warp) % a.stages;
+            std::uint32_t pass = static_cast<std::uint32_t>((warp - copy_warp) / a.stages);
+            bool moved = true;  // to another tile
+            int from = 0;       // row of 128 bytes
+            const CUtensorMap* map = lane == 0 ? &weights_map : &codes_map;
+            const int step = lane == 0 ? block_rows : static_cast<int>(a.out_rows);
+            const std::uint32_t stage = 2 * (weight_block + row_bytes);  // of both blocks: boxes are whole, past the last row too
+            std::int64_t q = warp - copy_warp;
+            for (; q < mine; q += copy_warps) {
+                if (moved) {
+                    const Tile t = tile_at<Experts, true>(a, first_item + nth * item_step);
+                    // past an odd last tile the second block's products are of no output
+                    const std::int64_t tile = static_cast<std::int64_t>(t.expert) * a.tiles + min(t.output / block_rows + rank, a.tiles - 1);
+                    from = static_cast<int>(lane == 0 ? tile * blocks * block_rows : t.row + rank * (t.columns / 2));
+                    moved = false;
+                }
+                bool free = true;
+                if (lane == 0) free = !*abort && barrier_wait(smem_address(&tail.empty[slot]), (pass & 1u) ^ 1u, waits);
+                if (!__shfl_sync(3u, free, 0)) {
+                    *abort = 1;
+                    break;
+                }
+                const std::uint32_t full = smem_address(&tail.full[slot]);
+                if (lane == 0 && rank == 0) barrier_expect_bytes(full, stage);
+                __syncwarp(3u);
+                tma_load_2d_pair(lane == 0 ? ring + slot * weight_block : rows_ring + slot * row_bytes, map, full, 0, from + k * step);
+                for (slot += copy_warps; slot >= a.stages; slot -= a.stages) ++pass;
+                for (k += copy_warps; k >= blocks; k -= blocks) ++nth, moved = true;
+            }
+            if (*abort && lane == 0 && rank == 0) {  // the copies under way, the other block's too: of q - 4, q - 8, ...
+                for (std::int64_t last = q - copy_warps; last >= 0 && last > q - copy_warps - a.stages; last -= copy_warps) {
+                    barrier_wait(smem_address(&tail.full[last % a.stages]), last / a.stages & 1, waits);
+                }
+            }
+        }
+    } else if (warp == mma_warp && rank == 1) {  // the first block's thread issues for both
+    } else if (warp == mma_warp) {
+        if (lane == 0) {
+            int slot = 0, buffer = 0;
+            std::uint32_t phase = 0, pass = 0;
+            for (std::int64_t item = first_item; item < items && !*abort; item += item_step) {
+                const Tile t = tile_at<Experts, true>(a, item);
+                const std::uint32_t instruction = i8_pair_instruction(t.columns);
+                if (!barrier_wait(smem_address(&tail.tmem_empty[buffer]), pass ^ 1u, waits)) *abort = 1;
+                tmem_fence_after();
+                const std::uint32_t sums = tmem + static_cast<std::uint32_t>(buffer * a.tile_rows);
+                for (int k = 0; k < blocks && !*abort; ++k) {
+                    if (!barrier_wait(smem_address(&tail.full[slot]), phase, waits)) {
+                        *abort = 1;
+                        break;
+                    }
+                    tmem_fence_after();
+                    const std::uint64_t w = sw128_descriptor(ring + slot * weight_block);
+                    const std::uint64_t x = sw128_descriptor(rows_ring + slot * row_bytes);
+#pragma unroll
+                    for (int step = 0; step < block_bytes / 32; ++step) {
+                        mma_i8_pair(sums, w + 2 * step, x + 2 * step, instruction, k > 0 || step > 0);
+                    }
+                    mma_commit_pair(smem_address(&tail.empty[slot]));
+                    if (++slot == a.stages) slot = 0, phase ^= 1u;
+                }
+                if (!*abort) mma_commit_pair(smem_address(&tail.tmem_full[buffer]));
+                if (++buffer == 2) buffer = 0, pass ^= 1u;
+            }
+            if (*abort) {  // the MMAs under way
+                mma_commit_pair(smem_address(&tail.drain));
+                barrier_wait(smem_address(&tail.drain), 0, waits);
+            }
+        }
+    } else {
+        const int quarter = warp % 4, half = warp / 4;
+        int buffer = 0;
+        std::uint32_t pass = 0;
+        for (std::int64_t item = first_item; item < items; item += item_step) {
+            const Tile t = tile_at<Experts, true>(a, item);
+            stage_rows<Experts>(a, t, tail, buffer);
+            if (epilogue_any(*abort != 0)) break;  // all of them, as the next ones wait for one another here
+            if (!barrier_wait(smem_address(&tail.tmem_full[buffer]), pass, waits)) {
+                *abort = 1;
+                continue;
+            }
+            tmem_fence_after();
+            const std::uint32_t sums = tmem + static_cast<std::uint32_t>(buffer * a.tile_rows) +
+                (static_cast<std::uint32_t>(quarter * 32) << 16);
+            store_tile<T, Experts>(a, t, tail, buffer, t.output + rank * block_rows + quarter * 32, sums, half);
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) barrier_arrive_at(smem_address(&tail.tmem_empty[buffer]), 0);
+            if (++buffer == 2) buffer = 0, pass ^= 1u;
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    cluster_arrive();  // the other block's memory is read, and this one's barriers are arrived on, no more
+    cluster_wait();
+    if (warp == mma_warp) {
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_columns) : "memory");
         if (lane == 0 && tail.status != 0 && a.status != nullptr) atomicOr(a.status, tail.status);
     }
 }
@@ -617,8 +802,58 @@ cudaError_t product(ProductArgs a, std::int64_t most_items, cudaStream_t stream)
     return cudaLaunchKernelEx(&config, product_kernel<T, Experts>, a);
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// `rows` rows of 128 bytes, copied `box` at a time (their swizzle is in memory already).
+bool encode(CUtensorMap& map, const void* memory, std::uint64_t rows, int box) {
+    static const EncodeTiled function = [] {
+        void* pointer = nullptr;
+        cudaDriverEntryPointQueryResult found{};
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &pointer, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            return static_cast<EncodeTiled>(nullptr);
+        }
+        return reinterpret_cast<EncodeTiled>(pointer);
+    }();
+    if (function == nullptr) return false;
+    const cuuint64_t sizes[2] = {block_bytes, rows}, strides[1] = {block_bytes};
+    const cuuint32_t boxes[2] = {block_bytes, static_cast<cuuint32_t>(box)}, steps[2] = {1, 1};
+    return function(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(memory), sizes, strides, boxes, steps,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, bool Experts>
+cudaError_t pair_product(ProductArgs a, std::int64_t most_items, cudaStream_t stream) {
+    static SharedAllowance allowance;
+    const int stage = weight_block + a.tile_rows / 2 * block_bytes;
+    a.stages = std::min(most_stages, 208 * 1024 / stage);
+    a.tmem_columns = 32;
+    while (a.tmem_columns < 2u * static_cast<unsigned>(a.tile_rows)) a.tmem_columns *= 2;
+    const cudaError_t status = allowance.allow(pair_kernel<T, Experts>, 210 * 1024);
+    if (status != cudaSuccess) return status;
+    CUtensorMap weights, codes;
+    const std::uint64_t blocks = static_cast<std::uint64_t>(a.arranged.tiles == nullptr ? 1 : a.experts) * a.tiles * a.k_blocks;
+    if (!encode(weights, a.weights, blocks * block_rows, block_rows) ||
+        !encode(codes, a.codes, static_cast<std::uint64_t>(a.k_blocks) * a.out_rows, a.tile_rows / 2)) {
+        return cudaErrorUnknown;
+    }
+    const auto pairs = static_cast<unsigned>(std::min<std::int64_t>(most_items, sm_count() / 2));
+    return launch_overlapped(pair_kernel<T, Experts>, dim3(2 * pairs), dim3(product_threads),
+                             static_cast<std::size_t>(a.stages * stage + 1024), stream, weights, codes, a);
+}
+
 template <bool Experts>
-cudaError_t product(Type type, const ProductArgs& a, std::int64_t most_items, cudaStream_t stream) {
+cudaError_t product(Type type, const ProductArgs& a, std::int64_t most_items, bool pair, cudaStream_t stream) {
+    if (pair) {
+        switch (type) {
+        case Type::f16: return pair_product<__half, Experts>(a, most_items, stream);
+        case Type::bf16: return pair_product<__nv_bfloat16, Experts>(a, most_items, stream);
+        default: return pair_product<float, Experts>(a, most_items, stream);
+        }
+    }
     switch (type) {
     case Type::f16: return product<__half, Experts>(a, most_items, stream);
     case Type::bf16: return product<__nv_bfloat16, Experts>(a, most_items, stream);
@@ -635,27 +870,35 @@ int splits_of(std::int64_t items, int tile_rows, int k_blocks) {
     return splits;
 }
 
-// Rows a tile: what takes the fewest cycles by a model of the kernel, whose constants fit its times within a fifth. A
-// block of inputs is loaded at 40 bytes a cycle or multiplied at two cycles a row (at least 240); a tile's stores, which
-// overlap the next tile's products, take 24 cycles a row.
-int rows_a_tile(double groups, double rows, int tiles, int k_blocks) {
-    int best = step_rows;
+struct Shape {
+    int tile_rows;
+    bool pair;  // two blocks a tile
+};
+
+// Rows a tile, and the kernel: what takes the fewest cycles by a model. A block of inputs is loaded at 60 bytes a cycle or
+// multiplied at two cycles a row (at least 240); a tile's stores, which overlap the next tile's products, take 24 cycles a
+// row.
+Shape shape_of(double groups, double rows, int tiles, int k_blocks) {
+    Shape best{step_rows, false};
     double least = -1.0;
-    for (int n = step_rows; n <= most_tile; n += step_rows) {
-        // rows of a group are spread around their mean, so beyond one tile the last is half full
-        const double items = groups * tiles * (groups == 1.0 ? std::ceil(rows / n) : std::max(1.0, rows / n + 0.5));
-        const int splits = splits_of(static_cast<std::int64_t>(items), n, k_blocks);
-        const double block = std::max({(weight_block + n * block_bytes) / 40.0, 2.0 * n, 240.0});
-        const double product = std::ceil(static_cast<double>(k_blocks) / splits) * block, stores = 600.0 + 24.0 * n;
-        const double cost = std::ceil(items * splits / sm_count()) * std::max(product, stores) + stores + (splits > 1 ? 1500.0 : 0.0);
-        if (least < 0.0 || cost < least) least = cost, best = n;
-        if (n >= rows && groups == 1.0) break;
+    for (const bool pair : {false, true}) {
+        const int step = pair ? pair_step_rows : step_rows, sets = sm_count() / (pair ? 2 : 1);
+        for (int n = step; n <= most_tile; n += step) {
+            // rows of a group are spread around their mean, so beyond one tile the last is half full
+            const double items = groups * (pair ? (tiles + 1) / 2 : tiles) * (groups == 1.0 ? std::ceil(rows / n) : std::max(1.0, rows / n + 0.5));
+            const int splits = pair ? 1 : splits_of(static_cast<std::int64_t>(items), n, k_blocks);
+            const double block = std::max({(weight_block + (pair ? n / 2 : n) * block_bytes) / 60.0, 2.0 * n, 240.0});
+            const double product = std::ceil(static_cast<double>(k_blocks) / splits) * block, stores = 600.0 + 24.0 * n;
+            const double cost = std::ceil(items * splits / sets) * std::max(product, stores) + stores + (splits > 1 ? 1500.0 : 0.0) + (pair ? 1500.0 : 0.0);
+            if (least < 0.0 || cost < least) least = cost, best = {n, pair};
+            if (n >= rows && groups == 1.0) break;
+        }
     }
     return best;
 }
 
 struct Plan {
-    int tile_rows;
+    Shape shape;
     std::int64_t out_rows, tiles;
     std::size_t codes, scales, place, pair, table, count, products, bytes;
 };
@@ -670,16 +913,16 @@ Plan plan_of(const BytesArgs& a) {
         return here;
     };
     if (a.choices == nullptr) {
-        p.tile_rows = rows_a_tile(1.0, static_cast<double>(std::max<std::int64_t>(a.tokens, 1)), tiles_of(a.outputs), blocks_of(a.inputs));
+        p.shape = shape_of(1.0, static_cast<double>(std::max<std::int64_t>(a.tokens, 1)), tiles_of(a.outputs), blocks_of(a.inputs));
         p.out_rows = padded(a.tokens);
-        p.tiles = (a.tokens + p.tile_rows - 1) / p.tile_rows;
+        p.tiles = (a.tokens + p.shape.tile_rows - 1) / p.shape.tile_rows;
     } else {
         const std::int64_t groups = std::min<std::int64_t>(a.experts, pairs);
-        p.tile_rows = rows_a_tile(static_cast<double>(std::max<std::int64_t>(groups, 1)),
-                                  static_cast<double>(pairs) / static_cast<double>(std::max<std::int64_t>(groups, 1)), tiles_of(a.outputs),
-                                  blocks_of(a.inputs));
+        p.shape = shape_of(static_cast<double>(std::max<std::int64_t>(groups, 1)),
+                           static_cast<double>(pairs) / static_cast<double>(std::max<std::int64_t>(groups, 1)), tiles_of(a.outputs),
+                           blocks_of(a.inputs));
         p.out_rows = padded(pairs + groups * (step_rows - 1));
-        p.tiles = pairs / p.tile_rows + groups;
+        p.tiles = pairs / p.shape.tile_rows + groups;
     }
     p.codes = take(static_cast<std::size_t>(blocks_of(a.inputs)) * p.out_rows * block_bytes);
     p.scales = take(p.out_rows * sizeof(float));
@@ -731,7 +974,7 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
                     reinterpret_cast<int4*>(memory + p.table), reinterpret_cast<int*>(memory + p.count)};
         const cudaError_t status = launch_overlapped(arrange_kernel, dim3(1), dim3(arrange_threads),
                                                      (a.experts + 64) * sizeof(int), stream, a.choices, pairs, a.experts,
-                                                     p.tile_rows, arranged);
+                                                     p.shape.tile_rows, arranged);
         if (status != cudaSuccess) return status;
     }
     QuantiseArgs q{};
@@ -752,23 +995,23 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
     r.weights = static_cast<const std::uint8_t*>(a.packed), r.scales = a.scales, r.bias = a.bias;
     r.codes = q.codes, r.row_scales = q.scales, r.arranged = arranged;
     r.rows = a.tokens, r.out_rows = p.out_rows;
-    r.outputs = a.outputs, r.tiles = tiles_of(a.outputs), r.k_blocks = q.k_blocks;
-    r.tile_rows = p.tile_rows;
-    const std::int64_t items = p.tiles * r.tiles;
-    r.splits = splits_of(items, r.tile_rows, r.k_blocks);
+    r.experts = a.experts, r.outputs = a.outputs, r.tiles = tiles_of(a.outputs), r.k_blocks = q.k_blocks;
+    r.tile_rows = p.shape.tile_rows;
+    const std::int64_t items = p.tiles * (p.shape.pair ? (r.tiles + 1) / 2 : r.tiles);
+    r.splits = p.shape.pair ? 1 : splits_of(items, r.tile_rows, r.k_blocks);
     r.status = a.status;
     if (a.choices == nullptr) {
         r.y = a.y;
-        return product<false>(a.type, r, items, stream);
+        return product<false>(a.type, r, items, p.shape.pair, stream);
     }
     if (a.weights == nullptr) {
         r.y = a.y;
-        return product<true>(a.type, r, items, stream);
+        return product<true>(a.type, r, items, p.shape.pair, stream);
     }
     auto* products = reinterpret_cast<float*>(memory + p.products);
     r.y = products;
     // FP32 products, so that a token's sum is rounded once
-    status = product<true>(Type::f32, r, items, stream);
+    status = product<true>(Type::f32, r, items, p.shape.pair, stream);
     if (status != cudaSuccess) return status;
     switch (a.type) {
     case Type::f16: return combine<__half>(a, products, stream);

@@ -157,6 +157,48 @@ static __device__ __forceinline__ void mma_commit(std::uint32_t bar) {
                  : "memory");
 }
 
+// The same by the two blocks of a cluster on one tile of 256 rows of A: issued by the first block's thread, block i
+// holding rows 128 i .. 128 i + 127 of A and of the accumulator, and half of B's rows.
+static __device__ __forceinline__ std::uint32_t i8_pair_instruction(int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<std::uint32_t>(n >> 3) << 17) | (static_cast<std::uint32_t>(256 >> 4) << 24);
+}
+
+static __device__ __forceinline__ void mma_i8_pair(std::uint32_t d_tmem, std::uint64_t a, std::uint64_t b, std::uint32_t idesc,
+                                            std::uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrives on the barrier at this place in both blocks.
+static __device__ __forceinline__ void mma_commit_pair(std::uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(static_cast<std::uint16_t>(3))
+        : "memory");
+}
+
+// Arrive (count one) on the barrier at this place in block `rank` of the cluster.
+static __device__ __forceinline__ void barrier_arrive_at(std::uint32_t bar, std::uint32_t rank) {
+    asm volatile(
+        "{\n\t.reg .b32 there;\n\tmapa.shared::cluster.u32 there, %0, %1;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [there];\n\t}" ::"r"(bar),
+        "r"(rank)
+        : "memory");
+}
+
+// A TMA copy into this block's memory whose bytes the barrier at this place in the pair's first block counts (a shared
+// address's bit 24 tells the two blocks apart).
+static __device__ __forceinline__ void tma_load_2d_pair(std::uint32_t dst, const CUtensorMap* map, std::uint32_t bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<std::uint64_t>(map)), "r"(bar & 0xFEFFFFFFu), "r"(x), "r"(y)
+        : "memory");
+}
+
 static __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 static __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 

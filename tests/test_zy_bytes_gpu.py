@@ -117,6 +117,14 @@ def test_matrix_shapes(cuda, inputs, outputs):
     check_matrix(5, inputs, outputs, TYPES[(inputs + outputs) % 3], bias=True)
 
 
+@pytest.mark.parametrize("name", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows,inputs,outputs", [(2000, 1024, 4096), (2049, 900, 5000), (1111, 128, 16400), (4096, 4096, 2048),
+                                                 (5000, 2000, 1130)])
+def test_matrix_of_many_rows(cuda, rows, inputs, outputs, name):
+    """Sizes at which two blocks share a tile, with odd numbers of tiles and last tiles of a few rows."""
+    check_matrix(rows, inputs, outputs, name, bias=rows % 2 == 1)
+
+
 @pytest.mark.parametrize("rows,inputs,outputs", [
     (1, 4096, 4096), (16, 4096, 16384), (40, 16384, 1024), (64, 8192, 700), (512, 1024, 4096), (700, 512, 3000),
     (2048, 2048, 2048), (4099, 640, 1111), (3, 131072, 260)])
@@ -295,7 +303,8 @@ def test_experts_forms(cuda, kind, rows_each, weighted, name):
 
 @pytest.mark.parametrize("tokens,chosen,experts,inputs,outputs", [
     (1, 1, 1, 1, 1), (1, 8, 64, 2048, 1024), (1, 2, 1024, 64, 130), (7, 8, 8, 128, 128), (64, 8, 128, 256, 300),
-    (1000, 2, 5, 129, 257), (2048, 4, 16, 512, 384), (5000, 1, 1000, 100, 50), (300, 6, 33, 1000, 520), (16, 1, 2, 4096, 64)])
+    (1000, 2, 5, 129, 257), (2048, 4, 16, 512, 384), (5000, 1, 1000, 100, 50), (300, 6, 33, 1000, 520), (16, 1, 2, 4096, 64),
+    (4000, 4, 8, 512, 1500), (6000, 2, 16, 1000, 1024), (2001, 8, 5, 256, 2100)])
 def test_experts_shapes(cuda, tokens, chosen, experts, inputs, outputs):
     check_experts(normal((tokens, inputs), 1).bfloat16(), some_codes((experts, outputs, inputs), 3),
                   normal((experts, outputs), 4, 0.01).abs(), some_choices(tokens, chosen, experts, 5),
