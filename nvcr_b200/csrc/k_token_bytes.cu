@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace nvcr_sm100::token {
 namespace {
@@ -69,6 +70,7 @@ __global__ void __launch_bounds__(arrange_threads) arrange_kernel(const std::int
     const int thread = threadIdx.x, lane = thread % 32, warp = thread / 32;
     for (int e = thread; e < experts; e += arrange_threads) counts[e] = 0;
     __syncthreads();
+#pragma unroll 4
     for (std::int64_t i = thread; i < pairs; i += arrange_threads) {
         const int e = choices[i];
         if (e >= 0 && e < experts) atomicAdd(&counts[e], 1);
@@ -101,6 +103,7 @@ __global__ void __launch_bounds__(arrange_threads) arrange_kernel(const std::int
         __syncthreads();
     }
     if (thread == 0) *out.tile_count = first_tile;
+#pragma unroll 4
     for (std::int64_t i = thread; i < pairs; i += arrange_threads) {
         const int e = choices[i];
         int row = -1;
@@ -130,63 +133,127 @@ struct QuantiseArgs {
     int outputs;
 };
 
-// Warps warps a row, a thread 16 values at a time, of which the first `held` stay in registers between the row's
-// maximum and its codes; longer rows are read again.
-template <typename T, int Warps>
+// Sixteen values of a row as they are in memory.
+template <typename T>
+struct Sixteen {
+    uint4 words[sizeof(T)];
+    __device__ __forceinline__ void load(const T* row, int at, int inputs, bool vector) {
+        if (vector && at + 16 <= inputs) {
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) words[i] = reinterpret_cast<const uint4*>(row + at)[i];
+        } else {
+            unsigned made[4 * sizeof(T)];
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(4 * sizeof(T)); ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    made[i] = at + i < inputs ? __float_as_uint(row[at + i]) : 0u;
+                } else {
+                    const auto* bits = reinterpret_cast<const std::uint16_t*>(row);
+                    const unsigned low = at + 2 * i < inputs ? bits[at + 2 * i] : 0u, high = at + 2 * i + 1 < inputs ? bits[at + 2 * i + 1] : 0u;
+                    made[i] = low | high << 16;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) words[i] = {made[4 * i], made[4 * i + 1], made[4 * i + 2], made[4 * i + 3]};
+        }
+    }
+    __device__ __forceinline__ unsigned word(int i) const {
+        const uint4& w = words[i / 4];
+        return i % 4 == 0 ? w.x : i % 4 == 1 ? w.y : i % 4 == 2 ? w.z : w.w;
+    }
+    // The largest magnitude's bits so far, by halves for 16-bit types: magnitudes are ordered as their bits are, infinities
+    // and then NaNs above all.
+    __device__ __forceinline__ unsigned largest(unsigned so_far) const {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(4 * sizeof(T)); ++i) {
+            if constexpr (sizeof(T) == 4) {
+                so_far = max(so_far, word(i) & 0x7fffffffu);
+            } else {
+                so_far = __vmaxu2(so_far, word(i) & 0x7fff7fffu);
+            }
+        }
+        return so_far;
+    }
+    __device__ __forceinline__ void values(float (&v)[16]) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(word(i));
+            } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                v[i] = __uint_as_float(i % 2 == 0 ? word(i / 2) << 16 : word(i / 2) & 0xffff0000u);
+            } else {
+                v[i] = half_bits(static_cast<std::uint16_t>(word(i / 2) >> (i % 2 * 16)));
+            }
+        }
+    }
+};
+
+// Warps warps a row, a thread 16 values at a time, of which the first Held stay in registers between the row's maximum and
+// its codes; longer rows are read again. One warp a row, with the whole of it in registers, where there are rows for all
+// warps of an SM: 8192 x 4096 BF16 30 -> @@ us.
+template <typename T, int Warps, int Held>
 __global__ void __launch_bounds__(256) quantise_kernel(QuantiseArgs a) {
-    constexpr int threads = Warps * 32, held = 2;
-    __shared__ float largest[8];
+    constexpr int threads = Warps * 32;
+    __shared__ unsigned maxima[8];
     join_chain();
     const int part = threadIdx.x % threads;
     const std::int64_t row = blockIdx.x * static_cast<std::int64_t>(8 / Warps) + threadIdx.x / threads;
     const bool there = row < a.rows;
     const T* x = static_cast<const T*>(a.x);
-    if (there) x += row / a.inner * a.stride + row % a.inner * a.inner_stride;
+    if (there) x += a.inner == 1 ? row * a.stride : row / a.inner * a.stride + row % a.inner * a.inner_stride;
     const int pieces = a.k_blocks * (block_bytes / 16);
-    float kept[held][16];
-    float most = 0.0f;
+    Sixteen<T> kept[Held];
+    unsigned largest = 0;
 #pragma unroll
-    for (int h = 0; h < held; ++h) {
-        const int piece = part + h * threads;
-        if (there && piece < pieces) {
-            load_sixteen(x, piece * 16, a.inputs, a.vector, kept[h]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) most = max_nan(most, fabsf(kept[h][i]));
-        }
-    }
-    for (int piece = part + held * threads; there && piece < pieces; piece += threads) {
-        float v[16];
-        load_sixteen(x, piece * 16, a.inputs, a.vector, v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) most = max_nan(most, fabsf(v[i]));
+    for (int h = 0; h < Held; ++h) {
+        if (there && part + h * threads < pieces) kept[h].load(x, (part + h * threads) * 16, a.inputs, a.vector);
     }
 #pragma unroll
-    for (int offset = 16; offset > 0; offset /= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, offset));
+    for (int h = 0; h < Held; ++h) {
+        if (there && part + h * threads < pieces) largest = kept[h].largest(largest);
+    }
+#pragma unroll 1
+    for (int piece = part + Held * threads; there && piece < pieces; piece += threads) {
+        Sixteen<T> v;
+        v.load(x, piece * 16, a.inputs, a.vector);
+        largest = v.largest(largest);
+    }
+    if constexpr (sizeof(T) == 2) largest = max(largest >> 16, largest & 0xffffu);
+    largest = __reduce_max_sync(0xffffffffu, largest);
     if constexpr (Warps > 1) {
-        if (threadIdx.x % 32 == 0) largest[threadIdx.x / 32] = most;
+        if (threadIdx.x % 32 == 0) maxima[threadIdx.x / 32] = largest;
         __syncthreads();
         const int first = threadIdx.x / threads * Warps;
 #pragma unroll
-        for (int w = 0; w < Warps; ++w) most = max_nan(most, largest[first + w]);
+        for (int w = 0; w < Warps; ++w) largest = max(largest, maxima[first + w]);
     }
     if (!there) return;
+    float most;
+    if constexpr (sizeof(T) == 4) {
+        most = __uint_as_float(largest);
+    } else {
+        const auto bits = static_cast<std::uint16_t>(largest);
+        most = widen(reinterpret_cast<const T&>(bits));
+    }
     const RowScale scale(most);
-    auto store = [&](const float (&v)[16], int piece) {
+    auto store = [&](const Sixteen<T>& sixteen, int piece) {
+        float v[16];
+        sixteen.values(v);
         const uint4 words = scale.codes(v);
+        std::uint8_t* block = a.codes + piece / 8 * a.out_rows * block_bytes;
         for (int f = 0; f < a.fan; ++f) {
             const std::int64_t to = a.place == nullptr ? row : a.place[row * a.fan + f];
-            if (to < 0) continue;
-            uint4* at = reinterpret_cast<uint4*>(a.codes + (piece / 8 * a.out_rows + to) * block_bytes);
-            at[(piece % 8) ^ static_cast<int>(to & 7)] = words;
+            if (to >= 0) reinterpret_cast<uint4*>(block + to * block_bytes)[(piece % 8) ^ static_cast<int>(to & 7)] = words;
         }
     };
 #pragma unroll
-    for (int h = 0; h < held; ++h) {
+    for (int h = 0; h < Held; ++h) {
         if (part + h * threads < pieces) store(kept[h], part + h * threads);
     }
-    for (int piece = part + held * threads; piece < pieces; piece += threads) {
-        float v[16];
-        load_sixteen(x, piece * 16, a.inputs, a.vector, v);
+#pragma unroll 1
+    for (int piece = part + Held * threads; piece < pieces; piece += threads) {
+        Sixteen<T> v;
+        v.load(x, piece * 16, a.inputs, a.vector);
         store(v, piece);
     }
     for (int f = part; f < a.fan; f += threads) {
@@ -274,16 +341,16 @@ struct Tile {
 
 // Tiles of one group of rows after another; with Pair the outputs are those of two blocks.
 template <bool Experts, bool Pair = false>
-__device__ __forceinline__ Tile tile_at(const ProductArgs& a, std::int64_t item) {
+__device__ __forceinline__ Tile tile_at(const ProductArgs& a, int item) {
     const int tiles = Pair ? (a.tiles + 1) / 2 : a.tiles;
-    const std::int64_t nth = item / tiles;
+    const int nth = item / tiles;
     Tile t;
-    t.output = static_cast<int>(item - nth * tiles) * (Pair ? 2 * block_rows : block_rows);
+    t.output = (item - nth * tiles) * (Pair ? 2 * block_rows : block_rows);
     if constexpr (Experts) {
         const int4 found = a.arranged.tiles[nth];
         t.expert = found.x, t.row = found.y, t.rows = found.z;
     } else {
-        t.expert = 0, t.row = nth * a.tile_rows;
+        t.expert = 0, t.row = static_cast<std::int64_t>(nth) * a.tile_rows;
         t.rows = static_cast<int>(min(static_cast<std::int64_t>(a.tile_rows), a.rows - t.row));
     }
     constexpr int step = Pair ? pair_step_rows : step_rows;
@@ -311,9 +378,19 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, const Tile& t, 
     const float bias = inside && a.bias != nullptr ? widen(static_cast<const T*>(a.bias)[channel]) : 0.0f;
     T* y = static_cast<T*>(a.y) + output;
     if constexpr (!Experts) y += t.row * a.outputs;
+    int ahead[16];  // the next columns, under way while the ones before are scaled
+    if (half * 16 < t.columns) tmem_load16(sums + static_cast<std::uint32_t>(half * 16), ahead);
+#pragma unroll 1
     for (int column = half * 16; column < t.columns; column += 32) {
         int acc[16];
-        tmem_load16(sums + static_cast<std::uint32_t>(column), acc);
+        tmem_load_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            acc[i] = ahead[i];
+            asm volatile("" : "+r"(acc[i]));  // not read before the wait
+        }
+        if (column + 32 < t.columns) tmem_load16(sums + static_cast<std::uint32_t>(column + 32), ahead);
+        if (!inside) continue;
         float row_scale[16];
         int row[16];
 #pragma unroll
@@ -325,8 +402,6 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, const Tile& t, 
                 row[4 * i] = r.x, row[4 * i + 1] = r.y, row[4 * i + 2] = r.z, row[4 * i + 3] = r.w;
             }
         }
-        tmem_load_wait();
-        if (!inside) continue;
         T* to = y + static_cast<std::int64_t>(column) * a.outputs;
         auto value = [&](int i) {
             const float v = __fmul_rn(__fmul_rn(__int2float_rn(acc[i]), scale), row_scale[i]);
@@ -349,6 +424,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, const Tile& t, 
             }
         }
     }
+    tmem_load_wait();
 }
 
 // A block takes tiles of 128 outputs by tile_rows rows one after another: four warps copy blocks of weights and rows into a
@@ -369,7 +445,7 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int splits = a.splits;
     const int rank = static_cast<int>(blockIdx.x) % splits;
-    const std::int64_t first_item = blockIdx.x / splits, item_step = gridDim.x / splits;
+    const int first_item = static_cast<int>(blockIdx.x) / splits, item_step = static_cast<int>(gridDim.x) / splits;
     const int k_from = static_cast<int>(static_cast<std::int64_t>(a.k_blocks) * rank / splits);
     const int k_to = static_cast<int>(static_cast<std::int64_t>(a.k_blocks) * (rank + 1) / splits);
 
@@ -403,22 +479,24 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
     unsigned* waits = &tail.status;
     launch_dependents();
     if (Experts || warp < copy_warp || warp >= copy_warp + copy_warps) grid_dependency_wait();
-    std::int64_t items = 0;
+    int items = 0;
     if (Experts) {
-        items = *a.arranged.tile_count * static_cast<std::int64_t>(a.tiles);
+        items = *a.arranged.tile_count * a.tiles;
     } else {
-        items = (a.rows + a.tile_rows - 1) / a.tile_rows * a.tiles;
+        items = static_cast<int>((a.rows + a.tile_rows - 1) / a.tile_rows) * a.tiles;
     }
 
     if (warp >= copy_warp && warp < copy_warp + copy_warps) {
         // The block's copies are numbered q = 0, 1, ..., a block of inputs each, tile after tile; this warp has every
-        // fourth one. Those that fill the ring go out a lane each, the later ones a lane an operand.
+        // fourth one. Those that fill the ring go out a lane each, the later ones a lane an operand. (There are four stages
+        // at least: a warp that ran ahead by two uses of a stage would take the parity of its barrier's phase before last for
+        // the last one's.)
         const int blocks = k_to - k_from;
-        const std::int64_t mine = first_item < items ? (items - first_item + item_step - 1) / item_step * blocks : 0;
+        const std::int64_t mine = first_item < items ? static_cast<std::int64_t>((items - first_item + item_step - 1) / item_step) * blocks : 0;
         auto of = [&](std::int64_t q, std::uint32_t& bytes, const std::uint8_t*& weights, const std::uint8_t*& rows) {
             const std::int64_t nth = q / blocks;
             const int k = k_from + static_cast<int>(q - nth * blocks);
-            const Tile t = tile_at<Experts>(a, first_item + nth * item_step);
+            const Tile t = tile_at<Experts>(a, first_item + static_cast<int>(nth) * item_step);
             bytes = static_cast<std::uint32_t>(t.columns) * block_bytes;
             weights = a.weights + ((static_cast<std::int64_t>(t.expert) * a.tiles + t.output / block_rows) * a.k_blocks + k) * weight_block;
             rows = a.codes + (t.row + k * a.out_rows) * block_bytes;
@@ -478,20 +556,21 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
         if (lane == 0) {
             int slot = 0, buffer = 0;
             std::uint32_t phase = 0, pass = 0;
-            for (std::int64_t item = first_item; item < items && !*abort; item += item_step) {
-                const Tile t = tile_at<Experts>(a, item);
+            const std::uint64_t first_weights = sw128_descriptor(ring), first_rows = sw128_descriptor(rows_ring);
+            Tile next = first_item < items ? tile_at<Experts>(a, first_item) : Tile{};
+            for (int item = first_item; item < items && !*abort; item += item_step) {
+                const Tile t = next;
+                if (items - item > item_step) next = tile_at<Experts>(a, item + item_step);  // its latency under this one's products
                 const std::uint32_t instruction = i8_instruction(t.columns);
-                if (!barrier_wait(smem_address(&tail.tmem_empty[buffer]), pass ^ 1u, waits)) *abort = 1;
+                bool going = barrier_wait(smem_address(&tail.tmem_empty[buffer]), pass ^ 1u, waits);
                 tmem_fence_after();
                 const std::uint32_t sums = tmem + static_cast<std::uint32_t>(buffer * a.tile_rows);
-                for (int k = k_from; k < k_to && !*abort; ++k) {
-                    if (!barrier_wait(smem_address(&tail.full[slot]), phase, waits)) {
-                        *abort = 1;
-                        break;
-                    }
+                for (int k = k_from; going && k < k_to; ++k) {
+                    going = barrier_wait(smem_address(&tail.full[slot]), phase, waits);
+                    if (!going) break;
                     tmem_fence_after();
-                    const std::uint64_t w = sw128_descriptor(ring + slot * weight_block);
-                    const std::uint64_t x = sw128_descriptor(rows_ring + slot * row_bytes);
+                    const std::uint64_t w = first_weights + static_cast<std::uint64_t>(slot * (weight_block >> 4));
+                    const std::uint64_t x = first_rows + static_cast<std::uint64_t>(slot * (static_cast<int>(row_bytes) >> 4));
 #pragma unroll
                     for (int step = 0; step < block_bytes / 32; ++step) {
                         mma_i8(sums, w + 2 * step, x + 2 * step, instruction, k > k_from || step > 0);
@@ -499,7 +578,11 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
                     mma_commit(smem_address(&tail.empty[slot]));
                     if (++slot == a.stages) slot = 0, phase ^= 1u;
                 }
-                if (!*abort) mma_commit(smem_address(&tail.tmem_full[buffer]));
+                if (going) {
+                    mma_commit(smem_address(&tail.tmem_full[buffer]));
+                } else {
+                    *abort = 1;
+                }
                 if (++buffer == 2) buffer = 0, pass ^= 1u;
             }
             if (*abort) {  // the MMAs under way
@@ -512,7 +595,7 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
         int buffer = 0;
         std::uint32_t pass = 0;
         if (splits > 1) cluster_wait();
-        for (std::int64_t item = first_item; item < items; item += item_step) {
+        for (int item = first_item; item < items; item += item_step) {
             const Tile t = tile_at<Experts>(a, item);
             if (splits == 1) stage_rows<Experts>(a, t, tail, buffer);
             if (epilogue_any(*abort != 0)) break;  // all of them, as the next ones wait for one another here
@@ -579,7 +662,11 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
 // rows in its shared memory, which the tensor cores of both read. A block of 128 inputs so takes 32 KB a block in place of
 // 48, where 128 x 256 tiles loaded 66 bytes a cycle and SM, which is all that L2 gave. The copies of both blocks count on
 // the first one's barriers, whose thread issues the MMAs: a thread that told it of the second one's, by an arrival with
-// release, took 1300 cycles a block of inputs.
+// release, took 1300 cycles a block of inputs. A stage of the ring holds two blocks of inputs, as a wait, four MMAs and a
+// commit take that thread 690 cycles, and the tensor cores 512.
+constexpr int pair_blocks = 2;                                // of inputs a stage
+constexpr unsigned copy_lanes = (2u << pair_blocks) - 1;      // of a copying warp
+
 template <typename T, bool Experts>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) pair_kernel(
     const __grid_constant__ CUtensorMap weights_map, const __grid_constant__ CUtensorMap codes_map, const ProductArgs a) {
@@ -587,11 +674,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
     __shared__ ProductTail tail;
     const std::uint32_t ring = (smem_address(dynamic) + 1023u) & ~1023u;
     const std::uint32_t row_bytes = static_cast<std::uint32_t>(a.tile_rows) / 2 * block_bytes;
-    const std::uint32_t rows_ring = ring + static_cast<std::uint32_t>(a.stages) * weight_block;
+    const std::uint32_t rows_ring = ring + static_cast<std::uint32_t>(a.stages) * pair_blocks * weight_block;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = static_cast<int>(blockIdx.x) % 2;
-    const std::int64_t first_item = blockIdx.x / 2, item_step = gridDim.x / 2;
-    const int blocks = a.k_blocks;
+    const int first_item = static_cast<int>(blockIdx.x) / 2, item_step = static_cast<int>(gridDim.x) / 2;
+    const int blocks = a.k_blocks, groups = (blocks + pair_blocks - 1) / pair_blocks;
 
     if (warp == copy_warp && lane == 0) {
         for (int s = 0; s < a.stages; ++s) {
@@ -624,44 +711,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
     unsigned* waits = &tail.status;
     launch_dependents();
     grid_dependency_wait();
-    const std::int64_t row_tiles = Experts ? *a.arranged.tile_count : (a.rows + a.tile_rows - 1) / a.tile_rows;
-    const std::int64_t items = row_tiles * ((a.tiles + 1) / 2);
+    const int row_tiles = Experts ? *a.arranged.tile_count : static_cast<int>((a.rows + a.tile_rows - 1) / a.tile_rows);
+    const int items = row_tiles * ((a.tiles + 1) / 2);
 
     if (warp >= copy_warp && warp < copy_warp + copy_warps) {
-        const std::int64_t mine = first_item < items ? (items - first_item + item_step - 1) / item_step * blocks : 0;
-        if (lane < 2) {
-            std::int64_t nth = (warp - copy_warp) / blocks;
-            int k = (warp - copy_warp) % blocks, slot = (warp - copy_warp) % a.stages;
+        const std::int64_t mine = first_item < items ? static_cast<std::int64_t>((items - first_item + item_step - 1) / item_step) * groups : 0;
+        // No more warps take turns than there are stages: one that ran ahead by two uses of a stage would take the parity of
+        // its barrier's phase before last for the last one's.
+        const int turns = min(copy_warps, a.stages);
+        if (lane <= pair_blocks && warp - copy_warp < turns) {  // the first lane copies weights, the others a block of codes each
+            std::int64_t nth = (warp - copy_warp) / groups;
+            int group = (warp - copy_warp) % groups, slot = (warp - copy_warp) % a.stages;
             std::uint32_t pass = static_cast<std::uint32_t>((warp - copy_warp) / a.stages);
             bool moved = true;  // to another tile
             int from = 0;       // row of 128 bytes
             const CUtensorMap* map = lane == 0 ? &weights_map : &codes_map;
             const int step = lane == 0 ? block_rows : static_cast<int>(a.out_rows);
-            const std::uint32_t stage = 2 * (weight_block + row_bytes);  // of both blocks: boxes are whole, past the last row too
+            const std::uint32_t to = lane == 0 ? ring : rows_ring + (lane - 1) * row_bytes;
+            const std::uint32_t to_step = pair_blocks * (lane == 0 ? weight_block : row_bytes);
+            // of both blocks: boxes are whole, past the last row and the last block of inputs too (zeros past the codes' end)
+            const std::uint32_t stage = 2 * pair_blocks * (weight_block + row_bytes);
             std::int64_t q = warp - copy_warp;
-            for (; q < mine; q += copy_warps) {
+            for (; q < mine; q += turns) {
                 if (moved) {
-                    const Tile t = tile_at<Experts, true>(a, first_item + nth * item_step);
+                    const Tile t = tile_at<Experts, true>(a, first_item + static_cast<int>(nth) * item_step);
                     // past an odd last tile the second block's products are of no output
                     const std::int64_t tile = static_cast<std::int64_t>(t.expert) * a.tiles + min(t.output / block_rows + rank, a.tiles - 1);
-                    from = static_cast<int>(lane == 0 ? tile * blocks * block_rows : t.row + rank * (t.columns / 2));
+                    from = static_cast<int>(lane == 0 ? tile * blocks * block_rows
+                                                      : t.row + rank * (t.columns / 2) + static_cast<std::int64_t>(lane - 1) * a.out_rows);
                     moved = false;
                 }
                 bool free = true;
                 if (lane == 0) free = !*abort && barrier_wait(smem_address(&tail.empty[slot]), (pass & 1u) ^ 1u, waits);
-                if (!__shfl_sync(3u, free, 0)) {
+                if (!__shfl_sync(copy_lanes, free, 0)) {
                     *abort = 1;
                     break;
                 }
                 const std::uint32_t full = smem_address(&tail.full[slot]);
                 if (lane == 0 && rank == 0) barrier_expect_bytes(full, stage);
-                __syncwarp(3u);
-                tma_load_2d_pair(lane == 0 ? ring + slot * weight_block : rows_ring + slot * row_bytes, map, full, 0, from + k * step);
-                for (slot += copy_warps; slot >= a.stages; slot -= a.stages) ++pass;
-                for (k += copy_warps; k >= blocks; k -= blocks) ++nth, moved = true;
+                __syncwarp(copy_lanes);
+                tma_load_2d_pair(to + slot * to_step, map, full, 0, from + group * pair_blocks * step);
+                for (slot += turns; slot >= a.stages; slot -= a.stages) ++pass;
+                for (group += turns; group >= groups; group -= groups) ++nth, moved = true;
             }
-            if (*abort && lane == 0 && rank == 0) {  // the copies under way, the other block's too: of q - 4, q - 8, ...
-                for (std::int64_t last = q - copy_warps; last >= 0 && last > q - copy_warps - a.stages; last -= copy_warps) {
+            if (*abort && lane == 0 && rank == 0) {  // the copies under way, the other block's too
+                for (std::int64_t last = q - turns; last >= 0 && last > q - turns - a.stages; last -= turns) {
                     barrier_wait(smem_address(&tail.full[last % a.stages]), last / a.stages & 1, waits);
                 }
             }
@@ -671,28 +765,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
         if (lane == 0) {
             int slot = 0, buffer = 0;
             std::uint32_t phase = 0, pass = 0;
-            for (std::int64_t item = first_item; item < items && !*abort; item += item_step) {
-                const Tile t = tile_at<Experts, true>(a, item);
+            const std::uint64_t first_weights = sw128_descriptor(ring), first_rows = sw128_descriptor(rows_ring);
+            Tile next = first_item < items ? tile_at<Experts, true>(a, first_item) : Tile{};
+            for (int item = first_item; item < items && !*abort; item += item_step) {
+                const Tile t = next;
+                if (items - item > item_step) next = tile_at<Experts, true>(a, item + item_step);  // its latency under this one's products
                 const std::uint32_t instruction = i8_pair_instruction(t.columns);
-                if (!barrier_wait(smem_address(&tail.tmem_empty[buffer]), pass ^ 1u, waits)) *abort = 1;
+                bool going = barrier_wait(smem_address(&tail.tmem_empty[buffer]), pass ^ 1u, waits);
                 tmem_fence_after();
                 const std::uint32_t sums = tmem + static_cast<std::uint32_t>(buffer * a.tile_rows);
-                for (int k = 0; k < blocks && !*abort; ++k) {
-                    if (!barrier_wait(smem_address(&tail.full[slot]), phase, waits)) {
-                        *abort = 1;
-                        break;
-                    }
+                for (int k = 0; going && k < blocks; k += pair_blocks) {
+                    going = barrier_wait(smem_address(&tail.full[slot]), phase, waits);
+                    if (!going) break;
                     tmem_fence_after();
-                    const std::uint64_t w = sw128_descriptor(ring + slot * weight_block);
-                    const std::uint64_t x = sw128_descriptor(rows_ring + slot * row_bytes);
+                    const std::uint64_t w = first_weights + static_cast<std::uint64_t>(slot * (pair_blocks * weight_block >> 4));
+                    const std::uint64_t x = first_rows + static_cast<std::uint64_t>(slot * (pair_blocks * static_cast<int>(row_bytes) >> 4));
 #pragma unroll
-                    for (int step = 0; step < block_bytes / 32; ++step) {
-                        mma_i8_pair(sums, w + 2 * step, x + 2 * step, instruction, k > 0 || step > 0);
+                    for (int block = 0; block < pair_blocks; ++block) {
+                        if (k + block >= blocks) break;
+#pragma unroll
+                        for (int step = 0; step < block_bytes / 32; ++step) {
+                            mma_i8_pair(sums, w + static_cast<std::uint64_t>(block * (weight_block >> 4) + 2 * step),
+                                        x + static_cast<std::uint64_t>(block * (static_cast<int>(row_bytes) >> 4) + 2 * step), instruction,
+                                        k > 0 || block > 0 || step > 0);
+                        }
                     }
                     mma_commit_pair(smem_address(&tail.empty[slot]));
                     if (++slot == a.stages) slot = 0, phase ^= 1u;
                 }
-                if (!*abort) mma_commit_pair(smem_address(&tail.tmem_full[buffer]));
+                if (going) {
+                    mma_commit_pair(smem_address(&tail.tmem_full[buffer]));
+                } else {
+                    *abort = 1;
+                }
                 if (++buffer == 2) buffer = 0, pass ^= 1u;
             }
             if (*abort) {  // the MMAs under way
@@ -704,7 +809,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
         const int quarter = warp % 4, half = warp / 4;
         int buffer = 0;
         std::uint32_t pass = 0;
-        for (std::int64_t item = first_item; item < items; item += item_step) {
+        for (int item = first_item; item < items; item += item_step) {
             const Tile t = tile_at<Experts, true>(a, item);
             stage_rows<Experts>(a, t, tail, buffer);
             if (epilogue_any(*abort != 0)) break;  // all of them, as the next ones wait for one another here
@@ -734,35 +839,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
 
 // ---- y[t] = sum_j weights[t][j] * products[t][j], in the order of j ----
 
-template <typename T>
-__global__ void __launch_bounds__(256) combine_kernel(const float* products, const std::int32_t* choices, const float* weights,
+// A thread Each outputs: four where rows of outputs are whole vectors.
+template <typename T, int Each>
+__global__ void __launch_bounds__(128) combine_kernel(const float* products, const std::int32_t* choices, const float* weights,
                                                       int chosen, int experts, int outputs, T* y) {
     join_chain();
     const std::int64_t token = blockIdx.x;
-    const int output = static_cast<int>(blockIdx.y * 256 + threadIdx.x);
+    const int output = static_cast<int>(blockIdx.y * 128 + threadIdx.x) * Each;
     if (output >= outputs) return;
-    float sum = 0.0f;
+    float sum[Each] = {};
+#pragma unroll 4
     for (int j = 0; j < chosen; ++j) {
         const std::int64_t pair = token * chosen + j;
         const int e = choices[pair];
-        if (e >= 0 && e < experts) sum = fmaf(weights[pair], products[pair * outputs + output], sum);
+        if (e < 0 || e >= experts) continue;
+        const float weight = weights[pair];
+        const float* from = products + pair * outputs + output;
+        if constexpr (Each == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(from);
+            sum[0] = fmaf(weight, v.x, sum[0]), sum[1] = fmaf(weight, v.y, sum[1]);
+            sum[2] = fmaf(weight, v.z, sum[2]), sum[3] = fmaf(weight, v.w, sum[3]);
+        } else {
+            sum[0] = fmaf(weight, *from, sum[0]);
+        }
     }
-    y[token * outputs + output] = narrow<T>(sum);
+#pragma unroll
+    for (int i = 0; i < Each; ++i) y[token * outputs + output + i] = narrow<T>(sum[i]);
 }
 
 // ---- launches ----
 
-template <typename T, int Warps>
+template <typename T, int Warps, int Held>
 cudaError_t quantise_rows(const QuantiseArgs& a, cudaStream_t stream) {
     const std::int64_t blocks = (a.rows + 8 / Warps - 1) / (8 / Warps);
-    return launch_overlapped(quantise_kernel<T, Warps>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
+    return launch_overlapped(quantise_kernel<T, Warps, Held>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
 }
 
 template <typename T>
 cudaError_t quantise(const QuantiseArgs& a, cudaStream_t stream) {
-    if (a.inputs <= 1024) return quantise_rows<T, 1>(a, stream);
-    if (a.inputs <= 2048) return quantise_rows<T, 2>(a, stream);
-    return quantise_rows<T, 8>(a, stream);
+    constexpr int held = 16 / sizeof(T);  // 64 registers
+    const bool many = a.rows >= 8 * sm_count();
+    if (a.inputs <= 1024) return quantise_rows<T, 1, 2>(a, stream);
+    if (many && a.inputs <= 512 * held) return quantise_rows<T, 1, held>(a, stream);
+    if (a.inputs <= 2048) return quantise_rows<T, 2, 2>(a, stream);
+    return quantise_rows<T, 8, 2>(a, stream);
 }
 
 cudaError_t quantise(Type type, const QuantiseArgs& a, cudaStream_t stream) {
@@ -780,6 +900,7 @@ cudaError_t product(ProductArgs a, std::int64_t most_items, cudaStream_t stream)
     const int room = 208 * 1024 - exchange;
     const int stage = weight_block + a.tile_rows * block_bytes;
     a.stages = std::min(most_stages, room / stage);
+    if (a.stages < copy_warps) return cudaErrorInvalidValue;  // as the copying warps' turns need (at 256 rows there are four)
     a.tmem_columns = 32;
     while (a.tmem_columns < 2u * static_cast<unsigned>(a.tile_rows)) a.tmem_columns *= 2;
     const int bytes = a.stages * stage + exchange + 1024;
@@ -828,7 +949,7 @@ bool encode(CUtensorMap& map, const void* memory, std::uint64_t rows, int box) {
 template <typename T, bool Experts>
 cudaError_t pair_product(ProductArgs a, std::int64_t most_items, cudaStream_t stream) {
     static SharedAllowance allowance;
-    const int stage = weight_block + a.tile_rows / 2 * block_bytes;
+    const int stage = pair_blocks * (weight_block + a.tile_rows / 2 * block_bytes);
     a.stages = std::min(most_stages, 208 * 1024 / stage);
     a.tmem_columns = 32;
     while (a.tmem_columns < 2u * static_cast<unsigned>(a.tile_rows)) a.tmem_columns *= 2;
@@ -836,7 +957,7 @@ cudaError_t pair_product(ProductArgs a, std::int64_t most_items, cudaStream_t st
     if (status != cudaSuccess) return status;
     CUtensorMap weights, codes;
     const std::uint64_t blocks = static_cast<std::uint64_t>(a.arranged.tiles == nullptr ? 1 : a.experts) * a.tiles * a.k_blocks;
-    if (!encode(weights, a.weights, blocks * block_rows, block_rows) ||
+    if (!encode(weights, a.weights, blocks * block_rows, pair_blocks * block_rows) ||
         !encode(codes, a.codes, static_cast<std::uint64_t>(a.k_blocks) * a.out_rows, a.tile_rows / 2)) {
         return cudaErrorUnknown;
     }
@@ -939,9 +1060,11 @@ Plan plan_of(const BytesArgs& a) {
 
 template <typename T>
 cudaError_t combine(const BytesArgs& a, const float* products, cudaStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>((a.outputs + 255) / 256));
-    return launch_overlapped(combine_kernel<T>, grid, dim3(256), 0, stream, products, a.choices, a.weights, a.chosen,
-                             a.experts, a.outputs, static_cast<T*>(a.y));
+    const int each = a.outputs % 4 == 0 ? 4 : 1;
+    const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>((a.outputs + 128 * each - 1) / (128 * each)));
+    auto kernel = each == 4 ? combine_kernel<T, 4> : combine_kernel<T, 1>;
+    return launch_overlapped(kernel, grid, dim3(128), 0, stream, products, a.choices, a.weights, a.chosen, a.experts, a.outputs,
+                             static_cast<T*>(a.y));
 }
 
 }  // namespace
@@ -998,6 +1121,7 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
     r.experts = a.experts, r.outputs = a.outputs, r.tiles = tiles_of(a.outputs), r.k_blocks = q.k_blocks;
     r.tile_rows = p.shape.tile_rows;
     const std::int64_t items = p.tiles * (p.shape.pair ? (r.tiles + 1) / 2 : r.tiles);
+    if (items > INT32_MAX - 1024) return cudaErrorInvalidValue;  // tiles are counted in 32 bits
     r.splits = p.shape.pair ? 1 : splits_of(items, r.tile_rows, r.k_blocks);
     r.status = a.status;
     if (a.choices == nullptr) {
