@@ -556,11 +556,15 @@ int nvcr_sm100_token_route(int type, const void* scores, int64_t stride, int64_t
  * logit, the first of equal ones. Logits of -infinity and NaN are left out; a
  * row of nothing else gives -1 and 0. Weights are summed in multiples of 2^-43:
  * smaller ones are never chosen. temperatures, top_ks, top_ps and min_ps hold a
- * value a row; where one is NULL, every row has the value after it. */
+ * value a row; where one is NULL, every row has the value after it. The
+ * workspace's size (0 for a few rows) comes first; it is 16-byte aligned, and the
+ * call's own until it has run. */
+int nvcr_sm100_token_sample_workspace(int type, int64_t rows, int32_t symbols, size_t* bytes);
 int nvcr_sm100_token_sample(int type, const void* logits, int64_t stride, int64_t rows, int32_t symbols,
                             const float* uniforms, const float* temperatures, float temperature,
                             const int32_t* top_ks, int32_t top_k, const float* top_ps, float top_p, const float* min_ps,
-                            float min_p, int64_t* chosen, float* probabilities, void* stream);
+                            float min_p, int64_t* chosen, float* probabilities, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 #ifdef __cplusplus
 }

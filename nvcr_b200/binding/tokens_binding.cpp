@@ -499,11 +499,15 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t count) {
         const EachRow<float> min_p(args[5], "min_p", at::kFloat, rows, device);
         const at::Tensor chosen = at::empty({rows}, logits.options().dtype(at::kLong));
         const at::Tensor probabilities = at::empty({rows}, logits.options().dtype(at::kFloat));
+        std::size_t bytes = 0;
+        check(nvcr_sm100_token_sample_workspace(type, rows, static_cast<std::int32_t>(symbols), &bytes));
+        at::Tensor room;
+        if (bytes > 0) room = workspace(bytes, device, args[6]);
         check(nvcr_sm100_token_sample(type, from, logits.stride(0), rows, static_cast<std::int32_t>(symbols),
                                       static_cast<const float*>(uniforms), temperature.values, temperature.value,
                                       top_k.values, top_k.value, top_p.values, top_p.value, min_p.values, min_p.value,
                                       chosen.data_ptr<std::int64_t>(), probabilities.data_ptr<float>(),
-                                      stream_of(args[6], device)));
+                                      bytes > 0 ? room.data_ptr() : nullptr, bytes, stream_of(args[6], device)));
         return pair(chosen, probabilities);
     });
 }

@@ -481,19 +481,35 @@ int nvcr_sm100_token_route(int type, const void* scores, int64_t stride, int64_t
     });
 }
 
+int nvcr_sm100_token_sample_workspace(int type, int64_t rows, int32_t symbols, size_t* bytes) {
+    return guarded([&] {
+        if (bytes == nullptr) return refuse("null argument");
+        if (!any_type(type)) return refuse("unknown type");
+        if (rows < 0 || rows > most_rows) return refuse("rows out of range");
+        if (symbols <= 0 || symbols > token::most_symbols) return refuse("symbols must be 1 to 2^20");
+        *bytes = token::sample_workspace(static_cast<token::Type>(type), rows, symbols);
+        return report_ok();
+    });
+}
+
 int nvcr_sm100_token_sample(int type, const void* logits, int64_t stride, int64_t rows, int32_t symbols,
                             const float* uniforms, const float* temperatures, float temperature,
                             const int32_t* top_ks, int32_t top_k, const float* top_ps, float top_p, const float* min_ps,
-                            float min_p, int64_t* chosen, float* probabilities, void* stream) {
+                            float min_p, int64_t* chosen, float* probabilities, void* workspace, size_t workspace_bytes,
+                            void* stream) {
     return guarded([&] {
         if (!any_type(type)) return refuse("unknown type");
         if (rows < 0 || rows > most_rows) return refuse("rows out of range");
         if (symbols <= 0 || symbols > token::most_symbols) return refuse("symbols must be 1 to 2^20");
+        if (!aligned(workspace)) return refuse("the workspace must be 16-byte aligned");
+        const std::size_t needed = token::sample_workspace(static_cast<token::Type>(type), rows, symbols);
+        if (workspace_bytes < needed || (needed > 0 && workspace == nullptr)) return refuse("the workspace is too small");
         if (rows > 0 && (logits == nullptr || uniforms == nullptr || chosen == nullptr || probabilities == nullptr)) {
             return refuse("null logits, uniforms, chosen or probabilities");
         }
         return launched(token::sample({static_cast<token::Type>(type), logits, stride, rows, symbols, uniforms, temperatures,
-                                       top_ks, top_ps, min_ps, temperature, top_k, top_p, min_p, chosen, probabilities},
+                                       top_ks, top_ps, min_ps, temperature, top_k, top_p, min_p, chosen, probabilities,
+                                       workspace},
                                       static_cast<cudaStream_t>(stream)));
     });
 }

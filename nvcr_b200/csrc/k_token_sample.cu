@@ -7,16 +7,21 @@
 // first few equal to it. Weights are FP64 and summed as whole multiples of 2^-43 of the largest, so that no order of
 // sums changes a choice, and which symbol is chosen does not hang on a rounding to FP32.
 //
-// A cluster of up to eight blocks has a row in its registers, read once (`cluster_kernel`):
+// A few rows are a cluster's each, of up to eight blocks, which has the row in its registers, read once (`cluster_kernel`):
 // * Where the symbols that can be kept are few (`candidates`: by min_p, top_k or ten octaves below the largest), they go
 //   to the first block, which sorts them and ends the row (`finish`). The rest is summed in FP32 for top_p's whole; a
-//   choice that hangs on that sum's error is made again by `row_by_block`, exactly.
+//   choice that hangs on that sum's error is made again exactly.
 // * Where they are many, a histogram of weights or counts over the cluster says between which logits the threshold lies,
 //   and these are sorted (`find`); the choice is found by sums of each warp's runs (`locate`).
+// Many rows go through three launches whose blocks wait for no other: parts of rows, whose candidates and sums go to memory
+// (`part_kernel`); a block a row, which ends it (`end_kernel`); the rows that were not ended, a cluster each
+// (`rest_kernel`). 256 rows of 131072 took 58 us by clusters, whose blocks were idle while they waited for one another.
+//
 // Longer rows and infinite logits take `row_by_block`, which finds the threshold's bits from memory
 // with one block.
 #include "token_elements.cuh"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -69,6 +74,8 @@ __device__ __forceinline__ double share_of(unsigned key, const Row& row) {
     // below 2^-46, less than half a unit: none; so are symbols that are left out, and all but the largest at temperature 0
     return key == row.top ? unit : key != 0 && y > -46.0 * table_size ? found : 0.0;
 }
+// One copy of it for code that runs once a row.
+__device__ __noinline__ double share_once(unsigned key, const Row& row) { return share_of(key, row); }
 // Rounded to whole units: below 2^52 the sum's low bits.
 __device__ __forceinline__ Weight weight_of(double share) {
     return static_cast<Weight>(__double_as_longlong(share + 4503599627370496.0)) & 0xfffffffffffffull;
@@ -138,6 +145,7 @@ __device__ __forceinline__ Weight before(Weight mine, Weight* scratch, Weight& a
     __syncthreads();
     Weight earlier = 0;
     all = 0;
+#pragma unroll 4
     for (int w = 0; w < warps; ++w) {
         if (w < warp) earlier += scratch[w];
         all += scratch[w];
@@ -187,13 +195,13 @@ __device__ Threshold find_by_block(const T* logits, int symbols, const Row& row,
             if (!by_weight) {
                 atomicAdd(&sums.low[bin], 1u);
             } else if (key != kept.key) {  // those are added below
-                const Weight w = weight_of(share_of(key, row));
+                const Weight w = weight_of(share_once(key, row));
                 if (w != 0) add(sums, bin, w);
             }
         }
         __syncthreads();
         if (by_weight && threadIdx.x == 0 && kept.key != 0 && (shift == 32 || kept.key >> shift == prefix)) {
-            add(sums, kept.key >> next & ((1u << width) - 1), kept.ties * weight_of(share_of(kept.key, row)));
+            add(sums, kept.key >> next & ((1u << width) - 1), kept.ties * weight_of(share_once(kept.key, row)));
         }
         __syncthreads();
         pass(sums, above, wanted, [&](int bin) { return static_cast<Weight>(sums.high[bin]) << 32 | sums.low[bin]; });
@@ -204,7 +212,7 @@ __device__ Threshold find_by_block(const T* logits, int symbols, const Row& row,
         shift = next;
     }
     __syncthreads();
-    const Weight each = by_weight ? weight_of(share_of(prefix, row)) : 1;
+    const Weight each = by_weight ? weight_of(share_once(prefix, row)) : 1;
     return {prefix, static_cast<unsigned>((wanted - above + each - 1) / each)};
 }
 
@@ -234,10 +242,10 @@ __device__ __noinline__ void row_by_block(const SampleArgs& a, std::int64_t r, S
             Weight mine = 0, all;
             for (int i = threadIdx.x; i < symbols; i += threads) {
                 const unsigned key = key_of(widen(logits[i]));
-                if (key > kept.key) mine += weight_of(share_of(key, row));
+                if (key > kept.key) mine += weight_of(share_once(key, row));
             }
             before(mine, sums.scratch, all);
-            if (kept.key != 0) all += kept.ties * weight_of(share_of(kept.key, row));
+            if (kept.key != 0) all += kept.ties * weight_of(share_once(kept.key, row));
             kept = stricter(kept, find_by_block(logits, symbols, row, true, part_of(s.top_p, all), kept, sums));
         }
     }
@@ -252,7 +260,7 @@ __device__ __noinline__ void row_by_block(const SampleArgs& a, std::int64_t r, S
         for (int i = from; i < to; ++i) {
             const unsigned key = key_of(widen(logits[i]));
             if (key == 0 || key < kept.key || (key == kept.key && nth++ >= kept.ties)) continue;
-            const double share = share_of(key, row);
+            const double share = share_once(key, row);
             if (share >= row.least && !visit(i, share)) return;
         }
     };
@@ -368,6 +376,31 @@ struct Elements {
     }
 };
 
+// Logits at .. of a row, with -infinity outside it.
+template <typename T>
+__device__ __forceinline__ uint4 load_vector(const T* logits, int symbols, int at) {
+    using Of = Elements<T>;
+    constexpr int each = Of::each;
+            uint4 v = Of::none();
+            if (at >= 0 && at + each <= symbols) {
+                v = *reinterpret_cast<const uint4*>(logits + at);
+            } else if (at + each > 0 && at < symbols) {
+                unsigned words[4] = {v.x, v.y, v.z, v.w};
+    #pragma unroll
+                for (int i = 0; i < each; ++i) {
+                    if (at + i < 0 || at + i >= symbols) continue;
+                    if constexpr (sizeof(T) == 4) {
+                        words[i] = __float_as_uint(logits[at + i]);
+                    } else {
+                        const unsigned bits = reinterpret_cast<const std::uint16_t*>(logits)[at + i];
+                        words[i / 2] = i % 2 == 0 ? (words[i / 2] & 0xffff0000u) | bits : (words[i / 2] & 0xffffu) | bits << 16;
+                    }
+                }
+                v = {words[0], words[1], words[2], words[3]};
+            }
+            return v;
+}
+
 // What a cluster keeps: keys above `key`, and those equal to it up to index `last`.
 struct Kept {
     unsigned key;
@@ -377,7 +410,7 @@ struct Kept {
 
 // 2048 in falling order, by 512 threads: four neighbours a thread, so that only exchanges over 128 places and more pass
 // through shared memory.
-__device__ __forceinline__ void sort(unsigned long long* shared) {
+__device__ __noinline__ void sort(unsigned long long* shared) {
     static_assert(most_candidates == 4 * threads);
     unsigned long long v[4];
     const int base = 4 * static_cast<int>(threadIdx.x);
@@ -452,28 +485,8 @@ struct ClusterRow {
     int vectors;  // of this thread
     int first;    // index of this thread's first element: of its n-th vector first + n * threads * each
 
-    // A vector, with -infinity outside the row.
     __device__ __forceinline__ uint4 load(int n) const {
-        const T* logits = static_cast<const T*>(a.logits) + r * a.stride;
-        const int at = first + n * threads * each;
-        uint4 v = Of::none();
-        if (at >= 0 && at + each <= a.symbols) {
-            v = *reinterpret_cast<const uint4*>(logits + at);
-        } else if (at + each > 0 && at < a.symbols) {
-            unsigned words[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < each; ++i) {
-                if (at + i < 0 || at + i >= a.symbols) continue;
-                if constexpr (sizeof(T) == 4) {
-                    words[i] = __float_as_uint(logits[at + i]);
-                } else {
-                    const unsigned bits = reinterpret_cast<const std::uint16_t*>(logits)[at + i];
-                    words[i / 2] = i % 2 == 0 ? (words[i / 2] & 0xffff0000u) | bits : (words[i / 2] & 0xffffu) | bits << 16;
-                }
-            }
-            v = {words[0], words[1], words[2], words[3]};
-        }
-        return v;
+        return load_vector(static_cast<const T*>(a.logits) + r * a.stride, a.symbols, first + n * threads * each);
     }
 
     // body(n, vector) for each, four loads at a time under way.
@@ -792,7 +805,7 @@ const int n = cell / warps;
         __syncwarp();
         const unsigned long long one = shared.weights[lane], two = shared.weights[lane + 32];
         int place_one = 0, place_two = 0;
-#pragma unroll 4
+#pragma unroll 2
         for (int k = 0; k < all_count; ++k) {
             const unsigned long long other = shared.weights[k];
             place_one += other > one, place_two += other > two;
@@ -839,7 +852,7 @@ const int n = cell / warps;
         shared.weights[2 * lane] = w[0], shared.weights[2 * lane + 1] = w[1];
         __syncwarp();
         Weight lower[2] = {0, 0};  // of those with lower indexes, whose complements are larger
-#pragma unroll 4
+#pragma unroll 2
         for (int k = 0; k < n; ++k) {
             const unsigned other = static_cast<unsigned>(shared.sorted[k]);
             const Weight weight = shared.weights[k];
@@ -863,19 +876,17 @@ const int n = cell / warps;
         if (threadIdx.x == 0) shared.kept = shared.low = shared.high = 0;
         int n = collect(counts, part);
         if (s.top_k > 0) n = min(n, s.top_k);
-        constexpr int most_each = most_candidates / threads;
         const int run = (n + threads - 1) / threads, from = static_cast<int>(threadIdx.x) * run;
-        Weight mine[most_each], sum = 0, all;
+        const int until = min(n, from + run);
+        Weight sum = 0, all;
         unsigned kept = 0;
-#pragma unroll
-        for (int i = 0; i < most_each; ++i) {
-            mine[i] = 0;
-            if (i < run && from + i < n) {
-                const double share = share_of(static_cast<unsigned>(shared.sorted[from + i] >> 32), row);
-                mine[i] = weight_of(share);
-                kept += share >= row.least;
-            }
-            sum += mine[i];
+#pragma unroll 1
+        for (int i = from; i < until; ++i) {
+            const double share = share_once(static_cast<unsigned>(shared.sorted[i] >> 32), row);
+            const Weight w = weight_of(share);
+            shared.weights[i] = w;
+            kept += share >= row.least;
+            sum += w;
         }
         Weight to = before(sum, shared.sums.scratch, all);
         double least_part = 0.0, most_part = 0.0;
@@ -884,14 +895,12 @@ const int n = cell / warps;
             least_part = p * (static_cast<double>(all) + bulk - slack), most_part = p * (static_cast<double>(all) + bulk + slack);
         }
         unsigned low = 0, high = 0;
-#pragma unroll
-        for (int i = 0; i < most_each; ++i) {
-            if (i < run && from + i < n) {
-                to += mine[i];
-                shared.weights[from + i] = to;
-                low += static_cast<double>(to) < least_part;
-                high += static_cast<double>(to) < most_part;
-            }
+#pragma unroll 1
+        for (int i = from; i < until; ++i) {
+            to += shared.weights[i];
+            shared.weights[i] = to;
+            low += static_cast<double>(to) < least_part;
+            high += static_cast<double>(to) < most_part;
         }
         kept = __reduce_add_sync(0xffffffffu, kept);
         low = __reduce_add_sync(0xffffffffu, low), high = __reduce_add_sync(0xffffffffu, high);
@@ -910,7 +919,7 @@ const int n = cell / warps;
         const Weight wanted = part_of_uniform(s.uniform, whole_kept);
         auto choose = [&](unsigned long long entry) {
             a.chosen[r] = static_cast<std::int64_t>(~static_cast<unsigned>(entry));
-            a.probabilities[r] = probability_of(share_of(static_cast<unsigned>(entry >> 32), row), whole_kept);
+            a.probabilities[r] = probability_of(share_once(static_cast<unsigned>(entry >> 32), row), whole_kept);
         };
         auto weight_at = [&](int i) { return shared.weights[i] - (i == 0 ? 0 : shared.weights[i - 1]); };
         if (n <= threads) {  // the weight of those with lower indexes, for each
@@ -929,20 +938,17 @@ const int n = cell / warps;
             shared.gathered[i] = i < n ? (shared.sorted[i] & 0xffffffffull) << 32 | static_cast<unsigned>(i) : 0ull;
         }
         sort(shared.gathered);
-        const int start = static_cast<int>(threadIdx.x) * most_each;
+        const int start = static_cast<int>(threadIdx.x) * (most_candidates / threads), stop = min(n, start + most_candidates / threads);
         sum = 0;
-#pragma unroll
-        for (int i = 0; i < most_each; ++i) {
-            mine[i] = start + i < n ? weight_at(static_cast<int>(shared.gathered[start + i] & 0xffffffffull)) : 0;
-            sum += mine[i];
-        }
+#pragma unroll 1
+        for (int i = start; i < stop; ++i) sum += weight_at(static_cast<int>(shared.gathered[i] & 0xffffffffull));
         to = before(sum, shared.sums.scratch, all);
-#pragma unroll
-        for (int i = 0; i < most_each; ++i) {
-            if (start + i < n && wanted >= to && wanted < to + mine[i]) {
-                choose(shared.sorted[static_cast<unsigned>(shared.gathered[start + i])]);
-            }
-            to += mine[i];
+#pragma unroll 1
+        for (int i = start; i < stop; ++i) {
+            const int at = static_cast<int>(shared.gathered[i] & 0xffffffffull);
+            const Weight w = weight_at(at);
+            if (wanted >= to && wanted < to + w) choose(shared.sorted[at]);
+            to += w;
         }
         return true;
     }
@@ -1109,6 +1115,292 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
     cluster_sync();  // no block ends while another one reads its memory
 }
 
+// ---- many rows ----
+
+constexpr int part_threads = 256;
+constexpr int part_vectors = 8;    // a thread
+constexpr int part_candidates = 2048;
+
+// What `part_kernel` tells of a part of a row.
+struct Part {
+    unsigned top;    // the largest key
+    float cut;       // the least logit of its candidates
+    unsigned count;  // of them; past part_candidates some are missing
+    float rest;      // the others' weights, the part's largest one's as one
+};
+
+struct ManyArgs {
+    int parts;  // a row
+    Part* told;
+    unsigned long long* candidates;  // [row][part][part_candidates]: a key and the complement of an index
+    unsigned* left;                  // how many rows `end_kernel` has left, and which
+};
+
+// What a row's settings ask for, the largest logit known.
+struct Wishes {
+    bool greedy, by_count, by_part;
+    int top_k;
+    float factor;  // octaves a logit
+    bool ordinary; // FP32 exponents will do
+    bool few;      // candidates can be told
+};
+__device__ __forceinline__ Wishes wishes_of(const SampleArgs& a, const Settings& s, float largest) {
+    Wishes w;
+    w.greedy = !(s.temperature > 0.0f);
+    w.top_k = w.greedy ? 1 : s.top_k;
+    w.by_count = w.greedy || (s.top_k > 0 && s.top_k < a.symbols);
+    w.by_part = !w.greedy && s.top_p < 1.0f;
+    w.factor = w.greedy ? 1.0f : 1.44269504f / s.temperature;
+    w.ordinary = largest < INFINITY && w.factor < 1e30f && w.factor > 1e-30f;
+    w.few = w.ordinary && (w.by_count || w.by_part || s.min_p > 0.0f) && (!w.by_count || w.top_k <= part_candidates / 2) &&
+        fabsf(largest * w.factor) < 1e4f;
+    return w;
+}
+
+// A part of a row: its largest logit, its candidates (a cut below its own largest, so those below the row's largest are
+// among them) and the sum of the others' weights.
+template <typename T>
+__global__ void __launch_bounds__(part_threads, 4) part_kernel(SampleArgs a, ManyArgs m) {
+    using Of = Elements<T>;
+    constexpr int each = Of::each, warps_here = part_threads / 32;
+    __shared__ uint4 queue[part_candidates];
+    __shared__ int places[part_candidates];
+    __shared__ unsigned bins_here[cut_bins], scratch[warps_here];
+    __shared__ float sums_here[warps_here];
+    __shared__ unsigned count, queued;
+    __shared__ int cut_bin;
+    join_chain();
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const std::int64_t r = blockIdx.x / m.parts;
+    const int part = static_cast<int>(blockIdx.x - r * m.parts);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *m.left = 0;
+    const T* logits = static_cast<const T*>(a.logits) + r * a.stride;
+    const int skew = static_cast<int>(reinterpret_cast<std::uintptr_t>(logits) % 16 / sizeof(T));
+    const int first = (part * part_vectors * part_threads + static_cast<int>(threadIdx.x)) * each - skew;
+    uint4 v[part_vectors];
+#pragma unroll
+    for (int k = 0; k < part_vectors; ++k) v[k] = load_vector(logits, a.symbols, first + k * part_threads * each);
+    const Settings s = settings_of(a, r);
+    float most = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < part_vectors; ++k) most = fmaxf(most, Of::largest(v[k]));
+    unsigned top = __reduce_max_sync(0xffffffffu, key_of(most));
+    if (threadIdx.x == 0) count = queued = 0, cut_bin = cut_bins;
+    if (lane == 0) scratch[warp] = top;
+    if (threadIdx.x < cut_bins) bins_here[threadIdx.x] = 0;
+    static_assert(cut_bins <= part_threads);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < warps_here; ++w) top = max(top, scratch[w]);
+    const float largest = top == 0 ? -INFINITY : logit_of(top);
+    const Wishes wishes = wishes_of(a, s, largest);
+    Part told{top, INFINITY, 0, 0.0f};
+    if (top != 0 && wishes.few) {
+        const float base = -largest * wishes.factor;
+        auto exponent = [&](float l) { return fmaf(l, wishes.factor, base); };
+        const bool by_least = !wishes.greedy && s.min_p > 0.0f;
+        float octaves = -10.0f;
+        if (by_least) {
+            octaves = fmaxf(log2f(fminf(s.min_p, 1.0f)) - 0.01f, -46.0f);
+        } else if (wishes.by_count) {
+            // at which top_k vectors have their largest logits above: so many candidates at least, and seldom many more
+#pragma unroll
+            for (int k = 0; k < part_vectors; ++k) {
+                const float x = exponent(Of::largest(v[k])) * -cut_steps;
+                if (x < static_cast<float>(cut_bins)) atomicAdd(&bins_here[static_cast<int>(x)], 1u);
+            }
+            __syncthreads();
+            if (warp == 0) {  // a lane eight bins
+                unsigned mine[cut_bins / 32], sum = 0;
+#pragma unroll
+                for (int i = 0; i < cut_bins / 32; ++i) sum += mine[i] = bins_here[lane * (cut_bins / 32) + i];
+                unsigned to = sum;
+                for (int o = 1; o < 32; o *= 2) {
+                    const unsigned u = __shfl_up_sync(0xffffffffu, to, o);
+                    if (lane >= o) to += u;
+                }
+                unsigned earlier = to - sum;
+                // a part's share of the row's, and half as many again: where that is too few, the row is left
+                const auto wanted = static_cast<unsigned>(min(wishes.top_k, 3 * wishes.top_k / (2 * m.parts) + 32));
+#pragma unroll
+                for (int i = 0; i < cut_bins / 32; ++i) {
+                    if (earlier < wanted && earlier + mine[i] >= wanted) cut_bin = lane * (cut_bins / 32) + i + 1;
+                    earlier += mine[i];
+                }
+            }
+            __syncthreads();
+            octaves = static_cast<float>(cut_bin) * (-1.0f / cut_steps) - 0.01f;
+        }
+        told.cut = wishes.greedy ? largest : largest + octaves / wishes.factor;
+        const bool sum_rest = wishes.by_part && !wishes.by_count;
+        float rest = 0.0f;
+#pragma unroll
+        for (int k = 0; k < part_vectors; ++k) {
+            if (Of::largest(v[k]) >= told.cut) {  // looked at below, by all threads
+                const unsigned nth = atomicAdd(&queued, 1u);
+                if (nth < part_candidates) queue[nth] = v[k], places[nth] = first + k * part_threads * each;
+            } else if (sum_rest) {
+#pragma unroll
+                for (int i = 0; i < each; ++i) rest += exp2_fast(exponent(Of::get(v[k], i)));
+            }
+        }
+        __syncthreads();
+        unsigned long long* list = m.candidates + (r * m.parts + part) * part_candidates;
+        const int all = static_cast<int>(min(queued, static_cast<unsigned>(part_candidates))) * each;
+        for (int e = threadIdx.x; e < all; e += part_threads) {
+            const float l = Of::pick(queue[e / each], e % each);
+            if (l >= told.cut) {
+                const unsigned nth = atomicAdd(&count, 1u);
+                if (nth < part_candidates) {
+                    list[nth] = static_cast<unsigned long long>(key_of(l)) << 32 | ~static_cast<unsigned>(places[e / each] + e % each);
+                }
+            } else if (l == l) {
+                rest += exp2_fast(exponent(l));
+            }
+        }
+        rest = warp_sum(rest);
+        if (lane == 0) sums_here[warp] = rest;
+        __syncthreads();
+        for (int w = 0; w < warps_here; ++w) told.rest += sums_here[w];
+        told.count = queued > part_candidates ? queued : count;
+    }
+    if (threadIdx.x == 0) m.told[r * m.parts + part] = told;
+}
+
+// A block a row: its candidates of all parts, those above the highest cut, in which nothing is missing.
+template <typename T>
+__global__ void __launch_bounds__(threads, 2) end_kernel(SampleArgs a, ManyArgs m) {
+    extern __shared__ unsigned char memory[];
+    auto& shared = *reinterpret_cast<Shared*>(memory);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    make_table(shared.table);
+    if (threadIdx.x == 0) shared.count = 0;
+    join_chain();
+    const std::int64_t r = blockIdx.x;
+    const Part* told = m.told + r * m.parts;
+    const Settings s = settings_of(a, r);
+    unsigned top = 0;
+    float cut = -INFINITY;
+    bool whole = true;
+    for (int p = lane; p < m.parts; p += 32) {
+        const Part part = told[p];
+        top = max(top, part.top);
+        if (part.top != 0) cut = fmaxf(cut, part.cut);
+        whole = whole && part.count <= part_candidates;
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) cut = fmaxf(cut, __shfl_xor_sync(0xffffffffu, cut, o));
+    whole = __all_sync(0xffffffffu, whole);
+    if (top == 0) {  // nothing to choose
+        if (threadIdx.x == 0) a.chosen[r] = -1, a.probabilities[r] = 0.0f;
+        return;
+    }
+    const float largest = logit_of(top);
+    const Wishes wishes = wishes_of(a, s, largest);
+    const Row row = row_of(top, s, shared.table);
+    bool done = false;
+    if (whole && wishes.few && cut < INFINITY) {  // a part whose largest is not ordinary has an infinite cut
+        const float base = -largest * wishes.factor;
+        auto exponent = [&](float l) { return fmaf(l, wishes.factor, base); };
+        double bulk = 0.0;
+        for (int p = lane; p < m.parts; p += 32) {
+            const Part part = told[p];
+            if (part.top != 0) bulk += static_cast<double>(part.rest) * exp2_fast(exponent(logit_of(part.top)));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o /= 2) bulk += __shfl_xor_sync(0xffffffffu, bulk, o);
+        __syncthreads();
+        // a warp a part
+        float held = 0.0f, rest = 0.0f;
+        for (int p = warp; p < m.parts; p += warps) {
+            const int count = static_cast<int>(told[p].count);
+            const unsigned long long* list = m.candidates + (r * m.parts + p) * part_candidates;
+            for (int i = lane; i < count; i += 32) {
+                const unsigned long long entry = list[i];
+                const float l = logit_of(static_cast<unsigned>(entry >> 32));
+                if (l >= cut) {
+                    const unsigned nth = atomicAdd(&shared.count, 1u);
+                    if (nth < most_candidates) shared.gathered[nth] = entry;
+                    held += exp2_fast(exponent(l));
+                } else {
+                    rest += exp2_fast(exponent(l));
+                }
+            }
+        }
+        held = warp_sum(held), rest = warp_sum(rest);
+        if (lane == 0) shared.parts[0][warp] = held, shared.parts[1][warp] = rest;
+        __syncthreads();
+        double all_held = 0.0;
+        for (int w = 0; w < warps; ++w) all_held += shared.parts[0][w], bulk += shared.parts[1][w];
+        const int count = static_cast<int>(shared.count);
+        const bool sum_rest = wishes.by_part && !wishes.by_count, by_least = row.least > 0.0 && !wishes.greedy;
+        // another rounding of the parts' largest logits' exponents
+        const double error = bulk_error(largest, wishes.factor) + 1e-5;
+        const bool enough = count <= most_candidates && bulk <= 1e30 &&
+            ((by_least && !(wishes.by_count && wishes.by_part)) ||
+             (wishes.by_count ? count >= wishes.top_k
+                              : all_held * (1.0 - error) >= static_cast<double>(fmaxf(s.top_p, 0.0f)) *
+                                      ((all_held + bulk) * (1.0 + error) + a.symbols / unit)));
+        if (enough) {
+            if (threadIdx.x == 0) shared.counts[0][0] = static_cast<unsigned long long>(count);
+            __syncthreads();
+            Settings set = s;
+            if (wishes.greedy) set.top_k = 1, set.top_p = 1.0f, set.min_p = 0.0f;
+            const double others = sum_rest ? bulk * unit : 0.0, slack = sum_rest ? others * error + a.symbols : 0.0;
+            ClusterRow<T> one{a, shared, r, 0, 1, 0, 0};
+            if (count <= 64) {
+                if (warp == 0) {
+                    done = one.finish_few(row, set, shared.counts[0], most_candidates, count, others, slack);
+                    if (lane == 0) shared.queued = done;
+                }
+                __syncthreads();
+                done = shared.queued != 0;
+            } else {
+                done = one.finish(row, set, shared.counts[0], most_candidates, others, slack);
+            }
+        }
+    }
+    if (!done && threadIdx.x == 0) m.left[1 + atomicAdd(m.left, 1u)] = static_cast<unsigned>(r);
+}
+
+// The rows that are left, a cluster each.
+template <typename T>
+__global__ void __launch_bounds__(threads, 2) rest_kernel(SampleArgs a, ManyArgs m, int blocks) {
+    extern __shared__ unsigned char memory[];
+    constexpr int each = Elements<T>::each;
+    auto& shared = *reinterpret_cast<Shared*>(memory);
+    const int lane = threadIdx.x % 32;
+    const int rank = static_cast<int>(blockIdx.x) % blocks;
+    join_chain();
+    const unsigned count = *m.left;
+    if (count == 0) return;
+    cluster_arrive();  // the others' memory is there once all have
+    make_table(shared.table);
+    cluster_wait();
+    __syncthreads();
+    for (unsigned nth = blockIdx.x / blocks; nth < count; nth += gridDim.x / blocks) {
+        const std::int64_t r = m.left[1 + nth];
+        const T* logits = static_cast<const T*>(a.logits) + r * a.stride;
+        const int skew = static_cast<int>(reinterpret_cast<std::uintptr_t>(logits) % 16 / sizeof(T));
+        const int all_vectors = (a.symbols + skew + each - 1) / each;
+        const int share = (all_vectors + blocks * threads - 1) / (blocks * threads);
+        ClusterRow<T> of_cluster{a, shared, r, rank, blocks, share, (rank * share * threads + static_cast<int>(threadIdx.x)) * each - skew};
+        const Settings s = settings_of(a, r);
+        unsigned top = 0;
+        for (int p = lane; p < m.parts; p += 32) top = max(top, m.told[r * m.parts + p].top);
+        top = __reduce_max_sync(0xffffffffu, top);
+        const Row row = row_of(top, s, shared.table);
+        const float largest = logit_of(top), factor = 1.44269504f / s.temperature;
+        if (row.temperature != 0.0 && !(largest < INFINITY && factor < 1e30f && factor > 1e-30f)) {
+            if (rank == 0) row_by_block<T>(a, r, shared.sums, shared.table);
+        } else {
+            of_cluster.whole(row, s, largest, factor);
+        }
+        cluster_sync();  // before the next row, or the end, while another block reads this one's memory
+    }
+}
+
 template <typename T, int Vectors>
 cudaError_t launch_cluster(const SampleArgs& a, int blocks, cudaStream_t stream) {
     static SharedAllowance allowance;
@@ -1130,8 +1422,66 @@ cudaError_t launch_cluster(const SampleArgs& a, int blocks, cudaStream_t stream)
     return cudaLaunchKernelEx(&config, cluster_kernel<T, Vectors>, a, blocks);
 }
 
+int parts_of(Type type, int symbols) {
+    const int part = part_threads * part_vectors * (type == Type::f32 ? 4 : 8);
+    return (symbols + 7 + part - 1) / part;  // a row may begin within a vector
+}
+int parts_of(const SampleArgs& a) {
+    const int each = a.type == Type::f32 ? 4 : 8, part = part_threads * part_vectors * each;
+    const bool whole = reinterpret_cast<std::uintptr_t>(a.logits) % 16 == 0 && a.stride % each == 0;
+    return whole ? (a.symbols + part - 1) / part : parts_of(a.type, a.symbols);
+}
+std::size_t rounded(std::size_t bytes) { return (bytes + 255) / 256 * 256; }
+// Blocks of a cluster that has a row in its registers.
+int blocks_of(Type type, int symbols) {
+    const int held = threads * 8 * (type == Type::f32 ? 4 : 8);
+    int blocks = 1;
+    while (blocks < most_blocks && blocks * held < symbols) blocks *= 2;
+    return blocks;
+}
+bool many_rows(Type type, std::int64_t rows, int symbols) {
+    return blocks_of(type, symbols) > 1 && rows * blocks_of(type, symbols) > 2 * sm_count() &&
+        symbols + 7 <= most_vectors * 4 * threads * most_blocks &&  // what a cluster's threads have
+        rows <= INT_MAX / parts_of(type, symbols);
+}
+
+template <typename T>
+cudaError_t launch_many(const SampleArgs& a, cudaStream_t stream) {
+    static SharedAllowance end_allowance, rest_allowance;
+    cudaError_t status = end_allowance.allow(end_kernel<T>, sizeof(Shared));
+    if (status == cudaSuccess) status = rest_allowance.allow(rest_kernel<T>, sizeof(Shared));
+    if (status != cudaSuccess) return status;
+    ManyArgs m{};
+    m.parts = parts_of(a);
+    const std::size_t parts = static_cast<std::size_t>(a.rows) * m.parts;
+    auto* memory = static_cast<unsigned char*>(a.workspace);
+    m.told = reinterpret_cast<Part*>(memory);
+    m.candidates = reinterpret_cast<unsigned long long*>(memory + rounded(parts * sizeof(Part)));
+    m.left = reinterpret_cast<unsigned*>(memory + rounded(parts * sizeof(Part)) + parts * part_candidates * 8);
+    status = kernels::launch_overlapped(part_kernel<T>, dim3(static_cast<unsigned>(parts)), dim3(part_threads), 0, stream, a, m);
+    if (status != cudaSuccess) return status;
+    status = kernels::launch_overlapped(end_kernel<T>, dim3(static_cast<unsigned>(a.rows)), dim3(threads), sizeof(Shared), stream, a, m);
+    if (status != cudaSuccess) return status;
+    const int blocks = blocks_of(a.type, a.symbols);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(std::min<std::int64_t>(a.rows, 2 * sm_count() / blocks) * blocks));
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = sizeof(Shared);
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = static_cast<unsigned>(blocks);
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, rest_kernel<T>, a, m, blocks);
+}
+
 template <typename T>
 cudaError_t launch(const SampleArgs& a, cudaStream_t stream) {
+    if (many_rows(a.type, a.rows, a.symbols)) return launch_many<T>(a, stream);
     constexpr int each = 16 / sizeof(T);
     const bool aligned = reinterpret_cast<std::uintptr_t>(a.logits) % 16 == 0 && (a.rows == 1 || a.stride % each == 0);
     const int vectors = (a.symbols + each - 1) / each + (aligned ? 0 : 1);  // a row may begin within one
@@ -1148,6 +1498,12 @@ cudaError_t launch(const SampleArgs& a, cudaStream_t stream) {
 }
 
 }  // namespace
+
+std::size_t sample_workspace(Type type, std::int64_t rows, int symbols) {
+    if (!many_rows(type, rows, symbols)) return 0;
+    const std::size_t parts = static_cast<std::size_t>(rows) * parts_of(type, symbols);
+    return rounded(parts * sizeof(Part)) + parts * part_candidates * 8 + rounded((static_cast<std::size_t>(rows) + 1) * sizeof(unsigned));
+}
 
 cudaError_t sample(const SampleArgs& a, cudaStream_t stream) {
     if (a.rows == 0) return cudaSuccess;

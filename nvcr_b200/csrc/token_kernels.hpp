@@ -200,8 +200,10 @@ struct SampleArgs {
     float min_p;
     std::int64_t* chosen;
     float* probabilities;
+    void* workspace;
 };
 constexpr int most_symbols = 1 << 20;
+std::size_t sample_workspace(Type type, std::int64_t rows, int symbols);
 cudaError_t sample(const SampleArgs& args, cudaStream_t stream);
 
 }  // namespace nvcr_sm100::token

@@ -89,7 +89,7 @@ EXPORTS = [
     "nvcr_sm100_token_attend", "nvcr_sm100_token_packed_bytes", "nvcr_sm100_token_pack", "nvcr_sm100_token_multiply",
     "nvcr_sm100_token_bytes_packed", "nvcr_sm100_token_bytes_pack", "nvcr_sm100_token_bytes_workspace",
     "nvcr_sm100_token_bytes_multiply", "nvcr_sm100_token_experts_workspace", "nvcr_sm100_token_experts_multiply",
-    "nvcr_sm100_token_route", "nvcr_sm100_token_sample",
+    "nvcr_sm100_token_route", "nvcr_sm100_token_sample", "nvcr_sm100_token_sample_workspace",
 ]
 
 _lib: ctypes.CDLL | None = None
@@ -210,7 +210,8 @@ def library() -> ctypes.CDLL:
                                                   vp, ctypes.c_int32, ctypes.c_int32, ctypes.c_int, ctypes.c_float, vp,
                                                   vp, vp]),
         "nvcr_sm100_token_sample": (ctypes.c_int, [ctypes.c_int, vp, i64, i64, ctypes.c_int32, vp, vp, ctypes.c_float, vp,
-                                                   ctypes.c_int32, vp, ctypes.c_float, vp, ctypes.c_float, vp, vp, vp]),
+                                                   ctypes.c_int32, vp, ctypes.c_float, vp, ctypes.c_float, vp, vp, vp, sz, vp]),
+        "nvcr_sm100_token_sample_workspace": (ctypes.c_int, [ctypes.c_int, i64, ctypes.c_int32, ctypes.POINTER(sz)]),
     }
     for name, (restype, argtypes) in signatures.items():
         function = getattr(lib, name)

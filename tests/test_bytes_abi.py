@@ -121,13 +121,17 @@ def test_sample_refuses(lib, room):
     def call(**changes):
         fields = dict(type=0, logits=room, stride=8, rows=2, symbols=8, uniforms=room, temperatures=None, temperature=1.0,
                       top_ks=None, top_k=0, top_ps=None, top_p=1.0, min_ps=None, min_p=0.0, chosen=room, probabilities=room,
-                      stream=None)
+                      workspace=None, bytes=0, stream=None)
         fields.update(changes)
         return lib.nvcr_sm100_token_sample(*fields.values())
 
     for changes in (dict(type=3), dict(type=-1), dict(rows=-1), dict(rows=1 << 31), dict(symbols=0), dict(symbols=(1 << 20) + 1),
-                    dict(logits=None), dict(uniforms=None), dict(chosen=None), dict(probabilities=None)):
+                    dict(logits=None), dict(uniforms=None), dict(chosen=None), dict(probabilities=None), dict(workspace=room + 8),
+                    dict(rows=1000, symbols=100000), dict(rows=1000, symbols=100000, workspace=room, bytes=4096)):
         assert call(**changes) == INVALID, changes
+    for changes in ((3, 1, 8), (0, -1, 8), (0, 1 << 31, 8), (0, 1, 0), (0, 1, (1 << 20) + 1)):
+        assert lib.nvcr_sm100_token_sample_workspace(*changes, size()) == INVALID
+    assert lib.nvcr_sm100_token_sample_workspace(0, 1, 8, None) == INVALID
     assert call(rows=0, logits=None, uniforms=None, chosen=None, probabilities=None) == 0
 
 

@@ -510,19 +510,21 @@ def plain_sample(logits, uniforms, temperature, top_k, top_p, min_p):
         with np.errstate(invalid="ignore"):
             share = np.where(row[index] == top, 1.0, np.exp((row[index] - top) / temperature[r]))
         share = np.nan_to_num(share)
+        # sums are of multiples of 2^-43, as the header says: what is smaller does not tip two equal halves
+        units = np.rint(share * 2.0 ** 43)
         n = len(index)
         if top_p[r] < 1.0:
-            n = 1 + int(np.searchsorted(np.cumsum(share), max(top_p[r], 0.0) * share.sum()))
+            n = 1 + int(np.searchsorted(np.cumsum(units), max(top_p[r], 0.0) * units.sum()))
         if min_p[r] > 0:
             n = min(n, int((share >= min(min_p[r], 1.0)).sum()))
         n = max(1, min(n, len(index)))
-        index, share = index[:n], share[:n]
+        index, share, units = index[:n], share[:n], units[:n]
         order = np.argsort(index)
-        sums = np.cumsum(share[order])
+        sums = np.cumsum(units[order])
         u = 0.0 if not uniforms[r] > 0 else uniforms[r]
         at = int(np.searchsorted(sums, u * sums[-1], side="right")) if u < 1.0 else n
-        at = order[min(at, np.flatnonzero(share[order] >= 2.0 ** -44)[-1])]
-        symbols.append(index[at]), probabilities.append(share[at] / sums[-1])
+        at = order[min(at, np.flatnonzero(units[order])[-1])]
+        symbols.append(index[at]), probabilities.append(share[at] * 2.0 ** 43 / sums[-1])
     return np.array(symbols), np.array(probabilities)
 
 
@@ -550,12 +552,52 @@ SETTINGS = [dict(), dict(top_k=1), dict(top_k=50), dict(top_k=3000), dict(top_p=
 
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("settings", SETTINGS, ids=str)
-@pytest.mark.parametrize("rows,symbols", [(1, 1), (3, 7), (20, 1000), (9, 32768), (5, 50001), (2, 200003)])
+@pytest.mark.parametrize("rows,symbols", [(1, 1), (3, 7), (20, 1000), (9, 32768), (5, 50001), (2, 200003), (3, 262144), (2, 300001)])
 def test_sample(cuda, rows, symbols, settings, name):
     import torch
 
     logits = normal((rows, symbols), rows, 2.0) + torch.relu(normal((rows, symbols), 7) - 2.5) * 6.0
     check_sample(logits.to(kind_of(name)), **settings)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("settings", SETTINGS, ids=str)
+def test_sample_of_many_rows(cuda, settings, name):
+    """So many rows that their parts are looked at one by one; flat and sharp ones, odd sizes, masks and extremes among
+    them."""
+    import torch
+
+    rows, symbols = 301, {"float16": 33001, "bfloat16": 40000, "float32": 17000}[name]
+    logits = normal((rows, symbols), 1, 2.0) + torch.relu(normal((rows, symbols), 7) - 2.5) * 6.0
+    logits *= torch.rand((rows, 1), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda") * 2.0
+    logits[0] = -math.inf
+    logits[1] = math.nan
+    logits[2, 100:] = -math.inf
+    logits[3, ::2] = math.nan
+    logits[4] = 0.0
+    logits[5] = -3.0
+    logits[5, symbols - 1] = 4.0
+    logits[6, 13] = math.inf
+    logits[7, 13] = logits[7, symbols - 2] = math.inf
+    logits[8] *= 1000.0
+    logits[9, : symbols // 2] -= 200.0
+    logits[10] = torch.round(logits[10])
+    logits[11] = torch.where(torch.arange(symbols, device="cuda") % 3 == 0, 5.0, -5.0)
+    logits[12, 20:] = -math.inf
+    logits[12, :20] = torch.finfo(torch.float16).min
+    check_sample(logits.to(kind_of(name)), **settings)
+
+
+def test_sample_of_many_rows_settings_of_each_row(cuda):
+    import torch
+
+    rows = 400
+    logits = normal((rows, 40001), 8, 3.0).half()
+    pick = lambda values, kind: torch.tensor([values[i % len(values)] for i in range(rows)], dtype=kind, device="cuda")  # noqa: E731
+    check_sample(logits, seed=5, temperature=pick([1.0, 0.0, 0.5, -1.0, math.nan, 1e-30, 1e30, math.inf, 0.02], torch.float32),
+                 top_k=pick([0, 5, -3, 100000, 64, 700], torch.int32),
+                 top_p=pick([1.0, 0.5, math.nan, -1.0, 2.0, 0.9, 1e-9], torch.float32),
+                 min_p=pick([0.0, 0.1, -1.0, 5.0, math.nan, 0.01, 0.5, 0.0, 1e-30], torch.float32))
 
 
 @pytest.mark.parametrize("settings", SETTINGS, ids=str)
