@@ -53,7 +53,7 @@ constexpr double unit = 8796093022208.0;  // 2^43: 2^20 weights stay below 2^63
 constexpr int table_size = 64;
 
 struct Row {
-    unsigned top;         // the largest key
+    float largest;
     double temperature;   // 0: the largest alone
     double least;         // of a kept share
     double factor;        // steps of 2^(1/64) a logit
@@ -62,8 +62,8 @@ struct Row {
 
 // A logit's share of the largest one's weight, in units. With y = 64 log2(e) (l - max) / temperature = n + f, |f| <= 1/2:
 // 2^(n / 64) from the table and its exponent, e^(f ln(2) / 64) by Taylor's polynomial, whose fifth term is below 4e-14.
-__device__ __forceinline__ double share_of(unsigned key, const Row& row) {
-    const double y = (static_cast<double>(logit_of(key)) - static_cast<double>(logit_of(row.top))) * row.factor;
+__device__ __forceinline__ double share_of(float logit, const Row& row) {
+    const double y = (static_cast<double>(logit) - static_cast<double>(row.largest)) * row.factor;
     const double whole = y + 6755399441055744.0;  // 1.5 * 2^52: rounds to a whole number, in the low word
     const int n = __double2loint(whole);
     const double f = y - (whole - 6755399441055744.0);
@@ -71,11 +71,12 @@ __device__ __forceinline__ double share_of(unsigned key, const Row& row) {
     const double p = fma(f, fma(f, fma(f, fma(f, c * c * c * c / 24.0, c * c * c / 6.0), c * c / 2.0), c), 1.0);
     const double w = row.table[n & (table_size - 1)] * p;
     const double found = __hiloint2double(__double2hiint(w) + (n >> 6) * (1 << 20), __double2loint(w));
-    // below 2^-46, less than half a unit: none; so are symbols that are left out, and all but the largest at temperature 0
-    return key == row.top ? unit : key != 0 && y > -46.0 * table_size ? found : 0.0;
+    // Infinite largest ones share; below 2^-46, less than half a unit, there is none, and none for a NaN (y is one), an
+    // infinity, or all but the largest at temperature 0, whose factor is infinite.
+    return logit == row.largest ? unit : y > -46.0 * table_size ? found : 0.0;
 }
 // One copy of it for code that runs once a row.
-__device__ __noinline__ double share_once(unsigned key, const Row& row) { return share_of(key, row); }
+__device__ __noinline__ double share_once(float logit, const Row& row) { return share_of(logit, row); }
 // Rounded to whole units: below 2^52 the sum's low bits.
 __device__ __forceinline__ Weight weight_of(double share) {
     return static_cast<Weight>(__double_as_longlong(share + 4503599627370496.0)) & 0xfffffffffffffull;
@@ -117,7 +118,7 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, std::int64_
 }
 __device__ __forceinline__ Row row_of(unsigned top, const Settings& s, const double* table) {
     const double temperature = s.temperature > 0.0f ? static_cast<double>(s.temperature) : 0.0;
-    return {top, temperature, s.min_p > 0.0f ? static_cast<double>(fminf(s.min_p, 1.0f)) * unit : 0.0,
+    return {logit_of(top), temperature, s.min_p > 0.0f ? static_cast<double>(fminf(s.min_p, 1.0f)) * unit : 0.0,
             table_size * 1.4426950408889634074 / temperature, table};
 }
 // By the block's first threads; the caller synchronises.
@@ -195,13 +196,13 @@ __device__ Threshold find_by_block(const T* logits, int symbols, const Row& row,
             if (!by_weight) {
                 atomicAdd(&sums.low[bin], 1u);
             } else if (key != kept.key) {  // those are added below
-                const Weight w = weight_of(share_once(key, row));
+                const Weight w = weight_of(share_once(logit_of(key), row));
                 if (w != 0) add(sums, bin, w);
             }
         }
         __syncthreads();
         if (by_weight && threadIdx.x == 0 && kept.key != 0 && (shift == 32 || kept.key >> shift == prefix)) {
-            add(sums, kept.key >> next & ((1u << width) - 1), kept.ties * weight_of(share_once(kept.key, row)));
+            add(sums, kept.key >> next & ((1u << width) - 1), kept.ties * weight_of(share_once(logit_of(kept.key), row)));
         }
         __syncthreads();
         pass(sums, above, wanted, [&](int bin) { return static_cast<Weight>(sums.high[bin]) << 32 | sums.low[bin]; });
@@ -212,7 +213,7 @@ __device__ Threshold find_by_block(const T* logits, int symbols, const Row& row,
         shift = next;
     }
     __syncthreads();
-    const Weight each = by_weight ? weight_of(share_once(prefix, row)) : 1;
+    const Weight each = by_weight ? weight_of(share_once(logit_of(prefix), row)) : 1;
     return {prefix, static_cast<unsigned>((wanted - above + each - 1) / each)};
 }
 
@@ -242,10 +243,10 @@ __device__ __noinline__ void row_by_block(const SampleArgs& a, std::int64_t r, S
             Weight mine = 0, all;
             for (int i = threadIdx.x; i < symbols; i += threads) {
                 const unsigned key = key_of(widen(logits[i]));
-                if (key > kept.key) mine += weight_of(share_once(key, row));
+                if (key > kept.key) mine += weight_of(share_once(logit_of(key), row));
             }
             before(mine, sums.scratch, all);
-            if (kept.key != 0) all += kept.ties * weight_of(share_once(kept.key, row));
+            if (kept.key != 0) all += kept.ties * weight_of(share_once(logit_of(kept.key), row));
             kept = stricter(kept, find_by_block(logits, symbols, row, true, part_of(s.top_p, all), kept, sums));
         }
     }
@@ -260,7 +261,7 @@ __device__ __noinline__ void row_by_block(const SampleArgs& a, std::int64_t r, S
         for (int i = from; i < to; ++i) {
             const unsigned key = key_of(widen(logits[i]));
             if (key == 0 || key < kept.key || (key == kept.key && nth++ >= kept.ties)) continue;
-            const double share = share_once(key, row);
+            const double share = share_once(logit_of(key), row);
             if (share >= row.least && !visit(i, share)) return;
         }
     };
@@ -401,11 +402,11 @@ __device__ __forceinline__ uint4 load_vector(const T* logits, int symbols, int a
             return v;
 }
 
-// What a cluster keeps: keys above `key`, and those equal to it up to index `last`.
+// What a cluster keeps: logits above `value`, and those equal to it up to index `last`. A NaN is not among them.
 struct Kept {
-    unsigned key;
+    float value;
     int last;
-    __device__ __forceinline__ bool holds(unsigned k, int index) const { return k > key || (k == key && k != 0 && index <= last); }
+    __device__ __forceinline__ bool holds(float l, int index) const { return l > value || (l == value && index <= last); }
 };
 
 // 2048 in falling order, by 512 threads: four neighbours a thread, so that only exchanges over 128 places and more pass
@@ -505,7 +506,15 @@ struct ClusterRow {
         }
     }
 
-    // Where the running sum of amounts, in the order of indexes, first exceeds wanted(their whole): visit(index, key, whole)
+    // body(first, elements 0 .. each / 2 - 1 of it) for both halves of a vector: as many FP64 values at once as there are
+    // registers for.
+    template <typename Body>
+    static __device__ __forceinline__ void for_halves(const uint4& v, Body&& body) {
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) body(h * (each / 2), h == 0 ? uint4{v.x, v.y, 0, 0} : uint4{v.z, v.w, 0, 0});
+    }
+
+    // Where the running sum of amounts, in the order of indexes, first exceeds wanted(their whole): visit(index, logit, whole)
     // there, by one thread of the cluster.
     template <typename Amount, typename Wanted, typename Visit>
     __device__ __forceinline__ void locate(Amount&& amount, Wanted&& wanted_of, Visit&& visit) {
@@ -513,8 +522,10 @@ struct ClusterRow {
         const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
         for_vectors([&](int n, const uint4& v) {
             Weight sum = 0;
+            for_halves(v, [&](int from, const uint4& half) {
 #pragma unroll
-            for (int i = 0; i < each; ++i) sum += amount(first + n * threads * each + i, key_of(Of::get(v, i)));
+                for (int i = 0; i < each / 2; ++i) sum += amount(first + n * threads * each + from + i, Of::get(half, i));
+            });
 #pragma unroll
             for (int o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (lane == 0) shared.cells[n * warps + warp] = sum;
@@ -542,7 +553,7 @@ const int n = cell / warps;
         const uint4 v = load(n);
         Weight sum = 0;
 #pragma unroll
-        for (int i = 0; i < each; ++i) sum += amount(first + n * threads * each + i, key_of(Of::get(v, i)));
+        for (int i = 0; i < each; ++i) sum += amount(first + n * threads * each + i, Of::get(v, i));
         Weight to = sum;
         for (int o = 1; o < 32; o *= 2) {
             const Weight u = __shfl_up_sync(0xffffffffu, to, o);
@@ -553,9 +564,9 @@ const int n = cell / warps;
 #pragma unroll
         for (int i = 0; i < each; ++i) {
             const int index = first + n * threads * each + i;
-            const unsigned key = key_of(Of::get(v, i));
-            const Weight w = amount(index, key);
-            if (wanted >= from && wanted < from + w) visit(index, key, all);
+            const float l = Of::get(v, i);
+            const Weight w = amount(index, l);
+            if (wanted >= from && wanted < from + w) visit(index, l, all);
             from += w;
         }
     }
@@ -602,7 +613,7 @@ const int n = cell / warps;
         }
     }
 
-    // A histogram of the symbols that bin_of(logit, key) puts in a bin, the largest logits in the first, by counts or
+    // A histogram of the symbols that bin_of(logit) puts in a bin, the largest logits in the first, by counts or
     // weights: the bin in which wanted_of(whole) is reached, or -1, and what of it is wanted there.
     template <typename BinOf, typename WantedOf>
     __device__ __forceinline__ int reach(const Row& row, bool by_weight, const Kept& kept, BinOf&& bin_of, WantedOf&& wanted_of,
@@ -613,25 +624,26 @@ const int n = cell / warps;
         if (threadIdx.x == 0) sums.found = -1;
         __syncthreads();
         for_vectors([&](int n, const uint4& v) {
-            int bin[each];
-            Weight w[each];
+            for_halves(v, [&](int from, const uint4& half) {
+                int bin[each / 2];
+                Weight w[each / 2];
 #pragma unroll
-            for (int i = 0; i < each; ++i) {
-                const float l = Of::get(v, i);
-                const unsigned key = key_of(l);
-                bin[i] = bin_of(l, key);
-                if (!kept.holds(key, first + n * threads * each + i)) bin[i] = -1;
-                if (by_weight) w[i] = weight_of(share_of(key, row));
-            }
-#pragma unroll
-            for (int i = 0; i < each; ++i) {
-                if (bin[i] < 0) continue;
-                if (!by_weight) {
-                    atomicAdd(&sums.low[bin[i]], 1u);
-                } else if (w[i] != 0) {
-                    add(sums, static_cast<unsigned>(bin[i]), w[i]);
+                for (int i = 0; i < each / 2; ++i) {
+                    const float l = Of::get(half, i);
+                    bin[i] = bin_of(l);
+                    if (!kept.holds(l, first + n * threads * each + from + i)) bin[i] = -1;
+                    if (by_weight) w[i] = weight_of(share_of(l, row));
                 }
-            }
+#pragma unroll
+                for (int i = 0; i < each / 2; ++i) {
+                    if (bin[i] < 0) continue;
+                    if (!by_weight) {
+                        atomicAdd(&sums.low[bin[i]], 1u);
+                    } else if (w[i] != 0) {
+                        add(sums, static_cast<unsigned>(bin[i]), w[i]);
+                    }
+                }
+            });
         });
         cluster_sync();
         if (rank == 0) {
@@ -678,7 +690,7 @@ const int n = cell / warps;
         };
         Weight wanted;
         const int octave = reach(
-            row, by_weight, kept, [&](float l, unsigned) { return octave_bin(l); },
+            row, by_weight, kept, octave_bin,
             [&](Weight all) { return by_weight ? part_of(s.top_p, all) : static_cast<Weight>(s.top_k); }, wanted);
         if (octave < 0) return kept;  // there is less than wanted: all of it
         unsigned low = 0, high = 0;   // the keys looked at, once they are known
@@ -693,7 +705,7 @@ const int n = cell / warps;
                     const unsigned key = key_of(l);
                     const int index = first + n * threads * each + i;
                     if (turn == 0 ? octave_bin(l) != octave : key < low || key > high) continue;
-                    if (!kept.holds(key, index)) continue;
+                    if (!kept.holds(l, index)) continue;
                     least = min(least, key), most = max(most, key);
                     gather(key, index, part);
                 }
@@ -726,7 +738,7 @@ const int n = cell / warps;
 #pragma unroll
                     for (int i = 0; i < most_each; ++i) {
                         mine[i] = i >= run || from + i >= n ? 0
-                            : by_weight ? weight_of(share_of(static_cast<unsigned>(shared.sorted[from + i] >> 32), row)) : 1;
+                            : by_weight ? weight_of(share_of(logit_of(static_cast<unsigned>(shared.sorted[from + i] >> 32)), row)) : 1;
                         sum += mine[i];
                     }
                     Weight earlier = before(sum, shared.sums.scratch, all);
@@ -741,13 +753,13 @@ const int n = cell / warps;
                 break;
             }
             if (low == high) {
-                const Weight one = by_weight ? weight_of(share_of(low, row)) : 1;
+                const Weight one = by_weight ? weight_of(share_of(logit_of(low), row)) : 1;
                 locate(
-                    [&](int index, unsigned key) { return static_cast<Weight>(key == low && kept.holds(key, index)); },
+                    [&](int index, float l) { return static_cast<Weight>(key_of(l) == low && kept.holds(l, index)); },
                     [&](Weight) { return (wanted + one - 1) / one - 1; },
-                    [&](int index, unsigned key, Weight) {
+                    [&](int index, float l, Weight) {
                         for (int b = 0; b < blocks; ++b) {
-                            put(&shared.told[0], b, static_cast<unsigned long long>(key) << 32 | ~static_cast<unsigned>(index));
+                            put(&shared.told[0], b, static_cast<unsigned long long>(key_of(l)) << 32 | ~static_cast<unsigned>(index));
                         }
                     });
                 break;
@@ -757,7 +769,10 @@ const int n = cell / warps;
             const unsigned from = low, to = high;
             const int found = reach(
                 row, by_weight, kept,
-                [&](float, unsigned key) { return key >= from && key <= to ? static_cast<int>((to - key) >> shift) : -1; },
+                [&](float l) {
+                    const unsigned key = key_of(l);
+                    return key >= from && key <= to ? static_cast<int>((to - key) >> shift) : -1;
+                },
                 [&](Weight) { return still; }, wanted);
             high = to - (static_cast<unsigned>(found) << shift);
             low = high - min(high - from, (1u << shift) - 1);
@@ -765,29 +780,28 @@ const int n = cell / warps;
         cluster_sync();
         const unsigned long long end = shared.told[0];
         __syncthreads();
-        return {static_cast<unsigned>(end >> 32), static_cast<int>(~static_cast<unsigned>(end))};
+        return {logit_of(static_cast<unsigned>(end >> 32)), static_cast<int>(~static_cast<unsigned>(end))};
     }
 
     // Any row of finite logits, exactly.
     __device__ __forceinline__ void whole(const Row& row, const Settings& s, float largest, float factor) {
-        Kept kept{0, 0};
+        Kept kept{-INFINITY, INT_MAX};
         if (row.temperature == 0.0) {
-            kept = {row.top, INT_MAX};
+            kept = {row.largest, INT_MAX};
         } else {
             if (s.top_k > 0 && s.top_k < a.symbols) kept = find(row, s, false, largest, factor, kept);
             if (s.top_p < 1.0f) kept = find(row, s, true, largest, factor, kept);
         }
         // with a temperature of 0, u is taken as 0: the first of the largest
         locate(
-            [&](int index, unsigned key) -> Weight {
-                if (!kept.holds(key, index)) return 0;
-                const double share = share_of(key, row);
-                return share >= row.least ? weight_of(share) : 0;
+            [&](int index, float l) -> Weight {
+                const double share = share_of(l, row);
+                return kept.holds(l, index) && share >= row.least ? weight_of(share) : 0;
             },
             [&](Weight all) { return row.temperature == 0.0 ? 0 : part_of_uniform(s.uniform, all); },
-            [&](int index, unsigned key, Weight all) {
+            [&](int index, float l, Weight all) {
                 a.chosen[r] = index;
-                a.probabilities[r] = row.temperature == 0.0 ? 1.0f : probability_of(share_of(key, row), all);
+                a.probabilities[r] = row.temperature == 0.0 ? 1.0f : probability_of(share_of(l, row), all);
             });
     }
 
@@ -822,7 +836,7 @@ const int n = cell / warps;
         for (int i = 0; i < 2; ++i) {
             const bool there = 2 * lane + i < n;
             entry[i] = there ? shared.sorted[2 * lane + i] : 0;
-            const double share = there ? share_of(static_cast<unsigned>(entry[i] >> 32), row) : 0.0;
+            const double share = there ? share_of(logit_of(static_cast<unsigned>(entry[i] >> 32)), row) : 0.0;
             w[i] = weight_of(share);
             kept += there && share >= row.least;
         }
@@ -863,7 +877,7 @@ const int n = cell / warps;
         for (int i = 0; i < 2; ++i) {
             if (2 * lane + i < n && wanted >= lower[i] && wanted < lower[i] + w[i]) {
                 a.chosen[r] = static_cast<std::int64_t>(~static_cast<unsigned>(entry[i]));
-                a.probabilities[r] = probability_of(share_of(static_cast<unsigned>(entry[i] >> 32), row), last);
+                a.probabilities[r] = probability_of(share_of(logit_of(static_cast<unsigned>(entry[i] >> 32)), row), last);
             }
         }
         return true;
@@ -882,7 +896,7 @@ const int n = cell / warps;
         unsigned kept = 0;
 #pragma unroll 1
         for (int i = from; i < until; ++i) {
-            const double share = share_once(static_cast<unsigned>(shared.sorted[i] >> 32), row);
+            const double share = share_once(logit_of(static_cast<unsigned>(shared.sorted[i] >> 32)), row);
             const Weight w = weight_of(share);
             shared.weights[i] = w;
             kept += share >= row.least;
@@ -919,7 +933,7 @@ const int n = cell / warps;
         const Weight wanted = part_of_uniform(s.uniform, whole_kept);
         auto choose = [&](unsigned long long entry) {
             a.chosen[r] = static_cast<std::int64_t>(~static_cast<unsigned>(entry));
-            a.probabilities[r] = probability_of(share_once(static_cast<unsigned>(entry >> 32), row), whole_kept);
+            a.probabilities[r] = probability_of(share_once(logit_of(static_cast<unsigned>(entry >> 32)), row), whole_kept);
         };
         auto weight_at = [&](int i) { return shared.weights[i] - (i == 0 ? 0 : shared.weights[i - 1]); };
         if (n <= threads) {  // the weight of those with lower indexes, for each
