@@ -12,8 +12,18 @@ back to the residual stream::
     hidden, normed = block_norm(delta, residual=hidden, ...)
     delta          = down.multiply(silu(gate) * up)             # gate, up = gate_up.multiply(normed)
 
+With ``experts`` the second block is each token's own few of many, in 8 bits::
+
+    choices, weights = route(scores.multiply(normed), chosen, renormalise=True)
+    gate, up       = gate_up.multiply(normed, choices)          # [tokens, chosen, inner] each
+    delta          = down.multiply(silu(gate) * up, choices, weights)
+
+``bits=8`` holds all weights in 8 bits, for long prompts: their products run on the
+tensor cores at their 8-bit rate, where those with 4-bit weights are made for a few rows.
+
 ``python -m nvcr_b200.token_model`` decodes a batch of sequences with random
-weights and prints the time of a step, eager and as a captured CUDA graph.
+weights and prints the time of a step, eager and as a captured CUDA graph;
+``--experts 8``, ``--bits 8`` and ``--temperature 0.8 --top-p 0.9`` try the rest.
 """
 from __future__ import annotations
 
@@ -38,13 +48,25 @@ class TokenModelConfig:
     group: int = 64
     positions: int = 4096
     dtype: torch.dtype = torch.float16
+    bits: int = 4  # of weights: 4 or 8
+    experts: int = 0  # of the second block; 0: one block for all tokens
+    chosen: int = 2  # experts of a token
+
+
+def _matrix(config: TokenModelConfig, make: torch.Generator, outputs: int,
+            inputs: int) -> tokens.PackedMatrix | tokens.ByteMatrix:
+    weights = torch.randn((outputs, inputs), generator=make, device="cuda") * inputs ** -0.5
+    return tokens.ByteMatrix.quantise(weights) if config.bits == 8 else tokens.PackedMatrix.quantise(weights, config.group)
 
 
 class _Layer:
     def __init__(self, config: TokenModelConfig, make: torch.Generator) -> None:
-        def matrix(outputs: int, inputs: int) -> tokens.PackedMatrix:
-            weights = torch.randn((outputs, inputs), generator=make, device="cuda") * inputs ** -0.5
-            return tokens.PackedMatrix.quantise(weights, config.group)
+        def matrix(outputs: int, inputs: int) -> tokens.PackedMatrix | tokens.ByteMatrix:
+            return _matrix(config, make, outputs, inputs)
+
+        def experts(outputs: int, inputs: int) -> tokens.ByteExperts:
+            shape = (config.experts, outputs, inputs)
+            return tokens.ByteExperts.quantise(torch.randn(shape, generator=make, device="cuda") * inputs ** -0.5)
 
         def vector(mean: float) -> torch.Tensor:
             return (torch.randn((config.width,), generator=make, device="cuda") * 0.1 + mean).to(config.dtype)
@@ -52,8 +74,14 @@ class _Layer:
         heads = config.heads + 2 * config.kv_heads
         self.qkv = matrix(heads * config.head_dim, config.width)
         self.out = matrix(config.width, config.heads * config.head_dim)
-        self.gate_up = matrix(2 * config.inner, config.width)
-        self.down = matrix(config.width, config.inner)
+        if config.experts:
+            weights = torch.randn((config.experts, config.width), generator=make, device="cuda") * config.width ** -0.5
+            self.scores = tokens.ByteMatrix.quantise(weights)
+            self.gate_up = experts(2 * config.inner, config.width)
+            self.down = experts(config.width, config.inner)
+        else:
+            self.gate_up = matrix(2 * config.inner, config.width)
+            self.down = matrix(config.width, config.inner)
         self.before = [vector(1.0), vector(1.0)]  # weights of the norms before and after each block, and its gate
         self.after = [vector(1.0), vector(1.0)]
         self.gates = [vector(0.5), vector(0.5)]
@@ -69,8 +97,7 @@ class TokenModel:
         self.max_length = self.columns * page_size
         self.embedding = torch.randn((config.symbols, config.width), generator=make, device="cuda").to(config.dtype)
         self.layers = [_Layer(config, make) for _ in range(config.layers)]
-        head = torch.randn((config.symbols, config.width), generator=make, device="cuda") * config.width ** -0.5
-        self.head = tokens.PackedMatrix.quantise(head, config.group)
+        self.head = _matrix(config, make, config.symbols, config.width)
         self.last_norm = torch.ones((config.width,), dtype=config.dtype, device="cuda")
         self.caches = [tokens.PagedCache.empty(batch * self.columns, config.kv_heads, page_size, config.head_dim,
                                                min(config.group, config.head_dim)) for _ in range(config.layers)]
@@ -109,11 +136,22 @@ class TokenModel:
                                         max_length=self.max_length)
             delta = layer.out.multiply(mixed.view(batch * count, -1))
             hidden, normed = self._between(hidden, delta, layer.after[0], layer.gates[0], layer.before[1])
-            inner_gate, up = layer.gate_up.multiply(normed).chunk(2, 1)
-            delta = layer.down.multiply(torch.nn.functional.silu(inner_gate) * up)
+            if config.experts:
+                choices, weights = tokens.route(layer.scores.multiply(normed), config.chosen, renormalise=True)
+                inner_gate, up = layer.gate_up.multiply(normed, choices).chunk(2, 2)
+                delta = layer.down.multiply(torch.nn.functional.silu(inner_gate) * up, choices, weights)
+            else:
+                inner_gate, up = layer.gate_up.multiply(normed).chunk(2, 1)
+                delta = layer.down.multiply(torch.nn.functional.silu(inner_gate) * up)
             after, gate = layer.after[1], layer.gates[1]
         _, normed = self._between(hidden, delta, after, gate, self.last_norm)
         return self.head.multiply(normed).view(batch, count, -1)
+
+    def step(self, symbols: torch.Tensor, uniforms: torch.Tensor, **settings) -> torch.Tensor:
+        """Appends int64 symbols [batch, count] and returns the one [batch, 1] that follows each sequence, chosen by its
+        uniform number (float32 [batch]) and `tokens.sample`'s settings."""
+        chosen, _ = tokens.sample(self.advance(symbols)[:, -1], uniforms, **settings)
+        return chosen[:, None]
 
     @staticmethod
     def _slots(pages: torch.Tensor, places: torch.Tensor, page_size: int) -> torch.Tensor:
@@ -129,9 +167,13 @@ class TokenModel:
         return tokens.block_norm(delta, residual=hidden, gate=gate, post=True, post_weight=after, pre_weight=before)
 
     def check(self) -> None:
-        """Raises if a kernel met a slot, position, page or length out of range."""
+        """Raises if a kernel met a slot, position, page or length out of range, or a wait in one ran out."""
         for cache in self.caches:
             cache.check()
+        parts = [self.head] + [part for layer in self.layers for part in vars(layer).values()]
+        for part in parts:
+            if isinstance(part, (tokens.ByteMatrix, tokens.ByteExperts)):
+                part.check()
 
 
 def main() -> None:
@@ -140,21 +182,30 @@ def main() -> None:
     parser.add_argument("--prompt", type=int, default=32)
     parser.add_argument("--steps", type=int, default=64)
     parser.add_argument("--layers", type=int, default=4)
+    parser.add_argument("--bits", type=int, choices=(4, 8), default=4, help="of the weights")
+    parser.add_argument("--experts", type=int, default=0, help="of a layer's second block (0: one block for all)")
+    parser.add_argument("--temperature", type=float, default=0.0, help="0: the symbol with the largest logit")
+    parser.add_argument("--top-p", type=float, default=1.0)
     options = parser.parse_args()
-    config = TokenModelConfig(layers=options.layers)
+    config = TokenModelConfig(layers=options.layers, bits=options.bits, experts=options.experts,
+                              chosen=min(2, max(1, options.experts)))
     model = TokenModel(config, options.batch, options.prompt + 2 * options.steps + 8)
     make = torch.Generator(device="cuda").manual_seed(1)
     prompt = torch.randint(0, config.symbols, (options.batch, options.prompt), generator=make, device="cuda")
     symbols = model.advance(prompt)[:, -1:].argmax(-1)
+    uniforms = torch.zeros((options.batch,), device="cuda")
 
     def step(x: torch.Tensor) -> torch.Tensor:
-        return model.advance(x).argmax(-1)
+        if options.temperature <= 0:
+            return model.advance(x).argmax(-1)
+        return model.step(x, uniforms, temperature=options.temperature, top_p=options.top_p)
 
     for _ in range(4):
         symbols = step(symbols)
     torch.cuda.synchronize()
     began = time.perf_counter()
     for _ in range(options.steps):
+        uniforms.uniform_(generator=make)
         symbols = step(symbols)
     torch.cuda.synchronize()
     eager = (time.perf_counter() - began) / options.steps
@@ -165,6 +216,7 @@ def main() -> None:
     torch.cuda.synchronize()
     began = time.perf_counter()
     for _ in range(options.steps):
+        uniforms.uniform_(generator=make)
         graph.replay()
     torch.cuda.synchronize()
     captured = (time.perf_counter() - began) / options.steps
