@@ -131,7 +131,72 @@ struct QuantiseArgs {
     float* scales;        // [out_rows]
     void* zeros;          // null, or the output whose rows without a place are zeros
     int outputs;
+    // for blocks that find the places themselves
+    const std::int32_t* choices;
+    int pairs, experts, tile_rows;
+    Arranged arranged;
 };
+
+constexpr int most_own_pairs = 1024;
+
+// The places of a few pairs, found by every block of `quantise_kernel` for itself, which saves a launch: `places` of the
+// block's own pairs first .. first + count - 1. The first block writes the tiles. 256 threads.
+__device__ __forceinline__ void find_places(const QuantiseArgs& a, int first, int count, int* choices, int* starts, int* places) {
+    __shared__ int scratch[16];
+    const int thread = threadIdx.x, lane = thread % 32, warp = thread / 32;
+    for (int e = thread; e < a.experts; e += 256) starts[e] = 0;
+    for (int i = thread; i < a.pairs; i += 256) {
+        const int e = a.choices[i];
+        choices[i] = e >= 0 && e < a.experts ? e : -1;
+    }
+    __syncthreads();
+    for (int i = thread; i < a.pairs; i += 256) {
+        if (choices[i] >= 0) atomicAdd(&starts[choices[i]], 1);
+    }
+    __syncthreads();
+    // a thread a run of experts: their rows, padded, and tiles before its first
+    const int run = (a.experts + 255) / 256, from = min(a.experts, thread * run), to = min(a.experts, from + run);
+    int rows = 0, tiles = 0;
+    for (int e = from; e < to; ++e) {
+        rows += (starts[e] + step_rows - 1) / step_rows * step_rows;
+        tiles += (starts[e] + a.tile_rows - 1) / a.tile_rows;
+    }
+    int row = rows, tile = tiles;
+    for (int o = 1; o < 32; o *= 2) {
+        const int r = __shfl_up_sync(0xffffffffu, row, o), t = __shfl_up_sync(0xffffffffu, tile, o);
+        if (lane >= o) row += r, tile += t;
+    }
+    if (lane == 31) scratch[warp] = row, scratch[8 + warp] = tile;
+    __syncthreads();
+    int all_tiles = 0;
+    for (int w = 0; w < 8; ++w) {
+        if (w < warp) row += scratch[w], tile += scratch[8 + w];
+        all_tiles += scratch[8 + w];
+    }
+    row -= rows, tile -= tiles;
+    for (int e = from; e < to; ++e) {
+        const int have = starts[e];
+        starts[e] = row;
+        if (blockIdx.x == 0) {
+            for (int t = 0; t * a.tile_rows < have; ++t) {
+                a.arranged.tiles[tile++] = {e, row + t * a.tile_rows, min(a.tile_rows, have - t * a.tile_rows), 0};
+            }
+        }
+        row += (have + step_rows - 1) / step_rows * step_rows;
+    }
+    if (blockIdx.x == 0 && thread == 0) *a.arranged.tile_count = all_tiles;
+    __syncthreads();
+    for (int n = warp; n < count; n += 8) {  // a warp a pair: those with the same expert before it
+        const int i = first + n, e = choices[i];
+        int before = 0;
+        for (int j = 0; j < i; j += 32) before += __popc(__ballot_sync(0xffffffffu, j + lane < i && choices[j + lane] == e));
+        if (lane == 0) {
+            places[n] = e < 0 ? -1 : starts[e] + before;
+            if (e >= 0) a.arranged.pair[starts[e] + before] = i;
+        }
+    }
+    __syncthreads();
+}
 
 // Sixteen values of a row as they are in memory.
 template <typename T>
@@ -190,12 +255,17 @@ struct Sixteen {
 
 // Warps warps a row, a thread 16 values at a time, of which the first Held stay in registers between the row's maximum and
 // its codes; longer rows are read again. One warp a row, with the whole of it in registers, where there are rows for all
-// warps of an SM: 8192 x 4096 BF16 30 -> @@ us.
-template <typename T, int Warps, int Held>
+// warps of an SM: 8192 x 4096 BF16 30 -> 24 us.
+template <typename T, int Warps, int Held, bool Arrange>
 __global__ void __launch_bounds__(256) quantise_kernel(QuantiseArgs a) {
+    extern __shared__ int own[];  // Arrange: places of the block's pairs, then choices and starts
     constexpr int threads = Warps * 32;
     __shared__ unsigned maxima[8];
     join_chain();
+    if constexpr (Arrange) {
+        const int first = static_cast<int>(blockIdx.x) * (8 / Warps) * a.fan, room = 8 / Warps * a.fan;
+        find_places(a, first, min(room, a.pairs - first), own + room, own + room + a.pairs, own);
+    }
     const int part = threadIdx.x % threads;
     const std::int64_t row = blockIdx.x * static_cast<std::int64_t>(8 / Warps) + threadIdx.x / threads;
     const bool there = row < a.rows;
@@ -236,13 +306,17 @@ __global__ void __launch_bounds__(256) quantise_kernel(QuantiseArgs a) {
         most = widen(reinterpret_cast<const T&>(bits));
     }
     const RowScale scale(most);
+    auto place = [&](int f) -> std::int64_t {
+        if constexpr (Arrange) return own[static_cast<int>(threadIdx.x) / threads * a.fan + f];
+        return a.place == nullptr ? row : a.place[row * a.fan + f];
+    };
     auto store = [&](const Sixteen<T>& sixteen, int piece) {
         float v[16];
         sixteen.values(v);
         const uint4 words = scale.codes(v);
         std::uint8_t* block = a.codes + piece / 8 * a.out_rows * block_bytes;
         for (int f = 0; f < a.fan; ++f) {
-            const std::int64_t to = a.place == nullptr ? row : a.place[row * a.fan + f];
+            const std::int64_t to = place(f);
             if (to >= 0) reinterpret_cast<uint4*>(block + to * block_bytes)[(piece % 8) ^ static_cast<int>(to & 7)] = words;
         }
     };
@@ -257,12 +331,12 @@ __global__ void __launch_bounds__(256) quantise_kernel(QuantiseArgs a) {
         store(v, piece);
     }
     for (int f = part; f < a.fan; f += threads) {
-        const std::int64_t to = a.place == nullptr ? row : a.place[row * a.fan + f];
+        const std::int64_t to = place(f);
         if (to >= 0) a.scales[to] = scale.told();
     }
     if (a.zeros != nullptr) {
         for (int f = 0; f < a.fan; ++f) {
-            if (a.place[row * a.fan + f] >= 0) continue;
+            if (place(f) >= 0) continue;
             T* out = static_cast<T*>(a.zeros) + (row * a.fan + f) * a.outputs;
             for (int i = part; i < a.outputs; i += threads) out[i] = narrow<T>(0.0f);
         }
@@ -871,8 +945,10 @@ __global__ void __launch_bounds__(128) combine_kernel(const float* products, con
 
 template <typename T, int Warps, int Held>
 cudaError_t quantise_rows(const QuantiseArgs& a, cudaStream_t stream) {
-    const std::int64_t blocks = (a.rows + 8 / Warps - 1) / (8 / Warps);
-    return launch_overlapped(quantise_kernel<T, Warps, Held>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
+    const auto blocks = static_cast<unsigned>((a.rows + 8 / Warps - 1) / (8 / Warps));
+    if (a.choices == nullptr) return launch_overlapped(quantise_kernel<T, Warps, Held, false>, dim3(blocks), dim3(256), 0, stream, a);
+    const std::size_t shared = sizeof(int) * (static_cast<std::size_t>(8 / Warps) * a.fan + a.pairs + a.experts);
+    return launch_overlapped(quantise_kernel<T, Warps, Held, true>, dim3(blocks), dim3(256), shared, stream, a);
 }
 
 template <typename T>
@@ -984,10 +1060,11 @@ cudaError_t product(Type type, const ProductArgs& a, std::int64_t most_items, bo
 
 constexpr int most_split_tile = 64;  // rows of a tile that a cluster shares: its sums have a place of their own
 
-// Blocks that share a tile's inputs: while they all run at once and each has two blocks of them.
+// Blocks that share a tile's inputs: while they all run at once and each has two blocks of them. No more than four: of
+// clusters of eight blocks with an SM each, 16 do not run at once (16 rows of 2048 -> 2048 11.4 us, 7.6 by four).
 int splits_of(std::int64_t items, int tile_rows, int k_blocks) {
     int splits = 1;
-    while (tile_rows <= most_split_tile && splits < 8 && items * splits * 2 <= sm_count() && k_blocks >= splits * 4) splits *= 2;
+    while (tile_rows <= most_split_tile && splits < 4 && items * splits * 2 <= sm_count() && k_blocks >= splits * 4) splits *= 2;
     return splits;
 }
 
@@ -999,28 +1076,28 @@ struct Shape {
 // Rows a tile, and the kernel: what takes the fewest cycles by a model. A block of inputs is loaded at 60 bytes a cycle or
 // multiplied at two cycles a row (at least 240); a tile's stores, which overlap the next tile's products, take 24 cycles a
 // row.
-Shape shape_of(double groups, double rows, int tiles, int k_blocks) {
+Shape shape_of(bool experts, double groups, double rows, int tiles, int k_blocks) {
     Shape best{step_rows, false};
     double least = -1.0;
     for (const bool pair : {false, true}) {
         const int step = pair ? pair_step_rows : step_rows, sets = sm_count() / (pair ? 2 : 1);
         for (int n = step; n <= most_tile; n += step) {
             // rows of a group are spread around their mean, so beyond one tile the last is half full
-            const double items = groups * (pair ? (tiles + 1) / 2 : tiles) * (groups == 1.0 ? std::ceil(rows / n) : std::max(1.0, rows / n + 0.5));
+            const double items = groups * (pair ? (tiles + 1) / 2 : tiles) * (!experts ? std::ceil(rows / n) : std::max(1.0, rows / n + 0.5));
             const int splits = pair ? 1 : splits_of(static_cast<std::int64_t>(items), n, k_blocks);
             const double block = std::max({(weight_block + (pair ? n / 2 : n) * block_bytes) / 60.0, 2.0 * n, 240.0});
             const double product = std::ceil(static_cast<double>(k_blocks) / splits) * block, stores = 600.0 + 24.0 * n;
             const double cost = std::ceil(items * splits / sets) * std::max(product, stores) + stores + (splits > 1 ? 1500.0 : 0.0) + (pair ? 1500.0 : 0.0);
             if (least < 0.0 || cost < least) least = cost, best = {n, pair};
-            if (n >= rows && groups == 1.0) break;
+            if (n >= rows && !experts) break;
         }
     }
     return best;
 }
 
+// Where the parts of a call's working memory are: for any shape of its tiles, which takes a microsecond to choose.
 struct Plan {
-    Shape shape;
-    std::int64_t out_rows, tiles;
+    std::int64_t out_rows, groups;
     std::size_t codes, scales, place, pair, table, count, products, bytes;
 };
 
@@ -1033,24 +1110,14 @@ Plan plan_of(const BytesArgs& a) {
         at += aligned(bytes);
         return here;
     };
-    if (a.choices == nullptr) {
-        p.shape = shape_of(1.0, static_cast<double>(std::max<std::int64_t>(a.tokens, 1)), tiles_of(a.outputs), blocks_of(a.inputs));
-        p.out_rows = padded(a.tokens);
-        p.tiles = (a.tokens + p.shape.tile_rows - 1) / p.shape.tile_rows;
-    } else {
-        const std::int64_t groups = std::min<std::int64_t>(a.experts, pairs);
-        p.shape = shape_of(static_cast<double>(std::max<std::int64_t>(groups, 1)),
-                           static_cast<double>(pairs) / static_cast<double>(std::max<std::int64_t>(groups, 1)), tiles_of(a.outputs),
-                           blocks_of(a.inputs));
-        p.out_rows = padded(pairs + groups * (step_rows - 1));
-        p.tiles = pairs / p.shape.tile_rows + groups;
-    }
+    p.groups = a.choices == nullptr ? 1 : std::max<std::int64_t>(std::min<std::int64_t>(a.experts, pairs), 1);
+    p.out_rows = a.choices == nullptr ? padded(a.tokens) : padded(pairs + p.groups * (step_rows - 1));
     p.codes = take(static_cast<std::size_t>(blocks_of(a.inputs)) * p.out_rows * block_bytes);
     p.scales = take(p.out_rows * sizeof(float));
     if (a.choices != nullptr) {
         p.place = take(pairs * sizeof(int));
         p.pair = take(p.out_rows * sizeof(int));
-        p.table = take(p.tiles * sizeof(int4));
+        p.table = take((pairs / step_rows + p.groups) * sizeof(int4));
         p.count = take(sizeof(int));
         if (a.weights != nullptr) p.products = take(static_cast<std::size_t>(pairs) * a.outputs * sizeof(float));
     }
@@ -1090,17 +1157,25 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
     const Plan p = plan_of(a);
     auto* memory = static_cast<std::uint8_t*>(a.workspace);
     const std::int64_t pairs = a.tokens * a.chosen;
+    const Shape shape = shape_of(a.choices != nullptr, static_cast<double>(p.groups), static_cast<double>(pairs) / static_cast<double>(p.groups),
+                                 tiles_of(a.outputs), blocks_of(a.inputs));
+    const std::int64_t row_tiles = a.choices == nullptr ? (pairs + shape.tile_rows - 1) / shape.tile_rows : pairs / shape.tile_rows + p.groups;
     const int elements = a.type == Type::f32 ? 4 : 2;
     Arranged arranged{};
     if (a.choices != nullptr) {
         arranged = {reinterpret_cast<int*>(memory + p.place), reinterpret_cast<int*>(memory + p.pair),
                     reinterpret_cast<int4*>(memory + p.table), reinterpret_cast<int*>(memory + p.count)};
-        const cudaError_t status = launch_overlapped(arrange_kernel, dim3(1), dim3(arrange_threads),
-                                                     (a.experts + 64) * sizeof(int), stream, a.choices, pairs, a.experts,
-                                                     p.shape.tile_rows, arranged);
-        if (status != cudaSuccess) return status;
     }
     QuantiseArgs q{};
+    if (a.choices != nullptr && pairs <= most_own_pairs) {
+        q.choices = a.choices, q.pairs = static_cast<int>(pairs), q.experts = a.experts, q.tile_rows = shape.tile_rows;
+        q.arranged = arranged;
+    } else if (a.choices != nullptr) {
+        const cudaError_t status = launch_overlapped(arrange_kernel, dim3(1), dim3(arrange_threads),
+                                                     (a.experts + 64) * sizeof(int), stream, a.choices, pairs, a.experts,
+                                                     shape.tile_rows, arranged);
+        if (status != cudaSuccess) return status;
+    }
     q.x = a.x, q.stride = a.x_stride, q.inner_stride = a.x_inner_stride;
     q.inner = a.inner;
     q.rows = a.tokens * q.inner;
@@ -1119,23 +1194,23 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
     r.codes = q.codes, r.row_scales = q.scales, r.arranged = arranged;
     r.rows = a.tokens, r.out_rows = p.out_rows;
     r.experts = a.experts, r.outputs = a.outputs, r.tiles = tiles_of(a.outputs), r.k_blocks = q.k_blocks;
-    r.tile_rows = p.shape.tile_rows;
-    const std::int64_t items = p.tiles * (p.shape.pair ? (r.tiles + 1) / 2 : r.tiles);
+    r.tile_rows = shape.tile_rows;
+    const std::int64_t items = row_tiles * (shape.pair ? (r.tiles + 1) / 2 : r.tiles);
     if (items > INT32_MAX - 1024) return cudaErrorInvalidValue;  // tiles are counted in 32 bits
-    r.splits = p.shape.pair ? 1 : splits_of(items, r.tile_rows, r.k_blocks);
+    r.splits = shape.pair ? 1 : splits_of(items, r.tile_rows, r.k_blocks);
     r.status = a.status;
     if (a.choices == nullptr) {
         r.y = a.y;
-        return product<false>(a.type, r, items, p.shape.pair, stream);
+        return product<false>(a.type, r, items, shape.pair, stream);
     }
     if (a.weights == nullptr) {
         r.y = a.y;
-        return product<true>(a.type, r, items, p.shape.pair, stream);
+        return product<true>(a.type, r, items, shape.pair, stream);
     }
     auto* products = reinterpret_cast<float*>(memory + p.products);
     r.y = products;
     // FP32 products, so that a token's sum is rounded once
-    status = product<true>(Type::f32, r, items, p.shape.pair, stream);
+    status = product<true>(Type::f32, r, items, shape.pair, stream);
     if (status != cudaSuccess) return status;
     switch (a.type) {
     case Type::f16: return combine<__half>(a, products, stream);

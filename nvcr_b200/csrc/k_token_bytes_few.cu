@@ -301,11 +301,16 @@ int power_of_two(int n) {
 
 }  // namespace
 
+// One or two rows always. Every block takes all rows as codes for itself and multiplies without the tensor cores, so with
+// more rows only where there is little to multiply: 3 rows of 4096 -> 4096 (50 M products) 8.7 us here and 9.1 by the tensor
+// cores, 4 rows 9.4 and 9.1, 8 rows of 1024 -> 1024 5.5 and 8.0, of 4096 -> 16384 26.6 and 17.9. By experts, whose other
+// way takes three launches: 4 tokens by 8 of 128, 2048 -> 1024 (67 M), 13 us and 23; 32 tokens by 2 of 8 (134 M) 20 and 15.
 bool few_rows(const BytesArgs& a) {
-    const int rows = a.choices == nullptr ? static_cast<int>(std::min<std::int64_t>(a.tokens, 1 << 20)) : a.inner;
-    if (power_of_two(std::min(rows, 1024)) * blocks_of(a.inputs) > most_room / block_bytes) return false;
-    if (a.choices == nullptr) return rows <= 8;
-    return a.chosen <= most_chosen && a.tokens * a.chosen <= 64;
+    const std::int64_t rows = a.choices == nullptr ? a.tokens : a.inner, pairs = a.choices == nullptr ? a.tokens : a.tokens * a.chosen;
+    if (rows > 16 || power_of_two(static_cast<int>(rows)) * blocks_of(a.inputs) > most_room / block_bytes) return false;
+    const std::int64_t products = static_cast<std::int64_t>(a.inputs) * a.outputs;
+    if (a.choices == nullptr) return rows <= 2 || (rows <= 8 && rows * products <= 3 << 24);
+    return a.chosen <= most_chosen && pairs <= 64 && pairs * products <= 1 << 26;
 }
 
 cudaError_t multiply_few(const BytesArgs& a, cudaStream_t stream) {
