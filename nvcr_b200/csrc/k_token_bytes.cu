@@ -48,6 +48,26 @@ __global__ void __launch_bounds__(256) pack_kernel(const std::int8_t* codes, std
     }
 }
 
+// ---- clusters ----
+
+__device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ int peer_load(const int* here, int rank) {
+    int v;
+    asm volatile("{\n\t.reg .b32 there;\n\tmapa.shared::cluster.u32 there, %1, %2;\n\tld.shared::cluster.b32 %0, [there];\n\t}"
+                 : "=r"(v)
+                 : "r"(smem_address(here)), "r"(rank)
+                 : "memory");
+    return v;
+}
+
 // ---- where the rows of each expert go ----
 
 constexpr int arrange_threads = 1024;
@@ -59,60 +79,69 @@ struct Arranged {
     int* tile_count;
 };
 
-// One block. Which of an expert's rows a pair gets is decided by atomics, and changes no output: rows are independent
-// and their sums exact.
-__global__ void __launch_bounds__(arrange_threads) arrange_kernel(const std::int32_t* choices, std::int64_t pairs, int experts,
-                                                                  int tile_rows, Arranged out) {
-    extern __shared__ int shared[];
-    int* counts = shared;             // [experts], then the next row of each
-    int* scratch = shared + experts;  // two sums of each warp
-    join_chain();
+constexpr int arrange_blocks = 8;
+
+// One cluster, a part of the pairs each block's; a thread an expert. Which of an expert's rows a pair gets is decided by
+// atomics, and changes no output: rows are independent and their sums exact. 16384 pairs of 32 experts: 9.7 us, 11
+// by one block, which more pairs would keep longer.
+__global__ void __cluster_dims__(arrange_blocks, 1, 1) __launch_bounds__(arrange_threads)
+    arrange_kernel(const std::int32_t* choices, std::int64_t pairs, int experts, int tile_rows, Arranged out) {
+    __shared__ int counts[arrange_threads], next[arrange_threads], scratch[64];
+    static_assert(most_experts <= arrange_threads);
     const int thread = threadIdx.x, lane = thread % 32, warp = thread / 32;
-    for (int e = thread; e < experts; e += arrange_threads) counts[e] = 0;
+    const int rank = static_cast<int>(blockIdx.x);
+    counts[thread] = 0;
+    join_chain();
     __syncthreads();
+    const std::int64_t from = pairs * rank / arrange_blocks, to = pairs * (rank + 1) / arrange_blocks;
 #pragma unroll 4
-    for (std::int64_t i = thread; i < pairs; i += arrange_threads) {
+    for (std::int64_t i = from + thread; i < to; i += arrange_threads) {
         const int e = choices[i];
         if (e >= 0 && e < experts) atomicAdd(&counts[e], 1);
     }
+    cluster_arrive();
+    cluster_wait();
+    int count = 0, before = 0;  // of the expert: all, and those of earlier blocks
+    int some[arrange_blocks];
+#pragma unroll
+    for (int b = 0; b < arrange_blocks; ++b) some[b] = peer_load(&counts[thread], b);
+#pragma unroll
+    for (int b = 0; b < arrange_blocks; ++b) count += some[b], before += b < rank ? some[b] : 0;
+    cluster_arrive();  // the others' counts are read
+    const int rows = (count + step_rows - 1) / step_rows * step_rows;
+    const int tiles = (count + tile_rows - 1) / tile_rows;
+    int row = rows, tile = tiles;
+    for (int o = 1; o < 32; o *= 2) {
+        const int r = __shfl_up_sync(0xffffffffu, row, o), t = __shfl_up_sync(0xffffffffu, tile, o);
+        if (lane >= o) row += r, tile += t;
+    }
+    if (lane == 31) scratch[warp] = row, scratch[32 + warp] = tile;
     __syncthreads();
-    int first_row = 0, first_tile = 0;
-    for (int from = 0; from < experts; from += arrange_threads) {
-        const int e = from + thread;
-        const int count = e < experts ? counts[e] : 0;
-        const int rows = (count + step_rows - 1) / step_rows * step_rows;
-        const int tiles = (count + tile_rows - 1) / tile_rows;
-        int row = rows, tile = tiles;
-        for (int o = 1; o < 32; o *= 2) {
-            const int r = __shfl_up_sync(0xffffffffu, row, o), t = __shfl_up_sync(0xffffffffu, tile, o);
-            if (lane >= o) row += r, tile += t;
-        }
-        if (lane == 31) scratch[warp] = row, scratch[32 + warp] = tile;
-        __syncthreads();
-        int rows_before = 0, tiles_before = 0, all_rows = 0, all_tiles = 0;
-        for (int w = 0; w < arrange_threads / 32; ++w) {
-            if (w < warp) rows_before += scratch[w], tiles_before += scratch[32 + w];
-            all_rows += scratch[w], all_tiles += scratch[32 + w];
-        }
-        row += first_row + rows_before - rows, tile += first_tile + tiles_before - tiles;
+    int all_tiles = 0;
+    for (int w = 0; w < arrange_threads / 32; ++w) {
+        if (w < warp) row += scratch[w], tile += scratch[32 + w];
+        all_tiles += scratch[32 + w];
+    }
+    row -= rows, tile -= tiles;
+    if (rank == 0) {
         for (int t = 0; t < tiles; ++t) {
-            out.tiles[tile + t] = {e, row + t * tile_rows, min(tile_rows, count - t * tile_rows), 0};
+            out.tiles[tile + t] = {thread, row + t * tile_rows, min(tile_rows, count - t * tile_rows), 0};
         }
-        if (e < experts) counts[e] = row;
-        first_row += all_rows, first_tile += all_tiles;
-        __syncthreads();
+        if (thread == 0) *out.tile_count = all_tiles;
     }
-    if (thread == 0) *out.tile_count = first_tile;
+    next[thread] = row + before;
+    __syncthreads();
 #pragma unroll 4
-    for (std::int64_t i = thread; i < pairs; i += arrange_threads) {
+    for (std::int64_t i = from + thread; i < to; i += arrange_threads) {
         const int e = choices[i];
-        int row = -1;
+        int at = -1;
         if (e >= 0 && e < experts) {
-            row = atomicAdd(&counts[e], 1);
-            out.pair[row] = static_cast<int>(i);
+            at = atomicAdd(&next[e], 1);
+            out.pair[at] = static_cast<int>(i);
         }
-        out.place[i] = row;
+        out.place[i] = at;
     }
+    cluster_wait();
 }
 
 // ---- rows as codes ----
@@ -379,15 +408,6 @@ __device__ __forceinline__ void bulk_load(std::uint32_t to, const void* from, st
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
                  "l"(__cvta_generic_to_global(from)), "r"(bytes), "r"(barrier)
                  : "memory");
-}
-
-__device__ __forceinline__ void cluster_arrive() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
-    __syncwarp();
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ void peer_store(std::uint32_t address, int rank, int v) {
@@ -1171,9 +1191,8 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
         q.choices = a.choices, q.pairs = static_cast<int>(pairs), q.experts = a.experts, q.tile_rows = shape.tile_rows;
         q.arranged = arranged;
     } else if (a.choices != nullptr) {
-        const cudaError_t status = launch_overlapped(arrange_kernel, dim3(1), dim3(arrange_threads),
-                                                     (a.experts + 64) * sizeof(int), stream, a.choices, pairs, a.experts,
-                                                     shape.tile_rows, arranged);
+        const cudaError_t status = launch_overlapped(arrange_kernel, dim3(arrange_blocks), dim3(arrange_threads), 0, stream, a.choices,
+                                                     pairs, a.experts, shape.tile_rows, arranged);
         if (status != cudaSuccess) return status;
     }
     q.x = a.x, q.stride = a.x_stride, q.inner_stride = a.x_inner_stride;
