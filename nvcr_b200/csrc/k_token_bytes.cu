@@ -939,26 +939,26 @@ __global__ void __launch_bounds__(128) combine_kernel(const float* products, con
                                                       int chosen, int experts, int outputs, T* y) {
     join_chain();
     const std::int64_t token = blockIdx.x;
-    const int output = static_cast<int>(blockIdx.y * 128 + threadIdx.x) * Each;
-    if (output >= outputs) return;
-    float sum[Each] = {};
+    for (int output = static_cast<int>(blockIdx.y * 128 + threadIdx.x) * Each; output < outputs; output += static_cast<int>(gridDim.y) * 128 * Each) {
+        float sum[Each] = {};
 #pragma unroll 4
-    for (int j = 0; j < chosen; ++j) {
-        const std::int64_t pair = token * chosen + j;
-        const int e = choices[pair];
-        if (e < 0 || e >= experts) continue;
-        const float weight = weights[pair];
-        const float* from = products + pair * outputs + output;
-        if constexpr (Each == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(from);
-            sum[0] = fmaf(weight, v.x, sum[0]), sum[1] = fmaf(weight, v.y, sum[1]);
-            sum[2] = fmaf(weight, v.z, sum[2]), sum[3] = fmaf(weight, v.w, sum[3]);
-        } else {
-            sum[0] = fmaf(weight, *from, sum[0]);
+        for (int j = 0; j < chosen; ++j) {
+            const std::int64_t pair = token * chosen + j;
+            const int e = choices[pair];
+            if (e < 0 || e >= experts) continue;
+            const float weight = weights[pair];
+            const float* from = products + pair * outputs + output;
+            if constexpr (Each == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(from);
+                sum[0] = fmaf(weight, v.x, sum[0]), sum[1] = fmaf(weight, v.y, sum[1]);
+                sum[2] = fmaf(weight, v.z, sum[2]), sum[3] = fmaf(weight, v.w, sum[3]);
+            } else {
+                sum[0] = fmaf(weight, *from, sum[0]);
+            }
         }
-    }
 #pragma unroll
-    for (int i = 0; i < Each; ++i) y[token * outputs + output + i] = narrow<T>(sum[i]);
+        for (int i = 0; i < Each; ++i) y[token * outputs + output + i] = narrow<T>(sum[i]);
+    }
 }
 
 // ---- launches ----
@@ -1148,7 +1148,7 @@ Plan plan_of(const BytesArgs& a) {
 template <typename T>
 cudaError_t combine(const BytesArgs& a, const float* products, cudaStream_t stream) {
     const int each = a.outputs % 4 == 0 ? 4 : 1;
-    const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>((a.outputs + 128 * each - 1) / (128 * each)));
+    const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(std::min((a.outputs + 128 * each - 1) / (128 * each), 65535)));
     auto kernel = each == 4 ? combine_kernel<T, 4> : combine_kernel<T, 1>;
     return launch_overlapped(kernel, grid, dim3(128), 0, stream, products, a.choices, a.weights, a.chosen, a.experts, a.outputs,
                              static_cast<T*>(a.y));
@@ -1181,6 +1181,7 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
                                  tiles_of(a.outputs), blocks_of(a.inputs));
     const std::int64_t row_tiles = a.choices == nullptr ? (pairs + shape.tile_rows - 1) / shape.tile_rows : pairs / shape.tile_rows + p.groups;
     const int elements = a.type == Type::f32 ? 4 : 2;
+    if (row_tiles * tiles_of(a.outputs) > INT32_MAX - 1024) return cudaErrorInvalidValue;  // tiles are counted in 32 bits
     Arranged arranged{};
     if (a.choices != nullptr) {
         arranged = {reinterpret_cast<int*>(memory + p.place), reinterpret_cast<int*>(memory + p.pair),
@@ -1215,7 +1216,6 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
     r.experts = a.experts, r.outputs = a.outputs, r.tiles = tiles_of(a.outputs), r.k_blocks = q.k_blocks;
     r.tile_rows = shape.tile_rows;
     const std::int64_t items = row_tiles * (shape.pair ? (r.tiles + 1) / 2 : r.tiles);
-    if (items > INT32_MAX - 1024) return cudaErrorInvalidValue;  // tiles are counted in 32 bits
     r.splits = shape.pair ? 1 : splits_of(items, r.tile_rows, r.k_blocks);
     r.status = a.status;
     if (a.choices == nullptr) {

@@ -732,6 +732,81 @@ def test_streams_and_graphs(cuda):
         assert same(outs[1], replayed) and same(step(), replayed)
 
 
+def test_large_calls_in_graphs(cuda):
+    """A prompt's product, experts of many pairs and the sampling of many rows, captured twice and replayed at once on two
+    streams with new inputs, and with shares of the work that change from replay to replay."""
+    import torch
+
+    from nvcr_b200 import tokens
+
+    matrix = tokens.ByteMatrix.quantise(normal((2100, 512), 1, 0.1))
+    experts = tokens.ByteExperts.quantise(normal((6, 700, 512), 2, 0.1))
+    x, weights = normal((1500, 512), 3).bfloat16(), torch.rand((1500, 2), device="cuda")
+    choices = some_choices(1500, 2, 6, 4)
+    logits, u = normal((200, 40000), 5, 3.0).bfloat16(), torch.rand(200, device="cuda")
+    top_p = torch.full((200,), 0.8, device="cuda")
+
+    def step():
+        return (matrix.multiply(x), experts.multiply(x, choices, weights), experts.multiply(x, choices),
+                *tokens.sample(logits, u, temperature=0.9, top_p=top_p))
+
+    same = lambda a, b: all(torch.equal(p, q) for p, q in zip(a, b))  # noqa: E731
+    step()
+    torch.cuda.synchronize()
+    side, graphs, outs = torch.cuda.Stream(), [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step())
+    for seed, kind in ((7, "one"), (8, "absent"), (9, "skewed")):
+        x.copy_(normal((1500, 512), seed).bfloat16())
+        choices.copy_(some_choices(1500, 2, 6, seed, kind))
+        logits.copy_(normal((200, 40000), seed, float(seed - 5)).bfloat16())
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in outs[0]]
+        assert same(outs[1], replayed) and same(step(), replayed)
+    matrix.check(), experts.check()
+
+
+def test_weights_written_just_before(cuda):
+    """A product enqueued right behind the kernels that write its weights, again and again with other ones."""
+    import torch
+
+    from nvcr_b200.tokens import ByteMatrix
+
+    x = torch.ones((1, 4096), device="cuda")
+    codes = torch.empty((4096, 4096), dtype=torch.int8, device="cuda")
+    scales = torch.ones(4096, device="cuda")
+    out = []
+    for n in range(30):
+        codes.fill_(n + 1)
+        out.append(ByteMatrix(codes, scales).multiply(x))
+    for n, y in enumerate(out):
+        want = (n + 1) * 127 * 4096 * torch.tensor(1.0 / 127.0)
+        assert (y - want).abs().max() <= 4 * E * want, n
+
+
+def test_results_are_the_same_bits_again(cuda):
+    """Whatever atomics decide inside: the same calls give the same bits."""
+    import torch
+
+    from nvcr_b200 import tokens
+
+    experts = tokens.ByteExperts(some_codes((9, 300, 256), 1), normal((9, 300), 2, 0.01).abs())
+    x, weights, choices = normal((3000, 256), 3).half(), normal((3000, 3), 4), some_choices(3000, 3, 9, 5, "absent")
+    logits, u = normal((180, 50001), 6, 2.0).half(), torch.rand(180, device="cuda")
+    calls = [lambda: (experts.multiply(x, choices, weights),), lambda: tokens.sample(logits, u, top_p=0.95),
+             lambda: tokens.sample(logits[:1], u[:1], top_k=2000), lambda: tokens.route(logits[:, :256], 8, kind="sigmoid")]
+    for call in calls:
+        first = [t.clone() for t in call()]
+        for _ in range(5):
+            assert all(torch.equal(a, b) for a, b in zip(first, call()))
+
+
 def test_workspaces_of_a_given_stream_are_its_own(cuda):
     """A call on a busy stream keeps its working memory until that stream has run it."""
     import torch
