@@ -127,7 +127,8 @@ __device__ __forceinline__ void make_table(double* table) {
 }
 
 struct Sums {
-    unsigned low[bins], high[bins];  // counts in low, or halves of the weights' sums
+    alignas(16) unsigned low[bins];  // counts, or halves of the weights' sums
+    alignas(16) unsigned high[bins];
     Weight scratch[warps];
     Weight found_weight;
     int found;
@@ -319,7 +320,12 @@ __device__ __forceinline__ void put(const void* here, int rank, unsigned long lo
 }
 __device__ __forceinline__ unsigned get(const unsigned* here, int rank) {
     unsigned v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at_block(here, rank)) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at_block(here, rank)));
+    return v;
+}
+__device__ __forceinline__ uint4 get_four(const unsigned* here, int rank) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at_block(here, rank)));
     return v;
 }
 
@@ -648,16 +654,26 @@ const int n = cell / warps;
         cluster_sync();
         if (rank == 0) {
             constexpr int run = bins / threads;
-            Weight mine[run], all = 0, sum = 0;
+            static_assert(run == 4);
+            Weight mine[run] = {0, 0, 0, 0}, all = 0, sum = 0;
+            const int first_bin = run * static_cast<int>(threadIdx.x);
+#pragma unroll 1
+            for (int from = 0; from < blocks; from += 4) {  // four blocks' loads under way: each takes some 700 cycles
+                uint4 low[4], high[4];
 #pragma unroll
-            for (int i = 0; i < run; ++i) {
-                const int bin = run * static_cast<int>(threadIdx.x) + i;
-                mine[i] = 0;
-                for (int b = 0; b < blocks; ++b) {
-                    mine[i] += static_cast<Weight>(get(&sums.high[bin], b)) << 32 | get(&sums.low[bin], b);
+                for (int b = 0; b < 4; ++b) {
+                    const int of = min(from + b, blocks - 1);
+                    low[b] = get_four(&sums.low[first_bin], of), high[b] = get_four(&sums.high[first_bin], of);
                 }
-                sum += mine[i];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    if (from + b >= blocks) break;
+                    mine[0] += static_cast<Weight>(high[b].x) << 32 | low[b].x, mine[1] += static_cast<Weight>(high[b].y) << 32 | low[b].y;
+                    mine[2] += static_cast<Weight>(high[b].z) << 32 | low[b].z, mine[3] += static_cast<Weight>(high[b].w) << 32 | low[b].w;
+                }
             }
+#pragma unroll
+            for (int i = 0; i < run; ++i) sum += mine[i];
             Weight earlier = before(sum, sums.scratch, all);
             const Weight want = wanted_of(all);
 #pragma unroll
@@ -1043,7 +1059,11 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
             cluster_sync();
             Weight mine = 0, all;
             if (threadIdx.x < cut_bins) {
-                for (int b = 0; b < blocks; ++b) mine += get(&shared.sums.low[threadIdx.x], b);
+                unsigned some[most_blocks];
+#pragma unroll
+                for (int b = 0; b < most_blocks; ++b) some[b] = get(&shared.sums.low[threadIdx.x], min(b, blocks - 1));
+#pragma unroll
+                for (int b = 0; b < most_blocks; ++b) mine += b < blocks ? some[b] : 0;
             }
             const Weight earlier = before(mine, shared.sums.scratch, all), wanted = static_cast<Weight>(s.top_k);
             if (earlier < wanted && earlier + mine >= wanted) shared.cut = static_cast<int>(threadIdx.x) + 1;
