@@ -339,7 +339,7 @@ struct Shared {
     unsigned long long maxima[most_blocks], totals[most_blocks], counts[2][most_blocks], sums_of[2][most_blocks];
     unsigned long long told[2];  // the first block to all
     float parts[2][warps];
-    unsigned count, queued;
+    unsigned count, queued, wide;
     unsigned kept, low, high;
     int cut;
 };
@@ -582,11 +582,11 @@ const int n = cell / warps;
     __device__ __forceinline__ int collect(const unsigned long long* counts, int part) {
         unsigned long long* from = shared.gathered;
         int n = 0;
-        for (int b = 0; b < blocks; ++b) n += static_cast<int>(counts[b]);
+        for (int b = 0; b < blocks; ++b) n += static_cast<int>(counts[b] & 0xffffffffu);
         unsigned long long* to = n <= threads ? shared.weights : shared.sorted;
         n = 0;
         for (int b = 0; b < blocks; ++b) {
-            const int count = static_cast<int>(counts[b]);
+            const int count = static_cast<int>(counts[b] & 0xffffffffu);
             for (int i = threadIdx.x; i < count; i += threads) to[n + i] = from[b * part + i];
             n += count;
         }
@@ -700,8 +700,9 @@ const int n = cell / warps;
     __device__ __noinline__ Kept find(const Row& row, const Settings& s, bool by_weight, float largest, float factor, Kept kept) {
         const int part = most_candidates / blocks;
         const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+        auto octave_of = [&](float l) { return __fmul_rn(__fsub_rn(l, largest), -44.0f * factor); };
         auto octave_bin = [&](float l) {
-            const float x = __fmul_rn(__fsub_rn(l, largest), -44.0f * factor);
+            const float x = octave_of(l);
             return x < static_cast<float>(bins) ? static_cast<int>(x) : -1;  // a NaN is in none
         };
         Weight wanted;
@@ -714,14 +715,28 @@ const int n = cell / warps;
             if (threadIdx.x == 0) shared.count = 0;
             __syncthreads();
             unsigned least = 0xffffffffu, most = 0;
+            const float from_logit = turn == 0 ? 0.0f : logit_of(low), to_logit = turn == 0 ? 0.0f : logit_of(high);
             for_vectors([&](int n, const uint4& v) {
+                unsigned in = 0;  // the elements looked at
 #pragma unroll
                 for (int i = 0; i < each; ++i) {
                     const float l = Of::get(v, i);
-                    const unsigned key = key_of(l);
+                    bool here;
+                    if (turn == 0) {
+                        const float x = octave_of(l);
+                        here = x >= static_cast<float>(octave) && x < static_cast<float>(octave + 1);
+                    } else {
+                        here = l >= from_logit && l <= to_logit;
+                    }
+                    in |= here ? 1u << i : 0u;
+                }
+                while (in != 0) {
+                    const int i = __ffs(static_cast<int>(in)) - 1;
+                    in &= in - 1;
+                    const float l = Of::pick(v, i);
                     const int index = first + n * threads * each + i;
-                    if (turn == 0 ? octave_bin(l) != octave : key < low || key > high) continue;
                     if (!kept.holds(l, index)) continue;
+                    const unsigned key = key_of(l);
                     least = min(least, key), most = max(most, key);
                     gather(key, index, part);
                 }
@@ -827,7 +842,7 @@ const int n = cell / warps;
         const int lane = threadIdx.x % 32;
         int filled = 0;
         for (int b = 0; b < blocks; ++b) {
-            const int count = static_cast<int>(counts[b]);
+            const int count = static_cast<int>(counts[b] & 0xffffffffu);
             for (int i = lane; i < count; i += 32) shared.weights[filled + i] = shared.gathered[b * part + i];
             filled += count;
         }
@@ -1011,7 +1026,7 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
 #pragma unroll
     for (int k = 0; k < Vectors; ++k) most = fmaxf(most, Of::largest(v[k]));
     unsigned top = __reduce_max_sync(0xffffffffu, key_of(most));
-    if (threadIdx.x == 0) shared.count = shared.queued = 0;
+    if (threadIdx.x == 0) shared.count = shared.queued = shared.wide = 0;
     if (lane == 0) shared.sums.scratch[warp] = top;
     __syncthreads();
     for (int w = 0; w < warps; ++w) top = max(top, static_cast<unsigned>(shared.sums.scratch[w]));
@@ -1043,6 +1058,7 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
         const double error = bulk_error(largest, factor);
         auto* queue = reinterpret_cast<uint4*>(shared.sorted);  // vectors with a candidate, in sorted and weights
         auto* places = reinterpret_cast<int*>(shared.sums.high);
+        constexpr float wide_cut = -14.5f;
         float cut = -10.0f;
         if (row.least > 0.0) {
             cut = fmaxf(log2f(fminf(s.min_p, 1.0f)) - 0.01f, -46.0f);
@@ -1072,9 +1088,12 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
         }
         for (int turn = 0;; ++turn) {
             float held = 0.0f, rest = 0.0f;  // weights of candidates and of the others
+            unsigned wide = 0;               // vectors with a candidate of the wider cut
 #pragma unroll
             for (int k = 0; k < Vectors; ++k) {
-                if (exponent(Of::largest(v[k])) >= cut) {  // looked at below, by all threads
+                const float x = exponent(Of::largest(v[k]));
+                wide += x >= wide_cut;
+                if (x >= cut) {  // looked at below, by all threads
                     const unsigned nth = atomicAdd(&shared.queued, 1u);
                     if (nth < static_cast<unsigned>(part)) queue[nth] = v[k], places[nth] = first + k * threads * each;
                 } else if (sum_rest) {
@@ -1094,25 +1113,28 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
                 }
             }
             held = warp_sum(held), rest = warp_sum(rest);
-            if (lane == 0) shared.parts[0][warp] = held, shared.parts[1][warp] = rest;
+            wide = __reduce_add_sync(0xffffffffu, wide);
+            if (lane == 0) shared.parts[0][warp] = held, shared.parts[1][warp] = rest, atomicAdd(&shared.wide, wide);
             __syncthreads();
             held = rest = 0.0f;
             for (int w = 0; w < warps; ++w) held += shared.parts[0][w], rest += shared.parts[1][w];
             const int parity = turn & 1;
             if (threadIdx.x < static_cast<unsigned>(blocks)) {
-                put(&shared.counts[parity][rank], static_cast<int>(threadIdx.x), max(shared.count, shared.queued));
+                put(&shared.counts[parity][rank], static_cast<int>(threadIdx.x),
+                    static_cast<unsigned long long>(shared.wide) << 32 | max(shared.count, shared.queued));
                 put(&shared.sums_of[parity][rank], static_cast<int>(threadIdx.x),
                     static_cast<unsigned long long>(__float_as_uint(held)) << 32 | __float_as_uint(rest));
             }
             __syncthreads();
-            if (threadIdx.x == 0) shared.count = shared.queued = 0;
+            if (threadIdx.x == 0) shared.count = shared.queued = shared.wide = 0;
             cluster_sync();
             int count = 0;
-            bool fits = true;
+            bool fits = true, wide_fits = true;
             double all_held = 0.0, bulk = 0.0;
             for (int b = 0; b < blocks; ++b) {
-                const int some = static_cast<int>(shared.counts[parity][b]);
+                const int some = static_cast<int>(shared.counts[parity][b] & 0xffffffffu);
                 fits = fits && some <= part;
+                wide_fits = wide_fits && shared.counts[parity][b] >> 32 <= static_cast<unsigned long long>(part);
                 count += some;
                 const unsigned long long both = shared.sums_of[parity][b];
                 all_held += __uint_as_float(static_cast<unsigned>(both >> 32)), bulk += __uint_as_float(static_cast<unsigned>(both));
@@ -1141,8 +1163,8 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
                 if (!done) row_by_block<T>(a, r, shared.sums, shared.table);
                 return;
             }
-            if (cut < -14.0f) break;
-            cut = -14.5f;
+            if (cut < -14.0f || !wide_fits) break;
+            cut = wide_cut;
         }
     }
     of_cluster.whole(row, s, largest, factor);
