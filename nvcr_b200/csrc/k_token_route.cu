@@ -243,9 +243,9 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
     }
     // How far a share s and its sum b with the bias may be off: of exponents up to 128, rounded twice or three times to 2^-24
     // of themselves, a factor of 1e-5 or 1.6e-5, which a sigmoid has times 1 - s; ex2, rcp and sums 4e-7, a softmax's sum
-    // 2e-6; b 2^-24 of itself; and what is flushed to zero.
+    // 2e-6; b 2^-24 of itself, and as much again with its error added; and what is flushed to zero.
     auto error = [&](float s, float b) {
-        return s * (a.sigmoid ? 4e-7f + (1.0f - s) * 1e-5f : 2e-5f) + 1.2e-7f * fabsf(b) + 1e-37f;
+        return s * (a.sigmoid ? 4e-7f + (1.0f - s) * 1e-5f : 2e-5f) + 1.8e-7f * fabsf(b) + 1e-37f;
     };
     unsigned key[Each];
     float furthest = 0.0f;
@@ -323,8 +323,13 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
     bound = max(1u, __shfl_sync(0xffffffffu, bound, min(a.count, 31)));
     auto* entries = reinterpret_cast<unsigned long long*>(keys);
     int candidates = 0;
+    float reach = -INFINITY;  // the most that an expert behind the candidates may have
 #pragma unroll
     for (int i = 0; i < Each; ++i) {
+        if (key[i] != 0 && key[i] < bound) {
+            const float b = share[i] + bias[i];
+            reach = fmaxf(reach, b + error(share[i], b));
+        }
         const unsigned holders = __ballot_sync(0xffffffffu, key[i] >= bound);
         const int at = candidates + __popc(holders & ((1u << lane) - 1));
         if (key[i] >= bound && at < 32) {
@@ -335,6 +340,8 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
         candidates += __popc(holders);
     }
     __syncwarp();
+    const unsigned reach_key = __reduce_max_sync(0xffffffffu, ordered(reach));
+    const float reach_of_all = value_of(reach_key);
     certain = certain && candidates <= 32;
     const int n = min(candidates, 32);
     const unsigned long long entry = lane < n ? entries[lane] : 0;
@@ -353,10 +360,23 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
     const float s = __shfl_sync(0xffffffffu, mine_here.x, from), mine = __shfl_sync(0xffffffffu, mine_here.y, from),
                 b = __shfl_sync(0xffffffffu, mine_here.z, from);
     {
-        const float after = __shfl_down_sync(0xffffffffu, v, 1), after_s = __shfl_down_sync(0xffffffffu, s, 1),
-                    after_l = __shfl_down_sync(0xffffffffu, mine, 1), after_b = __shfl_down_sync(0xffffffffu, b, 1);
-        const bool near = v - after <= error(s, v) + error(after_s, after) && !(mine == after_l && b == after_b);
-        if (lane < a.count && lane + 1 < n && near) certain = false;
+        // Each choice has to lie above all that come after it by both errors, but for those right after it that have the
+        // same score and bias. Equal ones at the last choice stand for it: the last of them is looked at too.
+        const float off = lane < n ? error(s, v) : 0.0f;
+        float after = lane < n ? v + off : -INFINITY;  // the most of this and of later ones
+        after = fmaxf(after, lane == 31 ? reach_of_all : -INFINITY);
+#pragma unroll
+        for (int apart = 1; apart < 32; apart *= 2) {
+            const float other = __shfl_down_sync(0xffffffffu, after, apart);
+            if (lane + apart < 32) after = fmaxf(after, other);
+        }
+        after = __shfl_down_sync(0xffffffffu, after, 1);
+        if (lane == 31) after = reach_of_all;
+        const float next_l = __shfl_down_sync(0xffffffffu, mine, 1), next_b = __shfl_down_sync(0xffffffffu, b, 1);
+        const bool tied = lane + 1 < n && mine == next_l && b == next_b;
+        const unsigned runs = __ballot_sync(0xffffffffu, tied) >> (a.count - 1);
+        const int last = a.count - 1 + __ffs(static_cast<int>(~runs)) - 1;
+        if (lane <= last && lane < n && !tied && !(v - off > after)) certain = false;
     }
     certain = __all_sync(0xffffffffu, certain);
     if (!certain) {

@@ -485,6 +485,35 @@ def test_route_near_ties(cuda):
     check_route(-scores, 12, "softmax", bias, 8, 3, True)
 
 
+def test_route_ties_before_a_larger_one(cuda):
+    """Equal scores with the last places of the choice between them, and after them in FP32 one that is larger by a step."""
+    import torch
+
+    scores = torch.full((3, 40), -2.0, device="cuda")
+    small = torch.tensor(1e-3, device="cuda")
+    scores[:, 30] = 10.0
+    scores[:, :2] = small
+    scores[:, 2] = torch.nextafter(small, torch.tensor(1.0, device="cuda"))
+    for count in (1, 2, 3, 4, 5):
+        check_route(scores, count, "softmax")
+        check_route(scores, count, "softmax", groups=4, kept=2)
+        check_route(scores - 20.0, count, "sigmoid")
+
+
+@pytest.mark.parametrize("kind", ["softmax", "sigmoid"])
+def test_route_sums_that_agree(cuda, kind):
+    """Biases that make up for the shares: every sum is the same but for a rounding, shares and so their errors are not."""
+    import torch
+
+    for seed, experts, count in ((1, 64, 6), (2, 256, 8), (3, 100, 31), (4, 32, 1)):
+        scores = normal((200, experts), seed, 3.0)
+        for row in range(0, 200, 8):
+            wide = scores[row].double()
+            share = torch.sigmoid(wide) if kind == "sigmoid" else torch.softmax(wide, 0)
+            shift = normal((experts,), seed + 10, 4e-7).double()
+            check_route(scores[row:row + 8], count, kind, (1.0 - share + shift).float())
+
+
 # ---- sampling ----
 
 def plain_sample(logits, uniforms, temperature, top_k, top_p, min_p):
