@@ -5,7 +5,9 @@
 // s, b and the sums are FP64 by definition: which expert is chosen hangs on differences of b, and FP32 would decide some of
 // them by its rounding. But FP32 says of most tokens that no difference is that small: `route_kernel` chooses in FP32, and
 // takes a token whose choices differ by less than that arithmetic's error again in FP64 (`exactly`), unless scores and
-// biases are equal. The weights are FP64 in either.
+// biases are equal. The weights are FP64 in either. 16384 tokens by 8 of 256 experts in groups: 32.8 us, 90 with all
+// tokens in FP64; 1270 warp instructions a token keep the schedulers busy for two thirds of that, where the scores'
+// bytes take 2.7.
 #include "token_elements.cuh"
 
 #include <cmath>

@@ -5,15 +5,16 @@
 ``TokenContext.attend`` is attention over such a cache; ``PackedMatrix`` is a
 4-bit weight matrix with group scales, for a few rows; ``ByteMatrix`` and
 ``ByteExperts`` are weights in 8 bits, for one row to a prompt's; ``route``
-chooses a token's experts and ``sample`` the next symbol. Tensors are torch tensors on the current
-CUDA device (another one's are refused); work is enqueued on torch's current
-stream unless ``stream`` names another (then the caller orders the two, and keeps
+chooses a token's experts and ``sample`` the next symbol. Tensors are torch
+tensors on the current CUDA device (another one's are refused); work is enqueued
+on torch's current stream unless ``stream`` names another (then the caller orders the two, and keeps
 the tensors alive). What the operators refuse raises ``ExecutorError``; there is
 no CPU fallback. They are forward operators: an output has no gradient, whether or
 not an input requires one.
 
 The same call on the same kind of GPU gives the same bits; a token's may change
-with the rest of its call, as the other rows and sequences decide the order of sums.
+with the rest of its call, as the other rows and sequences decide the order of sums
+(not in 8-bit products, `route` and `sample`).
 
 The 4-bit group form, of caches and weights alike: a group of consecutive values
 is held as codes c in 0..15, two a byte with the even index in the low half, an
