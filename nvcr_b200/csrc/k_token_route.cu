@@ -5,11 +5,12 @@
 // s, b and the sums are FP64 by definition: which expert is chosen hangs on differences of b, and FP32 would decide some of
 // them by its rounding. But FP32 says of most tokens that no difference is that small: `route_kernel` chooses in FP32, and
 // takes a token whose choices differ by less than that arithmetic's error again in FP64 (`exactly`), unless scores and
-// biases are equal. The weights are FP64 in either. 16384 tokens by 8 of 256 experts in groups: 32.8 us, 90 with all
+// biases are equal. The weights are FP64 in either. 16384 tokens by 8 of 256 experts in groups: 30.9 us, 90 with all
 // tokens in FP64; 1270 warp instructions a token keep the schedulers busy for two thirds of that, where the scores'
 // bytes take 2.7.
 #include "token_elements.cuh"
 
+#include <climits>
 #include <cmath>
 
 namespace nvcr_sm100::token {
@@ -189,12 +190,17 @@ __global__ void __launch_bounds__(route_warps * 32) exact_kernel(RouteArgs a) {
     if (token < a.tokens) exactly<T, Each>(a, token, keys_of + warp * a.experts);
 }
 
-// The order of floats that are no NaN, as that of unsigned integers above 0.
+// The order of floats that are no NaN, as that of unsigned integers; 0 for -infinity. -0 lies below +0: it comes as neither a
+// share nor a sum of one.
+constexpr unsigned least_key = 0x007fffffu;
 __device__ __forceinline__ unsigned ordered(float v) {
-    const unsigned bits = __float_as_uint(v + 0.0f);
-    return bits >> 31 ? ~bits : bits | 0x80000000u;
+    const int bits = __float_as_int(v);
+    return static_cast<unsigned>(bits ^ (bits >> 31 | INT_MIN)) - least_key;
 }
-__device__ __forceinline__ float value_of(unsigned key) { return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ float value_of(unsigned key) {
+    const unsigned bits = key + least_key;
+    return __uint_as_float(bits >> 31 ? bits & 0x7fffffffu : ~bits);
+}
 
 __device__ __forceinline__ float reciprocal(float v) {
     float r;
@@ -215,21 +221,22 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
     if (token >= a.tokens) return;
     const T* row = static_cast<const T*>(a.scores) + token * a.stride;
     float score[Each], bias[Each];
-    float most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < Each; ++i) {
         const int e = i * 32 + lane;
         score[i] = e < a.experts ? widen(row[e]) : -INFINITY;
         bias[i] = a.bias != nullptr && e < a.experts ? a.bias[e] : 0.0f;
-        most = fmaxf(most, score[i]);
     }
     constexpr float log2e = 1.44269504f;
+    float most = -INFINITY, largest_share = 1.0f;
     float share[Each];
     bool certain = true;
     if (a.sigmoid) {
 #pragma unroll
         for (int i = 0; i < Each; ++i) share[i] = reciprocal(1.0f + exp2_fast(score[i] * -log2e));
     } else {
+#pragma unroll
+        for (int i = 0; i < Each; ++i) most = fmaxf(most, score[i]);
 #pragma unroll
         for (int offset = 16; offset > 0; offset /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
         certain = most < INFINITY;
@@ -239,9 +246,9 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
             share[i] = score[i] > -INFINITY ? exp2_fast((score[i] - most) * log2e) : 0.0f;
             sum += share[i];
         }
-        const float inverse = reciprocal(token::warp_sum(sum));
+        largest_share = reciprocal(token::warp_sum(sum));
 #pragma unroll
-        for (int i = 0; i < Each; ++i) share[i] *= inverse;
+        for (int i = 0; i < Each; ++i) share[i] *= largest_share;
     }
     // How far a share s and its sum b with the bias may be off: of exponents up to 128, rounded twice or three times to 2^-24
     // of themselves, a factor of 1e-5 or 1.6e-5, which a sigmoid has times 1 - s; ex2, rcp and sums 4e-7, a softmax's sum
@@ -250,15 +257,12 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
         return s * (a.sigmoid ? 4e-7f + (1.0f - s) * 1e-5f : 2e-5f) + 1.8e-7f * fabsf(b) + 1e-37f;
     };
     unsigned key[Each];
-    float furthest = 0.0f;
 #pragma unroll
     for (int i = 0; i < Each; ++i) {
-        const float b = share[i] + bias[i];
-        const bool there = score[i] > -INFINITY && b > -INFINITY;  // a NaN is left out
-        key[i] = there ? ordered(b) : 0;
-        furthest = fmaxf(furthest, there ? fabsf(b) : 0.0f);
+        const float b = score[i] > -INFINITY ? share[i] + bias[i] : -INFINITY;
+        key[i] = ordered(fmaxf(b, -INFINITY));  // a NaN is left out
     }
-    certain = certain && furthest <= 1e30f;
+    constexpr float most_exact = 1e30f;  // larger sums with biases could pass FP32's range
     auto* keys = reinterpret_cast<unsigned*>(keys_of + warp * room_of(a));
     if (a.kept_groups < a.groups) {
         const int size = a.experts / a.groups;
@@ -296,6 +300,7 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
             const float other = __shfl_sync(0xffffffffu, value, g);
             place += other > value || (other == value && g < lane);
         }
+        certain = certain && (!some || fabsf(value) <= most_exact);
         const bool stays = lane < a.groups && place < a.kept_groups;
         const unsigned kept = __ballot_sync(0xffffffffu, stays);
         // the least that a group that stays may have, and the most of the others (groups without an expert are of no matter)
@@ -314,25 +319,31 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
     unsigned bound = 0;
 #pragma unroll
     for (int i = 0; i < Each; ++i) bound = max(bound, key[i]);
-#pragma unroll
-    for (int size = 2; size <= 32; size *= 2) {
-#pragma unroll
-        for (int apart = size / 2; apart > 0; apart /= 2) {
-            const unsigned other = __shfl_xor_sync(0xffffffffu, bound, apart);
-            bound = ((lane & apart) == 0) == ((lane & size) == 0) ? max(bound, other) : min(bound, other);
+    if (a.count < 16) {  // by taking the largest off
+        unsigned largest = 0;
+#pragma unroll 1
+        for (int k = 0; k <= a.count; ++k) {
+            largest = __reduce_max_sync(0xffffffffu, bound);
+            if (bound == largest) bound = 0;
         }
+        bound = max(1u, largest);
+    } else {
+#pragma unroll
+        for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+            for (int apart = size / 2; apart > 0; apart /= 2) {
+                const unsigned other = __shfl_xor_sync(0xffffffffu, bound, apart);
+                bound = ((lane & apart) == 0) == ((lane & size) == 0) ? max(bound, other) : min(bound, other);
+            }
+        }
+        bound = max(1u, __shfl_sync(0xffffffffu, bound, min(a.count, 31)));
     }
-    bound = max(1u, __shfl_sync(0xffffffffu, bound, min(a.count, 31)));
     auto* entries = reinterpret_cast<unsigned long long*>(keys);
     int candidates = 0;
-    float reach = -INFINITY;  // the most that an expert behind the candidates may have
 #pragma unroll
     for (int i = 0; i < Each; ++i) {
-        if (key[i] != 0 && key[i] < bound) {
-            const float b = share[i] + bias[i];
-            reach = fmaxf(reach, b + error(share[i], b));
-        }
         const unsigned holders = __ballot_sync(0xffffffffu, key[i] >= bound);
+        if (holders == 0) continue;
         const int at = candidates + __popc(holders & ((1u << lane) - 1));
         if (key[i] >= bound && at < 32) {
             entries[at] = static_cast<unsigned long long>(key[i]) << 32 | ~static_cast<unsigned>(i * 32 + lane);
@@ -342,8 +353,11 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
         candidates += __popc(holders);
     }
     __syncwarp();
-    const unsigned reach_key = __reduce_max_sync(0xffffffffu, ordered(reach));
-    const float reach_of_all = value_of(reach_key);
+    // The most that an expert behind the candidates may have: below the bound, and with a bias of its own any share.
+    const float edge = value_of(bound);
+    const float reach = bound == 1 ? -INFINITY
+        : a.bias == nullptr        ? edge + error(edge, edge)
+                                   : edge + ((a.sigmoid ? 2.8e-6f : 2e-5f * largest_share) + 1.8e-7f * fabsf(edge) + 1e-37f);
     certain = certain && candidates <= 32;
     const int n = min(candidates, 32);
     const unsigned long long entry = lane < n ? entries[lane] : 0;
@@ -366,19 +380,19 @@ __global__ void __launch_bounds__(route_warps * 32, 8) route_kernel(RouteArgs a)
         // same score and bias. Equal ones at the last choice stand for it: the last of them is looked at too.
         const float off = lane < n ? error(s, v) : 0.0f;
         float after = lane < n ? v + off : -INFINITY;  // the most of this and of later ones
-        after = fmaxf(after, lane == 31 ? reach_of_all : -INFINITY);
+        after = fmaxf(after, lane == 31 ? reach : -INFINITY);
 #pragma unroll
         for (int apart = 1; apart < 32; apart *= 2) {
             const float other = __shfl_down_sync(0xffffffffu, after, apart);
             if (lane + apart < 32) after = fmaxf(after, other);
         }
         after = __shfl_down_sync(0xffffffffu, after, 1);
-        if (lane == 31) after = reach_of_all;
+        if (lane == 31) after = reach;
         const float next_l = __shfl_down_sync(0xffffffffu, mine, 1), next_b = __shfl_down_sync(0xffffffffu, b, 1);
         const bool tied = lane + 1 < n && mine == next_l && b == next_b;
         const unsigned runs = __ballot_sync(0xffffffffu, tied) >> (a.count - 1);
         const int last = a.count - 1 + __ffs(static_cast<int>(~runs)) - 1;
-        if (lane <= last && lane < n && !tied && !(v - off > after)) certain = false;
+        if (lane <= last && lane < n && !tied && !(v - off > after && fabsf(v) <= most_exact)) certain = false;
     }
     certain = __all_sync(0xffffffffu, certain);
     if (!certain) {
