@@ -1176,6 +1176,23 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
 
 // ---- many rows ----
 
+// Two FP32 values in one instruction.
+struct Two {
+    unsigned long long bits;
+    __device__ __forceinline__ Two(float one, float two) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(one), "f"(two)); }
+    __device__ __forceinline__ void add(const Two& v) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(bits) : "l"(v.bits)); }
+    __device__ __forceinline__ Two by(const Two& factor, const Two& more) const {
+        Two made(*this);
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(made.bits) : "l"(bits), "l"(factor.bits), "l"(more.bits));
+        return made;
+    }
+    __device__ __forceinline__ float2 values() const {
+        float2 v;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(bits));
+        return v;
+    }
+};
+
 constexpr int part_threads = 256;
 constexpr int part_vectors = 8;    // a thread
 constexpr int part_candidates = 2048;
@@ -1237,12 +1254,19 @@ __global__ void __launch_bounds__(part_threads, 4) part_kernel(SampleArgs a, Man
     const int skew = static_cast<int>(reinterpret_cast<std::uintptr_t>(logits) % 16 / sizeof(T));
     const int first = (part * part_vectors * part_threads + static_cast<int>(threadIdx.x)) * each - skew;
     uint4 v[part_vectors];
+    const int block_first = part * part_vectors * part_threads * each - skew;
+    if (block_first >= 0 && block_first + part_vectors * part_threads * each <= a.symbols) {
+        const auto* from = reinterpret_cast<const uint4*>(logits + first);
 #pragma unroll
-    for (int k = 0; k < part_vectors; ++k) v[k] = load_vector(logits, a.symbols, first + k * part_threads * each);
+        for (int k = 0; k < part_vectors; ++k) v[k] = from[k * part_threads];
+    } else {
+#pragma unroll
+        for (int k = 0; k < part_vectors; ++k) v[k] = load_vector(logits, a.symbols, first + k * part_threads * each);
+    }
     const Settings s = settings_of(a, r);
-    float most = -INFINITY;
+    float of_vector[part_vectors], most = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < part_vectors; ++k) most = fmaxf(most, Of::largest(v[k]));
+    for (int k = 0; k < part_vectors; ++k) of_vector[k] = Of::largest(v[k]), most = fmaxf(most, of_vector[k]);
     unsigned top = __reduce_max_sync(0xffffffffu, key_of(most));
     if (threadIdx.x == 0) count = queued = 0, cut_bin = cut_bins;
     if (lane == 0) scratch[warp] = top;
@@ -1265,7 +1289,7 @@ __global__ void __launch_bounds__(part_threads, 4) part_kernel(SampleArgs a, Man
             // at which top_k vectors have their largest logits above: so many candidates at least, and seldom many more
 #pragma unroll
             for (int k = 0; k < part_vectors; ++k) {
-                const float x = exponent(Of::largest(v[k])) * -cut_steps;
+                const float x = exponent(of_vector[k]) * -cut_steps;
                 if (x < static_cast<float>(cut_bins)) atomicAdd(&bins_here[static_cast<int>(x)], 1u);
             }
             __syncthreads();
@@ -1292,17 +1316,22 @@ __global__ void __launch_bounds__(part_threads, 4) part_kernel(SampleArgs a, Man
         }
         told.cut = wishes.greedy ? largest : largest + octaves / wishes.factor;
         const bool sum_rest = wishes.by_part && !wishes.by_count;
-        float rest = 0.0f;
+        const Two factors(wishes.factor, wishes.factor), bases(base, base);
+        Two sums(0.0f, 0.0f);
 #pragma unroll
         for (int k = 0; k < part_vectors; ++k) {
-            if (Of::largest(v[k]) >= told.cut) {  // looked at below, by all threads
+            if (of_vector[k] >= told.cut) {  // looked at below, by all threads
                 const unsigned nth = atomicAdd(&queued, 1u);
                 if (nth < part_candidates) queue[nth] = v[k], places[nth] = first + k * part_threads * each;
             } else if (sum_rest) {
 #pragma unroll
-                for (int i = 0; i < each; ++i) rest += exp2_fast(exponent(Of::get(v[k], i)));
+                for (int i = 0; i < each; i += 2) {
+                    const float2 x = Two(Of::get(v[k], i), Of::get(v[k], i + 1)).by(factors, bases).values();
+                    sums.add(Two(exp2_fast(x.x), exp2_fast(x.y)));
+                }
             }
         }
+        float rest = sums.values().x + sums.values().y;
         __syncthreads();
         unsigned long long* list = m.candidates + (r * m.parts + part) * part_candidates;
         const int all = static_cast<int>(min(queued, static_cast<unsigned>(part_candidates))) * each;
