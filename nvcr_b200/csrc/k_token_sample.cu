@@ -37,6 +37,7 @@ constexpr int bins = 2048;
 constexpr int most_blocks = 8;
 constexpr int most_candidates = 2048;
 constexpr int most_vectors = 16;  // a thread
+constexpr int most_counted = 128; // symbols whose places are counted, not sorted
 constexpr int cut_bins = 256;     // of `cut`, so many an octave:
 constexpr float cut_steps = 5.5f;
 
@@ -478,6 +479,34 @@ __device__ __noinline__ void sort(unsigned long long* shared) {
     __syncthreads();
 }
 
+// As `sort`, up to 512: one a thread.
+__device__ __noinline__ void sort_few(unsigned long long* shared, int n) {
+    const int i = static_cast<int>(threadIdx.x);
+    int all = 32;
+    while (all < n) all *= 2;
+    __syncthreads();
+    unsigned long long v = i < n ? shared[i] : 0;
+#pragma unroll 1
+    for (int size = 2; size <= all; size *= 2) {
+#pragma unroll 1
+        for (int apart = size / 2; apart > 0; apart /= 2) {
+            unsigned long long other;
+            if (apart >= 32) {
+                __syncthreads();
+                if (i < all) shared[i] = v;
+                __syncthreads();
+                other = shared[i ^ apart];
+            } else {
+                other = __shfl_xor_sync(0xffffffffu, v, apart);
+            }
+            v = ((i & size) == 0) == ((i & apart) == 0) ? max(v, other) : min(v, other);
+        }
+    }
+    __syncthreads();
+    if (i < all) shared[i] = v;
+    __syncthreads();
+}
+
 // FP32 sums of weights that are not candidates, as a share of them: three roundings of 2^-24 of an exponent of at most 46,
 // and two of largest * factor, times ln 2; ex2.approx's error (2^-22) and up to 160 additions.
 __device__ __forceinline__ double bulk_error(float largest, float factor) {
@@ -580,20 +609,20 @@ struct ClusterRow {
         }
     }
 
-    // The gathered symbols of all blocks, sorted; how many there are. Up to a block's threads each one's place is counted,
-    // by a group of threads: 64 take 1.0 us less than the sort's 21 exchanges with a barrier each.
+    // The gathered symbols of all blocks, sorted; how many there are. Of up to 128 each one's place is counted, by a group of
+    // threads: 64 take 1.0 us less than the sort of 2048, but 309 by 512 threads 10 us more.
     __device__ __forceinline__ int collect(const unsigned long long* counts, int part) {
         unsigned long long* from = shared.gathered;
         int n = 0;
         for (int b = 0; b < blocks; ++b) n += static_cast<int>(counts[b] & 0xffffffffu);
-        unsigned long long* to = n <= threads ? shared.weights : shared.sorted;
+        unsigned long long* to = n <= most_counted ? shared.weights : shared.sorted;
         n = 0;
         for (int b = 0; b < blocks; ++b) {
             const int count = static_cast<int>(counts[b] & 0xffffffffu);
             for (int i = threadIdx.x; i < count; i += threads) to[n + i] = from[b * part + i];
             n += count;
         }
-        if (n <= threads) {
+        if (n <= most_counted) {
             __syncthreads();
             const int group = group_of(n), i = static_cast<int>(threadIdx.x) / group;
             const unsigned long long mine = i < n ? to[i] : 0;
@@ -602,6 +631,10 @@ struct ClusterRow {
             for (int o = group / 2; o > 0; o /= 2) place += __shfl_xor_sync(0xffffffffu, place, o);
             if (i < n && threadIdx.x % group == 0) shared.sorted[place] = mine;
             __syncthreads();
+            return n;
+        }
+        if (n <= threads) {
+            sort_few(shared.sorted, n);
             return n;
         }
         for (int i = n + threadIdx.x; i < most_candidates; i += threads) shared.sorted[i] = 0;
@@ -970,7 +1003,7 @@ struct ClusterRow {
             a.probabilities[r] = probability_of(share_once(logit_of(static_cast<unsigned>(entry >> 32)), row), whole_kept);
         };
         auto weight_at = [&](int i) { return shared.weights[i] - (i == 0 ? 0 : shared.weights[i - 1]); };
-        if (n <= threads) {  // the weight of those with lower indexes, for each
+        if (n <= most_counted) {  // the weight of those with lower indexes, for each
             const int group = group_of(n), i = static_cast<int>(threadIdx.x) / group;
             const unsigned index = i < n ? static_cast<unsigned>(shared.sorted[i]) : 0;  // its complement
             Weight lower = 0;
@@ -985,8 +1018,13 @@ struct ClusterRow {
         for (int i = threadIdx.x; i < most_candidates; i += threads) {
             shared.gathered[i] = i < n ? (shared.sorted[i] & 0xffffffffull) << 32 | static_cast<unsigned>(i) : 0ull;
         }
-        sort(shared.gathered);
-        const int start = static_cast<int>(threadIdx.x) * (most_candidates / threads), stop = min(n, start + most_candidates / threads);
+        if (n <= threads) {
+            sort_few(shared.gathered, n);
+        } else {
+            sort(shared.gathered);
+        }
+        const int each_thread = n <= threads ? 1 : most_candidates / threads;
+        const int start = static_cast<int>(threadIdx.x) * each_thread, stop = min(n, start + each_thread);
         sum = 0;
 #pragma unroll 1
         for (int i = start; i < stop; ++i) sum += weight_at(static_cast<int>(shared.gathered[i] & 0xffffffffull));
@@ -1399,20 +1437,31 @@ __global__ void __launch_bounds__(threads, 2) end_kernel(SampleArgs a, ManyArgs 
 #pragma unroll
         for (int o = 16; o > 0; o /= 2) bulk += __shfl_xor_sync(0xffffffffu, bulk, o);
         __syncthreads();
-        // a warp a part
+        // a part by one warp, or by as many as there are for each
         float held = 0.0f, rest = 0.0f;
-        for (int p = warp; p < m.parts; p += warps) {
+        const int sharing = max(1, warps / m.parts);
+        for (int p = warp / sharing; p < m.parts; p += warps / sharing) {
             const int count = static_cast<int>(told[p].count);
             const unsigned long long* list = m.candidates + (r * m.parts + p) * part_candidates;
-            for (int i = lane; i < count; i += 32) {
-                const unsigned long long entry = list[i];
-                const float l = logit_of(static_cast<unsigned>(entry >> 32));
-                if (l >= cut) {
-                    const unsigned nth = atomicAdd(&shared.count, 1u);
-                    if (nth < most_candidates) shared.gathered[nth] = entry;
-                    held += exp2_fast(exponent(l));
-                } else {
-                    rest += exp2_fast(exponent(l));
+            for (int from = warp % sharing * 128; from < count; from += sharing * 128) {
+                unsigned long long entry[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int i = from + k * 32 + lane;
+                    entry[k] = i < count ? list[i] : 0;
+                }
+#pragma unroll 1
+                for (int k = 0; k < 4; ++k) {
+                    const unsigned long long one = k == 0 ? entry[0] : k == 1 ? entry[1] : k == 2 ? entry[2] : entry[3];
+                    if (one == 0) break;
+                    const float l = logit_of(static_cast<unsigned>(one >> 32));
+                    if (l >= cut) {
+                        const unsigned nth = atomicAdd(&shared.count, 1u);
+                        if (nth < most_candidates) shared.gathered[nth] = one;
+                        held += exp2_fast(exponent(l));
+                    } else {
+                        rest += exp2_fast(exponent(l));
+                    }
                 }
             }
         }
