@@ -1101,8 +1101,10 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
         auto* places = reinterpret_cast<int*>(shared.sums.high);
         constexpr float wide_cut = -14.5f;
         float cut = -10.0f;
-        if (row.least > 0.0) {
-            cut = fmaxf(log2f(fminf(s.min_p, 1.0f)) - 0.01f, -46.0f);
+        const bool by_least = row.least > 0.0 && !(by_count && by_part);  // top_p's whole is that of the first top_k
+        const float least_cut = by_least ? fmaxf(log2f(fminf(s.min_p, 1.0f)) - 0.01f, -46.0f) : -INFINITY;
+        if (!by_count && by_least) {
+            cut = least_cut;
         } else if (by_count) {
             // at which top_k vectors have their largest logits above: so many candidates at least, and seldom many more
             for (int i = threadIdx.x; i < cut_bins; i += threads) shared.sums.low[i] = 0;
@@ -1125,7 +1127,7 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
             const Weight earlier = before(mine, shared.sums.scratch, all), wanted = static_cast<Weight>(s.top_k);
             if (earlier < wanted && earlier + mine >= wanted) shared.cut = static_cast<int>(threadIdx.x) + 1;
             __syncthreads();
-            cut = static_cast<float>(shared.cut) * (-1.0f / cut_steps) - 0.001f;
+            cut = fmaxf(static_cast<float>(shared.cut) * (-1.0f / cut_steps) - 0.001f, least_cut);
         }
         for (int turn = 0;; ++turn) {
             float held = 0.0f, rest = 0.0f;  // weights of candidates and of the others
@@ -1182,7 +1184,7 @@ __global__ void __launch_bounds__(threads, Vectors == 8 ? 2 : 1) cluster_kernel(
             }
             if (!fits || !(bulk <= 1e30)) break;  // a NaN among the sums too
             const bool complete = cut <= -46.0f;  // what is left out has no weight
-            const bool enough = complete || (row.least > 0.0 && !(by_count && by_part)) ||
+            const bool enough = complete || cut == least_cut ||
                 (by_count ? count >= s.top_k
                           : all_held * (1.0 - error) >= static_cast<double>(fmaxf(s.top_p, 0.0f)) *
                                  ((all_held + bulk) * (1.0 + error) + a.symbols / unit));
@@ -1253,10 +1255,14 @@ struct ManyArgs {
 // What a row's settings ask for, the largest logit known.
 struct Wishes {
     bool greedy, by_count, by_part;
+    bool by_least;  // min_p tells the candidates; not where top_p's whole is that of the first top_k
     int top_k;
     float factor;  // octaves a logit
     bool ordinary; // FP32 exponents will do
     bool few;      // candidates can be told
+    __device__ __forceinline__ float least_octaves(const Settings& s) const {
+        return fmaxf(log2f(fminf(s.min_p, 1.0f)) - 0.01f, -46.0f);
+    }
 };
 __device__ __forceinline__ Wishes wishes_of(const SampleArgs& a, const Settings& s, float largest) {
     Wishes w;
@@ -1264,6 +1270,7 @@ __device__ __forceinline__ Wishes wishes_of(const SampleArgs& a, const Settings&
     w.top_k = w.greedy ? 1 : s.top_k;
     w.by_count = w.greedy || (s.top_k > 0 && s.top_k < a.symbols);
     w.by_part = !w.greedy && s.top_p < 1.0f;
+    w.by_least = !w.greedy && s.min_p > 0.0f && !(w.by_count && w.by_part);
     w.factor = w.greedy ? 1.0f : 1.44269504f / s.temperature;
     w.ordinary = largest < INFINITY && w.factor < 1e30f && w.factor > 1e-30f;
     w.few = w.ordinary && (w.by_count || w.by_part || s.min_p > 0.0f) && (!w.by_count || w.top_k <= part_candidates / 2) &&
@@ -1319,11 +1326,8 @@ __global__ void __launch_bounds__(part_threads, 4) part_kernel(SampleArgs a, Man
     if (top != 0 && wishes.few) {
         const float base = -largest * wishes.factor;
         auto exponent = [&](float l) { return fmaf(l, wishes.factor, base); };
-        const bool by_least = !wishes.greedy && s.min_p > 0.0f;
-        float octaves = -10.0f;
-        if (by_least) {
-            octaves = fmaxf(log2f(fminf(s.min_p, 1.0f)) - 0.01f, -46.0f);
-        } else if (wishes.by_count) {
+        float octaves = wishes.by_least ? wishes.least_octaves(s) : -10.0f;
+        if (wishes.by_count && !wishes.greedy) {
             // at which top_k vectors have their largest logits above: so many candidates at least, and seldom many more
 #pragma unroll
             for (int k = 0; k < part_vectors; ++k) {
@@ -1350,7 +1354,8 @@ __global__ void __launch_bounds__(part_threads, 4) part_kernel(SampleArgs a, Man
                 }
             }
             __syncthreads();
-            octaves = static_cast<float>(cut_bin) * (-1.0f / cut_steps) - 0.01f;
+            const float by_count = static_cast<float>(cut_bin) * (-1.0f / cut_steps) - 0.01f;
+            octaves = wishes.by_least ? fmaxf(octaves, by_count) : by_count;
         }
         told.cut = wishes.greedy ? largest : largest + octaves / wishes.factor;
         const bool sum_rest = wishes.by_part && !wishes.by_count;
@@ -1471,11 +1476,11 @@ __global__ void __launch_bounds__(threads, 2) end_kernel(SampleArgs a, ManyArgs 
         double all_held = 0.0;
         for (int w = 0; w < warps; ++w) all_held += shared.parts[0][w], bulk += shared.parts[1][w];
         const int count = static_cast<int>(shared.count);
-        const bool sum_rest = wishes.by_part && !wishes.by_count, by_least = row.least > 0.0 && !wishes.greedy;
+        const bool sum_rest = wishes.by_part && !wishes.by_count;
         // another rounding of the parts' largest logits' exponents
         const double error = bulk_error(largest, wishes.factor) + 1e-5;
         const bool enough = count <= most_candidates && bulk <= 1e30 &&
-            ((by_least && !(wishes.by_count && wishes.by_part)) ||
+            ((wishes.by_least && cut == largest + wishes.least_octaves(s) / wishes.factor) ||
              (wishes.by_count ? count >= wishes.top_k
                               : all_held * (1.0 - error) >= static_cast<double>(fmaxf(s.top_p, 0.0f)) *
                                       ((all_held + bulk) * (1.0 + error) + a.symbols / unit)));
