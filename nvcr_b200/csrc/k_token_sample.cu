@@ -479,31 +479,76 @@ __device__ __noinline__ void sort(unsigned long long* shared) {
     __syncthreads();
 }
 
-// As `sort`, up to 512: one a thread.
-__device__ __noinline__ void sort_few(unsigned long long* shared, int n) {
-    const int i = static_cast<int>(threadIdx.x);
-    int all = 32;
-    while (all < n) all *= 2;
+constexpr int most_crowded = 256;  // entries of a bin that are compared with one another
+
+// n entries in falling order, n up to 2048: to bins by equal steps of their logits (shift < 0), or by their indexes'
+// leading bits, and within a bin by comparing them all. 1300 take 3 us where `sort` takes 12; it is left for those that
+// crowd in few bins.
+__device__ __noinline__ void arrange(unsigned long long* list, int n, int shift, Sums& sums) {
+    constexpr int most = most_candidates / threads, each = bins / threads;
+    static_assert(each == 4);
+    const int thread = static_cast<int>(threadIdx.x);
     __syncthreads();
-    unsigned long long v = i < n ? shared[i] : 0;
-#pragma unroll 1
-    for (int size = 2; size <= all; size *= 2) {
-#pragma unroll 1
-        for (int apart = size / 2; apart > 0; apart /= 2) {
-            unsigned long long other;
-            if (apart >= 32) {
-                __syncthreads();
-                if (i < all) shared[i] = v;
-                __syncthreads();
-                other = shared[i ^ apart];
-            } else {
-                other = __shfl_xor_sync(0xffffffffu, v, apart);
-            }
-            v = ((i & size) == 0) == ((i & apart) == 0) ? max(v, other) : min(v, other);
+    reinterpret_cast<uint4*>(sums.low)[thread] = {0, 0, 0, 0};
+    unsigned long long entry[most];
+    unsigned top = 0, least = 0xffffffffu;
+#pragma unroll
+    for (int k = 0; k < most; ++k) {
+        const int i = k * threads + thread;
+        entry[k] = i < n ? list[i] : 0;
+        if (entry[k] != 0) top = max(top, static_cast<unsigned>(entry[k] >> 32)), least = min(least, static_cast<unsigned>(entry[k] >> 32));
+    }
+    float largest = 0.0f, scale = 0.0f;
+    if (shift < 0) {
+        top = __reduce_max_sync(0xffffffffu, top), least = __reduce_min_sync(0xffffffffu, least);
+        if (thread % 32 == 0) sums.scratch[thread / 32] = static_cast<Weight>(top) << 32 | least;
+        __syncthreads();
+#pragma unroll 4
+        for (int w = 0; w < warps; ++w) {
+            const Weight both = sums.scratch[w];
+            top = max(top, static_cast<unsigned>(both >> 32)), least = min(least, static_cast<unsigned>(both));
         }
+        largest = logit_of(top);
+        scale = (bins - 1) / (largest - logit_of(least));
     }
     __syncthreads();
-    if (i < all) shared[i] = v;
+    int bin[most];
+    unsigned place[most];
+#pragma unroll
+    for (int k = 0; k < most; ++k) {
+        if (entry[k] == 0) continue;
+        const auto high = static_cast<unsigned>(entry[k] >> 32);
+        // falling in the logit, whatever is rounded; a NaN, of an infinite scale, is the largest's
+        bin[k] = shift < 0 ? min(bins - 1, static_cast<int>((largest - logit_of(high)) * scale)) : static_cast<int>(~high >> shift);
+        place[k] = atomicAdd(&sums.low[bin[k]], 1u);
+    }
+    __syncthreads();
+    const uint4 count = reinterpret_cast<const uint4*>(sums.low)[thread];
+    Weight all;
+    const auto first = static_cast<unsigned>(before(count.x + count.y + count.z + count.w, sums.scratch, all));
+    reinterpret_cast<uint4*>(sums.high)[thread] = {first, first + count.x, first + count.x + count.y, first + count.x + count.y + count.z};
+    if (__syncthreads_or(max(max(count.x, count.y), max(count.z, count.w)) > most_crowded)) {
+        for (int i = n + thread; i < most_candidates; i += threads) list[i] = 0;
+        sort(list);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < most; ++k) {
+        if (entry[k] != 0) list[sums.high[bin[k]] + place[k]] = entry[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < most; ++k) {
+        if (entry[k] == 0) continue;
+        const unsigned start = sums.high[bin[k]], end = start + sums.low[bin[k]];
+        place[k] = start;
+        for (unsigned i = start; i < end; ++i) place[k] += list[i] > entry[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < most; ++k) {
+        if (entry[k] != 0) list[place[k]] = entry[k];
+    }
     __syncthreads();
 }
 
@@ -610,7 +655,7 @@ struct ClusterRow {
     }
 
     // The gathered symbols of all blocks, sorted; how many there are. Of up to 128 each one's place is counted, by a group of
-    // threads: 64 take 1.0 us less than the sort of 2048, but 309 by 512 threads 10 us more.
+    // threads.
     __device__ __forceinline__ int collect(const unsigned long long* counts, int part) {
         unsigned long long* from = shared.gathered;
         int n = 0;
@@ -633,12 +678,7 @@ struct ClusterRow {
             __syncthreads();
             return n;
         }
-        if (n <= threads) {
-            sort_few(shared.sorted, n);
-            return n;
-        }
-        for (int i = n + threadIdx.x; i < most_candidates; i += threads) shared.sorted[i] = 0;
-        sort(shared.sorted);
+        arrange(shared.sorted, n, -1, shared.sums);
         return n;
     }
     // Threads for each of n, a power of two.
@@ -1015,16 +1055,11 @@ struct ClusterRow {
             return true;
         }
         // in the order of indexes: the largest complement first
-        for (int i = threadIdx.x; i < most_candidates; i += threads) {
-            shared.gathered[i] = i < n ? (shared.sorted[i] & 0xffffffffull) << 32 | static_cast<unsigned>(i) : 0ull;
+        for (int i = threadIdx.x; i < n; i += threads) {
+            shared.gathered[i] = (shared.sorted[i] & 0xffffffffull) << 32 | static_cast<unsigned>(i);
         }
-        if (n <= threads) {
-            sort_few(shared.gathered, n);
-        } else {
-            sort(shared.gathered);
-        }
-        const int each_thread = n <= threads ? 1 : most_candidates / threads;
-        const int start = static_cast<int>(threadIdx.x) * each_thread, stop = min(n, start + each_thread);
+        arrange(shared.gathered, n, max(0, 21 - __clz(max(a.symbols - 1, 1))), shared.sums);
+        const int start = static_cast<int>(threadIdx.x) * run, stop = min(n, start + run);
         sum = 0;
 #pragma unroll 1
         for (int i = start; i < stop; ++i) sum += weight_at(static_cast<int>(shared.gathered[i] & 0xffffffffull));
