@@ -552,10 +552,11 @@ __device__ __noinline__ void arrange(unsigned long long* list, int n, int shift,
     __syncthreads();
 }
 
-// FP32 sums of weights that are not candidates, as a share of them: three roundings of 2^-24 of an exponent of at most 46,
-// and two of largest * factor, times ln 2; ex2.approx's error (2^-22) and up to 160 additions.
+// FP32 sums of weights that are not candidates may be off by this share of them: exponents of up to 46 by 2.2 * 2^-24 of
+// themselves (the factor's rounding and their own) and by 2^-24 of largest * factor, times ln 2; ex2.approx 2^-22, and up to
+// 181 additions one after another.
 __device__ __forceinline__ double bulk_error(float largest, float factor) {
-    return 3e-5 + 2e-7 * fabs(static_cast<double>(largest) * static_cast<double>(factor));
+    return 1.6e-5 + 5e-8 * fabs(static_cast<double>(largest) * static_cast<double>(factor));
 }
 
 template <typename T>
@@ -1478,11 +1479,12 @@ __global__ void __launch_bounds__(threads, 2) end_kernel(SampleArgs a, ManyArgs 
         for (int o = 16; o > 0; o /= 2) bulk += __shfl_xor_sync(0xffffffffu, bulk, o);
         __syncthreads();
         // a part by one warp, or by as many as there are for each
-        float held = 0.0f, rest = 0.0f;
+        double held_here = 0.0, rest_here = 0.0;
         const int sharing = max(1, warps / m.parts);
         for (int p = warp / sharing; p < m.parts; p += warps / sharing) {
             const int count = static_cast<int>(told[p].count);
             const unsigned long long* list = m.candidates + (r * m.parts + p) * part_candidates;
+            float held = 0.0f, rest = 0.0f;
             for (int from = warp % sharing * 128; from < count; from += sharing * 128) {
                 unsigned long long entry[4];
 #pragma unroll
@@ -1504,16 +1506,17 @@ __global__ void __launch_bounds__(threads, 2) end_kernel(SampleArgs a, ManyArgs 
                     }
                 }
             }
+            held_here += held, rest_here += rest;
         }
-        held = warp_sum(held), rest = warp_sum(rest);
+        const float held = warp_sum(static_cast<float>(held_here)), rest = warp_sum(static_cast<float>(rest_here));
         if (lane == 0) shared.parts[0][warp] = held, shared.parts[1][warp] = rest;
         __syncthreads();
         double all_held = 0.0;
         for (int w = 0; w < warps; ++w) all_held += shared.parts[0][w], bulk += shared.parts[1][w];
         const int count = static_cast<int>(shared.count);
         const bool sum_rest = wishes.by_part && !wishes.by_count;
-        // another rounding of the parts' largest logits' exponents
-        const double error = bulk_error(largest, wishes.factor) + 1e-5;
+        // exponents in two steps, each with a rounding of its own largest logit's
+        const double error = 2.0 * bulk_error(largest, wishes.factor);
         const bool enough = count <= most_candidates && bulk <= 1e30 &&
             ((wishes.by_least && cut == largest + wishes.least_octaves(s) / wishes.factor) ||
              (wishes.by_count ? count >= wishes.top_k
