@@ -19,9 +19,9 @@
 //
 // Longer rows and infinite logits take `row_by_block`, which finds the threshold's bits from memory with one block.
 //
-// One row of 32768 FP32 logits (top_k 50, top_p 0.95) 10.7 us: launch, four exchanges of a cluster, one warp's end of the
-// row. 256 rows of 131072 BF16 logits (top_p 0.9, min_p 0.01) 42 us, of which 10 are the logits at HBM's rate: parts take
-// 26, ends 21, whose time is the latency of sums and FP64 weights, some of it side by side.
+// One row of 32768 FP32 logits (top_k 50, top_p 0.95) 11 us: launch, four exchanges of a cluster, one warp's end of the
+// row. 256 rows of 131072 BF16 logits (top_p 0.9, min_p 0.01) 37 us, of which 10 are the logits at HBM's rate: parts take
+// 25, by an exponential a logit; ends 13, by the latency of sums and FP64 weights, some of it side by side.
 #include "token_elements.cuh"
 
 #include <algorithm>
