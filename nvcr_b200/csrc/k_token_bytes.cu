@@ -416,8 +416,9 @@ __device__ __forceinline__ void peer_store(std::uint32_t address, int rank, int 
                  : "memory");
 }
 
-// A barrier of the epilogue's threads: whether any of them says so.
+// A barrier of the epilogue's threads: whether any of them says so. bar.red takes whole warps.
 __device__ __forceinline__ bool epilogue_any(bool mine) {
+    __syncwarp();
     int any;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
@@ -472,6 +473,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, const Tile& t, 
     const float bias = inside && a.bias != nullptr ? widen(static_cast<const T*>(a.bias)[channel]) : 0.0f;
     T* y = static_cast<T*>(a.y) + output;
     if constexpr (!Experts) y += t.row * a.outputs;
+    __syncwarp();
     int ahead[16];  // the next columns, under way while the ones before are scaled
     if (half * 16 < t.columns) tmem_load16(sums + static_cast<std::uint32_t>(half * 16), ahead);
 #pragma unroll 1
@@ -484,39 +486,41 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, const Tile& t, 
             asm volatile("" : "+r"(acc[i]));  // not read before the wait
         }
         if (column + 32 < t.columns) tmem_load16(sums + static_cast<std::uint32_t>(column + 32), ahead);
-        if (!inside) continue;
-        float row_scale[16];
-        int row[16];
+        if (inside) {
+            float row_scale[16];
+            int row[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 v = reinterpret_cast<const float4*>(tail.row_scales[buffer])[column / 4 + i];
-            row_scale[4 * i] = v.x, row_scale[4 * i + 1] = v.y, row_scale[4 * i + 2] = v.z, row_scale[4 * i + 3] = v.w;
-            if constexpr (Experts) {
-                const int4 r = reinterpret_cast<const int4*>(tail.rows[buffer])[column / 4 + i];
-                row[4 * i] = r.x, row[4 * i + 1] = r.y, row[4 * i + 2] = r.z, row[4 * i + 3] = r.w;
-            }
-        }
-        T* to = y + static_cast<std::int64_t>(column) * a.outputs;
-        auto value = [&](int i) {
-            const float v = __fmul_rn(__fmul_rn(__int2float_rn(acc[i]), scale), row_scale[i]);
-            return narrow<T>(a.bias != nullptr ? __fadd_rn(v, bias) : v);
-        };
-        if (column + 16 <= t.rows) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 4; ++i) {
+                const float4 v = reinterpret_cast<const float4*>(tail.row_scales[buffer])[column / 4 + i];
+                row_scale[4 * i] = v.x, row_scale[4 * i + 1] = v.y, row_scale[4 * i + 2] = v.z, row_scale[4 * i + 3] = v.w;
                 if constexpr (Experts) {
-                    y[static_cast<std::int64_t>(row[i]) * a.outputs] = value(i);
-                } else {
-                    *to = value(i);
-                    to += a.outputs;
+                    const int4 r = reinterpret_cast<const int4*>(tail.rows[buffer])[column / 4 + i];
+                    row[4 * i] = r.x, row[4 * i + 1] = r.y, row[4 * i + 2] = r.z, row[4 * i + 3] = r.w;
                 }
             }
-        } else {
+            T* to = y + static_cast<std::int64_t>(column) * a.outputs;
+            auto value = [&](int i) {
+                const float v = __fmul_rn(__fmul_rn(__int2float_rn(acc[i]), scale), row_scale[i]);
+                return narrow<T>(a.bias != nullptr ? __fadd_rn(v, bias) : v);
+            };
+            if (column + 16 <= t.rows) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if (column + i < t.rows) y[static_cast<std::int64_t>(Experts ? row[i] : column + i) * a.outputs] = value(i);
+                for (int i = 0; i < 16; ++i) {
+                    if constexpr (Experts) {
+                        y[static_cast<std::int64_t>(row[i]) * a.outputs] = value(i);
+                    } else {
+                        *to = value(i);
+                        to += a.outputs;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (column + i < t.rows) y[static_cast<std::int64_t>(Experts ? row[i] : column + i) * a.outputs] = value(i);
+                }
             }
         }
+        __syncwarp();  // the TMEM instructions take whole warps: reconverge before the next columns
     }
     tmem_load_wait();
 }
@@ -693,7 +697,8 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
             const Tile t = tile_at<Experts>(a, item);
             if (splits == 1) stage_rows<Experts>(a, t, tail, buffer);
             if (epilogue_any(*abort != 0)) break;  // all of them, as the next ones wait for one another here
-            if (!barrier_wait(smem_address(&tail.tmem_full[buffer]), pass, waits)) {
+            // the TMEM loads take whole warps, so a warp takes one decision
+            if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&tail.tmem_full[buffer]), pass, waits))) {
                 *abort = 1;
                 continue;
             }
@@ -907,7 +912,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
             const Tile t = tile_at<Experts, true>(a, item);
             stage_rows<Experts>(a, t, tail, buffer);
             if (epilogue_any(*abort != 0)) break;  // all of them, as the next ones wait for one another here
-            if (!barrier_wait(smem_address(&tail.tmem_full[buffer]), pass, waits)) {
+            // the TMEM loads take whole warps, so a warp takes one decision
+            if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&tail.tmem_full[buffer]), pass, waits))) {
                 *abort = 1;
                 continue;
             }
