@@ -529,6 +529,14 @@ int nvcr_sm100_token_experts_multiply(int type, const void* x, int64_t x_stride,
                                       int32_t inputs, void* y, void* workspace, size_t workspace_bytes,
                                       uint32_t* status, void* stream);
 
+/* Failure-detection self-test: this thread's next call of the two products above
+ * runs with block `block` of its product kernel copying nothing, and with waits
+ * that give up after limit_ms (1..4000): those for what that block should have
+ * copied do, as any wait in the kernel would, and the CUDA context stays usable.
+ * Calls of a few rows, which wait for nothing, and blocks that the kernel does not
+ * have are as always. */
+int nvcr_sm100_token_test_wait_timeout(unsigned int limit_ms, int32_t block);
+
 /* Routing of tokens to experts (at most 1024) by scores [tokens][experts] (F16,
  * BF16 or F32): s = softmax of a token's scores, or their sigmoid when `sigmoid`
  * is not 0; b = s + bias (FP32 [experts], may be NULL). The experts are `groups`

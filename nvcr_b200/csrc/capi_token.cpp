@@ -121,6 +121,18 @@ bool byte_matrix_shape(std::int64_t matrices, std::int32_t outputs, std::int32_t
 }
 constexpr const char* byte_matrix_reason = "a matrix has 1 to 2^24 outputs and 1 to 131072 inputs";
 
+// Of this thread's next call of a product in 8 bits, which takes it.
+struct WaitTest {
+    unsigned long long limit_ns = 0;
+    std::int32_t block = -1;
+};
+thread_local WaitTest wait_test;
+
+void take_wait_test(token::BytesArgs& args) {
+    args.wait_ns = wait_test.limit_ns, args.withheld = wait_test.block;
+    wait_test = {};
+}
+
 bool aligned(const void* buffer) { return reinterpret_cast<std::uintptr_t>(buffer) % 16 == 0; }
 
 // Null when the experts' call can be made, else why not. Rows of experts are padded by up to 15, and counted in 32 bits.
@@ -418,6 +430,7 @@ int nvcr_sm100_token_bytes_multiply(int type, const void* x, int64_t x_stride, i
         args.x = x, args.x_stride = x_stride;
         args.packed = packed, args.scales = scales, args.bias = bias, args.y = y;
         args.workspace = workspace, args.status = status;
+        take_wait_test(args);
         return launched(token::multiply_bytes(args, static_cast<cudaStream_t>(stream)));
     });
 }
@@ -457,7 +470,17 @@ int nvcr_sm100_token_experts_multiply(int type, const void* x, int64_t x_stride,
         if (rows_each != 0) args.inner = chosen, args.x_inner_stride = x_row_stride;
         args.packed = packed, args.scales = scales, args.y = y;
         args.workspace = workspace, args.status = status;
+        take_wait_test(args);
         return launched(token::multiply_bytes(args, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+int nvcr_sm100_token_test_wait_timeout(unsigned int limit_ms, int32_t block) {
+    return guarded([&] {
+        if (limit_ms == 0 || limit_ms > 4000) return refuse("the limit must be 1 to 4000 ms");
+        if (block < 0) return refuse("block out of range");
+        wait_test = {limit_ms * 1000000ull, block};
+        return report_ok();
     });
 }
 

@@ -392,6 +392,8 @@ struct ProductArgs {
     unsigned tmem_columns;
     void* y;
     unsigned* status;
+    unsigned long long wait_ns;  // after which a wait gives up
+    int withheld;                // the block that copies nothing, so that waits do (a self-test), or -1
 };
 
 struct ProductTail {
@@ -402,6 +404,7 @@ struct ProductTail {
     std::uint32_t tmem;
     unsigned status;  // of waits: told to the caller's at the end
     int abort;
+    int given_up;     // by a block of the cluster, which tells all: its sums are missing
 };
 
 __device__ __forceinline__ void bulk_load(std::uint32_t to, const void* from, std::uint32_t bytes, std::uint32_t barrier) {
@@ -558,7 +561,7 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
         }
         barrier_init(smem_address(&tail.drain), 1);
         tail.status = 0;
-        tail.abort = 0;
+        tail.abort = tail.given_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async_shared();
     }
@@ -590,7 +593,8 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
         // at least: a warp that ran ahead by two uses of a stage would take the parity of its barrier's phase before last for
         // the last one's.)
         const int blocks = k_to - k_from;
-        const std::int64_t mine = first_item < items ? static_cast<std::int64_t>((items - first_item + item_step - 1) / item_step) * blocks : 0;
+        const bool copying = first_item < items && static_cast<int>(blockIdx.x) != a.withheld;
+        const std::int64_t mine = copying ? static_cast<std::int64_t>((items - first_item + item_step - 1) / item_step) * blocks : 0;
         auto of = [&](std::int64_t q, std::uint32_t& bytes, const std::uint8_t*& weights, const std::uint8_t*& rows) {
             const std::int64_t nth = q / blocks;
             const int k = k_from + static_cast<int>(q - nth * blocks);
@@ -631,7 +635,7 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
                     moved = false;
                 }
                 bool free = true;
-                if (lane == 0) free = !*abort && barrier_wait(smem_address(&tail.empty[slot]), (pass & 1u) ^ 1u, waits);
+                if (lane == 0) free = !*abort && barrier_wait_for(smem_address(&tail.empty[slot]), (pass & 1u) ^ 1u, waits, a.wait_ns);
                 if (!__shfl_sync(3u, free, 0)) {
                     *abort = 1;
                     break;
@@ -646,7 +650,7 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
             }
             if (*abort && lane == 0) {  // the copies under way: of q - 4, q - 8, ...
                 for (std::int64_t last = q - copy_warps; last >= 0 && last > q - copy_warps - a.stages; last -= copy_warps) {
-                    if (last < mine) barrier_wait(smem_address(&tail.full[last % a.stages]), last / a.stages & 1, waits);
+                    if (last < mine) barrier_wait_for(smem_address(&tail.full[last % a.stages]), last / a.stages & 1, waits, a.wait_ns);
                 }
             }
         }
@@ -660,11 +664,11 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
                 const Tile t = next;
                 if (items - item > item_step) next = tile_at<Experts>(a, item + item_step);  // its latency under this one's products
                 const std::uint32_t instruction = i8_instruction(t.columns);
-                bool going = barrier_wait(smem_address(&tail.tmem_empty[buffer]), pass ^ 1u, waits);
+                bool going = barrier_wait_for(smem_address(&tail.tmem_empty[buffer]), pass ^ 1u, waits, a.wait_ns);
                 tmem_fence_after();
                 const std::uint32_t sums = tmem + static_cast<std::uint32_t>(buffer * a.tile_rows);
                 for (int k = k_from; going && k < k_to; ++k) {
-                    going = barrier_wait(smem_address(&tail.full[slot]), phase, waits);
+                    going = barrier_wait_for(smem_address(&tail.full[slot]), phase, waits, a.wait_ns);
                     if (!going) break;
                     tmem_fence_after();
                     const std::uint64_t w = first_weights + static_cast<std::uint64_t>(slot * (weight_block >> 4));
@@ -685,7 +689,7 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
             }
             if (*abort) {  // the MMAs under way
                 mma_commit(smem_address(&tail.drain));
-                barrier_wait(smem_address(&tail.drain), 0, waits);
+                barrier_wait_for(smem_address(&tail.drain), 0, waits, a.wait_ns);
             }
         }
     } else {
@@ -698,7 +702,7 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
             if (splits == 1) stage_rows<Experts>(a, t, tail, buffer);
             if (epilogue_any(*abort != 0)) break;  // all of them, as the next ones wait for one another here
             // the TMEM loads take whole warps, so a warp takes one decision
-            if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&tail.tmem_full[buffer]), pass, waits))) {
+            if (!__all_sync(0xffffffffu, barrier_wait_for(smem_address(&tail.tmem_full[buffer]), pass, waits, a.wait_ns))) {
                 *abort = 1;
                 continue;
             }
@@ -728,9 +732,10 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
 
     if (splits > 1) {
         if (warp >= epilogue_warps) cluster_wait();
+        if (*abort && lane < splits) peer_store(smem_address(&tail.given_up), lane, 1);  // the warp that gave up is one of them
         cluster_arrive();
         cluster_wait();
-        if (first_item < items && !*abort) {
+        if (first_item < items && !*static_cast<volatile int*>(&tail.given_up)) {
             const Tile t = tile_at<Experts>(a, first_item);
             const int mine = block_rows / splits;
             const int* sums = reinterpret_cast<const int*>(dynamic + (exchange - raw));
@@ -814,7 +819,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
     const int items = row_tiles * ((a.tiles + 1) / 2);
 
     if (warp >= copy_warp && warp < copy_warp + copy_warps) {
-        const std::int64_t mine = first_item < items ? static_cast<std::int64_t>((items - first_item + item_step - 1) / item_step) * groups : 0;
+        const bool copying = first_item < items && static_cast<int>(blockIdx.x) != a.withheld;
+        const std::int64_t mine = copying ? static_cast<std::int64_t>((items - first_item + item_step - 1) / item_step) * groups : 0;
         // No more warps take turns than there are stages: one that ran ahead by two uses of a stage would take the parity of
         // its barrier's phase before last for the last one's.
         const int turns = min(copy_warps, a.stages);
@@ -841,7 +847,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
                     moved = false;
                 }
                 bool free = true;
-                if (lane == 0) free = !*abort && barrier_wait(smem_address(&tail.empty[slot]), (pass & 1u) ^ 1u, waits);
+                if (lane == 0) free = !*abort && barrier_wait_for(smem_address(&tail.empty[slot]), (pass & 1u) ^ 1u, waits, a.wait_ns);
                 if (!__shfl_sync(copy_lanes, free, 0)) {
                     *abort = 1;
                     break;
@@ -855,7 +861,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
             }
             if (*abort && lane == 0 && rank == 0) {  // the copies under way, the other block's too
                 for (std::int64_t last = q - turns; last >= 0 && last > q - turns - a.stages; last -= turns) {
-                    barrier_wait(smem_address(&tail.full[last % a.stages]), last / a.stages & 1, waits);
+                    barrier_wait_for(smem_address(&tail.full[last % a.stages]), last / a.stages & 1, waits, a.wait_ns);
                 }
             }
         }
@@ -870,11 +876,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
                 const Tile t = next;
                 if (items - item > item_step) next = tile_at<Experts, true>(a, item + item_step);  // its latency under this one's products
                 const std::uint32_t instruction = i8_pair_instruction(t.columns);
-                bool going = barrier_wait(smem_address(&tail.tmem_empty[buffer]), pass ^ 1u, waits);
+                bool going = barrier_wait_for(smem_address(&tail.tmem_empty[buffer]), pass ^ 1u, waits, a.wait_ns);
                 tmem_fence_after();
                 const std::uint32_t sums = tmem + static_cast<std::uint32_t>(buffer * a.tile_rows);
                 for (int k = 0; going && k < blocks; k += pair_blocks) {
-                    going = barrier_wait(smem_address(&tail.full[slot]), phase, waits);
+                    going = barrier_wait_for(smem_address(&tail.full[slot]), phase, waits, a.wait_ns);
                     if (!going) break;
                     tmem_fence_after();
                     const std::uint64_t w = first_weights + static_cast<std::uint64_t>(slot * (pair_blocks * weight_block >> 4));
@@ -901,7 +907,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
             }
             if (*abort) {  // the MMAs under way
                 mma_commit_pair(smem_address(&tail.drain));
-                barrier_wait(smem_address(&tail.drain), 0, waits);
+                barrier_wait_for(smem_address(&tail.drain), 0, waits, a.wait_ns);
             }
         }
     } else {
@@ -913,7 +919,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
             stage_rows<Experts>(a, t, tail, buffer);
             if (epilogue_any(*abort != 0)) break;  // all of them, as the next ones wait for one another here
             // the TMEM loads take whole warps, so a warp takes one decision
-            if (!__all_sync(0xffffffffu, barrier_wait(smem_address(&tail.tmem_full[buffer]), pass, waits))) {
+            if (!__all_sync(0xffffffffu, barrier_wait_for(smem_address(&tail.tmem_full[buffer]), pass, waits, a.wait_ns))) {
                 *abort = 1;
                 continue;
             }
@@ -1223,7 +1229,7 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
     r.tile_rows = shape.tile_rows;
     const std::int64_t items = row_tiles * (shape.pair ? (r.tiles + 1) / 2 : r.tiles);
     r.splits = shape.pair ? 1 : splits_of(items, r.tile_rows, r.k_blocks);
-    r.status = a.status;
+    r.status = a.status, r.wait_ns = a.wait_ns != 0 ? a.wait_ns : wait_limit_ns, r.withheld = a.withheld;
     if (a.choices == nullptr) {
         r.y = a.y;
         return product<false>(a.type, r, items, shape.pair, stream);

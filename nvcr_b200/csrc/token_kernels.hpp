@@ -157,6 +157,9 @@ struct BytesArgs {
     void* y;           // [tokens][chosen][outputs], or with weights [tokens][outputs]
     void* workspace;
     unsigned* status;  // null: not wanted
+    // self-test: after how long a wait gives up (0: the kernels' limit), and the block that copies nothing (-1: none)
+    unsigned long long wait_ns = 0;
+    int withheld = -1;
 };
 std::size_t byte_matrix_bytes(std::int64_t matrices, int outputs, int inputs);
 cudaError_t pack_bytes(const std::int8_t* codes, std::int64_t matrices, int outputs, int inputs, void* packed,

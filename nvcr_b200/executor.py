@@ -89,7 +89,8 @@ EXPORTS = [
     "nvcr_sm100_token_attend", "nvcr_sm100_token_packed_bytes", "nvcr_sm100_token_pack", "nvcr_sm100_token_multiply",
     "nvcr_sm100_token_bytes_packed", "nvcr_sm100_token_bytes_pack", "nvcr_sm100_token_bytes_workspace",
     "nvcr_sm100_token_bytes_multiply", "nvcr_sm100_token_experts_workspace", "nvcr_sm100_token_experts_multiply",
-    "nvcr_sm100_token_route", "nvcr_sm100_token_sample", "nvcr_sm100_token_sample_workspace",
+    "nvcr_sm100_token_test_wait_timeout", "nvcr_sm100_token_route", "nvcr_sm100_token_sample",
+    "nvcr_sm100_token_sample_workspace",
 ]
 
 _lib: ctypes.CDLL | None = None
@@ -206,6 +207,7 @@ def library() -> ctypes.CDLL:
         "nvcr_sm100_token_experts_multiply": (ctypes.c_int, [ctypes.c_int, vp, i64, i64, ctypes.c_int, i64, vp,
                                                              ctypes.c_int32, vp, vp, vp] + [ctypes.c_int32] * 3 +
                                               [vp, vp, sz, vp, vp]),
+        "nvcr_sm100_token_test_wait_timeout": (ctypes.c_int, [ctypes.c_uint, ctypes.c_int32]),
         "nvcr_sm100_token_route": (ctypes.c_int, [ctypes.c_int, vp, i64, i64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int,
                                                   vp, ctypes.c_int32, ctypes.c_int32, ctypes.c_int, ctypes.c_float, vp,
                                                   vp, vp]),
