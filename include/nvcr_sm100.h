@@ -519,8 +519,9 @@ int nvcr_sm100_token_bytes_multiply(int type, const void* x, int64_t x_stride, i
  * with `rows_each` not 0 [tokens][chosen][inputs]; scales are [experts][outputs].
  * Without weights (NULL) y is [tokens][chosen][outputs]; with them, y[t] =
  * sum_j weights[t][j] * product, [tokens][outputs], added in FP32 in the order
- * of j and rounded once. A choice outside 0 .. experts - 1 has no product: zeros,
- * and nothing in the sum. choices and weights (FP32) are contiguous. */
+ * of j and rounded once (where a wait runs out, none of them is written). A choice
+ * outside 0 .. experts - 1 has no product: zeros, and nothing in the sum. choices
+ * and weights (FP32) are contiguous. */
 int nvcr_sm100_token_experts_workspace(int64_t tokens, int32_t chosen, int weighted, int32_t experts, int32_t outputs,
                                        int32_t inputs, size_t* bytes);
 int nvcr_sm100_token_experts_multiply(int type, const void* x, int64_t x_stride, int64_t x_row_stride, int rows_each,

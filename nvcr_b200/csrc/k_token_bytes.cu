@@ -77,6 +77,7 @@ struct Arranged {
     int* pair;        // [rows]: the pair of a row
     int4* tiles;      // expert, first row, rows
     int* tile_count;
+    int* given_up;    // whether a block of the product has: some products are missing
 };
 
 constexpr int arrange_blocks = 8;
@@ -127,7 +128,7 @@ __global__ void __cluster_dims__(arrange_blocks, 1, 1) __launch_bounds__(arrange
         for (int t = 0; t < tiles; ++t) {
             out.tiles[tile + t] = {thread, row + t * tile_rows, min(tile_rows, count - t * tile_rows), 0};
         }
-        if (thread == 0) *out.tile_count = all_tiles;
+        if (thread == 0) *out.tile_count = all_tiles, *out.given_up = 0;
     }
     next[thread] = row + before;
     __syncthreads();
@@ -213,7 +214,7 @@ __device__ __forceinline__ void find_places(const QuantiseArgs& a, int first, in
         }
         row += (have + step_rows - 1) / step_rows * step_rows;
     }
-    if (blockIdx.x == 0 && thread == 0) *a.arranged.tile_count = all_tiles;
+    if (blockIdx.x == 0 && thread == 0) *a.arranged.tile_count = all_tiles, *a.arranged.given_up = 0;
     __syncthreads();
     for (int n = warp; n < count; n += 8) {  // a warp a pair: those with the same expert before it
         const int i = first + n, e = choices[i];
@@ -429,6 +430,13 @@ __device__ __forceinline__ bool epilogue_any(bool mine) {
         : "r"(static_cast<int>(mine))
         : "memory");
     return any != 0;
+}
+
+// What a block whose wait ran out leaves behind: its status, and that sums over experts are not to be made.
+template <bool Experts>
+__device__ __forceinline__ void give_up(const ProductArgs& a, unsigned status) {
+    if (a.status != nullptr) atomicOr(a.status, status);
+    if (Experts) atomicExch(a.arranged.given_up, 1);
 }
 
 struct Tile {
@@ -758,7 +766,7 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
     __syncthreads();
     if (warp == mma_warp) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_columns) : "memory");
-        if (lane == 0 && tail.status != 0 && a.status != nullptr) atomicOr(a.status, tail.status);
+        if (lane == 0 && tail.status != 0) give_up<Experts>(a, tail.status);
     }
 }
 
@@ -939,7 +947,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
     cluster_wait();
     if (warp == mma_warp) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_columns) : "memory");
-        if (lane == 0 && tail.status != 0 && a.status != nullptr) atomicOr(a.status, tail.status);
+        if (lane == 0 && tail.status != 0) give_up<Experts>(a, tail.status);
     }
 }
 
@@ -948,8 +956,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads, 1) 
 // A thread Each outputs: four where rows of outputs are whole vectors.
 template <typename T, int Each>
 __global__ void __launch_bounds__(128) combine_kernel(const float* products, const std::int32_t* choices, const float* weights,
-                                                      int chosen, int experts, int outputs, T* y) {
+                                                      int chosen, int experts, int outputs, const int* given_up, T* y) {
     join_chain();
+    const bool whole = *given_up == 0;  // else products are missing, and nothing is written
     const std::int64_t token = blockIdx.x;
     for (int output = static_cast<int>(blockIdx.y * 128 + threadIdx.x) * Each; output < outputs; output += static_cast<int>(gridDim.y) * 128 * Each) {
         float sum[Each] = {};
@@ -969,7 +978,9 @@ __global__ void __launch_bounds__(128) combine_kernel(const float* products, con
             }
         }
 #pragma unroll
-        for (int i = 0; i < Each; ++i) y[token * outputs + output + i] = narrow<T>(sum[i]);
+        for (int i = 0; i < Each; ++i) {
+            if (whole) y[token * outputs + output + i] = narrow<T>(sum[i]);
+        }
     }
 }
 
@@ -1150,7 +1161,7 @@ Plan plan_of(const BytesArgs& a) {
         p.place = take(pairs * sizeof(int));
         p.pair = take(p.out_rows * sizeof(int));
         p.table = take((pairs / step_rows + p.groups) * sizeof(int4));
-        p.count = take(sizeof(int));
+        p.count = take(2 * sizeof(int));
         if (a.weights != nullptr) p.products = take(static_cast<std::size_t>(pairs) * a.outputs * sizeof(float));
     }
     p.bytes = at;
@@ -1158,12 +1169,12 @@ Plan plan_of(const BytesArgs& a) {
 }
 
 template <typename T>
-cudaError_t combine(const BytesArgs& a, const float* products, cudaStream_t stream) {
+cudaError_t combine(const BytesArgs& a, const float* products, const int* given_up, cudaStream_t stream) {
     const int each = a.outputs % 4 == 0 ? 4 : 1;
     const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(std::min((a.outputs + 128 * each - 1) / (128 * each), 65535)));
     auto kernel = each == 4 ? combine_kernel<T, 4> : combine_kernel<T, 1>;
     return launch_overlapped(kernel, grid, dim3(128), 0, stream, products, a.choices, a.weights, a.chosen, a.experts, a.outputs,
-                             static_cast<T*>(a.y));
+                             given_up, static_cast<T*>(a.y));
 }
 
 }  // namespace
@@ -1197,7 +1208,8 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
     Arranged arranged{};
     if (a.choices != nullptr) {
         arranged = {reinterpret_cast<int*>(memory + p.place), reinterpret_cast<int*>(memory + p.pair),
-                    reinterpret_cast<int4*>(memory + p.table), reinterpret_cast<int*>(memory + p.count)};
+                    reinterpret_cast<int4*>(memory + p.table), reinterpret_cast<int*>(memory + p.count),
+                    reinterpret_cast<int*>(memory + p.count) + 1};
     }
     QuantiseArgs q{};
     if (a.choices != nullptr && pairs <= most_own_pairs) {
@@ -1244,9 +1256,9 @@ cudaError_t multiply_bytes(const BytesArgs& a, cudaStream_t stream) {
     status = product<true>(Type::f32, r, items, shape.pair, stream);
     if (status != cudaSuccess) return status;
     switch (a.type) {
-    case Type::f16: return combine<__half>(a, products, stream);
-    case Type::bf16: return combine<__nv_bfloat16>(a, products, stream);
-    default: return combine<float>(a, products, stream);
+    case Type::f16: return combine<__half>(a, products, arranged.given_up, stream);
+    case Type::bf16: return combine<__nv_bfloat16>(a, products, arranged.given_up, stream);
+    default: return combine<float>(a, products, arranged.given_up, stream);
     }
 }
 

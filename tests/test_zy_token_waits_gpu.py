@@ -142,3 +142,10 @@ def test_a_block_of_a_pair_gives_up(cuda, block):
     assert not written.all() and written.any()
     written = experts_case(2000, 2, 4, 4096, 2048, block, weighted=False)
     assert not written.all() and written.any()
+
+
+@pytest.mark.parametrize("block", [0, 5])
+@pytest.mark.parametrize("tokens,chosen,experts,inputs,outputs", [(100, 2, 4, 2048, 300), (1000, 2, 5, 129, 257), (2000, 2, 4, 4096, 2048)])
+def test_sums_over_experts_of_a_call_that_gave_up_are_not_written(cuda, tokens, chosen, experts, inputs, outputs, block):
+    """Every token's sum needs products of several blocks, so none of the call's is stored."""
+    assert not experts_case(tokens, chosen, experts, inputs, outputs, block, weighted=True).any()
