@@ -2,7 +2,8 @@
 // codes q = rint(x / s) with a scale s of their own, one matrix for all rows or the matrix of the expert that each
 // row has chosen. The sums are exact in int32, so their order, and a split of them, change no bit.
 //
-// Three launches at most: where the rows of each expert go (`arrange`), the rows as codes (`quantise`), the product.
+// Four launches at most: where the rows of each expert go (`arrange`; up to 1024 pairs the next one finds that itself), the
+// rows as codes (`quantise`), the product, and for weighted sums over experts their products' sums (`combine`).
 // Both operands lie in memory as the tensor cores read them from shared memory, in the 128-byte swizzle: weights as
 // blocks of 128 outputs by 128 inputs, rows as [128 inputs][row][128 bytes]. So every tile is one contiguous copy,
 // with neither a tensor map nor an alignment that a caller has to keep.
@@ -27,6 +28,8 @@ std::size_t aligned(std::size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // ---- weights: [matrix][tile of outputs][block of inputs][128][128], zeros past the edges, laid out once ----
 
+// Products read one matrix's weights before they wait for the kernel before them, so a kernel that writes weights neither
+// starts early nor lets the next one: no programmatic launch here.
 __global__ void __launch_bounds__(256) pack_kernel(const std::int8_t* codes, std::int64_t blocks, int outputs, int inputs,
                                                    int tiles, int k_blocks, uint4* packed) {
     // a thread a 16-byte piece: piece c of row r lies at piece c ^ (r % 8)
@@ -619,8 +622,9 @@ __global__ void __launch_bounds__(product_threads, 1) product_kernel(const Produ
         if (filling) {
             of(own, bytes, weights, rows);
             barrier_expect_bytes(own_full, weight_block + bytes);
-            // The kernel before this one lets it start when all before that one have ended, and weights are written by
-            // kernels that let nothing start early: one matrix's need not wait. Which expert's, the tiles have said.
+            // The kernel before this one makes the codes; it lets this one start only after its own wait, so when all
+            // before it have ended, and weights are written by kernels that let nothing start early: one matrix's need not
+            // wait. Which expert's, the tiles have said.
             bulk_load(ring + own * weight_block, weights, weight_block, own_full);
         }
         __syncwarp();

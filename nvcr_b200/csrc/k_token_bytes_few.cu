@@ -1,6 +1,12 @@
 // Products in 8 bits for a few rows, where the weights' bytes are the work and a launch's latency most of the time: one
-// launch, in which every block takes its rows of x as codes into shared memory while its first weights are on their way
-// to registers, and multiplies them by dp4a (one row of 4096 -> 4096: 6.9 us, of which 2.6 are the weights at HBM's rate). Sums are exact in int32, so their splits and orders change no bit.
+// launch, in which every block loads its first weights, takes its rows of x as codes into shared memory and multiplies
+// them by dp4a (one row of 4096 -> 4096: 7.0 to 7.3 us, of which 2.6 are the weights at HBM's rate). Sums are exact in
+// int32, so their splits and orders change no bit.
+//
+// The first weights are meant to be on their way while the codes are made, but two blocks an SM leave 64 registers a
+// thread, of which the weights are 32 and a piece of x in FP32 another 16: all variants spill 156 to 252 bytes a thread
+// then, and a register whose load is under way is stored only once it has come. So how much of the two runs side by side is
+// not known.
 //
 // A warp has eight outputs at a time: rows 16 g + 4 h + {0..3} and those 8 below, whose pieces of a swizzled block lie
 // alike, so that a lane's piece of x serves two loads of weights.

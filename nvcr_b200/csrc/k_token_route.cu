@@ -7,7 +7,8 @@
 // takes a token whose choices differ by less than that arithmetic's error again in FP64 (`exactly`), unless scores and
 // biases are equal. The weights are FP64 in either. 16384 tokens by 8 of 256 experts in groups: 30.9 us, 90 with all
 // tokens in FP64; 1130 warp instructions a token keep the schedulers busy for 68% of that, where the scores'
-// bytes take 2.7.
+// bytes take 2.7. More than 256 experts, 31 choices or 32 groups go in FP64 throughout: 16384 tokens by 8 of 512 in 118 us, by
+// 32 of 256, or by 8 of 256 in 64 groups, in 148.
 #include "token_elements.cuh"
 
 #include <climits>

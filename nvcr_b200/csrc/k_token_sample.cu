@@ -17,7 +17,9 @@
 // (`part_kernel`); a block a row, which ends it (`end_kernel`); the rows that were not ended, a cluster each
 // (`rest_kernel`). 256 rows of 131072 took 58 us by clusters, whose blocks were idle while they waited for one another.
 //
-// Longer rows and infinite logits take `row_by_block`, which finds the threshold's bits from memory with one block.
+// Longer rows (past 2^18 FP32 symbols, 2^19 in 16 bits), infinite logits and, of a few rows, choices that hang on the FP32
+// sum's error take `row_by_block`, which finds the threshold's bits from memory with one block in up to eight passes: one
+// row of 32768 FP32 logits 47 us (by an infinity 125), of 131072 166, of 2^18 + 1 940, of 2^20 4.2 ms.
 //
 // One row of 32768 FP32 logits (top_k 50, top_p 0.95) 11 us: launch, four exchanges of a cluster, one warp's end of the
 // row. 256 rows of 131072 BF16 logits (top_p 0.9, min_p 0.01) 37 us, of which 10 are the logits at HBM's rate: parts take

@@ -12,9 +12,12 @@
 
 namespace nvcr_sm100::token {
 
-// The first thing every kernel does: a token model's step is a chain of short
+// The first thing a kernel does: a token model's step is a chain of short
 // launches, so each starts while the one before it ends, and waits for it here,
-// before it touches memory; then the next may start the same way.
+// before it touches memory; then the next may start the same way. (Products in
+// 8 bits let the next one start before they wait, and the one-matrix ones have
+// weights on their way by then, which only kernels that let nothing start early
+// write.)
 __device__ __forceinline__ void join_chain() {
     kernels::grid_dependency_wait();
     kernels::launch_dependents();
